@@ -639,6 +639,71 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
                                   int64_t* age, float* error, int64_t* n_spawned, void* scratch,
                                   int64_t scratch_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Window attention over packed windows, and the gated residual norm
+ * (dtype: 0 fp32, 1 bf16, 2 fp16).
+ *
+ * Window w holds queries [q_offsets[w], q_offsets[w+1]) and keys
+ * [k_offsets[w], k_offsets[w+1]) (device int32, windows + 1 each, non-decreasing;
+ * values outside [0, tq] or [0, tk] are clamped).  With group = heads / kv_heads,
+ * query head h reads key head h / group:
+ *   s_ij = scale q_i.k_j + table[bucket_map[d(i, j)]][h],  p = softmax_j s,  out_i = sum_j p_ij v_j
+ * causal: key j is visible where j <= i + (keys - queries), both counted in their
+ * window.  A row that sees no key, and a row outside every window, is zero.
+ *   q[tq][heads][dim], k and v[tk][kv_heads][dim]  token and head strides in elements, unit last stride
+ *   out[tq][heads][dim], d_q, d_k, d_v             contiguous
+ *   lse[heads][tq]     fp32, base-2 log of the row's sum (null: not wanted); +inf for a row without keys
+ *   table[buckets][heads]  null: no bias.  bucket_map[2 ry + 1][2 rx + 1] maps the key's position less the
+ *                      query's, clamped to +-ry and +-rx, to a row of the table; a value outside
+ *                      [0, buckets) adds no bias.  At most 4096 entries.
+ *   q_pos[tq][axes], k_pos[tk][axes]  int32 (y, x), or (x) with axes = 1; clamped to +-2^29
+ * entries: (2 ry + 1)(2 rx + 1), 0 without a table.
+ * ------------------------------------------------------------------------- */
+OSS_API int64_t oss_window_attention_scratch_bytes(int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                                                   int64_t kv_heads, int64_t dim, int64_t entries);
+OSS_API int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                                         int64_t kv_heads, int64_t dim, const void* q, int64_t q_st, int64_t q_sh,
+                                         const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                                         int64_t v_sh, const int32_t* q_offsets, const int32_t* k_offsets, float scale,
+                                         int32_t causal, const void* table, int32_t table_dtype, int64_t buckets,
+                                         const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
+                                         const int32_t* k_pos, int32_t axes, void* out, float* lse, void* scratch,
+                                         int64_t scratch_bytes, void* stream);
+/* buckets: rows of the table whose gradient is wanted, else 0. */
+OSS_API int64_t oss_window_attention_backward_scratch_bytes(int64_t tq, int64_t heads, int64_t buckets);
+/* d_table[buckets][heads] in the table's dtype, null: not wanted.  Every gradient is the same
+ * on every run: sums have a fixed order, those of d_table are 64-bit integers. */
+OSS_API int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                                          int64_t kv_heads, int64_t dim, const void* q, int64_t q_st, int64_t q_sh,
+                                          const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                                          int64_t v_sh, const int32_t* q_offsets, const int32_t* k_offsets, float scale,
+                                          int32_t causal, const void* table, int32_t table_dtype, int64_t buckets,
+                                          const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
+                                          const int32_t* k_pos, int32_t axes, const void* out, const float* lse,
+                                          const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
+                                          void* d_v, void* d_table, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* n = norm(h) weight + bias,  y = x + scale act(gate) n,  z = norm(y) next_weight + next_bias.
+ * layer: 1 mean and variance, 0 mean of squares.  gate_kind: 0 none, 1 gate[rows], 2 gate[rows][channels];
+ * act: 0 none, 1 sigmoid, 2 silu.  Row strides in elements; y, z and the gradients are contiguous.
+ * scale, bias, next_bias, z and stats may be null (1, 0, 0, not wanted); stats[rows][4] is what the
+ * backward needs.  Parameters [channels] share param_dtype. */
+OSS_API int oss_gated_norm_forward(int32_t dtype, int64_t rows, int64_t channels, const void* x, int64_t x_st,
+                                   const void* h, int64_t h_st, const void* gate, int64_t gate_st, int32_t gate_kind,
+                                   int32_t act, int32_t layer, float eps, int32_t param_dtype, const void* weight,
+                                   const void* bias, const void* scale, const void* next_weight, const void* next_bias,
+                                   void* y, void* z, float* stats, void* stream);
+OSS_API int64_t oss_gated_norm_backward_scratch_bytes(int64_t rows, int64_t channels);
+/* d_y or d_z null: zero.  Gradients that are null are not wanted. */
+OSS_API int oss_gated_norm_backward(int32_t dtype, int64_t rows, int64_t channels, const void* x, int64_t x_st,
+                                    const void* h, int64_t h_st, const void* gate, int64_t gate_st, int32_t gate_kind,
+                                    int32_t act, int32_t layer, float eps, int32_t param_dtype, const void* weight,
+                                    const void* bias, const void* scale, const void* next_weight, const void* next_bias,
+                                    const float* stats, const void* d_y, int64_t dy_st, const void* d_z, int64_t dz_st,
+                                    void* d_x, void* d_h, void* d_gate, void* d_weight, void* d_bias, void* d_scale,
+                                    void* d_next_weight, void* d_next_bias, void* scratch, int64_t scratch_bytes,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

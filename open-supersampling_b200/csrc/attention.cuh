@@ -1,0 +1,225 @@
+// Window attention over packed windows: the parameters, the walk over the
+// windows' tiles and the bucketed position bias that all its kernels share.
+//
+// Window w holds queries [q_off[w], q_off[w+1]) and keys [k_off[w], k_off[w+1]).
+//   s_ij = scale q_i.k_j + table[bucket[clamp(kpos_j - qpos_i)], h]
+//   p_ij = softmax over the visible j of s_ij,   o_i = sum_j p_ij v_j
+// All softmax arithmetic is in base 2: the kernels hold s log2(e).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace oss {
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Entries of the expanded position bias, (2 ry + 1) (2 rx + 1): a head's bias and its 64-bit
+// gradient sums stay in shared memory beside the tiles (16 + 32 KB).
+constexpr int kMaxBiasEntries = 4096;
+constexpr int kMaxHeadDim = 128;
+// Positions are clamped to this magnitude on load, so that their differences and the linear
+// codes y (2 rx + 1) + x of positions that need no clamp stay within int32.
+constexpr int kMaxPosition = 1 << 29;
+
+enum AttnType { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+struct AttnBias {
+    const void* table;       // [buckets][heads], null: no bias
+    int table_type;          // AttnType
+    int buckets;             // rows of table
+    const int32_t* map;      // [2 ry + 1][2 rx + 1] -> row of table; outside [0, buckets): no bias
+    int ry, rx;
+    const int32_t* q_pos;    // [tq][axes], (y, x) or (x)
+    const int32_t* k_pos;    // [tk][axes]
+    int axes;
+};
+
+struct AttnParams {
+    const void *q, *k, *v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // strides in elements: token, head
+    const int32_t *q_off, *k_off;                // [windows + 1]
+    int windows, tq, tk;
+    int heads, kv_heads, dim;
+    float scale;
+    int causal;
+    AttnBias bias;
+    void* out;        // [tq][heads][dim]
+    float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
+    // forward only
+    int pack;         // query heads of one key head that share a tile's rows (1 or the group)
+    int splits;       // parts that a window's keys are cut into
+    float* part_o;    // [splits][tq][heads][dim], splits > 1 only
+    float* part_ml;   // [splits][tq][heads][2]
+    // backward only
+    const void* dout;  // [tq][heads][dim]
+    int64_t do_st, do_sh;
+    const float* delta;  // [heads][tq], sum_j p_ij dp_ij
+    void *dq, *dk, *dv;  // contiguous [tq][heads][dim], [tk][kv_heads][dim]
+    unsigned long long* bias_acc;  // [buckets][heads], fixed point
+    uint32_t* bias_bad;            // [buckets][heads], nonzero where a term was not finite
+    const uint32_t* bias_max;      // [2]: largest finite |dout|, |v| (bits of non-negative floats)
+};
+
+__host__ __device__ __forceinline__ int bias_entries(const AttnBias& b) {
+    return b.table == nullptr ? 0 : (2 * b.ry + 1) * (2 * b.rx + 1);
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of packed windows without a host read of the offsets.  Window w of the
+// W + 2 below (the rows before the first offset and behind the last one are
+// windows without partners, so that their outputs are written too) owns the
+// slots from floor(off[w] / rows) + w on: that is at least ceil(len / rows) of
+// them, the total floor(t / rows) + W + 2 is known on the host, and a slot's
+// window is found with a 32-way search (three probes for 32k windows).  Slots
+// that come out empty return at once.
+__host__ __device__ __forceinline__ int attn_slots(int64_t t, int windows, int rows) {
+    return static_cast<int>(t / rows) + windows + 2;
+}
+
+__device__ __forceinline__ int attn_offset(const int32_t* off, int windows, int t, int w) {
+    if (w <= 0) return 0;
+    if (w >= windows + 2) return t;
+    return min(max(__ldg(off + w - 1), 0), t);
+}
+
+struct AttnTile {
+    int window;      // in [0, windows), or -1: rows outside every window
+    int begin, len;  // the window's tokens on the walked side
+    int first;       // first row of the tile, counted in rows of the window
+    int obegin, olen;  // the window's tokens on the other side
+};
+
+// Called by whole warps. `per`: rows for each token (packed heads). False: nothing to do.
+__device__ __forceinline__ bool attn_tile(const int32_t* off, int t, const int32_t* other, int ot, int windows, int per,
+                                          int rows, int slot, AttnTile& tile) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = windows + 2;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5;
+        const int w = lo + lane * step;
+        bool before = false;
+        if (w < hi) before = static_cast<int>(static_cast<int64_t>(attn_offset(off, windows, t, w)) * per / rows) + w <= slot;
+        const unsigned hit = __ballot_sync(0xffffffffu, before) | 1u;
+        const int n = __ffs(~hit) == 0 ? 32 : __ffs(~hit) - 1;  // leading probes at or before the slot
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    tile.begin = attn_offset(off, windows, t, lo);
+    tile.len = max(attn_offset(off, windows, t, lo + 1) - tile.begin, 0);
+    const int64_t first =
+        static_cast<int64_t>(slot - (static_cast<int>(static_cast<int64_t>(tile.begin) * per / rows) + lo)) * rows;
+    if (first < 0 || first >= static_cast<int64_t>(tile.len) * per) return false;
+    tile.first = static_cast<int>(first);
+    tile.window = lo >= 1 && lo <= windows ? lo - 1 : -1;
+    tile.obegin = tile.olen = 0;
+    if (tile.window >= 0) {
+        tile.obegin = attn_offset(other, windows, ot, lo);
+        tile.olen = max(attn_offset(other, windows, ot, lo + 1) - tile.obegin, 0);
+    }
+    return true;
+}
+
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float to_f(T x) {
+    return static_cast<float>(x);
+}
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) {
+    return x;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) {
+    return __float2half_rn(x);
+}
+
+__device__ __forceinline__ float load_typed(const void* p, int type, int64_t i) {
+    if (type == kF32) return static_cast<const float*>(p)[i];
+    if (type == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_typed(void* p, int type, int64_t i, float x) {
+    if (type == kF32)
+        static_cast<float*>(p)[i] = x;
+    else if (type == kBF16)
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else
+        static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- bias ------------------------------------------------------------------
+// A head's expanded bias, times log2(e): entry (dy + ry) (2 rx + 1) + dx + rx.
+__device__ __forceinline__ float bias_entry(const AttnBias& b, int heads, int head, int e) {
+    const int bucket = __ldg(b.map + e);
+    if (bucket < 0 || bucket >= b.buckets) return 0.0f;
+    return load_typed(b.table, b.table_type, static_cast<int64_t>(bucket) * heads + head) * kLog2e;
+}
+__device__ __forceinline__ int2 bias_pos(const int32_t* pos, int axes, int64_t token) {
+    int2 p = axes == 2 ? make_int2(__ldg(pos + token * 2), __ldg(pos + token * 2 + 1)) : make_int2(0, __ldg(pos + token));
+    p.x = min(max(p.x, -kMaxPosition), kMaxPosition);
+    p.y = min(max(p.y, -kMaxPosition), kMaxPosition);
+    return p;  // .x the first axis (y), .y the second (x)
+}
+__device__ __forceinline__ int bias_index(const AttnBias& b, int2 qp, int2 kp) {
+    const int dy = min(max(kp.x - qp.x, -b.ry), b.ry) + b.ry;
+    const int dx = min(max(kp.y - qp.y, -b.rx), b.rx) + b.rx;
+    return dy * (2 * b.rx + 1) + dx;
+}
+
+// Gradient of the bias: sums of ds in 64-bit fixed point, which come out the same in any
+// order.  |ds| summed over a row is at most 2 |dout| |v| dim, so with the exponent below the
+// sum over all rows stays under 2^61.
+__device__ __forceinline__ float bias_fixed_scale(const uint32_t* bias_max, int dim, int tq) {
+    const double bound =
+        2.0 * static_cast<double>(__uint_as_float(bias_max[0])) * static_cast<double>(__uint_as_float(bias_max[1])) * dim;
+    int e = 126;
+    // a finite fp32 ds is below 2^128 whatever the bound says
+    if (bound > 0.0) e = 60 - (32 - __clz(tq)) - min(ilogb(bound), 128);
+    return exp2f(static_cast<float>(min(max(e, -126), 126)));
+}
+
+// 64-bit add into two shared 32-bit words (native integer atomics; the carry goes by hand).
+__device__ __forceinline__ void bias_add_shared(uint32_t* lo, uint32_t* hi, int e, long long v) {
+    const uint32_t vl = static_cast<uint32_t>(v);
+    uint32_t vh = static_cast<uint32_t>(static_cast<unsigned long long>(v) >> 32);
+    const uint32_t old = atomicAdd(lo + e, vl);
+    vh += (old + vl < old) ? 1u : 0u;
+    if (vh != 0u) atomicAdd(hi + e, vh);
+}
+
+// A block's sum of one entry joins the global sum of its bucket.
+__device__ __forceinline__ void bias_flush(const AttnParams& p, int head, int e, uint32_t lo, uint32_t hi) {
+    if ((lo | hi) == 0u) return;
+    const int bucket = __ldg(p.bias.map + e);
+    if (bucket >= 0 && bucket < p.bias.buckets)
+        atomicAdd(p.bias_acc + static_cast<int64_t>(bucket) * p.heads + head, (static_cast<unsigned long long>(hi) << 32) | lo);
+}
+__device__ __forceinline__ void bias_mark_bad(const AttnParams& p, int head, int e) {
+    const int bucket = __ldg(p.bias.map + e);
+    if (bucket >= 0 && bucket < p.bias.buckets) p.bias_bad[static_cast<int64_t>(bucket) * p.heads + head] = 1u;
+}
+
+__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+
+// ---- launchers (attention_simt.cu) -------------------------------------------
+// type: AttnType of q, k, v and out.
+cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
+// dtable (null: no gradient of the table), delta: p.delta, written here.
+cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, float* delta, int sms, cudaStream_t s);
+
+}  // namespace oss

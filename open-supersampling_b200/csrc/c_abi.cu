@@ -7,6 +7,8 @@
 #include <mutex>
 #include <string>
 
+#include "attention.cuh"
+#include "gated_norm.cuh"
 #include "internal.h"
 #include "oss_common.cuh"
 
@@ -1248,6 +1250,252 @@ int oss_tile_bin_counting_sort(int64_t n, int64_t num_tiles, const int32_t* tile
     OSS_CUDA_TRY(oss::scan_exclusive_i32(tile_count, tile_offsets, tiles, false, nullptr, scan_scratch, s));
     OSS_CUDA_TRY(oss::launch_set_i32(tile_offsets + tiles, static_cast<int32_t>(n), s));
     OSS_CUDA_TRY(oss::radix_sort_pairs(keys, vals, n, static_cast<uint32_t>(tiles), sorted_gid, radix_scratch, s));
+    return OSS_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Window attention and the gated residual norm.
+namespace {
+
+constexpr int kSms = 148;  // sizes of scratch follow the B200's SM count on every host
+
+int check_attention_sizes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
+                          int64_t dim) {
+    OSS_CHECK(dtype >= 0 && dtype <= 2, OSS_ERR_INVALID, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    OSS_CHECK(tq >= 0 && tk >= 0 && windows >= 0, OSS_ERR_INVALID, "token and window counts must be non-negative");
+    OSS_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, OSS_ERR_INVALID,
+              "heads must be a positive multiple of kv_heads");
+    OSS_CHECK(dim >= 1 && dim <= oss::kMaxHeadDim, OSS_ERR_INVALID, "head dim must be in [1, 128]");
+    OSS_CHECK(heads <= 65535, OSS_ERR_RANGE, "more than 65535 heads");
+    OSS_CHECK(tq <= INT_MAX / 2 && tk <= INT_MAX / 2 && windows <= INT_MAX / 4, OSS_ERR_RANGE,
+              "token or window count exceeds 2^30");
+    return OSS_OK;
+}
+
+int check_attention_bias(const oss::AttnBias& b, int64_t buckets, int64_t ry, int64_t rx, int64_t tq, int64_t tk,
+                         int64_t heads) {
+    if (b.table == nullptr) return OSS_OK;
+    OSS_CHECK(b.table_type >= 0 && b.table_type <= 2, OSS_ERR_INVALID,
+              "table dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    OSS_CHECK(buckets > 0 && buckets * heads <= INT_MAX, OSS_ERR_INVALID, "the bias table needs rows, at most 2^31 values");
+    OSS_CHECK(b.axes == 1 || b.axes == 2, OSS_ERR_INVALID, "positions have one or two axes");
+    OSS_CHECK(ry >= 0 && rx >= 0 && ry <= oss::kMaxBiasEntries && rx <= oss::kMaxBiasEntries &&
+                  (2 * ry + 1) * (2 * rx + 1) <= oss::kMaxBiasEntries,
+              OSS_ERR_RANGE, "the bucket map has more than 4096 entries");
+    OSS_CHECK(b.map != nullptr && (tq == 0 || b.q_pos != nullptr) && (tk == 0 || b.k_pos != nullptr), OSS_ERR_INVALID,
+              "a bias table needs a bucket map and the positions of queries and keys");
+    return OSS_OK;
+}
+
+// Heads of one key head share a tile's rows where windows hold few queries (on average at most
+// 16): each key is then read once for the group. Their expanded biases have to fit as one does.
+int attention_pack(int64_t tq, int64_t windows, int64_t heads, int64_t kv_heads, int64_t entries) {
+    const int64_t group = heads / kv_heads;
+    return group > 1 && tq <= 16 * windows && entries * group <= oss::kMaxBiasEntries ? static_cast<int>(group) : 1;
+}
+
+// Parts that the keys of each window are cut into, so that few rows still fill the card: three
+// tiles in flight on each SM, at least 256 keys in a part on average.
+int attention_splits(int64_t tq, int64_t tk, int64_t windows, int64_t heads, int pack) {
+    if (tq == 0 || windows == 0) return 1;
+    const int64_t rows = tq * pack;
+    const int64_t busy = ((rows + 63) / 64 > (windows < tq ? windows : tq) ? (rows + 63) / 64 : (windows < tq ? windows : tq)) *
+                         (heads / pack);
+    const int64_t want = 3 * kSms / busy, most = tk / windows / 256;
+    const int64_t n = want < most ? want : most;
+    return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+
+int64_t attention_split_bytes(int64_t tq, int64_t heads, int64_t dim, int splits) {
+    if (splits == 1) return 0;
+    return oss::arena_bytes(splits * tq * heads * dim, 4) + oss::arena_bytes(splits * tq * heads * 2, 4);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t oss_window_attention_scratch_bytes(int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
+                                           int64_t dim, int64_t entries) {
+    if (heads <= 0 || kv_heads <= 0) return 0;
+    const int pack = attention_pack(tq, windows, heads, kv_heads, entries);
+    return attention_split_bytes(tq, heads, dim, attention_splits(tq, tk, windows, heads, pack));
+}
+
+int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
+                                 int64_t dim, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                 int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* q_offsets,
+                                 const int32_t* k_offsets, float scale, int32_t causal, const void* table,
+                                 int32_t table_dtype, int64_t buckets, const int32_t* bucket_map, int64_t ry, int64_t rx,
+                                 const int32_t* q_pos, const int32_t* k_pos, int32_t axes, void* out, float* lse,
+                                 void* scratch, int64_t scratch_bytes, void* stream) {
+    const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
+    if (rc != OSS_OK) return rc;
+    OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
+    oss::AttnParams p{};
+    p.bias = {table, table_dtype, static_cast<int>(buckets), bucket_map, static_cast<int>(ry), static_cast<int>(rx),
+              q_pos, k_pos, axes};
+    const int rb = check_attention_bias(p.bias, buckets, ry, rx, tq, tk, heads);
+    if (rb != OSS_OK) return rb;
+    if (tq == 0) return OSS_OK;
+    OSS_CHECK(q != nullptr && out != nullptr && (tk == 0 || (k != nullptr && v != nullptr)), OSS_ERR_INVALID,
+              "q, k, v and out must be non-null");
+    OSS_CHECK(q_offsets != nullptr && k_offsets != nullptr, OSS_ERR_INVALID, "offsets must be non-null");
+    const int entries = oss::bias_entries(p.bias);
+    p.q = q, p.k = k, p.v = v;
+    p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
+    p.q_off = q_offsets, p.k_off = k_offsets;
+    p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
+    p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
+    p.scale = scale, p.causal = causal != 0;
+    p.out = out, p.lse = lse;
+    p.pack = attention_pack(tq, windows, heads, kv_heads, entries);
+    OSS_CHECK(tq * p.pack <= INT_MAX, OSS_ERR_RANGE, "token count times heads of a group exceeds int32 range");
+    p.splits = attention_splits(tq, tk, windows, heads, p.pack);
+    if (p.splits > 1) {
+        OSS_CHECK(scratch != nullptr && scratch_bytes >= attention_split_bytes(tq, heads, dim, p.splits), OSS_ERR_SCRATCH,
+                  "scratch smaller than oss_window_attention_scratch_bytes");
+        oss::Arena arena{static_cast<char*>(scratch), scratch_bytes, 0};
+        p.part_o = arena.take<float>(p.splits * tq * heads * dim);
+        p.part_ml = arena.take<float>(p.splits * tq * heads * 2);
+    }
+    OSS_CUDA_TRY(oss::launch_attn_forward(p, dtype, static_cast<cudaStream_t>(stream)));
+    return OSS_OK;
+}
+
+int64_t oss_window_attention_backward_scratch_bytes(int64_t tq, int64_t heads, int64_t buckets) {
+    if (tq < 0 || heads <= 0 || buckets < 0) return 0;
+    return oss::arena_bytes(tq * heads, 4) + oss::arena_bytes(buckets * heads, 8) + oss::arena_bytes(buckets * heads, 4) +
+           oss::arena_bytes(2, 4);
+}
+
+int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
+                                  int64_t dim, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* q_offsets,
+                                  const int32_t* k_offsets, float scale, int32_t causal, const void* table,
+                                  int32_t table_dtype, int64_t buckets, const int32_t* bucket_map, int64_t ry, int64_t rx,
+                                  const int32_t* q_pos, const int32_t* k_pos, int32_t axes, const void* out,
+                                  const float* lse, const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
+                                  void* d_v, void* d_table, void* scratch, int64_t scratch_bytes, void* stream) {
+    const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
+    if (rc != OSS_OK) return rc;
+    OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
+    oss::AttnParams p{};
+    p.bias = {table, table_dtype, static_cast<int>(buckets), bucket_map, static_cast<int>(ry), static_cast<int>(rx),
+              q_pos, k_pos, axes};
+    const int rb = check_attention_bias(p.bias, buckets, ry, rx, tq, tk, heads);
+    if (rb != OSS_OK) return rb;
+    OSS_CHECK(d_table == nullptr || table != nullptr, OSS_ERR_INVALID, "d_table needs a bias table");
+    if (tq == 0 && tk == 0 && d_table == nullptr) return OSS_OK;
+    OSS_CHECK(tq == 0 || (q != nullptr && out != nullptr && lse != nullptr && d_out != nullptr && d_q != nullptr),
+              OSS_ERR_INVALID, "q, out, lse, d_out and d_q must be non-null");
+    OSS_CHECK(tk == 0 || (k != nullptr && v != nullptr && d_k != nullptr && d_v != nullptr), OSS_ERR_INVALID,
+              "k, v, d_k and d_v must be non-null");
+    OSS_CHECK(q_offsets != nullptr && k_offsets != nullptr, OSS_ERR_INVALID, "offsets must be non-null");
+    const int64_t sums = d_table == nullptr ? 0 : buckets;
+    OSS_CHECK(scratch != nullptr && scratch_bytes >= oss_window_attention_backward_scratch_bytes(tq, heads, sums),
+              OSS_ERR_SCRATCH, "scratch smaller than oss_window_attention_backward_scratch_bytes");
+    p.q = q, p.k = k, p.v = v;
+    p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
+    p.q_off = q_offsets, p.k_off = k_offsets;
+    p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
+    p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
+    p.scale = scale, p.causal = causal != 0, p.pack = 1, p.splits = 1;
+    p.out = const_cast<void*>(out), p.lse = const_cast<float*>(lse);
+    p.dout = d_out, p.do_st = do_st, p.do_sh = do_sh, p.dq = d_q, p.dk = d_k, p.dv = d_v;
+    oss::Arena arena{static_cast<char*>(scratch), scratch_bytes, 0};
+    float* delta = arena.take<float>(tq * heads);
+    p.delta = delta;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d_table != nullptr) {
+        char* sums_at = arena.base + arena.used;
+        p.bias_acc = arena.take<unsigned long long>(buckets * heads);
+        p.bias_bad = arena.take<uint32_t>(buckets * heads);
+        p.bias_max = arena.take<uint32_t>(2);
+        OSS_CUDA_TRY(cudaMemsetAsync(sums_at, 0, arena.base + arena.used - sums_at, s));
+    }
+    OSS_CUDA_TRY(oss::launch_attn_backward(p, dtype, d_table, delta, kSms, s));
+    return OSS_OK;
+}
+
+namespace {
+
+int check_gated_norm(const oss::GatedNorm& p, int32_t dtype, int64_t channels) {
+    OSS_CHECK(dtype >= 0 && dtype <= 2, OSS_ERR_INVALID, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    OSS_CHECK(p.param_type >= 0 && p.param_type <= 2, OSS_ERR_INVALID,
+              "parameter dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    OSS_CHECK(p.rows >= 0, OSS_ERR_INVALID, "rows must be non-negative");
+    OSS_CHECK(channels >= 1 && channels <= 8192, OSS_ERR_INVALID, "channels must be in [1, 8192]");
+    OSS_CHECK(p.gate_kind >= 0 && p.gate_kind <= 2, OSS_ERR_INVALID, "gate kind must be 0 (none), 1 (row) or 2 (full)");
+    OSS_CHECK(p.act >= 0 && p.act <= 2, OSS_ERR_INVALID, "gate activation must be 0 (none), 1 (sigmoid) or 2 (silu)");
+    OSS_CHECK(p.eps >= 0.0f, OSS_ERR_INVALID, "eps must be non-negative");
+    OSS_CHECK(p.rows == 0 || (p.x != nullptr && p.h != nullptr && (p.gate_kind == 0 || p.gate != nullptr)),
+              OSS_ERR_INVALID, "x, h and the gate must be non-null");
+    OSS_CHECK(p.weight != nullptr, OSS_ERR_INVALID, "weight must be non-null");
+    return OSS_OK;
+}
+
+}  // namespace
+
+int oss_gated_norm_forward(int32_t dtype, int64_t rows, int64_t channels, const void* x, int64_t x_st, const void* h,
+                           int64_t h_st, const void* gate, int64_t gate_st, int32_t gate_kind, int32_t act, int32_t layer,
+                           float eps, int32_t param_dtype, const void* weight, const void* bias, const void* scale,
+                           const void* next_weight, const void* next_bias, void* y, void* z, float* stats, void* stream) {
+    oss::GatedNorm p{};
+    p.rows = rows, p.c = static_cast<int>(channels), p.inv_c = 1.0f / static_cast<float>(channels), p.eps = eps;
+    p.layer = layer != 0, p.gate_kind = gate_kind, p.act = act, p.param_type = param_dtype;
+    p.x = x, p.h = h, p.gate = gate, p.x_st = x_st, p.h_st = h_st, p.g_st = gate_st;
+    p.weight = weight, p.bias = bias, p.scale = scale, p.next_weight = next_weight, p.next_bias = next_bias;
+    p.y = y, p.z = z, p.stats = reinterpret_cast<float4*>(stats);
+    const int rc = check_gated_norm(p, dtype, channels);
+    if (rc != OSS_OK) return rc;
+    if (rows == 0) return OSS_OK;
+    OSS_CHECK(y != nullptr && (z == nullptr || next_weight != nullptr), OSS_ERR_INVALID,
+              "y must be non-null, and z needs next_weight");
+    OSS_CHECK(aligned(stats, 16), OSS_ERR_INVALID, "stats must be 16-byte aligned");
+    OSS_CUDA_TRY(oss::launch_gated_norm_forward(p, dtype, static_cast<cudaStream_t>(stream)));
+    return OSS_OK;
+}
+
+int64_t oss_gated_norm_backward_scratch_bytes(int64_t rows, int64_t channels) {
+    if (rows <= 0 || channels < 1 || channels > 8192) return 0;
+    return 4 * oss::gated_norm_partial_floats(rows, static_cast<int>(channels));
+}
+
+int oss_gated_norm_backward(int32_t dtype, int64_t rows, int64_t channels, const void* x, int64_t x_st, const void* h,
+                            int64_t h_st, const void* gate, int64_t gate_st, int32_t gate_kind, int32_t act,
+                            int32_t layer, float eps, int32_t param_dtype, const void* weight, const void* bias,
+                            const void* scale, const void* next_weight, const void* next_bias, const float* stats,
+                            const void* d_y, int64_t dy_st, const void* d_z, int64_t dz_st, void* d_x, void* d_h,
+                            void* d_gate, void* d_weight, void* d_bias, void* d_scale, void* d_next_weight,
+                            void* d_next_bias, void* scratch, int64_t scratch_bytes, void* stream) {
+    oss::GatedNorm p{};
+    p.rows = rows, p.c = static_cast<int>(channels), p.inv_c = 1.0f / static_cast<float>(channels), p.eps = eps;
+    p.layer = layer != 0, p.gate_kind = gate_kind, p.act = act, p.param_type = param_dtype;
+    p.x = x, p.h = h, p.gate = gate, p.x_st = x_st, p.h_st = h_st, p.g_st = gate_st;
+    p.weight = weight, p.bias = bias, p.scale = scale, p.next_weight = next_weight, p.next_bias = next_bias;
+    p.stats = const_cast<float4*>(reinterpret_cast<const float4*>(stats));
+    p.dy = d_y, p.dz = d_z, p.dy_st = dy_st, p.dz_st = dz_st, p.dx = d_x, p.dh = d_h, p.dgate = d_gate;
+    p.dparam[0] = d_weight, p.dparam[1] = d_scale, p.dparam[2] = d_next_weight, p.dparam[3] = d_bias;
+    p.dparam[4] = d_next_bias;
+    const int rc = check_gated_norm(p, dtype, channels);
+    if (rc != OSS_OK) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        for (void* d : p.dparam)
+            if (d != nullptr) OSS_CUDA_TRY(cudaMemsetAsync(d, 0, channels * (param_dtype == 0 ? 4 : 2), s));
+        return OSS_OK;
+    }
+    OSS_CHECK(stats != nullptr && aligned(stats, 16), OSS_ERR_INVALID, "stats must be non-null and 16-byte aligned");
+    OSS_CHECK(d_z == nullptr || next_weight != nullptr, OSS_ERR_INVALID, "d_z needs next_weight");
+    OSS_CHECK(layer || (d_bias == nullptr && d_next_bias == nullptr), OSS_ERR_INVALID,
+              "only layer norms have gradients of biases");
+    OSS_CHECK(scratch != nullptr && scratch_bytes >= oss_gated_norm_backward_scratch_bytes(rows, channels),
+              OSS_ERR_SCRATCH, "scratch smaller than oss_gated_norm_backward_scratch_bytes");
+    p.partial = static_cast<float*>(scratch);
+    OSS_CUDA_TRY(oss::launch_gated_norm_backward(p, dtype, s));
     return OSS_OK;
 }
 

@@ -2,7 +2,8 @@
 (reference oss/cuda/oss_cuda/__init__.py:1-10)."""
 
 from ._raster import pair_capacity_overflowed
-from .attention import fused_window_cross_attention
+from .attention import fused_window_cross_attention, log_position_buckets, window_position_buckets
+from .norm import gated_residual_norm
 from .rasterizer import rasterize_gaussians, rasterize_gaussians_batched
 from .tile_bin import tile_bin_counting_sort
 
@@ -20,6 +21,9 @@ __all__ = [
     "rasterize_gaussians_batched",
     "warp_canvas_cuda",
     "fused_window_cross_attention",
+    "window_position_buckets",
+    "log_position_buckets",
+    "gated_residual_norm",
     "tile_bin_counting_sort",
     "pair_capacity_overflowed",
 ]
