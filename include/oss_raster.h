@@ -669,6 +669,10 @@ OSS_API int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, 
                                          const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
                                          const int32_t* k_pos, int32_t axes, void* out, float* lse, void* scratch,
                                          int64_t scratch_bytes, void* stream);
+/* Waits inside the tensor-core kernels are bounded; one that runs out (which would be a fault of the
+ * library) leaves NaN in its rows and is counted.  count: blocks that this happened to on the current
+ * device since the library was loaded.  Synchronises. */
+OSS_API int oss_window_attention_timeouts(uint32_t* count);
 /* buckets: rows of the table whose gradient is wanted, else 0. */
 OSS_API int64_t oss_window_attention_backward_scratch_bytes(int64_t tq, int64_t heads, int64_t buckets);
 /* d_table[buckets][heads] in the table's dtype, null: not wanted.  Every gradient is the same

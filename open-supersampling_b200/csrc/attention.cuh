@@ -219,6 +219,10 @@ __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) 
 // ---- launchers (attention_simt.cu) -------------------------------------------
 // type: AttnType of q, k, v and out.
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
+// attention_mma.cu: bf16 and fp16, without the join of split keys.
+cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s);
+// Waits of the tensor-core kernels that ran out of their limit since the library was loaded.
+cudaError_t attn_timeouts(unsigned int* count);
 // dtable (null: no gradient of the table), delta: p.delta, written here.
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, float* delta, int sms, cudaStream_t s);
 

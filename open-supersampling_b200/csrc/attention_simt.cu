@@ -550,10 +550,12 @@ cudaError_t fwd_rows(const AttnParams& p, cudaStream_t s) {
     return static_cast<int64_t>(p.tq) * p.pack <= 16ll * p.windows ? fwd_one<T, DP, 1>(p, s) : fwd_one<T, DP, 4>(p, s);
 }
 
+cudaError_t fwd_f32(const AttnParams& p, cudaStream_t s) {
+    return p.dim <= 32 ? fwd_rows<float, 32>(p, s) : p.dim <= 64 ? fwd_rows<float, 64>(p, s) : fwd_rows<float, 128>(p, s);
+}
+
 template <typename T>
-cudaError_t fwd_type(const AttnParams& p, cudaStream_t s) {
-    cudaError_t err = p.dim <= 32 ? fwd_rows<T, 32>(p, s) : p.dim <= 64 ? fwd_rows<T, 64>(p, s) : fwd_rows<T, 128>(p, s);
-    if (err != cudaSuccess || p.splits == 1) return err;
+cudaError_t join_parts(const AttnParams& p, cudaStream_t s) {
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads;
     k_attn_join<T><<<static_cast<unsigned>((rows + 7) / 8), kThreads, 0, s>>>(p);
     return cudaGetLastError();
@@ -596,8 +598,9 @@ cudaError_t bwd_type(const AttnParams& p, cudaStream_t s, float* delta, uint32_t
 }  // namespace
 
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s) {
-    if (type == kF32) return fwd_type<float>(p, s);
-    return type == kBF16 ? fwd_type<__nv_bfloat16>(p, s) : fwd_type<__half>(p, s);
+    const cudaError_t err = type == kF32 ? fwd_f32(p, s) : launch_attn_forward_mma(p, type, s);
+    if (err != cudaSuccess || p.splits == 1) return err;
+    return type == kF32 ? join_parts<float>(p, s) : type == kBF16 ? join_parts<__nv_bfloat16>(p, s) : join_parts<__half>(p, s);
 }
 
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, float* delta, int sms, cudaStream_t s) {

@@ -1365,6 +1365,14 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     return OSS_OK;
 }
 
+int oss_window_attention_timeouts(uint32_t* count) {
+    OSS_CHECK(count != nullptr, OSS_ERR_INVALID, "count must be non-null");
+    unsigned int n = 0;
+    OSS_CUDA_TRY(oss::attn_timeouts(&n));
+    *count = n;
+    return OSS_OK;
+}
+
 int64_t oss_window_attention_backward_scratch_bytes(int64_t tq, int64_t heads, int64_t buckets) {
     if (tq < 0 || heads <= 0 || buckets < 0) return 0;
     return oss::arena_bytes(tq * heads, 4) + oss::arena_bytes(buckets * heads, 8) + oss::arena_bytes(buckets * heads, 4) +
