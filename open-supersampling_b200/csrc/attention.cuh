@@ -55,11 +55,19 @@ struct AttnParams {
     // backward only
     const void* dout;  // [tq][heads][dim]
     int64_t do_st, do_sh;
-    const float* delta;  // [heads][tq], sum_j p_ij dp_ij
+    float* delta;        // [heads][tq], sum_j p_ij dp_ij
     void *dq, *dk, *dv;  // contiguous [tq][heads][dim], [tk][kv_heads][dim]
     unsigned long long* bias_acc;  // [buckets][heads], fixed point
     uint32_t* bias_bad;            // [buckets][heads], nonzero where a term was not finite
     const uint32_t* bias_max;      // [2]: largest finite |dout|, |v| (bits of non-negative floats)
+    // backward of 16-bit types only
+    int short_max;      // windows of up to so many keys go to the kernel for short windows
+    int qsplits;        // parts that the queries of a tile of keys are cut into
+    int short_blocks, dq_blocks, dkv_blocks;  // blocks for each (key) head of the three kernels
+    int* flags;         // [0]: nonzero where some window has more than short_max keys
+    float *part_dk, *part_dv;    // [qsplits][tk][kv_heads][dim], qsplits > 1 only
+    double* bias_part;           // [heads][bias_short + bias_long][entries]; null: no gradient of the table
+    int bias_short, bias_long;   // blocks of a head that sum the bias gradient, of short windows and of others
 };
 
 __host__ __device__ __forceinline__ int bias_entries(const AttnBias& b) {
@@ -216,14 +224,18 @@ __device__ __forceinline__ void bias_mark_bad(const AttnParams& p, int head, int
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 
-// ---- launchers (attention_simt.cu) -------------------------------------------
+// ---- launchers -----------------------------------------------------------------
 // type: AttnType of q, k, v and out.
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
-// attention_mma.cu: bf16 and fp16, without the join of split keys.
+// dtable (null: no gradient of the table).
+cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
+// attention_simt.cu: delta (p.flags null or set) and p.bias_max (where not null).
+cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s);
+// attention_mma.cu, attention_mma_bwd.cu: bf16 and fp16, the forward without the join of split keys.
 cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s);
+cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
 // Waits of the tensor-core kernels that ran out of their limit since the library was loaded.
 cudaError_t attn_timeouts(unsigned int* count);
-// dtable (null: no gradient of the table), delta: p.delta, written here.
-cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, float* delta, int sms, cudaStream_t s);
+cudaError_t attn_timeouts_bwd(unsigned int* count);
 
 }  // namespace oss

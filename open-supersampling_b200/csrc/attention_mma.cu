@@ -14,178 +14,11 @@
 // With head dims up to 64 the exponentials (16 a clock and SM) bound long windows: 64-key tiles
 // leave room for four blocks (128 of 512 tensor-memory columns each). With 128 the products do,
 // and 128-key tiles feed them from shared memory at the full rate.
-#include <type_traits>
-
-#include "attention.cuh"
+#include "attention_mma.cuh"
 #include "internal.h"
-#include "tcgen05.cuh"
 
 namespace oss {
 namespace {
-
-constexpr int kRows = 128;  // queries of a tile, threads of a block
-
-__device__ unsigned int g_attn_timeouts;  // waits that ran out of their limit, since the library was loaded
-
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-
-// One operand of the tile loads.
-template <typename T>
-struct Operand {
-    const T* p;
-    int64_t st, sh;
-    bool vec;  // every row starts on 16 bytes and ends on them
-    __device__ Operand(const void* q, int64_t st_, int64_t sh_, int dim) : p(static_cast<const T*>(q)), st(st_), sh(sh_) {
-        vec = ((reinterpret_cast<uintptr_t>(q) & 15) | ((st_ | sh_ | dim) & 7)) == 0;
-    }
-};
-
-// rows_pad rows of panels at dst: row r is token (first + r) / pack of the window, zeros from
-// `rows` on and from dim to the next 16 columns.
-template <typename T>
-__device__ __forceinline__ void load_panel(uint32_t dst, int panel_rows, const Operand<T>& o, int64_t token0, int head0,
-                                           int pack, int first, int rows, int rows_pad, int dim) {
-    const int chunks = ((dim + 15) / 16) * 2;
-    const uint32_t inv = (65536u + chunks - 1) / chunks;  // i / chunks for i < 2048
-    for (int i = threadIdx.x; i < rows_pad * chunks; i += kRows) {
-        const int r = static_cast<int>((static_cast<uint32_t>(i) * inv) >> 16), c = i - r * chunks;
-        int64_t token = token0;
-        int head = head0;
-        if (pack == 1) {
-            token += first + r;
-        } else {
-            token += (first + r) / pack;
-            head += (first + r) % pack;
-        }
-        const uint32_t to = dst + (c >> 3) * panel_rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        const bool live = r < rows && c * 8 < dim;
-        const T* from = o.p + (live ? token * o.st + head * o.sh + c * 8 : 0);
-        if (o.vec) {
-            tc::cp_async16(to, from, live);
-        } else {
-            uint32_t w[4] = {0, 0, 0, 0};
-            if (live) {
-                const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(s[e]) << (16 * (e & 1));
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        }
-    }
-}
-
-// ---- bias of a tile ----------------------------------------------------------------
-// How the entries of a tile of queries x keys are found. Most tiles need no clamping: windows
-// never leave the map, and far tokens all clamp to one entry.
-enum BiasMode { kLinear, kLinearX, kClamp, kOne };
-
-struct Range {  // of positions
-    int y0, y1, x0, x1;
-};
-__device__ __forceinline__ BiasMode bias_mode(const AttnBias& b, const Range& q, const Range& k) {
-    const int ylo = k.y0 - q.y1, yhi = k.y1 - q.y0, xlo = k.x0 - q.x1, xhi = k.x1 - q.x0;
-    const bool yin = ylo >= -b.ry && yhi <= b.ry, xin = xlo >= -b.rx && xhi <= b.rx;
-    const bool yone = ylo >= b.ry || yhi <= -b.ry, xone = xlo >= b.rx || xhi <= -b.rx;
-    if (yone && xone) return kOne;
-    if (yone && xin) return kLinearX;
-    return yin && xin ? kLinear : kClamp;
-}
-__device__ __forceinline__ Range warp_range(int2 p) {
-    return {__reduce_min_sync(0xffffffffu, p.x), __reduce_max_sync(0xffffffffu, p.x), __reduce_min_sync(0xffffffffu, p.y),
-            __reduce_max_sync(0xffffffffu, p.y)};
-}
-__device__ __forceinline__ Range join(const Range& a, const Range& b) {
-    return {min(a.y0, b.y0), max(a.y1, b.y1), min(a.x0, b.x0), max(a.x1, b.x1)};
-}
-
-template <int KT>
-struct KeyPos {  // of a tile, in shared memory
-    int y[KT], x[KT], code[KT];  // code: y (2 rx + 1) + x
-    Range range[KT / 32];
-};
-
-// Fills it; threads 0 .. KT - 1. n > 0 live keys.
-template <int KT>
-__device__ __forceinline__ void load_key_pos(KeyPos<KT>* s, const AttnBias& b, int64_t token, int n) {
-    const int j = threadIdx.x;
-    if (j >= KT) return;
-    const int2 p = bias_pos(b.k_pos, b.axes, token + min(j, n - 1));
-    s->y[j] = p.x;
-    s->x[j] = p.y;
-    s->code[j] = p.x * (2 * b.rx + 1) + p.y;
-    const Range r = warp_range(p);
-    if ((j & 31) == 0) s->range[j >> 5] = r;
-}
-template <int KT>
-__device__ __forceinline__ Range key_range(const KeyPos<KT>* s) {
-    Range r = s->range[0];
-#pragma unroll
-    for (int w = 1; w < KT / 32; ++w) r = join(r, s->range[w]);
-    return r;
-}
-
-// x[c] = x[c] c2 + bias of keys j0 + c, for a row at qp.
-template <int KT, int N>
-__device__ __forceinline__ void add_bias(float (&x)[N], float c2, const AttnBias& b, BiasMode mode, const float* E,
-                                         const KeyPos<KT>* k, int j0, int2 qp) {
-    const int w = 2 * b.rx + 1;
-    if (mode == kOne) {
-        const float e = E[bias_index(b, qp, make_int2(k->y[j0], k->x[j0]))];
-#pragma unroll
-        for (int c = 0; c < N; ++c) x[c] = fmaf(x[c], c2, e);
-    } else if (mode == kClamp) {
-#pragma unroll
-        for (int c = 0; c < N; ++c) x[c] = fmaf(x[c], c2, E[bias_index(b, qp, make_int2(k->y[j0 + c], k->x[j0 + c]))]);
-    } else {
-        const int* code = mode == kLinear ? k->code + j0 : k->x + j0;
-        const int dy = mode == kLinear ? -qp.x : min(max(k->y[j0] - qp.x, -b.ry), b.ry);
-        const float* at = E + (dy + b.ry) * w + b.rx - qp.y;
-#pragma unroll
-        for (int c = 0; c < N; c += 4) {
-            const int4 q = *reinterpret_cast<const int4*>(code + c);
-            x[c] = fmaf(x[c], c2, at[q.x]);
-            x[c + 1] = fmaf(x[c + 1], c2, at[q.y]);
-            x[c + 2] = fmaf(x[c + 2], c2, at[q.z]);
-            x[c + 3] = fmaf(x[c + 3], c2, at[q.w]);
-        }
-    }
-}
-
-// 16 columns of a row of an output tile, times `by`, into the panels at dst.
-template <typename T>
-__device__ __forceinline__ void stage16(uint32_t dst, const float* o, int c, float by) {
-    const int r = threadIdx.x;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2(o[8 * h + 2 * i] * by, o[8 * h + 2 * i + 1] * by, T{});
-        const int chunk = (c >> 3) + h;
-        const uint32_t to = dst + (chunk >> 3) * kRows * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-    }
-}
-__device__ __forceinline__ void write_part(float* to, const float* o, int c, int dim) {
-    if ((dim & 3) == 0) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            if (c + i < dim) *reinterpret_cast<float4*>(to + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (c + i < dim) to[c + i] = o[i];
-    }
-}
 
 // ---- a row again, where a product met what its mask hides --------------------------------
 // 0 times a NaN or an infinity behind the causal mask is NaN. A row that comes out not finite is
@@ -211,7 +44,7 @@ __device__ __noinline__ void forward_row(const AttnParams& p, int64_t token, int
         if (part != nullptr)
             write_part(part, o + c, c, p.dim);
         else
-            stage16<T>(stage, o + c, c, inv);
+            stage16<T>(stage, threadIdx.x, o + c, c, inv);
     }
 }
 
@@ -424,7 +257,7 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
             if (p.splits > 1) {
                 if (live) write_part(p.part_o + part * p.dim, o, c, p.dim);
             } else {
-                stage16<T>(sq, o, c, alive ? inv : __uint_as_float(0x7fffffffu));
+                stage16<T>(sq, tid, o, c, alive ? inv : __uint_as_float(0x7fffffffu));
             }
         }
         if (p.causal && live && !fine) {
@@ -434,27 +267,9 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
         }
         if (p.splits > 1) continue;
         __syncthreads();
-        const int chunks = (p.dim + 7) / 8;
-        const uint32_t cinv = (65536u + chunks - 1) / chunks;
-        const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.dim % 8 == 0;
-        for (int i = tid; i < rows * chunks; i += kRows) {
-            const int r = static_cast<int>((static_cast<uint32_t>(i) * cinv) >> 16), c = i - r * chunks;
-            const int64_t tok = t.begin + (t.first + r) / p.pack;
-            const int hd = head0 + (p.pack == 1 ? 0 : (t.first + r) % p.pack);
-            const uint32_t src = sq + (c >> 3) * kRows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src));
-            unsigned short* dst = static_cast<unsigned short*>(p.out) + (tok * p.heads + hd) * p.dim + c * 8;
-            if (vec) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c * 8 + e < p.dim) dst[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
-            }
-        }
+        store_panel<T, kRows>(sq, p.out, p.heads, p.dim, t.begin, head0, p.pack, t.first, rows);
     }
-    if (!alive && tid == 0) atomicAdd(&g_attn_timeouts, 1u);
+    if (!alive && tid == 0) count_timeout();
     tc::fence_before();
     __syncthreads();
     if (warp == 0) tc::tmem_free<kCols>(tmem);
@@ -484,7 +299,7 @@ cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t 
 }
 
 cudaError_t attn_timeouts(unsigned int* count) {
-    return cudaMemcpyFromSymbol(count, g_attn_timeouts, sizeof(unsigned int));
+    return cudaMemcpyFromSymbol(count, g_timeouts, sizeof(unsigned int));
 }
 
 }  // namespace oss

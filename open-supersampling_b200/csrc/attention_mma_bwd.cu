@@ -1,0 +1,993 @@
+// Window attention of 16-bit types on the tensor cores (tcgen05): backward.
+//
+// Per tile of 128 queries x keys, with thread = query row (two threads a row where a tile has 128 keys):
+//   S = Q K^T, dP = dO V^T          into tensor memory
+//   P = 2^(S - lse), dS = P (dP - delta)   in registers, written to shared memory as 16-bit values
+//   dV += P^T dO, dK += dS^T Q, dQ += dS K from shared memory: a row-major P is a K-major operand for
+//                                   dQ and an MN-major one for the other two, so nothing is transposed
+//
+// Windows of up to 64 keys (the Gaussians of a tile) take one kernel: a block holds the window's
+// keys and walks its queries, so that q, k, v and dout are read once and every gradient leaves
+// the block finished; delta comes from the row of P and dP itself. Longer windows take two, one
+// that walks keys for dQ and one that walks queries for dK and dV (seven products instead of five,
+// but no sums across blocks: every gradient has a fixed order of additions).
+//
+// fp16 keeps dS times a power of two that puts its bound 2 dim max|dout| max|v| at 2^15, so that
+// gradients of any size stay within the type's range.
+//
+// The bias gradient is summed per tile in shared 32-bit integers (native atomics; the same in any
+// order) at 2^-30 of the tile's sum of |dS|, which no entry exceeds, and then in fp64 by the entry's
+// own thread. Blocks keep their head and their tiles from run to run; their sums are added in order
+// at the end.
+#include "attention_mma.cuh"
+#include "internal.h"
+
+namespace oss {
+namespace {
+
+constexpr int kShortKeys = 64;
+
+template <typename T>
+constexpr int kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+
+// Power of two that dS is kept times.
+template <typename T>
+__device__ __forceinline__ float ds_scale(const AttnParams& p) {
+    if constexpr (kIsBf16<T>) return 1.0f;
+    const float bound = 2.0f * p.dim * __uint_as_float(p.bias_max[0]) * __uint_as_float(p.bias_max[1]);
+    if (!(bound > 0.0f)) return 1.0f;
+    return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
+}
+
+struct BiasSum {      // of a tile, uniform over the block
+    BiasMode mode;
+    float fixed;      // 0: nothing to add
+    bool bad;         // some terms are not finite
+};
+
+// The sum of finite |ds| of a warp's rows, negative where some is not finite.
+template <int N>
+__device__ __forceinline__ float warp_size(const float (&ds)[N]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) m += fabsf(ds[c]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
+    if (is_finite(m)) return m;
+    m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+        if (is_finite(ds[c])) m += fabsf(ds[c]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
+    return -fmaxf(fminf(m, 3.0e38f), 1.0e-38f);
+}
+
+template <int WARPS>
+__device__ __forceinline__ BiasSum bias_sum(BiasMode mode, const float* wsize) {
+    float m = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        m += fabsf(wsize[w]);
+        bad |= wsize[w] < 0.0f;
+    }
+    BiasSum b{mode, 0.0f, bad};
+    if (m > 0.0f) b.fixed = exp2f(static_cast<float>(min(max(29 - ilogbf(fminf(m, 3.0e38f)), -126), 126)));
+    return b;
+}
+
+// Adds a thread's 64 terms of keys j0 .. to the block's integers (wsum: a warp's sum where the tile
+// has one entry).
+template <int KT>
+__device__ __forceinline__ void bias_add(const AttnParams& p, const BiasSum& b, const float (&ds)[64], int n16, int head,
+                                         const KeyPos<KT>* k, int j0, int2 qp, int* I, float* wsum) {
+    if (b.mode == kOne) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+            if (j0 + c < n16) sum += ds[c];
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if ((threadIdx.x & 31) == 0) *wsum = sum;
+        return;
+    }
+    const int w = 2 * p.bias.rx + 1;
+    const int* code = b.mode == kLinear ? k->code + j0 : k->x + j0;
+    const int dy = b.mode == kLinear ? -qp.x : min(max(k->y[0] - qp.x, -p.bias.ry), p.bias.ry);
+    const int off = (dy + p.bias.ry) * w + p.bias.rx - qp.y;
+#pragma unroll
+    for (int c = 0; c < 64; ++c) {
+        if (j0 + c >= n16) break;
+        const float x = ds[c];
+        if (x == 0.0f) continue;
+        const int e = b.mode == kClamp ? bias_index(p.bias, qp, make_int2(k->y[j0 + c], k->x[j0 + c])) : code[c] + off;
+        if (b.bad && !is_finite(x))
+            bias_mark_bad(p, head, e);
+        else
+            atomicAdd(I + e, __float2int_rn(x * b.fixed));
+    }
+}
+
+// After a barrier: the integers join the block's fp64 sums.
+template <int THREADS, int WARPS, int KT>
+__device__ __forceinline__ void bias_join(const AttnParams& p, const BiasSum& b, int entries, int head, const KeyPos<KT>* k,
+                                          int2 qp, int* I, const float* wsum, double* acc) {
+    if (b.mode == kOne) {
+        if (threadIdx.x == 0) {
+            const int e = bias_index(p.bias, qp, make_int2(k->y[0], k->x[0]));
+            double sum = 0.0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum += static_cast<double>(wsum[w]);
+            if (b.bad)
+                bias_mark_bad(p, head, e);
+            else
+                acc[e] += sum;
+        }
+        return;
+    }
+    if (b.fixed == 0.0f) return;
+    const double unit = 1.0 / static_cast<double>(b.fixed);
+    for (int e = threadIdx.x; e < entries; e += THREADS) {
+        const int v = I[e];
+        if (v != 0) {
+            acc[e] += static_cast<double>(v) * unit;
+            I[e] = 0;
+        }
+    }
+}
+
+// A row of 64 values as 16-bit into a panel.
+template <typename T>
+__device__ __forceinline__ void write_row(uint32_t panel, int row, const float (&x)[64], float by) {
+#pragma unroll
+    for (int c = 0; c < 64; c += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack2(x[c + 2 * i] * by, x[c + 2 * i + 1] * by, T{});
+        const uint32_t to = panel + row * 128 + ((((c >> 3)) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+}
+
+// 16 columns of a row of a gradient, straight to memory.
+template <typename T>
+__device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim, float by) {
+    if (dim % 8 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (c + 8 * h >= dim) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack2(o[8 * h + 2 * i] * by, o[8 * h + 2 * i + 1] * by, T{});
+            *reinterpret_cast<uint4*>(to + c + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (c + i < dim) to[c + i] = from_f<T>(o[i] * by);
+    }
+}
+
+// Scores and dP of a thread's 64 keys from tensor memory, and the weights: s becomes p, dp stays.
+// Zero where the mask is, whatever stands there.
+template <int KT>
+__device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], float (&dp)[64], uint32_t ts, uint32_t tdp, int n16,
+                                        int j0, bool whole, int see, float lse, BiasMode mode, const float* E, bool biased,
+                                        const KeyPos<KT>* kp, int2 qp) {
+    const float c2 = p.scale * kLog2e;
+#pragma unroll
+    for (int c = 0; c < 64; c += 16) {
+        if (j0 + c < n16) {
+            tc::tmem_ld16(ts + j0 + c, s + c);
+            tc::tmem_ld16(tdp + j0 + c, dp + c);
+        }
+    }
+    tc::wait_ld();
+#pragma unroll
+    for (int c = 0; c < 64; c += 16) {
+        float(&x)[16] = *reinterpret_cast<float(*)[16]>(s + c);
+        if (j0 + c >= n16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = dp[c + i] = 0.0f;
+            continue;
+        }
+        if (biased) {
+            add_bias<KT, 16>(x, c2, p.bias, mode, E, kp, j0 + c, qp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = ex2(x[i] - lse);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], c2, -lse));
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool on = j0 + c + i < see;
+                x[i] = on ? x[i] : 0.0f;
+                dp[c + i] = on ? dp[c + i] : 0.0f;
+            }
+        }
+    }
+}
+
+// ---- rows again, where a product met what its mask hides ------------------------------------
+template <typename T>
+__device__ __forceinline__ float dot_row(const T* a, const T* b, int dim) {
+    float s = 0.0f;
+    for (int c = 0; c < dim; ++c) s = fmaf(to_f(a[c]), to_f(b[c]), s);
+    return s;
+}
+template <typename T>
+__device__ __forceinline__ float score_of(const AttnParams& p, int64_t q, int64_t k, int head, int kvh) {
+    float s = dot_row(static_cast<const T*>(p.q) + q * p.q_st + head * p.q_sh, static_cast<const T*>(p.k) + k * p.k_st + kvh * p.k_sh,
+                      p.dim) * (p.scale * kLog2e);
+    if (p.bias.table != nullptr)
+        s += bias_entry(p.bias, p.heads, head, bias_index(p.bias, bias_pos(p.bias.q_pos, p.bias.axes, q), bias_pos(p.bias.k_pos, p.bias.axes, k)));
+    return s;
+}
+
+// dq of one row over the keys [k0, k0 + see) that it sees, staged in the panels at `stage`.
+template <typename T>
+__device__ __noinline__ void query_row(const AttnParams& p, int64_t q, int head, int64_t k0, int see, float lse, float delta, float up,
+                                       uint32_t stage) {
+    float o[kMaxHeadDim];
+    const int kvh = head / (p.heads / p.kv_heads);
+    const T* g = static_cast<const T*>(p.dout) + q * p.do_st + head * p.do_sh;
+    for (int c = 0; c < kMaxHeadDim; ++c) o[c] = 0.0f;
+    for (int64_t k = k0; k < k0 + see; ++k) {
+        const float w = ex2(score_of<T>(p, q, k, head, kvh) - lse);
+        const float d = to_f(from_f<T>(w * (dot_row(g, static_cast<const T*>(p.v) + k * p.v_st + kvh * p.v_sh, p.dim) - delta) * up));
+        const T* kk = static_cast<const T*>(p.k) + k * p.k_st + kvh * p.k_sh;
+        for (int c = 0; c < p.dim; ++c) o[c] = fmaf(d, to_f(kk[c]), o[c]);
+    }
+    for (int c = 0; c < ((p.dim + 15) & ~15); c += 16) stage16<T>(stage, threadIdx.x & (kRows - 1), o + c, c, p.scale / up);
+}
+
+// dk (want_v: dv) of key k, the j-th of its window, over the query tiles [i0, i1) of its heads.
+template <typename T>
+__device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int kvh, int64_t q0, int lq, int lk, int i0, int i1, float up,
+                                     bool want_v, T* out, float* part) {
+    float o[kMaxHeadDim];
+    const int group = p.heads / p.kv_heads, qtiles = (lq + kRows - 1) / kRows;
+    for (int c = 0; c < kMaxHeadDim; ++c) o[c] = 0.0f;
+    for (int it = i0; it < i1; ++it) {
+        const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows;
+        for (int i = max(first, j - (lk - lq)); i < min(first + kRows, lq); ++i) {
+            const int64_t q = q0 + i;
+            float w = ex2(score_of<T>(p, q, k, head, kvh) - p.lse[static_cast<int64_t>(head) * p.tq + q]);
+            const T* g = static_cast<const T*>(p.dout) + q * p.do_st + head * p.do_sh;
+            const T* with = g;
+            if (!want_v) {
+                w *= (dot_row(g, static_cast<const T*>(p.v) + k * p.v_st + kvh * p.v_sh, p.dim) -
+                      p.delta[static_cast<int64_t>(head) * p.tq + q]) * up;
+                with = static_cast<const T*>(p.q) + q * p.q_st + head * p.q_sh;
+            }
+            w = to_f(from_f<T>(w));
+            for (int c = 0; c < p.dim; ++c) o[c] = fmaf(w, to_f(with[c]), o[c]);
+        }
+    }
+    const float by = want_v ? 1.0f : p.scale / up;
+    for (int c = 0; c < p.dim; ++c) {
+        if (part != nullptr)
+            part[c] = o[c] * by;
+        else
+            out[c] = from_f<T>(o[c] * by);
+    }
+}
+
+// A row of dk or dv out of tensor memory. Whole warps; rows of lanes with `live`.
+template <typename T, int DP>
+__device__ __forceinline__ void finish_key_row(const AttnParams& p, uint32_t at, bool live, bool any, int64_t k, int j, int kvh, int64_t q0,
+                                               int lq, int lk, int i0, int i1, int z, float up, bool want_v, bool alive) {
+    const int64_t row = (k * p.kv_heads + kvh) * p.dim;
+    T* out = static_cast<T*>(want_v ? p.dv : p.dk) + row;
+    float* part = p.qsplits > 1 ? (want_v ? p.part_dv : p.part_dk) + static_cast<int64_t>(z) * p.tk * p.kv_heads * p.dim + row : nullptr;
+    const float by = !alive ? __uint_as_float(0x7fffffffu) : want_v ? 1.0f : p.scale / up;
+    bool fine = true;
+#pragma unroll
+    for (int c = 0; c < DP; c += 16) {
+        if (c >= p.dim) continue;
+        float o[16];
+        if (any) {
+            tc::tmem_ld16(at + c, o);
+            tc::wait_ld();
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
+        if (!live) continue;
+        if (part != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= by;
+            write_part(part, o, c, p.dim);
+        } else {
+            write_out<T>(out, o, c, p.dim, by);
+        }
+    }
+    if (p.causal && live && !fine && alive) key_row<T>(p, k, j, kvh, q0, lq, lk, i0, i1, up, want_v, out, part);
+}
+
+// ---- which windows there are -----------------------------------------------------------------
+// flags[0]: some window has more than short_max keys.
+__global__ void __launch_bounds__(256) k_attn_flags(AttnParams p, int* flags) {
+    bool longer = false;
+    for (int w = blockIdx.x * 256 + threadIdx.x; w < p.windows; w += gridDim.x * 256)
+        longer |= attn_offset(p.k_off, p.windows, p.tk, w + 2) - attn_offset(p.k_off, p.windows, p.tk, w + 1) > p.short_max;
+    if (__syncthreads_or(longer) && threadIdx.x == 0) atomicOr(flags, 1);
+}
+
+// ---- short windows ---------------------------------------------------------------------------
+template <int DP>
+struct ShortSmem {
+    static constexpr int kT = kRows * DP * 2, kK = kShortKeys * DP * 2, kP = kRows * kShortKeys * 2;
+    // dS, P, Q, dO, K, V; dS and P end before 16 KB that may be read past them (rows of keys 64 and on,
+    // which nothing uses)
+    static constexpr int kTiles = 2 * kP + 2 * kT + 2 * kK;
+    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<kShortKeys>)) + 64 + 64 + 32;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(const __grid_constant__ AttnParams p) {
+    using L = ShortSmem<DP>;
+    constexpr int kCols = DP == 64 ? 256 : 512, KT = kShortKeys;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sd = tc::smem_addr(base), sp = sd + L::kP, sq = sp + L::kP, sg = sq + L::kT, sk = sg + L::kT, sv = sk + L::kK;
+    KeyPos<KT>* kp = reinterpret_cast<KeyPos<KT>*>(base + L::kTiles);
+    Range* qrange = reinterpret_cast<Range*>(kp + 1);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    float* wsize = reinterpret_cast<float*>(slot_tmem + 4);
+    float* wsum = wsize + 4;
+    const int group = p.heads / p.kv_heads, entries = bias_entries(p.bias), kvh = blockIdx.y;
+    const bool grad_bias = p.bias_part != nullptr;
+    double* acc = reinterpret_cast<double*>(base + L::kBytes);
+    int* I = reinterpret_cast<int*>(acc + (grad_bias ? group * entries : 0));
+    float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+
+    const int tid = threadIdx.x, warp = tid >> 5, z = blockIdx.z;
+    const int dim16 = (p.dim + 15) & ~15;
+    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
+        og(p.dout, p.do_st, p.do_sh, p.dim);
+    if (tid == 0) {
+        tc::mbar_init(bar_s, 1);
+        tc::mbar_init(bar_o, 1);
+        tc::mbar_init_fence();
+    }
+    if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
+    for (int e = tid; e < entries * group; e += kRows) {
+        E[e] = bias_entry(p.bias, p.heads, kvh * group + e / entries, e % entries);
+        if (grad_bias) acc[e] = 0.0;
+    }
+    if (grad_bias)
+        for (int e = tid; e < entries; e += kRows) I[e] = 0;
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t t_dv = 2 * KT, t_dk = 2 * KT + DP;  // columns; S at 0, dP at 64, dQ over both
+    const uint32_t id_grad = tc::idesc(kIsBf16<T>, dim16, true, true), id_q = tc::idesc(kIsBf16<T>, dim16, false, true);
+    const float up = ds_scale<T>(p);
+    int par_s = 0, par_o = 0;
+    bool alive = true;
+
+    // rows outside every window
+    if (z == 0) {
+        const int q_lo = attn_offset(p.q_off, p.windows, p.tq, 1), q_hi = attn_offset(p.q_off, p.windows, p.tq, p.windows + 1);
+        const int k_lo = attn_offset(p.k_off, p.windows, p.tk, 1), k_hi = attn_offset(p.k_off, p.windows, p.tk, p.windows + 1);
+        const int nq = q_lo + max(p.tq - q_hi, 0), nk = k_lo + max(p.tk - k_hi, 0);
+        for (int r = blockIdx.x; r < nq + nk; r += gridDim.x) {
+            const bool of_q = r < nq;
+            const int i = of_q ? r : r - nq, lo = of_q ? q_lo : k_lo, hi = of_q ? q_hi : k_hi;
+            const int64_t token = i < lo ? i : hi + (i - lo);
+            for (int c = tid; c < p.dim * (of_q ? group : 2); c += kRows) {
+                if (of_q) {
+                    static_cast<T*>(p.dq)[(token * p.heads + kvh * group) * p.dim + c] = from_f<T>(0.0f);
+                } else if (p.qsplits == 1) {
+                    static_cast<T*>(c < p.dim ? p.dk : p.dv)[(token * p.kv_heads + kvh) * p.dim + c % p.dim] = from_f<T>(0.0f);
+                } else {
+                    for (int s = 0; s < p.qsplits; ++s)
+                        (c < p.dim ? p.part_dk : p.part_dv)[((static_cast<int64_t>(s) * p.tk + token) * p.kv_heads + kvh) * p.dim + c % p.dim] = 0.0f;
+                }
+            }
+        }
+    }
+
+    for (int w = blockIdx.x; w < p.windows; w += gridDim.x) {
+        const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
+        const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), lk = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
+        if (lk > p.short_max) continue;
+        if (lk == 0) {
+            const int64_t n = static_cast<int64_t>(lq) * group * p.dim;
+            if (z == 0)
+                for (int64_t i = tid; i < n; i += kRows)
+                    static_cast<T*>(p.dq)[((q0 + i / (group * p.dim)) * p.heads + kvh * group) * p.dim + i % (group * p.dim)] = from_f<T>(0.0f);
+            continue;
+        }
+        const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
+        const int i0 = min(z * per, total), i1 = min(i0 + per, total);
+        const int n = lk, n16 = (n + 15) & ~15;
+        float lse = INFINITY;
+        int2 qp = make_int2(0, 0);
+        // Q, dO and the row's scalars of one tile
+        auto fetch = [&](int it) {
+            const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
+            load_panel<T>(sq, kRows, oq, q0, head, 1, first, rows, kRows, p.dim);
+            load_panel<T>(sg, kRows, og, q0, head, 1, first, rows, kRows, p.dim);
+            tc::cp_async_commit();
+            lse = tid < rows ? p.lse[static_cast<int64_t>(head) * p.tq + q0 + first + tid] : INFINITY;
+            if (entries > 0) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(tid, rows - 1));
+        };
+        __syncthreads();  // the window before has read its keys
+        if (i0 < i1) {
+            load_panel<T>(sk, KT, ok, k0, kvh, 1, 0, n, n16, p.dim);
+            load_panel<T>(sv, KT, ov, k0, kvh, 1, 0, n, n16, p.dim);
+            fetch(i0);
+            if (entries > 0) load_key_pos<KT>(kp, p.bias, k0, n);
+        }
+        for (int it = i0; it < i1; ++it) {
+            const int g = it / qtiles, head = kvh * group + g, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
+            if (entries > 0) {
+                const Range r = warp_range(qp);
+                if ((tid & 31) == 0) qrange[warp] = r;
+            }
+            tc::cp_async_wait<0>();
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
+                tc::mma_nt(tmem, sq, kRows, sk, KT, dim16, id);
+                tc::mma_nt(tmem + KT, sg, kRows, sv, KT, dim16, id);
+                tc::commit(bar_s);
+            }
+            const int see = tid >= rows ? 0 : p.causal ? min(max(first + tid + lk - lq + 1, 0), lk) : lk;
+            const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= n);
+            BiasMode mode = kOne;
+            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            par_s ^= 1;
+            tc::fence_after();
+            float s[64], dp[64];
+            weights<KT>(p, s, dp, ts, ts + KT, n16, 0, whole, see, lse, mode, E + g * entries, entries > 0, kp, qp);
+            float delta = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 64; ++c) delta = fmaf(s[c], dp[c], delta);
+            write_row<T>(sp, tid, s, 1.0f);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            write_row<T>(sd, tid, dp, up);
+            if (grad_bias) {
+                const float m = warp_size(dp);
+                if ((tid & 31) == 0) wsize[warp] = m;
+            }
+            if (p.causal && tid < rows) p.delta[static_cast<int64_t>(head) * p.tq + q0 + first + tid] = delta;
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                for (int k = 0; k < kRows; k += 16) {
+                    tc::mma_ss(tmem + t_dv, tc::desc(sp + k * 128, L::kP), tc::desc(sg + k * 128, kRows * 128), id_grad, it > i0 || k > 0);
+                    tc::mma_ss(tmem + t_dk, tc::desc(sd + k * 128, L::kP), tc::desc(sq + k * 128, kRows * 128), id_grad, it > i0 || k > 0);
+                }
+                for (int k = 0; k < n16; k += 16)
+                    tc::mma_ss(tmem, tc::desc(sd + k * 2, 16), tc::desc(sk + k * 128, KT * 128), id_q, k > 0);
+                tc::commit(bar_o);
+            }
+            BiasSum bs{kOne, 0.0f, false};
+            if (grad_bias) {
+                bs = bias_sum<4>(mode, wsize);
+                if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, 0, qp, I, wsum + warp);
+            }
+            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            par_o ^= 1;
+            tc::fence_after();
+            const int2 qp_now = qp;
+            const float lse_now = lse;
+            if (it + 1 < i1) fetch(it + 1);
+            bool fine = true;
+#pragma unroll
+            for (int c = 0; c < DP; c += 16) {
+                if (c >= dim16) continue;
+                float o[16];
+                tc::tmem_ld16(ts + c, o);
+                tc::wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
+                stage16<T>(sd, tid, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
+            }
+            if (p.causal && tid < rows && !fine && alive) query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, delta, up, sd);
+            tc::fence_before();
+            __syncthreads();
+            if (grad_bias && (bs.fixed != 0.0f || bs.bad))
+                bias_join<kRows, 4, KT>(p, bs, entries, head, kp, qp_now, I, wsum, acc + g * entries);
+            store_panel<T, kRows>(sd, p.dq, p.heads, p.dim, q0, head, 1, first, rows);
+        }
+        if (warp < 2) {
+            finish_key_row<T, DP>(p, ts + t_dv, tid < n, i0 < i1, k0 + min(tid, n - 1), tid, kvh, q0, lq, lk, i0, i1, z, up, true, alive);
+            finish_key_row<T, DP>(p, ts + t_dk, tid < n, i0 < i1, k0 + min(tid, n - 1), tid, kvh, q0, lq, lk, i0, i1, z, up, false, alive);
+        }
+        tc::fence_before();
+    }
+    if (grad_bias) {
+        __syncthreads();
+        for (int e = tid; e < entries * group; e += kRows)
+            p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * (p.bias_short + p.bias_long) + z * gridDim.x + blockIdx.x) * entries +
+                        e % entries] = acc[e];
+    }
+    if (!alive && tid == 0) count_timeout();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) tc::tmem_free<kCols>(tmem);
+}
+
+// ---- long windows: dq ------------------------------------------------------------------------
+template <int DP>
+struct LongSmem {
+    static constexpr int kT = kRows * DP * 2, kP = kRows * kRows * 2;
+    static constexpr int kBuf = DP == 64 ? 2 : 1;  // of what the kernel walks
+    static constexpr int kMisc = static_cast<int>(sizeof(KeyPos<kRows>)) * kBuf + 64 + 64 + 64;
+    static constexpr int kDq = 2 * kT + 2 * kBuf * kT + kP;
+    static constexpr int kDkv = 2 * kT + 2 * kBuf * kT + 2 * kP;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_constant__ AttnParams p) {
+    if (*p.flags == 0) return;
+    using L = LongSmem<DP>;
+    constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sq = tc::smem_addr(base), sg = sq + L::kT, sk = sg + L::kT, sv = sk + kBuf * L::kT, sd = sv + kBuf * L::kT;
+    KeyPos<KT>* kps = reinterpret_cast<KeyPos<KT>*>(base + L::kDq);
+    Range* qrange = reinterpret_cast<Range*>(kps + kBuf);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    float* wsize = reinterpret_cast<float*>(bars + 8);
+    float* wsum = wsize + 8;
+    const int entries = bias_entries(p.bias), head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
+    const bool grad_bias = p.bias_part != nullptr;
+    double* acc = reinterpret_cast<double*>(base + L::kDq + L::kMisc);
+    int* I = reinterpret_cast<int*>(acc + (grad_bias ? entries : 0));
+    float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+
+    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
+    const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tq, p.windows, kRows);
+    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
+        og(p.dout, p.do_st, p.do_sh, p.dim);
+    if (tid == 0) {
+        tc::mbar_init(bar_s, 1);
+        tc::mbar_init(bar_o, 1);
+        tc::mbar_init_fence();
+    }
+    if (warp == 0) tc::tmem_alloc<512>(tc::smem_addr(slot_tmem));
+    for (int e = tid; e < entries; e += kThreads) {
+        E[e] = bias_entry(p.bias, p.heads, head, e);
+        if (grad_bias) acc[e] = 0.0, I[e] = 0;
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t id_q = tc::idesc(kIsBf16<T>, dim16, false, true);
+    const float up = ds_scale<T>(p);
+    int par_s = 0, par_o = 0;
+    bool alive = true;
+
+    for (int it = blockIdx.x; it < slots; it += gridDim.x) {
+        AttnTile t;
+        if (!attn_tile(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, p.causal ? slots - 1 - it : it, t)) continue;
+        if (t.window < 0 || t.olen <= p.short_max) continue;
+        const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
+        const bool live = row < rows;
+        const int see = !live ? 0 : p.causal ? min(max(t.first + row + shift + 1, 0), t.olen) : t.olen;
+        const int most = p.causal ? min(max(t.first + rows + shift, 0), t.olen) : t.olen;
+        const int least = p.causal ? min(max(t.first + shift + 1, 0), t.olen) : t.olen;
+        const int tiles = (most + KT - 1) / KT;
+        const int64_t token = t.begin + t.first + min(row, rows - 1);
+        const float lse = live ? p.lse[static_cast<int64_t>(head) * p.tq + token] : INFINITY;
+        const float delta = live ? p.delta[static_cast<int64_t>(head) * p.tq + token] : 0.0f;
+        const int2 qp = entries > 0 ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0);
+        auto fetch = [&](int kt) {
+            const int b = kBuf == 2 ? kt & 1 : 0, n = min(KT, most - kt * KT), n16 = (n + 15) & ~15;
+            load_panel<T, kThreads>(sk + b * L::kT, KT, ok, t.obegin + kt * KT, kvh, 1, 0, n, n16, p.dim);
+            load_panel<T, kThreads>(sv + b * L::kT, KT, ov, t.obegin + kt * KT, kvh, 1, 0, n, n16, p.dim);
+            if (entries > 0) load_key_pos<KT>(kps + b, p.bias, t.obegin + kt * KT, n);
+        };
+        __syncthreads();  // the tile before has been read
+        if (tiles > 0) {
+            load_panel<T, kThreads>(sq, kRows, oq, t.begin, head, 1, t.first, rows, kRows, p.dim);
+            load_panel<T, kThreads>(sg, kRows, og, t.begin, head, 1, t.first, rows, kRows, p.dim);
+            fetch(0);
+            if (entries > 0) {
+                const Range r = warp_range(qp);
+                if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
+            }
+        }
+        tc::cp_async_commit();
+        BiasSum bs{kOne, 0.0f, false};
+        for (int kt = 0; kt < tiles; ++kt) {
+            const int b = kBuf == 2 ? kt & 1 : 0, n = min(KT, most - kt * KT), n16 = (n + 15) & ~15;
+            KeyPos<KT>* kp = kps + b;
+            tc::cp_async_wait<0>();
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
+                tc::mma_nt(tmem, sq, kRows, sk + b * L::kT, KT, dim16, id);
+                tc::mma_nt(tmem + KT, sg, kRows, sv + b * L::kT, KT, dim16, id);
+                tc::commit(bar_s);
+            }
+            if (grad_bias && kt > 0 && (bs.fixed != 0.0f || bs.bad))  // of the tile before
+                bias_join<kThreads, 8, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (kt - 1) & 1 : 0), qp, I, wsum, acc);
+            if (kBuf == 2) {
+                if (kt > 0) {  // dQ of the tile before: its keys and dS are free
+                    alive = tc::mbar_wait(bar_o, par_o) && alive;
+                    par_o ^= 1;
+                }
+                if (grad_bias) __syncthreads();  // its key positions have been read
+                if (kt + 1 < tiles) fetch(kt + 1);
+                tc::cp_async_commit();
+            }
+            BiasMode mode = kOne;
+            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            par_s ^= 1;
+            tc::fence_after();
+            float s[64], dp[64];
+            weights<KT>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, entries > 0, kp, qp);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
+            if (grad_bias) {
+                const float m = warp_size(dp);
+                if ((tid & 31) == 0) wsize[warp] = m;
+            }
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                for (int k = 0; k < n16; k += 16)
+                    tc::mma_ss(tmem + 2 * KT, tc::desc(sd + (k >> 6) * kRows * 128 + (k & 63) * 2, 16),
+                               tc::desc(sk + b * L::kT + k * 128, KT * 128), id_q, kt > 0 || k > 0);
+                tc::commit(bar_o);
+            }
+            if (grad_bias) {
+                bs = bias_sum<8>(mode, wsize);
+                if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, j0, qp, I, wsum + warp);
+            }
+            if (kBuf == 1) {
+                alive = tc::mbar_wait(bar_o, par_o) && alive;
+                par_o ^= 1;
+                if (kt + 1 < tiles) {
+                    if (grad_bias) {
+                        __syncthreads();
+                        if (bs.fixed != 0.0f || bs.bad) bias_join<kThreads, 8, KT>(p, bs, entries, head, kp, qp, I, wsum, acc);
+                        bs = BiasSum{kOne, 0.0f, false};
+                        __syncthreads();
+                    } else if (entries > 0) {
+                        __syncthreads();
+                    }
+                    fetch(kt + 1);
+                }
+                tc::cp_async_commit();
+            }
+        }
+        if (tiles > 0 && kBuf == 2) {
+            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            par_o ^= 1;
+        }
+        tc::fence_after();
+        __syncthreads();
+        if (grad_bias && tiles > 0 && (bs.fixed != 0.0f || bs.bad))
+            bias_join<kThreads, 8, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (tiles - 1) & 1 : 0), qp, I, wsum, acc);
+        if (tid < kRows) {
+            bool fine = true;
+#pragma unroll
+            for (int c = 0; c < DP; c += 16) {
+                if (c >= dim16) continue;
+                float o[16];
+                if (tiles > 0) {
+                    tc::tmem_ld16(ts + 2 * KT + c, o);
+                    tc::wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
+                stage16<T>(sq, row, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
+            }
+            if (p.causal && live && !fine && alive) query_row<T>(p, token, head, t.obegin, see, lse, delta, up, sq);
+        }
+        tc::fence_before();
+        __syncthreads();
+        store_panel<T, kThreads>(sq, p.dq, p.heads, p.dim, t.begin, head, 1, t.first, rows);
+    }
+    if (grad_bias) {
+        __syncthreads();
+        for (int e = tid; e < entries; e += kThreads)
+            p.bias_part[(static_cast<int64_t>(head) * (p.bias_short + p.bias_long) + p.bias_short + blockIdx.x) * entries + e] = acc[e];
+    }
+    if (!alive && tid == 0) count_timeout();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) tc::tmem_free<512>(tmem);
+}
+
+// ---- long windows: dk, dv --------------------------------------------------------------------
+template <typename T, int DP>
+__global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
+    if (*p.flags == 0) return;
+    using L = LongSmem<DP>;
+    constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sk = tc::smem_addr(base), sv = sk + L::kT, sq = sv + L::kT, sg = sq + kBuf * L::kT, sp = sg + kBuf * L::kT,
+                   sd = sp + L::kP;
+    KeyPos<KT>* kp = reinterpret_cast<KeyPos<KT>*>(base + L::kDkv);
+    Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of both buffers' queries: 4 warps each, written in turn
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    const int entries = bias_entries(p.bias), kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
+    float* E = reinterpret_cast<float*>(base + L::kDkv + L::kMisc);
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+
+    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
+    const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tk, p.windows, KT);
+    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
+        og(p.dout, p.do_st, p.do_sh, p.dim);
+    if (tid == 0) {
+        tc::mbar_init(bar_s, 1);
+        tc::mbar_init(bar_o, 1);
+        tc::mbar_init_fence();
+    }
+    if (warp == 0) tc::tmem_alloc<512>(tc::smem_addr(slot_tmem));
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t t_dv = 2 * KT, t_dk = 2 * KT + DP;
+    const uint32_t id_grad = tc::idesc(kIsBf16<T>, dim16, true, true);
+    const float up = ds_scale<T>(p);
+    int par_s = 0, par_o = 0, head_of_E = -1;
+    bool alive = true;
+
+    for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
+        AttnTile t;
+        if (!attn_tile(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, slot, t)) continue;
+        if (t.window < 0 || t.len <= p.short_max) continue;
+        const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;
+        const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
+        const int i0 = min(z * per, total), i1 = min(i0 + per, total);
+        // causal: query tiles before this one see none of the tile's keys
+        const int qt0 = p.causal ? min(max(t.first - (lk - lq), 0) / kRows, qtiles) : 0;
+        auto next = [&](int it) { return it < i1 && it % qtiles < qt0 ? it - it % qtiles + qt0 : it; };
+        auto fetch = [&](int it, int b) {
+            const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
+            load_panel<T, kThreads>(sq + b * L::kT, kRows, oq, t.obegin, head, 1, first, rows, kRows, p.dim);
+            load_panel<T, kThreads>(sg + b * L::kT, kRows, og, t.obegin, head, 1, first, rows, kRows, p.dim);
+        };
+        __syncthreads();
+        int it = next(i0), b = 0;
+        const bool any = it < i1;
+        if (any) {
+            load_panel<T, kThreads>(sk, KT, ok, t.begin, kvh, 1, t.first, n, n16, p.dim);
+            load_panel<T, kThreads>(sv, KT, ov, t.begin, kvh, 1, t.first, n, n16, p.dim);
+            fetch(it, 0);
+            if (entries > 0) load_key_pos<KT>(kp, p.bias, t.begin + t.first, n);
+        }
+        tc::cp_async_commit();
+        bool begun = false;
+        while (it < i1) {
+            const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
+            const int after = next(it + 1);
+            const bool live = row < rows;
+            const int64_t token = t.obegin + first + min(row, rows - 1);
+            const float lse = live ? p.lse[static_cast<int64_t>(head) * p.tq + token] : INFINITY;
+            const float delta = live ? p.delta[static_cast<int64_t>(head) * p.tq + token] : 0.0f;
+            int2 qp = make_int2(0, 0);
+            if (entries > 0) {
+                qp = bias_pos(p.bias.q_pos, p.bias.axes, token);
+                const Range r = warp_range(qp);
+                if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
+                if (head != head_of_E)  // everyone is past the last tile's lookups: its barrier before dV and dK
+                    for (int e = tid; e < entries; e += kThreads) E[e] = bias_entry(p.bias, p.heads, head, e);
+                head_of_E = head;
+            }
+            tc::cp_async_wait<0>();
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
+                tc::mma_nt(tmem, sq + b * L::kT, kRows, sk, KT, dim16, id);
+                tc::mma_nt(tmem + KT, sg + b * L::kT, kRows, sv, KT, dim16, id);
+                tc::commit(bar_s);
+            }
+            if (kBuf == 2) {
+                if (begun) {
+                    alive = tc::mbar_wait(bar_o, par_o) && alive;
+                    par_o ^= 1;
+                }
+                if (after < i1) fetch(after, b ^ 1);
+                tc::cp_async_commit();
+            }
+            const int see = !live ? 0 : p.causal ? min(max(first + row + lk - lq + 1, 0), lk) : lk;
+            const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= t.first + n);
+            BiasMode mode = kOne;
+            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            par_s ^= 1;
+            tc::fence_after();
+            float s[64], dp[64];
+            weights<KT>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, lse, mode, E, entries > 0, kp, qp);
+            write_row<T>(sp + (j0 >> 6) * kRows * 128, row, s, 1.0f);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
+            tc::fence_async();
+            tc::fence_before();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after();
+                for (int k = 0; k < kRows; k += 16) {
+                    tc::mma_ss(tmem + t_dv, tc::desc(sp + k * 128, kRows * 128), tc::desc(sg + b * L::kT + k * 128, kRows * 128), id_grad, begun || k > 0);
+                    tc::mma_ss(tmem + t_dk, tc::desc(sd + k * 128, kRows * 128), tc::desc(sq + b * L::kT + k * 128, kRows * 128), id_grad, begun || k > 0);
+                }
+                tc::commit(bar_o);
+            }
+            if (kBuf == 1) {
+                alive = tc::mbar_wait(bar_o, par_o) && alive;
+                par_o ^= 1;
+                if (after < i1) fetch(after, 0);
+                tc::cp_async_commit();
+            } else {
+                b ^= 1;
+            }
+            begun = true;
+            it = after;
+        }
+        if (begun && kBuf == 2) {
+            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            par_o ^= 1;
+        }
+        tc::fence_after();
+        const bool of_v = tid < kRows;
+        finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, t.begin + t.first + min(row, n - 1), t.first + row, kvh, t.obegin, lq,
+                              lk, i0, i1, z, up, of_v, alive);
+        tc::fence_before();
+    }
+    if (!alive && tid == 0) count_timeout();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) tc::tmem_free<512>(tmem);
+}
+
+// ---- sums across blocks ------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_join_dkv(AttnParams p) {
+    const int64_t n = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= n) return;
+    float k = 0.0f, v = 0.0f;
+    for (int s = 0; s < p.qsplits; ++s) {
+        k += p.part_dk[s * n + i];
+        v += p.part_dv[s * n + i];
+    }
+    static_cast<T*>(p.dk)[i] = from_f<T>(k);
+    static_cast<T*>(p.dv)[i] = from_f<T>(v);
+}
+
+// The parts of each entry, in order, into the first part.
+__global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
+    const int entries = bias_entries(p.bias), e = blockIdx.x * 256 + threadIdx.x;
+    if (e >= entries) return;
+    const int parts = p.bias_short + p.bias_long, used = *p.flags != 0 ? parts : p.bias_short;
+    double* at = p.bias_part + static_cast<int64_t>(blockIdx.y) * parts * entries + e;
+    double sum = 0.0;
+    for (int s = 0; s < used; ++s) sum += at[static_cast<int64_t>(s) * entries];
+    at[0] = sum;
+}
+
+// Entries to the rows of the table that they map to: in 64-bit fixed point, so that several
+// entries of one row add up the same in any order. A block a head.
+__global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dtable) {
+    const int entries = bias_entries(p.bias), head = blockIdx.x, tid = threadIdx.x;
+    const double* sum = p.bias_part + static_cast<int64_t>(head) * (p.bias_short + p.bias_long) * entries;
+    __shared__ unsigned long long top;
+    if (tid == 0) top = 0ull;
+    __syncthreads();
+    unsigned long long m = 0ull;
+    for (int e = tid; e < entries; e += 1024) m = max(m, static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
+    atomicMax(&top, m);
+    __syncthreads();
+    const double most = __longlong_as_double(static_cast<long long>(top));
+    const int shift = most > 0.0 ? 48 - ilogb(most) : 0;  // 4096 entries of at most 2^49
+    for (int e = tid; e < entries; e += 1024) {
+        const int bucket = __ldg(p.bias.map + e);
+        if (bucket >= 0 && bucket < p.bias.buckets)
+            atomicAdd(p.bias_acc + static_cast<int64_t>(bucket) * p.heads + head,
+                      static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], shift))));
+    }
+    __threadfence();
+    __syncthreads();
+    for (int b = tid; b < p.bias.buckets; b += 1024) {
+        const int64_t i = static_cast<int64_t>(b) * p.heads + head;
+        const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -shift);
+        store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
+    }
+}
+
+template <typename K>
+cudaError_t smem_of(K kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int DP>
+cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
+    const int entries = bias_entries(p.bias), group = p.heads / p.kv_heads, sum = p.bias_part != nullptr;
+    cudaError_t err;
+    const int b_short = 1024 + ShortSmem<DP>::kBytes + entries * group * (4 + 8 * sum) + entries * 4 * sum;
+    if (p.short_max == 0) {
+        // only rows and windows without partners: no bias is looked up
+        AttnParams none = p;
+        none.bias.table = nullptr;
+        none.bias_part = nullptr;
+        const int bytes = 1024 + ShortSmem<DP>::kBytes;
+        if ((err = smem_of(k_attn_bwd_short<T, DP>, bytes)) != cudaSuccess) return err;
+        k_attn_bwd_short<T, DP><<<dim3(p.short_blocks, p.kv_heads, 1), kRows, bytes, s>>>(none);
+    } else {
+        if ((err = smem_of(k_attn_bwd_short<T, DP>, b_short)) != cudaSuccess) return err;
+        k_attn_bwd_short<T, DP><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), kRows, b_short, s>>>(p);
+    }
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    const int b_dq = 1024 + LongSmem<DP>::kDq + LongSmem<DP>::kMisc + entries * (4 + 12 * sum);
+    if ((err = smem_of(k_attn_dq_long<T, DP>, b_dq)) != cudaSuccess) return err;
+    k_attn_dq_long<T, DP><<<dim3(p.dq_blocks, p.heads), 2 * kRows, b_dq, s>>>(p);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    const int b_kv = 1024 + LongSmem<DP>::kDkv + LongSmem<DP>::kMisc + entries * 4;
+    if ((err = smem_of(k_attn_dkv_long<T, DP>, b_kv)) != cudaSuccess) return err;
+    k_attn_dkv_long<T, DP><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_kv, s>>>(p);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    if (p.qsplits > 1) {
+        const int64_t n = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
+        k_attn_join_dkv<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+        if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    }
+    if (dtable != nullptr) {
+        k_attn_bias_parts<<<dim3((entries + 255) / 256, p.heads), 256, 0, s>>>(p);
+        if ((err = cudaGetLastError()) != cudaSuccess) return err;
+        k_attn_bias_table<<<p.heads, 1024, 0, s>>>(p, dtable);
+        err = cudaGetLastError();
+    }
+    return err;
+}
+
+}  // namespace
+
+cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
+    k_attn_flags<<<p.windows < 16384 ? 1 + p.windows / 1024 : 16, 256, 0, s>>>(p, p.flags);
+    cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+    if ((err = launch_attn_delta(p, type, sms, s)) != cudaSuccess) return err;
+    if (type == kBF16) return p.dim <= 64 ? bwd_one<__nv_bfloat16, 64>(p, dtable, s) : bwd_one<__nv_bfloat16, 128>(p, dtable, s);
+    return p.dim <= 64 ? bwd_one<__half, 64>(p, dtable, s) : bwd_one<__half, 128>(p, dtable, s);
+}
+
+cudaError_t attn_timeouts_bwd(unsigned int* count) {
+    return cudaMemcpyFromSymbol(count, g_timeouts, sizeof(unsigned int));
+}
+
+}  // namespace oss

@@ -272,9 +272,10 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
 
 // ---- backward ----------------------------------------------------------------
 // delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for the bias
-// gradient's fixed point). A warp a row.
+// gradient's fixed point, and fp16's range). A warp a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* delta, uint32_t* bias_max) {
+    if (p.flags != nullptr && *p.flags == 0 && bias_max == nullptr) return;  // short windows find their own
     const int lane = threadIdx.x & 31;
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads;
     const int64_t vrows = bias_max == nullptr ? 0 : static_cast<int64_t>(p.tk) * p.kv_heads;
@@ -585,14 +586,13 @@ cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s, int sms) {
 }
 
 template <typename T>
-cudaError_t bwd_type(const AttnParams& p, cudaStream_t s, float* delta, uint32_t* bias_max, int sms) {
+cudaError_t delta_type(const AttnParams& p, cudaStream_t s, int sms) {
+    uint32_t* bias_max = const_cast<uint32_t*>(p.bias_max);
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads + (bias_max ? static_cast<int64_t>(p.tk) * p.kv_heads : 0);
     const int64_t blocks = (rows + 7) / 8;
-    if (blocks > 0)
-        k_attn_delta<T><<<static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms), kThreads, 0, s>>>(p, delta, bias_max);
-    cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return err;
-    return p.dim <= 32 ? bwd_dim<T, 32>(p, s, sms) : p.dim <= 64 ? bwd_dim<T, 64>(p, s, sms) : bwd_dim<T, 128>(p, s, sms);
+    if (blocks == 0) return cudaSuccess;
+    k_attn_delta<T><<<static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms), kThreads, 0, s>>>(p, p.delta, bias_max);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -603,12 +603,16 @@ cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s) {
     return type == kF32 ? join_parts<float>(p, s) : type == kBF16 ? join_parts<__nv_bfloat16>(p, s) : join_parts<__half>(p, s);
 }
 
-cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, float* delta, int sms, cudaStream_t s) {
-    uint32_t* bias_max = p.bias_acc == nullptr ? nullptr : const_cast<uint32_t*>(p.bias_max);
-    cudaError_t err = type == kF32    ? bwd_type<float>(p, s, delta, bias_max, sms)
-                      : type == kBF16 ? bwd_type<__nv_bfloat16>(p, s, delta, bias_max, sms)
-                                      : bwd_type<__half>(p, s, delta, bias_max, sms);
-    if (err != cudaSuccess || p.bias_acc == nullptr) return err;
+cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s) {
+    return type == kF32 ? delta_type<float>(p, s, sms) : type == kBF16 ? delta_type<__nv_bfloat16>(p, s, sms) : delta_type<__half>(p, s, sms);
+}
+
+cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
+    if (type != kF32) return launch_attn_backward_mma(p, type, dtable, sms, s);
+    cudaError_t err = delta_type<float>(p, s, sms);
+    if (err != cudaSuccess) return err;
+    err = p.dim <= 32 ? bwd_dim<float, 32>(p, s, sms) : p.dim <= 64 ? bwd_dim<float, 64>(p, s, sms) : bwd_dim<float, 128>(p, s, sms);
+    if (err != cudaSuccess || dtable == nullptr) return err;
     k_attn_bias_grad<<<(p.bias.buckets * p.heads + kThreads - 1) / kThreads, kThreads, 0, s>>>(p, dtable);
     return cudaGetLastError();
 }

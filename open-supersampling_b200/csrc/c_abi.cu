@@ -1313,6 +1313,54 @@ int64_t attention_split_bytes(int64_t tq, int64_t heads, int64_t dim, int splits
     return oss::arena_bytes(splits * tq * heads * dim, 4) + oss::arena_bytes(splits * tq * heads * 2, 4);
 }
 
+// How the backward of 16-bit types is cut: see oss::AttnParams.
+void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
+    const int64_t group = p.heads / p.kv_heads;
+    // short windows keep the biases and sums of a whole group of heads
+    p.short_max = entries * group <= oss::kMaxBiasEntries ? 64 : 0;
+    // Parts of the queries, so that few tiles of keys still fill the card: at least 4 tiles of 128
+    // queries in each on average.
+    const int64_t windows = p.windows < 1 ? 1 : p.windows;
+    const int64_t items = (windows > p.tk / 128 ? windows : p.tk / 128) * p.kv_heads;
+    const int64_t want = 2 * kSms / items, most = p.tq / windows * group / 512;
+    const int64_t n = want < most ? want : most;
+    p.qsplits = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+    // resident blocks, or as many as there are tiles
+    auto blocks = [](int64_t tiles, int64_t resident, int64_t heads) {
+        const int64_t per = (resident + heads - 1) / heads;
+        return static_cast<int>(tiles < per ? (tiles < 1 ? 1 : tiles) : per);
+    };
+    p.short_blocks = blocks(windows, (p.dim <= 64 ? 2 : 1) * kSms, p.kv_heads * p.qsplits);
+    p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (sums ? 1 : 4) * kSms, p.heads);
+    p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, 128), 4 * kSms, p.kv_heads * p.qsplits);
+    p.bias_short = p.short_max > 0 ? p.short_blocks * p.qsplits : 0;
+    p.bias_long = p.dq_blocks;
+}
+
+// Lays the backward's scratch out; without a base, counts its bytes. `zeroed`: the bytes from
+// *zero_at on that have to be zero at the start.
+int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t entries, int64_t sum_rows, char* base, int64_t size,
+                                   char** zero_at, int64_t* zeroed) {
+    const bool sums = sum_rows > 0;
+    oss::Arena arena{base, size, 0};
+    p.delta = arena.take<float>(static_cast<int64_t>(p.tq) * p.heads);
+    if (dtype != oss::kF32) {
+        attention_backward_plan(p, entries, sums);
+        const int64_t keys = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
+        p.part_dk = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
+        p.part_dv = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
+        p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * (p.bias_short + p.bias_long) * entries) : nullptr;
+    }
+    const int64_t from = arena.used;
+    p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
+    p.bias_bad = sums ? arena.take<uint32_t>(sum_rows * p.heads) : nullptr;
+    p.bias_max = sums || dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
+    if (dtype == oss::kBF16) p.bias_max = nullptr;
+    p.flags = dtype != oss::kF32 ? arena.take<int>(1) : nullptr;
+    if (zero_at != nullptr) *zero_at = base + from, *zeroed = arena.used - from;
+    return arena.used;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1367,16 +1415,22 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
 
 int oss_window_attention_timeouts(uint32_t* count) {
     OSS_CHECK(count != nullptr, OSS_ERR_INVALID, "count must be non-null");
-    unsigned int n = 0;
-    OSS_CUDA_TRY(oss::attn_timeouts(&n));
-    *count = n;
+    unsigned int forward = 0, backward = 0;
+    OSS_CUDA_TRY(oss::attn_timeouts(&forward));
+    OSS_CUDA_TRY(oss::attn_timeouts_bwd(&backward));
+    *count = forward + backward;
     return OSS_OK;
 }
 
-int64_t oss_window_attention_backward_scratch_bytes(int64_t tq, int64_t heads, int64_t buckets) {
-    if (tq < 0 || heads <= 0 || buckets < 0) return 0;
-    return oss::arena_bytes(tq * heads, 4) + oss::arena_bytes(buckets * heads, 8) + oss::arena_bytes(buckets * heads, 4) +
-           oss::arena_bytes(2, 4);
+int64_t oss_window_attention_backward_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                                                    int64_t kv_heads, int64_t dim, int64_t entries, int64_t buckets) {
+    if (check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim) != OSS_OK || entries < 0 ||
+        entries > oss::kMaxBiasEntries || buckets < 0 || buckets * heads > INT_MAX)
+        return 0;
+    oss::AttnParams p{};
+    p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
+    p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
+    return attention_backward_scratch(p, dtype, entries, buckets, nullptr, 0, nullptr, nullptr);
 }
 
 int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
@@ -1403,7 +1457,9 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
               "k, v, d_k and d_v must be non-null");
     OSS_CHECK(q_offsets != nullptr && k_offsets != nullptr, OSS_ERR_INVALID, "offsets must be non-null");
     const int64_t sums = d_table == nullptr ? 0 : buckets;
-    OSS_CHECK(scratch != nullptr && scratch_bytes >= oss_window_attention_backward_scratch_bytes(tq, heads, sums),
+    OSS_CHECK(scratch != nullptr &&
+                  scratch_bytes >= oss_window_attention_backward_scratch_bytes(dtype, tq, tk, windows, heads, kv_heads, dim,
+                                                                               oss::bias_entries(p.bias), sums),
               OSS_ERR_SCRATCH, "scratch smaller than oss_window_attention_backward_scratch_bytes");
     p.q = q, p.k = k, p.v = v;
     p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
@@ -1413,18 +1469,13 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
     p.scale = scale, p.causal = causal != 0, p.pack = 1, p.splits = 1;
     p.out = const_cast<void*>(out), p.lse = const_cast<float*>(lse);
     p.dout = d_out, p.do_st = do_st, p.do_sh = do_sh, p.dq = d_q, p.dk = d_k, p.dv = d_v;
-    oss::Arena arena{static_cast<char*>(scratch), scratch_bytes, 0};
-    float* delta = arena.take<float>(tq * heads);
-    p.delta = delta;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (d_table != nullptr) {
-        char* sums_at = arena.base + arena.used;
-        p.bias_acc = arena.take<unsigned long long>(buckets * heads);
-        p.bias_bad = arena.take<uint32_t>(buckets * heads);
-        p.bias_max = arena.take<uint32_t>(2);
-        OSS_CUDA_TRY(cudaMemsetAsync(sums_at, 0, arena.base + arena.used - sums_at, s));
-    }
-    OSS_CUDA_TRY(oss::launch_attn_backward(p, dtype, d_table, delta, kSms, s));
+    char* zero_at = nullptr;
+    int64_t zeroed = 0;
+    attention_backward_scratch(p, dtype, oss::bias_entries(p.bias), sums, static_cast<char*>(scratch), scratch_bytes, &zero_at,
+                               &zeroed);
+    if (zeroed > 0) OSS_CUDA_TRY(cudaMemsetAsync(zero_at, 0, zeroed, s));
+    OSS_CUDA_TRY(oss::launch_attn_backward(p, dtype, d_table, kSms, s));
     return OSS_OK;
 }
 

@@ -74,10 +74,13 @@ def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buck
         tk, kv = k.size(0), k.size(1)
         dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
         dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if want_table else None
-        nbytes = lib.oss_window_attention_backward_scratch_bytes(tq, h, table.size(0) if want_table else 0)
+        windows = q_offsets.numel() - 1
+        nbytes = lib.oss_window_attention_backward_scratch_bytes(DTYPES[q.dtype], tq, tk, windows, h, kv, d,
+                                                                 0 if table is None else buckets.numel(),
+                                                                 table.size(0) if want_table else 0)
         scratch = torch.empty((max(1, nbytes),), device=q.device, dtype=torch.uint8)
         _lib.check(
-            lib.oss_window_attention_backward(DTYPES[q.dtype], tq, tk, q_offsets.numel() - 1, h, kv, d, *_strided(q),
+            lib.oss_window_attention_backward(DTYPES[q.dtype], tq, tk, windows, h, kv, d, *_strided(q),
                                               *_strided(k), *_strided(v), q_offsets.data_ptr(), k_offsets.data_ptr(),
                                               scale, int(causal), *_bias_args(table, buckets, q_pos, k_pos),
                                               out.data_ptr(), lse.data_ptr(), *_strided(grad), dq.data_ptr(),
