@@ -129,6 +129,66 @@ __device__ __forceinline__ bool attn_tile(const int32_t* off, int t, const int32
     return true;
 }
 
+// The tiles of slots [slot, end) one after the other: a search for the first, then window by
+// window (neighbouring offsets share cache lines).
+struct AttnWalk {
+    const int32_t *off, *other;
+    int t, ot, windows, per, rows;
+    int slot, end, w;
+    AttnTile tile;
+
+    // Called by whole warps. False: no tile.
+    __device__ __forceinline__ bool start(const int32_t* off_, int t_, const int32_t* other_, int ot_, int windows_, int per_,
+                                          int rows_, int slot_, int end_) {
+        off = off_, t = t_, other = other_, ot = ot_, windows = windows_, per = per_, rows = rows_, slot = slot_, end = end_;
+        const int lane = threadIdx.x & 31;
+        int lo = 0, hi = windows + 2;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
+            const unsigned hit = __ballot_sync(0xffffffffu, at < hi && slot_of(at) <= slot) | 1u;
+            const int n = hit == 0xffffffffu ? 32 : __ffs(~hit) - 1;  // leading probes at or before the slot
+            lo += (n - 1) * step;
+            hi = min(hi, lo + step);
+        }
+        enter(lo);
+        return settle();
+    }
+    __device__ __forceinline__ bool next() {
+        ++slot;
+        const int64_t first = static_cast<int64_t>(tile.first) + rows;
+        if (slot >= end || first >= static_cast<int64_t>(tile.len) * per) return settle();
+        tile.first = static_cast<int>(first);
+        return true;
+    }
+    __device__ __forceinline__ int slot_of(int at) const {
+        return static_cast<int>(static_cast<int64_t>(attn_offset(off, windows, t, at)) * per / rows) + at;
+    }
+    __device__ __forceinline__ void enter(int at) {
+        w = at;
+        tile.begin = attn_offset(off, windows, t, w);
+        tile.len = max(attn_offset(off, windows, t, w + 1) - tile.begin, 0);
+        tile.window = w >= 1 && w <= windows ? w - 1 : -1;
+        tile.obegin = tile.olen = 0;
+        if (tile.window >= 0) {
+            tile.obegin = attn_offset(other, windows, ot, w);
+            tile.olen = max(attn_offset(other, windows, ot, w + 1) - tile.obegin, 0);
+        }
+    }
+    __device__ __forceinline__ bool settle() {
+        while (slot < end) {
+            const int64_t first = static_cast<int64_t>(slot - slot_of(w)) * rows;
+            if (first >= 0 && first < static_cast<int64_t>(tile.len) * per) {
+                tile.first = static_cast<int>(first);
+                return true;
+            }
+            if (w >= windows + 1) return false;
+            enter(w + 1);
+            slot = max(slot, slot_of(w));
+        }
+        return false;
+    }
+};
+
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ float to_f(T x) {

@@ -55,11 +55,11 @@ struct FwdSmem {
     static constexpr int kBytes = kQ + 2 * kK + static_cast<int>(sizeof(KeyPos<KT>)) + 64 + 4 * static_cast<int>(sizeof(Range));
 };
 
-template <typename T, int KT, int DP>
+template <typename T, int KT, int DP, bool BIAS>
 __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const __grid_constant__ AttnParams p) {
     using L = FwdSmem<KT, DP>;
     constexpr int kCols = KT + DP;  // 128 or 256: S (P over it), then O
-    constexpr int kBf16 = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr int kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sq = tc::smem_addr(base), sk = sq + L::kQ, sv = sk + L::kK;
@@ -72,9 +72,9 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
 
     const int tid = threadIdx.x, warp = tid >> 5;
     const int head0 = blockIdx.y * p.pack, kvh = head0 / (p.heads / p.kv_heads);
-    const int entries = bias_entries(p.bias), dim16 = (p.dim + 15) & ~15;
-    const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
-    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim);
+    const int entries = BIAS ? bias_entries(p.bias) : 0, dim16 = (p.dim + 15) & ~15;
+    const Loader<T, kRows> lq(p.q, p.q_st, p.q_sh, p.dim, head0), lk(p.k, p.k_st, p.k_sh, p.dim, kvh),
+        lv(p.v, p.v_st, p.v_sh, p.dim, kvh);
     const float c2 = p.scale * kLog2e;
 
     if (tid == 0) {
@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
         tc::mbar_init_fence();
     }
     if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
-    for (int e = tid; e < entries * p.pack; e += kRows) E[e] = bias_entry(p.bias, p.heads, head0 + e / entries, e % entries);
+    if constexpr (BIAS)
+        for (int e = tid; e < entries * p.pack; e += kRows) E[e] = bias_entry(p.bias, p.heads, head0 + e / entries, e % entries);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -93,32 +94,48 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
     int par_s = 0, par_o = 0;  // parities of the next wait
     bool alive = true;
 
-    for (int it = blockIdx.x; it < slots; it += gridDim.x) {
-        AttnTile t;
-        // causal windows: the last tiles see the most keys and go first
-        if (!attn_tile(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, p.causal ? slots - 1 - it : it, t)) continue;
+    const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
+    const int chunk = (slots + gridDim.x - 1) / gridDim.x;
+    // causal windows: the last tiles see the most keys and go first
+    const int slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
+    AttnWalk walk;
+    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk)); more;
+         more = walk.next()) {
+        const AttnTile& t = walk.tile;
         const int rows = min(kRows, t.len * p.pack - t.first);
         const int row = t.first + tid;
         const bool live = tid < rows;
-        const int see = !live ? 0 : p.causal ? min(max(row / p.pack + t.olen - t.len + 1, 0), t.olen) : t.olen;
-        const int most = p.causal ? min(max((t.first + rows - 1) / p.pack + t.olen - t.len + 1, 0), t.olen) : t.olen;
-        const int least = p.causal ? min(max(t.first / p.pack + t.olen - t.len + 1, 0), t.olen) : t.olen;  // of the live rows
-        const int tiles = (most + KT - 1) / KT, per = (tiles + p.splits - 1) / p.splits;
-        const int tile0 = min(static_cast<int>(blockIdx.z) * per, tiles), tile1 = min(tile0 + per, tiles);
-        const int64_t token = t.begin + (live ? row / p.pack : 0);
-        const int head = head0 + (live ? row % p.pack : 0);
+        int qt = row, qh = 0;  // the row's token in the window, and head
+        if (p.pack > 1) qt = row / p.pack, qh = row - qt * p.pack;
+        const int shift = t.olen - t.len;
+        int most = t.olen, least = t.olen;  // keys that the last row sees, and the first
+        if (p.causal) {
+            most = min(max((p.pack > 1 ? (t.first + rows - 1) / p.pack : t.first + rows - 1) + shift + 1, 0), t.olen);
+            least = min(max((p.pack > 1 ? t.first / p.pack : t.first) + shift + 1, 0), t.olen);
+        }
+        int tile0 = 0, tile1 = (most + KT - 1) / KT;
+        if (p.splits > 1) {
+            const int per = (tile1 + p.splits - 1) / p.splits;
+            tile0 = min(static_cast<int>(blockIdx.z) * per, tile1);
+            tile1 = min(tile0 + per, tile1);
+        }
+        const int64_t token = t.begin + (live ? qt : 0);
+        const int head = head0 + (live ? qh : 0);
 
         float m = -INFINITY, l = 0.0f;  // m: what the weights are taken against
         int2 qp = make_int2(0, 0);
         __syncthreads();  // the last tile's staging has been read
         if (tile0 < tile1) {
             const int k0 = tile0 * KT, n = min(KT, most - k0), n16 = (n + 15) & ~15;
-            load_panel<T>(sq, kRows, oq, t.begin, head0, p.pack, t.first, rows, kRows, p.dim);
-            load_panel<T>(sk, KT, ok, t.obegin + k0, kvh, 1, 0, n, n16, p.dim);
+            if (p.pack == 1)
+                lq.load(sq, kRows, t.begin + t.first, rows, kRows);
+            else
+                lq.load_packed(sq, kRows, t.begin, p.q_sh, p.pack, t.first, rows, kRows);
+            lk.load(sk, KT, t.obegin + k0, n, n16);
             tc::cp_async_commit();
-            load_panel<T>(sv, KT, ov, t.obegin + k0, kvh, 1, 0, n, n16, p.dim);
+            lv.load(sv, KT, t.obegin + k0, n, n16);
             tc::cp_async_commit();
-            if (entries > 0) {
+            if (BIAS) {
                 load_key_pos<KT>(kp, p.bias, t.obegin + k0, n);
                 // rows past the last one take its position: no entry outside the map is looked up
                 qp = bias_pos(p.bias.q_pos, p.bias.axes, t.begin + (t.first + min(tid, rows - 1)) / p.pack);
@@ -136,55 +153,53 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
             tc::fence_before();
             __syncthreads();
             if (kt > tile0) {  // O of the tile before: P and V are free
-                alive = alive && tc::mbar_wait(bar_o, par_o);
+                alive = tc::mbar_wait(bar_o, par_o) && alive;
                 par_o ^= 1;
             }
             if (tid == 0) {
                 tc::fence_after();
-                tc::mma_nt(tmem, sq, kRows, sk, KT, dim16, tc::idesc(kBf16, n16, false, false));
+                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk, dim16, tc::idesc(kBf16, n16, false, false));
                 tc::commit(bar_s);
             }
             if (kt > tile0) {
-                load_panel<T>(sv, KT, ov, t.obegin + k0, kvh, 1, 0, n, n16, p.dim);
+                lv.load(sv, KT, t.obegin + k0, n, n16);
                 tc::cp_async_commit();
             }
             BiasMode mode = kOne;
-            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
-            alive = alive && tc::mbar_wait(bar_s, par_s);
+            if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
-            if (kt + 1 < tile1) {
-                const int n2 = min(KT, most - k0 - KT);
-                load_panel<T>(sk, KT, ok, t.obegin + k0 + KT, kvh, 1, 0, n2, (n2 + 15) & ~15, p.dim);
-            }
-            tc::cp_async_commit();  // a group for each tile, an empty one after the last
-
-            // the row's scores, in base 2
+            // the row's scores
             float s[KT];
 #pragma unroll
             for (int c = 0; c < KT; c += 16)
                 if (c < n16) tc::tmem_ld16(ts + c, s + c);
+            if (kt + 1 < tile1) {
+                const int n2 = min(KT, most - k0 - KT);
+                lk.load(sk, KT, t.obegin + k0 + KT, n2, (n2 + 15) & ~15);
+            }
+            tc::cp_async_commit();  // a group for each tile, an empty one after the last
             tc::wait_ld();
-            const bool whole = n == n16 && k0 + n <= least;  // rows past the last one come to nothing anyway
+            if (BIAS) {
+#pragma unroll
+                for (int c = 0; c < KT; c += 16)
+                    if (c < n16) add_bias<KT, 16>(*reinterpret_cast<float(*)[16]>(s + c), c2, p.bias, mode, E + (live ? qh : 0) * entries, kp, c, qp);
+            }
+            if (n != n16 || k0 + n > least) {  // some rows see less of the tile
+                const int see = live ? (p.causal ? min(qt + shift + 1, t.olen) : t.olen) - k0 : 0;
+#pragma unroll
+                for (int c = 0; c < KT; ++c) s[c] = c < see ? s[c] : -INFINITY;
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < KT; c += 16) {
                 if (c >= n16) continue;
-                float(&x)[16] = *reinterpret_cast<float(*)[16]>(s + c);
-                if (entries > 0) {
-                    add_bias<KT, 16>(x, c2, p.bias, mode, E + (live ? row % p.pack : 0) * entries, kp, c, qp);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] *= c2;
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = k0 + c + i < see ? x[i] : -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+                for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(s[c + i], s[c + i + 1]));
             }
-            // fmaxf passes NaN scores by: their weights are NaN whatever m is, and so is the row
+            // the maximum passes NaN scores by: their weights are NaN whatever m is, and so is the row
+            if (!BIAS) top *= c2;
             const bool rise = top > m + 8.0f || (m == -INFINITY && top > m);
             const float keep = rise ? ex2(m - top) : 1.0f;
             if (rise) m = top;
@@ -200,22 +215,28 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
                     tc::tmem_st16(to + c, o);
                 }
             }
-            const float off = m == -INFINITY ? 0.0f : m;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            // two values an instruction: the scaling and the sum are packed
+            const float off = m == -INFINITY ? 0.0f : -m;
+            const float2 by = make_float2(BIAS ? 1.0f : c2, BIAS ? 1.0f : c2), off2 = make_float2(off, off);
+            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
             for (int c = 0; c < KT; c += 16) {
                 if (c >= n16) continue;
                 uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float a = ex2(s[c + i] - off), b = ex2(s[c + i + 1] - off);
-                    sum0 += a;
-                    sum1 += b;
-                    w[i / 2] = pack2(a, b, T{});
+                for (int i = 0; i < 16; i += 4) {
+                    float2 a = make_float2(s[c + i], s[c + i + 1]), b = make_float2(s[c + i + 2], s[c + i + 3]);
+                    a = BIAS ? __fadd2_rn(a, off2) : __ffma2_rn(a, by, off2);
+                    b = BIAS ? __fadd2_rn(b, off2) : __ffma2_rn(b, by, off2);
+                    a.x = ex2(a.x), a.y = ex2(a.y), b.x = ex2(b.x), b.y = ex2(b.y);
+                    sum0 = __fadd2_rn(sum0, a);
+                    sum1 = __fadd2_rn(sum1, b);
+                    w[i / 2] = pack2(a.x, a.y, T{});
+                    w[i / 2 + 1] = pack2(b.x, b.y, T{});
                 }
                 tc::tmem_st8(ts + c / 2, w);
             }
-            l = l * keep + (sum0 + sum1);
+            l = l * keep + ((sum0.x + sum0.y) + (sum1.x + sum1.y));
             tc::wait_st();
             tc::cp_async_wait<1>();  // V of this tile
             tc::fence_async();
@@ -223,13 +244,13 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after();
-                tc::mma_tn(tmem + KT, tmem, sv, KT, n16, id_o, kt > tile0);
+                tc::mma_tn<KT>(tmem + KT, tmem, sv, n16, id_o, kt > tile0);
                 tc::commit(bar_o);
             }
-            if (entries > 0 && kt + 1 < tile1) load_key_pos<KT>(kp, p.bias, t.obegin + k0 + KT, min(KT, most - k0 - KT));
+            if (BIAS && kt + 1 < tile1) load_key_pos<KT>(kp, p.bias, t.obegin + k0 + KT, min(KT, most - k0 - KT));
         }
         if (tile0 < tile1) {
-            alive = alive && tc::mbar_wait(bar_o, par_o);
+            alive = tc::mbar_wait(bar_o, par_o) && alive;
             par_o ^= 1;
             tc::fence_after();
         }
@@ -253,7 +274,7 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
                 for (int i = 0; i < 16; ++i) o[i] = 0.0f;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);  // columns past dim are 0
+            for (int i = 0; i < 16; ++i) fine = fine && (!p.causal || is_finite(o[i]));  // columns past dim are 0
             if (p.splits > 1) {
                 if (live) write_part(p.part_o + part * p.dim, o, c, p.dim);
             } else {
@@ -261,8 +282,8 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
             }
         }
         if (p.causal && live && !fine) {
-            forward_row<T>(p, token, head, entries > 0 ? p.bias.k_pos : nullptr, t.obegin, tile0 * KT, min(see, tile1 * KT),
-                           m == -INFINITY ? 0.0f : m, E + (row % p.pack) * entries, qp, sq,
+            forward_row<T>(p, token, head, BIAS ? p.bias.k_pos : nullptr, t.obegin, tile0 * KT,
+                           min(min(qt + shift + 1, t.olen), tile1 * KT), m == -INFINITY ? 0.0f : m, E + qh * entries, qp, sq,
                            p.splits > 1 ? p.part_o + part * p.dim : nullptr, inv);
         }
         if (p.splits > 1) continue;
@@ -275,27 +296,30 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
     if (warp == 0) tc::tmem_free<kCols>(tmem);
 }
 
-template <typename T, int KT, int DP>
+template <typename T, int KT, int DP, bool BIAS>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
-    using L = FwdSmem<KT, DP>;
     const int entries = bias_entries(p.bias);
-    const int bytes = 1024 + L::kBytes + 4 * entries * p.pack;
-    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, KT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = 1024 + FwdSmem<KT, DP>::kBytes + 4 * entries * p.pack;
+    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, KT, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
     // Blocks stay for several tiles of one head; four rounds of them even out tiles of unequal
     // length, one where each has to expand a bias first.
-    const int groups = p.heads / p.pack, resident = 148 * (KT == 64 ? 4 : 2) * (entries > 0 ? 1 : 4);
+    const int groups = p.heads / p.pack, resident = 148 * (KT == 64 ? 4 : 2) * (BIAS ? 1 : 4);
     const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
     const int per_head = (resident + groups * p.splits - 1) / (groups * p.splits);
-    k_attn_fwd_mma<T, KT, DP><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows, bytes, s>>>(p);
+    k_attn_fwd_mma<T, KT, DP, BIAS><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows, bytes, s>>>(p);
     return cudaGetLastError();
+}
+template <typename T>
+cudaError_t fwd_type(const AttnParams& p, cudaStream_t s) {
+    if (p.bias.table != nullptr) return p.dim <= 64 ? fwd_one<T, 64, 64, true>(p, s) : fwd_one<T, 128, 128, true>(p, s);
+    return p.dim <= 64 ? fwd_one<T, 64, 64, false>(p, s) : fwd_one<T, 128, 128, false>(p, s);
 }
 
 }  // namespace
 
 cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s) {
-    if (type == kBF16) return p.dim <= 64 ? fwd_one<__nv_bfloat16, 64, 64>(p, s) : fwd_one<__nv_bfloat16, 128, 128>(p, s);
-    return p.dim <= 64 ? fwd_one<__half, 64, 64>(p, s) : fwd_one<__half, 128, 128>(p, s);
+    return type == kBF16 ? fwd_type<__nv_bfloat16>(p, s) : fwd_type<__half>(p, s);
 }
 
 cudaError_t attn_timeouts(unsigned int* count) {

@@ -25,51 +25,71 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
     return r;
 }
 
-// One operand of the tile loads.
-template <typename T>
-struct Operand {
-    const T* p;
-    int64_t st, sh;
-    bool vec;  // every row starts on 16 bytes and ends on them
-    __device__ Operand(const void* q, int64_t st_, int64_t sh_, int dim) : p(static_cast<const T*>(q)), st(st_), sh(sh_) {
-        vec = ((reinterpret_cast<uintptr_t>(q) & 15) | ((st_ | sh_ | dim) & 7)) == 0;
+// A thread's share of the loads of one operand into panels: 16-byte chunk c of rows r0, r0 + step, ...
+template <typename T, int THREADS>
+struct Loader {
+    const T* p;     // the head's chunk c
+    int64_t st;     // token stride
+    int dim, c, r0, step, shift;
+    bool on, zero;  // on: the chunk belongs to the 16-column steps; zero: it lies past dim
+    bool vec;       // every row starts on 16 bytes and ends on them
+
+    __device__ __forceinline__ Loader(const void* q, int64_t st_, int64_t sh, int dim_, int head) : st(st_), dim(dim_) {
+        const int chunks = ((dim + 15) / 16) * 2;
+        shift = 32 - __clz(chunks - 1);  // lanes a row: the next power of two
+        c = threadIdx.x & ((1 << shift) - 1);
+        r0 = threadIdx.x >> shift;
+        step = THREADS >> shift;  // 8 at least, so a chunk keeps its place in the swizzle from row to row
+        on = c < chunks;
+        zero = c * 8 >= dim;
+        p = static_cast<const T*>(q) + head * sh + (zero ? 0 : c * 8);
+        vec = ((reinterpret_cast<uintptr_t>(q) & 15) | ((st_ | sh | dim) & 7)) == 0;
+    }
+    __device__ __forceinline__ uint32_t place(uint32_t dst, int panel_rows) const {
+        return dst + (c >> 3) * panel_rows * 128 + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+    }
+    // `rows` rows from token on, zeros from there to rows_pad; of the head `skip` elements further.
+    __device__ __forceinline__ void load(uint32_t dst, int panel_rows, int64_t token, int rows, int rows_pad, int64_t skip = 0) const {
+        if (!on) return;
+        uint32_t to = place(dst, panel_rows);
+        const T* from = p + (token + r0) * st + skip;
+        int r = r0;
+        if (!zero) {
+            if (vec) {
+                for (; r < rows; r += step, to += step * 128, from += step * st) tc::cp_async16(to, from);
+            } else {
+                for (; r < rows; r += step, to += step * 128, from += step * st) store_some(to, from);
+            }
+        }
+        for (; r < rows_pad; r += step, to += step * 128) store_zero(to);
+    }
+    // The same for rows that are the heads of a group: row r is token r / pack, head r % pack.
+    __device__ __forceinline__ void load_packed(uint32_t dst, int panel_rows, int64_t token, int64_t sh, int pack, int first, int rows,
+                                                int rows_pad) const {
+        if (!on) return;
+        uint32_t to = place(dst, panel_rows);
+        for (int r = r0; r < rows_pad; r += step, to += step * 128) {
+            const T* from = p + (token + (first + r) / pack) * st + (first + r) % pack * sh;
+            if (zero || r >= rows)
+                store_zero(to);
+            else if (vec)
+                tc::cp_async16(to, from);
+            else
+                store_some(to, from);
+        }
+    }
+    __device__ __forceinline__ static void store_zero(uint32_t to) {
+        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0) : "memory");
+    }
+    __device__ __forceinline__ void store_some(uint32_t to, const T* from) const {
+        uint32_t w[4] = {0, 0, 0, 0};
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(__ldg(s + e)) << (16 * (e & 1));
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
 };
-
-// rows_pad rows of panels at dst: row r is token (first + r) / pack of the window, zeros from
-// `rows` on and from dim to the next 16 columns.
-template <typename T, int THREADS = kRows>
-__device__ __forceinline__ void load_panel(uint32_t dst, int panel_rows, const Operand<T>& o, int64_t token0, int head0,
-                                           int pack, int first, int rows, int rows_pad, int dim) {
-    const int chunks = ((dim + 15) / 16) * 2;
-    const uint32_t inv = (65536u + chunks - 1) / chunks;  // i / chunks for i < 2048
-    for (int i = threadIdx.x; i < rows_pad * chunks; i += THREADS) {
-        const int r = static_cast<int>((static_cast<uint32_t>(i) * inv) >> 16), c = i - r * chunks;
-        int64_t token = token0;
-        int head = head0;
-        if (pack == 1) {
-            token += first + r;
-        } else {
-            token += (first + r) / pack;
-            head += (first + r) % pack;
-        }
-        const uint32_t to = dst + (c >> 3) * panel_rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        const bool live = r < rows && c * 8 < dim;
-        const T* from = o.p + (live ? token * o.st + head * o.sh + c * 8 : 0);
-        if (o.vec) {
-            tc::cp_async16(to, from, live);
-        } else {
-            uint32_t w[4] = {0, 0, 0, 0};
-            if (live) {
-                const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(s[e]) << (16 * (e & 1));
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        }
-    }
-}
 
 // ---- bias of a tile ----------------------------------------------------------------
 // How the entries of a tile of queries x keys are found. Most tiles need no clamping: windows
@@ -165,17 +185,17 @@ __device__ __forceinline__ void stage16(uint32_t dst, int r, const float* o, int
 template <typename T, int THREADS>
 __device__ __forceinline__ void store_panel(uint32_t src0, void* out, int heads, int dim, int64_t token0, int head0, int pack,
                                             int first, int rows) {
-    const int chunks = (dim + 7) / 8;
-    const uint32_t inv = (65536u + chunks - 1) / chunks;
+    const int chunks = (dim + 7) / 8, shift = chunks > 1 ? 32 - __clz(chunks - 1) : 0;
+    const int c = threadIdx.x & ((1 << shift) - 1), step = THREADS >> shift;
+    if (c >= chunks) return;
     const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && dim % 8 == 0;
-    for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {
-        const int r = static_cast<int>((static_cast<uint32_t>(i) * inv) >> 16), c = i - r * chunks;
-        const int64_t token = token0 + (pack == 1 ? first + r : (first + r) / pack);
-        const int head = head0 + (pack == 1 ? 0 : (first + r) % pack);
+    for (int r = threadIdx.x >> shift; r < rows; r += step) {
+        const int64_t row = pack == 1 ? (token0 + first + r) * heads + head0
+                                      : (token0 + (first + r) / pack) * heads + head0 + (first + r) % pack;
         const uint32_t src = src0 + (c >> 3) * kRows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         uint32_t w[4];
         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src));
-        unsigned short* dst = static_cast<unsigned short*>(out) + (token * heads + head) * dim + c * 8;
+        unsigned short* dst = static_cast<unsigned short*>(out) + row * dim + c * 8;
         if (vec) {
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {

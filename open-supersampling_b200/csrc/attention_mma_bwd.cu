@@ -171,9 +171,9 @@ __device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim,
 
 // Scores and dP of a thread's 64 keys from tensor memory, and the weights: s becomes p, dp stays.
 // Zero where the mask is, whatever stands there.
-template <int KT>
+template <int KT, bool BIAS>
 __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], float (&dp)[64], uint32_t ts, uint32_t tdp, int n16,
-                                        int j0, bool whole, int see, float lse, BiasMode mode, const float* E, bool biased,
+                                        int j0, bool whole, int see, float lse, BiasMode mode, const float* E,
                                         const KeyPos<KT>* kp, int2 qp) {
     const float c2 = p.scale * kLog2e;
 #pragma unroll
@@ -181,33 +181,42 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], flo
         if (j0 + c < n16) {
             tc::tmem_ld16(ts + j0 + c, s + c);
             tc::tmem_ld16(tdp + j0 + c, dp + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[c + i] = dp[c + i] = 0.0f;
         }
     }
     tc::wait_ld();
+    const float2 by = make_float2(BIAS ? 1.0f : c2, BIAS ? 1.0f : c2), off = make_float2(-lse, -lse);
 #pragma unroll
     for (int c = 0; c < 64; c += 16) {
-        float(&x)[16] = *reinterpret_cast<float(*)[16]>(s + c);
-        if (j0 + c >= n16) {
+        if (j0 + c >= n16) continue;
+        if constexpr (BIAS) add_bias<KT, 16>(*reinterpret_cast<float(*)[16]>(s + c), c2, p.bias, mode, E, kp, j0 + c, qp);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = dp[c + i] = 0.0f;
-            continue;
+        for (int i = 0; i < 16; i += 2) {
+            const float2 x = make_float2(s[c + i], s[c + i + 1]), y = BIAS ? __fadd2_rn(x, off) : __ffma2_rn(x, by, off);
+            s[c + i] = ex2(y.x);
+            s[c + i + 1] = ex2(y.y);
         }
-        if (biased) {
-            add_bias<KT, 16>(x, c2, p.bias, mode, E, kp, j0 + c, qp);
+    }
+    if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = ex2(x[i] - lse);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], c2, -lse));
+        for (int c = 0; c < 64; ++c) {
+            const bool on = j0 + c < see;
+            s[c] = on ? s[c] : 0.0f;
+            dp[c] = on ? dp[c] : 0.0f;
         }
-        if (!whole) {
+    }
+}
+
+// dp becomes p (dp - delta).
+__device__ __forceinline__ void score_gradients(const float (&s)[64], float (&dp)[64], float delta) {
+    const float2 off = make_float2(-delta, -delta);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool on = j0 + c + i < see;
-                x[i] = on ? x[i] : 0.0f;
-                dp[c + i] = on ? dp[c + i] : 0.0f;
-            }
-        }
+    for (int c = 0; c < 64; c += 2) {
+        const float2 d = __fmul2_rn(make_float2(s[c], s[c + 1]), __fadd2_rn(make_float2(dp[c], dp[c + 1]), off));
+        dp[c] = d.x;
+        dp[c + 1] = d.y;
     }
 }
 
@@ -329,7 +338,7 @@ struct ShortSmem {
     static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<kShortKeys>)) + 64 + 64 + 32;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(const __grid_constant__ AttnParams p) {
     using L = ShortSmem<DP>;
     constexpr int kCols = DP == 64 ? 256 : 512, KT = kShortKeys;
@@ -342,8 +351,8 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
     float* wsize = reinterpret_cast<float*>(slot_tmem + 4);
     float* wsum = wsize + 4;
-    const int group = p.heads / p.kv_heads, entries = bias_entries(p.bias), kvh = blockIdx.y;
-    const bool grad_bias = p.bias_part != nullptr;
+    const int group = p.heads / p.kv_heads, entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y;
+    const bool grad_bias = BIAS && p.bias_part != nullptr;
     double* acc = reinterpret_cast<double*>(base + L::kBytes);
     int* I = reinterpret_cast<int*>(acc + (grad_bias ? group * entries : 0));
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
@@ -351,14 +360,15 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
 
     const int tid = threadIdx.x, warp = tid >> 5, z = blockIdx.z;
     const int dim16 = (p.dim + 15) & ~15;
-    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
-        og(p.dout, p.do_st, p.do_sh, p.dim);
+    const Loader<T, kRows> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
+        oq(p.q, p.q_st, p.q_sh, p.dim, kvh * group), og(p.dout, p.do_st, p.do_sh, p.dim, kvh * group);
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
         tc::mbar_init_fence();
     }
     if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
+    if constexpr (BIAS)
     for (int e = tid; e < entries * group; e += kRows) {
         E[e] = bias_entry(p.bias, p.heads, kvh * group + e / entries, e % entries);
         if (grad_bias) acc[e] = 0.0;
@@ -416,22 +426,22 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
         // Q, dO and the row's scalars of one tile
         auto fetch = [&](int it) {
             const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
-            load_panel<T>(sq, kRows, oq, q0, head, 1, first, rows, kRows, p.dim);
-            load_panel<T>(sg, kRows, og, q0, head, 1, first, rows, kRows, p.dim);
+            oq.load(sq, kRows, q0 + first, rows, kRows, (it / qtiles) * p.q_sh);
+            og.load(sg, kRows, q0 + first, rows, kRows, (it / qtiles) * p.do_sh);
             tc::cp_async_commit();
             lse = tid < rows ? p.lse[static_cast<int64_t>(head) * p.tq + q0 + first + tid] : INFINITY;
-            if (entries > 0) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(tid, rows - 1));
+            if (BIAS) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(tid, rows - 1));
         };
         __syncthreads();  // the window before has read its keys
         if (i0 < i1) {
-            load_panel<T>(sk, KT, ok, k0, kvh, 1, 0, n, n16, p.dim);
-            load_panel<T>(sv, KT, ov, k0, kvh, 1, 0, n, n16, p.dim);
+            ok.load(sk, KT, k0, n, n16);
+            ov.load(sv, KT, k0, n, n16);
             fetch(i0);
-            if (entries > 0) load_key_pos<KT>(kp, p.bias, k0, n);
+            if (BIAS) load_key_pos<KT>(kp, p.bias, k0, n);
         }
         for (int it = i0; it < i1; ++it) {
             const int g = it / qtiles, head = kvh * group + g, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
-            if (entries > 0) {
+            if (BIAS) {
                 const Range r = warp_range(qp);
                 if ((tid & 31) == 0) qrange[warp] = r;
             }
@@ -442,25 +452,28 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             if (tid == 0) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
-                tc::mma_nt(tmem, sq, kRows, sk, KT, dim16, id);
-                tc::mma_nt(tmem + KT, sg, kRows, sv, KT, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv, dim16, id);
                 tc::commit(bar_s);
             }
             const int see = tid >= rows ? 0 : p.causal ? min(max(first + tid + lk - lq + 1, 0), lk) : lk;
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= n);
             BiasMode mode = kOne;
-            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[64], dp[64];
-            weights<KT>(p, s, dp, ts, ts + KT, n16, 0, whole, see, lse, mode, E + g * entries, entries > 0, kp, qp);
-            float delta = 0.0f;
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, 0, whole, see, lse, mode, E + g * entries, kp, qp);
+            float2 d0 = make_float2(0.0f, 0.0f), d1 = d0;
 #pragma unroll
-            for (int c = 0; c < 64; ++c) delta = fmaf(s[c], dp[c], delta);
+            for (int c = 0; c < 64; c += 4) {
+                d0 = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(dp[c], dp[c + 1]), d0);
+                d1 = __ffma2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(dp[c + 2], dp[c + 3]), d1);
+            }
+            const float delta = (d0.x + d0.y) + (d1.x + d1.y);
             write_row<T>(sp, tid, s, 1.0f);
-#pragma unroll
-            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            score_gradients(s, dp, delta);
             write_row<T>(sd, tid, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
@@ -472,12 +485,12 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after();
-                for (int k = 0; k < kRows; k += 16) {
-                    tc::mma_ss(tmem + t_dv, tc::desc(sp + k * 128, L::kP), tc::desc(sg + k * 128, kRows * 128), id_grad, it > i0 || k > 0);
-                    tc::mma_ss(tmem + t_dk, tc::desc(sd + k * 128, L::kP), tc::desc(sq + k * 128, kRows * 128), id_grad, it > i0 || k > 0);
-                }
-                for (int k = 0; k < n16; k += 16)
-                    tc::mma_ss(tmem, tc::desc(sd + k * 2, 16), tc::desc(sk + k * 128, KT * 128), id_q, k > 0);
+                tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, L::kP), tc::desc(sg, kRows * 128), id_grad, it > i0);
+                tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, L::kP), tc::desc(sq, kRows * 128), id_grad, it > i0);
+                const uint64_t dd = tc::desc(sd, 16), dk = tc::desc(sk, KT * 128);
+#pragma unroll
+                for (int k = 0; k < KT; k += 16)
+                    if (k < n16) tc::mma_ss(tmem, dd + k * 2 / 16, dk + k * 128 / 16, id_q, k > 0);
                 tc::commit(bar_o);
             }
             BiasSum bs{kOne, 0.0f, false};
@@ -515,7 +528,7 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
         }
         tc::fence_before();
     }
-    if (grad_bias) {
+    if constexpr (BIAS) if (grad_bias) {
         __syncthreads();
         for (int e = tid; e < entries * group; e += kRows)
             p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * (p.bias_short + p.bias_long) + z * gridDim.x + blockIdx.x) * entries +
@@ -537,7 +550,7 @@ struct LongSmem {
     static constexpr int kDkv = 2 * kT + 2 * kBuf * kT + 2 * kP;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_constant__ AttnParams p) {
     if (*p.flags == 0) return;
     using L = LongSmem<DP>;
@@ -551,8 +564,8 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
     float* wsize = reinterpret_cast<float*>(bars + 8);
     float* wsum = wsize + 8;
-    const int entries = bias_entries(p.bias), head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
-    const bool grad_bias = p.bias_part != nullptr;
+    const int entries = BIAS ? bias_entries(p.bias) : 0, head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
+    const bool grad_bias = BIAS && p.bias_part != nullptr;
     double* acc = reinterpret_cast<double*>(base + L::kDq + L::kMisc);
     int* I = reinterpret_cast<int*>(acc + (grad_bias ? entries : 0));
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
@@ -560,8 +573,8 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
 
     const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tq, p.windows, kRows);
-    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
-        og(p.dout, p.do_st, p.do_sh, p.dim);
+    const Loader<T, kThreads> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
+        oq(p.q, p.q_st, p.q_sh, p.dim, head), og(p.dout, p.do_st, p.do_sh, p.dim, head);
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
@@ -581,9 +594,10 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     int par_s = 0, par_o = 0;
     bool alive = true;
 
-    for (int it = blockIdx.x; it < slots; it += gridDim.x) {
-        AttnTile t;
-        if (!attn_tile(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, p.causal ? slots - 1 - it : it, t)) continue;
+    const int chunk = (slots + gridDim.x - 1) / gridDim.x, slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
+    AttnWalk walk;
+    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, slot0, min(slots, slot0 + chunk)); more; more = walk.next()) {
+        const AttnTile& t = walk.tile;
         if (t.window < 0 || t.olen <= p.short_max) continue;
         const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
         const bool live = row < rows;
@@ -597,16 +611,16 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
         const int2 qp = entries > 0 ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0);
         auto fetch = [&](int kt) {
             const int b = kBuf == 2 ? kt & 1 : 0, n = min(KT, most - kt * KT), n16 = (n + 15) & ~15;
-            load_panel<T, kThreads>(sk + b * L::kT, KT, ok, t.obegin + kt * KT, kvh, 1, 0, n, n16, p.dim);
-            load_panel<T, kThreads>(sv + b * L::kT, KT, ov, t.obegin + kt * KT, kvh, 1, 0, n, n16, p.dim);
-            if (entries > 0) load_key_pos<KT>(kps + b, p.bias, t.obegin + kt * KT, n);
+            ok.load(sk + b * L::kT, KT, t.obegin + kt * KT, n, n16);
+            ov.load(sv + b * L::kT, KT, t.obegin + kt * KT, n, n16);
+            if (BIAS) load_key_pos<KT>(kps + b, p.bias, t.obegin + kt * KT, n);
         };
         __syncthreads();  // the tile before has been read
         if (tiles > 0) {
-            load_panel<T, kThreads>(sq, kRows, oq, t.begin, head, 1, t.first, rows, kRows, p.dim);
-            load_panel<T, kThreads>(sg, kRows, og, t.begin, head, 1, t.first, rows, kRows, p.dim);
+            oq.load(sq, kRows, t.begin + t.first, rows, kRows);
+            og.load(sg, kRows, t.begin + t.first, rows, kRows);
             fetch(0);
-            if (entries > 0) {
+            if (BIAS) {
                 const Range r = warp_range(qp);
                 if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
             }
@@ -623,8 +637,8 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
             if (tid == 0) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
-                tc::mma_nt(tmem, sq, kRows, sk + b * L::kT, KT, dim16, id);
-                tc::mma_nt(tmem + KT, sg, kRows, sv + b * L::kT, KT, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk + b * L::kT, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv + b * L::kT, dim16, id);
                 tc::commit(bar_s);
             }
             if (grad_bias && kt > 0 && (bs.fixed != 0.0f || bs.bad))  // of the tile before
@@ -639,14 +653,13 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
                 tc::cp_async_commit();
             }
             BiasMode mode = kOne;
-            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[64], dp[64];
-            weights<KT>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, entries > 0, kp, qp);
-#pragma unroll
-            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, kp, qp);
+            score_gradients(s, dp, delta);
             write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
@@ -657,9 +670,11 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after();
-                for (int k = 0; k < n16; k += 16)
-                    tc::mma_ss(tmem + 2 * KT, tc::desc(sd + (k >> 6) * kRows * 128 + (k & 63) * 2, 16),
-                               tc::desc(sk + b * L::kT + k * 128, KT * 128), id_q, kt > 0 || k > 0);
+                const uint64_t dd = tc::desc(sd, 16), dk = tc::desc(sk + b * L::kT, KT * 128);
+#pragma unroll
+                for (int k = 0; k < KT; k += 16)
+                    if (k < n16)
+                        tc::mma_ss(tmem + 2 * KT, dd + ((k >> 6) * kRows * 128 + (k & 63) * 2) / 16, dk + k * 128 / 16, id_q, kt > 0 || k > 0);
                 tc::commit(bar_o);
             }
             if (grad_bias) {
@@ -675,7 +690,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
                         if (bs.fixed != 0.0f || bs.bad) bias_join<kThreads, 8, KT>(p, bs, entries, head, kp, qp, I, wsum, acc);
                         bs = BiasSum{kOne, 0.0f, false};
                         __syncthreads();
-                    } else if (entries > 0) {
+                    } else if (BIAS) {
                         __syncthreads();
                     }
                     fetch(kt + 1);
@@ -726,7 +741,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
 }
 
 // ---- long windows: dk, dv --------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
     if (*p.flags == 0) return;
     using L = LongSmem<DP>;
@@ -739,14 +754,14 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
     Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of both buffers' queries: 4 warps each, written in turn
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
-    const int entries = bias_entries(p.bias), kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
+    const int entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
     float* E = reinterpret_cast<float*>(base + L::kDkv + L::kMisc);
     const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
 
     const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tk, p.windows, KT);
-    const Operand<T> oq(p.q, p.q_st, p.q_sh, p.dim), ok(p.k, p.k_st, p.k_sh, p.dim), ov(p.v, p.v_st, p.v_sh, p.dim),
-        og(p.dout, p.do_st, p.do_sh, p.dim);
+    const Loader<T, kThreads> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
+        oq(p.q, p.q_st, p.q_sh, p.dim, kvh * group), og(p.dout, p.do_st, p.do_sh, p.dim, kvh * group);
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
@@ -763,9 +778,10 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
 
-    for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
-        AttnTile t;
-        if (!attn_tile(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, slot, t)) continue;
+    const int chunk = (slots + gridDim.x - 1) / gridDim.x, slot0 = blockIdx.x * chunk;
+    AttnWalk walk;
+    for (bool more = walk.start(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, slot0, min(slots, slot0 + chunk)); more; more = walk.next()) {
+        const AttnTile& t = walk.tile;
         if (t.window < 0 || t.len <= p.short_max) continue;
         const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
@@ -774,18 +790,18 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
         const int qt0 = p.causal ? min(max(t.first - (lk - lq), 0) / kRows, qtiles) : 0;
         auto next = [&](int it) { return it < i1 && it % qtiles < qt0 ? it - it % qtiles + qt0 : it; };
         auto fetch = [&](int it, int b) {
-            const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
-            load_panel<T, kThreads>(sq + b * L::kT, kRows, oq, t.obegin, head, 1, first, rows, kRows, p.dim);
-            load_panel<T, kThreads>(sg + b * L::kT, kRows, og, t.obegin, head, 1, first, rows, kRows, p.dim);
+            const int first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
+            oq.load(sq + b * L::kT, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.q_sh);
+            og.load(sg + b * L::kT, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.do_sh);
         };
         __syncthreads();
         int it = next(i0), b = 0;
         const bool any = it < i1;
         if (any) {
-            load_panel<T, kThreads>(sk, KT, ok, t.begin, kvh, 1, t.first, n, n16, p.dim);
-            load_panel<T, kThreads>(sv, KT, ov, t.begin, kvh, 1, t.first, n, n16, p.dim);
+            ok.load(sk, KT, t.begin + t.first, n, n16);
+            ov.load(sv, KT, t.begin + t.first, n, n16);
             fetch(it, 0);
-            if (entries > 0) load_key_pos<KT>(kp, p.bias, t.begin + t.first, n);
+            if (BIAS) load_key_pos<KT>(kp, p.bias, t.begin + t.first, n);
         }
         tc::cp_async_commit();
         bool begun = false;
@@ -797,7 +813,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
             const float lse = live ? p.lse[static_cast<int64_t>(head) * p.tq + token] : INFINITY;
             const float delta = live ? p.delta[static_cast<int64_t>(head) * p.tq + token] : 0.0f;
             int2 qp = make_int2(0, 0);
-            if (entries > 0) {
+            if (BIAS) {
                 qp = bias_pos(p.bias.q_pos, p.bias.axes, token);
                 const Range r = warp_range(qp);
                 if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
@@ -812,8 +828,8 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
             if (tid == 0) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
-                tc::mma_nt(tmem, sq + b * L::kT, kRows, sk, KT, dim16, id);
-                tc::mma_nt(tmem + KT, sg + b * L::kT, kRows, sv, KT, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem, sq + b * L::kT, sk, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg + b * L::kT, sv, dim16, id);
                 tc::commit(bar_s);
             }
             if (kBuf == 2) {
@@ -827,25 +843,22 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
             const int see = !live ? 0 : p.causal ? min(max(first + row + lk - lq + 1, 0), lk) : lk;
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= t.first + n);
             BiasMode mode = kOne;
-            if (entries > 0) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[64], dp[64];
-            weights<KT>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, lse, mode, E, entries > 0, kp, qp);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, lse, mode, E, kp, qp);
             write_row<T>(sp + (j0 >> 6) * kRows * 128, row, s, 1.0f);
-#pragma unroll
-            for (int c = 0; c < 64; ++c) dp[c] = s[c] * (dp[c] - delta);
+            score_gradients(s, dp, delta);
             write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after();
-                for (int k = 0; k < kRows; k += 16) {
-                    tc::mma_ss(tmem + t_dv, tc::desc(sp + k * 128, kRows * 128), tc::desc(sg + b * L::kT + k * 128, kRows * 128), id_grad, begun || k > 0);
-                    tc::mma_ss(tmem + t_dk, tc::desc(sd + k * 128, kRows * 128), tc::desc(sq + b * L::kT + k * 128, kRows * 128), id_grad, begun || k > 0);
-                }
+                tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, kRows * 128), tc::desc(sg + b * L::kT, kRows * 128), id_grad, begun);
+                tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, kRows * 128), tc::desc(sq + b * L::kT, kRows * 128), id_grad, begun);
                 tc::commit(bar_o);
             }
             if (kBuf == 1) {
@@ -935,31 +948,28 @@ cudaError_t smem_of(K kernel, int bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool BIAS>
 cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
     const int entries = bias_entries(p.bias), group = p.heads / p.kv_heads, sum = p.bias_part != nullptr;
     cudaError_t err;
     const int b_short = 1024 + ShortSmem<DP>::kBytes + entries * group * (4 + 8 * sum) + entries * 4 * sum;
     if (p.short_max == 0) {
         // only rows and windows without partners: no bias is looked up
-        AttnParams none = p;
-        none.bias.table = nullptr;
-        none.bias_part = nullptr;
         const int bytes = 1024 + ShortSmem<DP>::kBytes;
-        if ((err = smem_of(k_attn_bwd_short<T, DP>, bytes)) != cudaSuccess) return err;
-        k_attn_bwd_short<T, DP><<<dim3(p.short_blocks, p.kv_heads, 1), kRows, bytes, s>>>(none);
+        if ((err = smem_of(k_attn_bwd_short<T, DP, false>, bytes)) != cudaSuccess) return err;
+        k_attn_bwd_short<T, DP, false><<<dim3(p.short_blocks, p.kv_heads, 1), kRows, bytes, s>>>(p);
     } else {
-        if ((err = smem_of(k_attn_bwd_short<T, DP>, b_short)) != cudaSuccess) return err;
-        k_attn_bwd_short<T, DP><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), kRows, b_short, s>>>(p);
+        if ((err = smem_of(k_attn_bwd_short<T, DP, BIAS>, b_short)) != cudaSuccess) return err;
+        k_attn_bwd_short<T, DP, BIAS><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), kRows, b_short, s>>>(p);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int b_dq = 1024 + LongSmem<DP>::kDq + LongSmem<DP>::kMisc + entries * (4 + 12 * sum);
-    if ((err = smem_of(k_attn_dq_long<T, DP>, b_dq)) != cudaSuccess) return err;
-    k_attn_dq_long<T, DP><<<dim3(p.dq_blocks, p.heads), 2 * kRows, b_dq, s>>>(p);
+    if ((err = smem_of(k_attn_dq_long<T, DP, BIAS>, b_dq)) != cudaSuccess) return err;
+    k_attn_dq_long<T, DP, BIAS><<<dim3(p.dq_blocks, p.heads), 2 * kRows, b_dq, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int b_kv = 1024 + LongSmem<DP>::kDkv + LongSmem<DP>::kMisc + entries * 4;
-    if ((err = smem_of(k_attn_dkv_long<T, DP>, b_kv)) != cudaSuccess) return err;
-    k_attn_dkv_long<T, DP><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_kv, s>>>(p);
+    if ((err = smem_of(k_attn_dkv_long<T, DP, BIAS>, b_kv)) != cudaSuccess) return err;
+    k_attn_dkv_long<T, DP, BIAS><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_kv, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     if (p.qsplits > 1) {
         const int64_t n = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
@@ -975,6 +985,12 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
     return err;
 }
 
+template <typename T>
+cudaError_t bwd_type(const AttnParams& p, void* dtable, cudaStream_t s) {
+    if (p.bias.table != nullptr) return p.dim <= 64 ? bwd_one<T, 64, true>(p, dtable, s) : bwd_one<T, 128, true>(p, dtable, s);
+    return p.dim <= 64 ? bwd_one<T, 64, false>(p, dtable, s) : bwd_one<T, 128, false>(p, dtable, s);
+}
+
 }  // namespace
 
 cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
@@ -982,8 +998,7 @@ cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     if ((err = launch_attn_delta(p, type, sms, s)) != cudaSuccess) return err;
-    if (type == kBF16) return p.dim <= 64 ? bwd_one<__nv_bfloat16, 64>(p, dtable, s) : bwd_one<__nv_bfloat16, 128>(p, dtable, s);
-    return p.dim <= 64 ? bwd_one<__half, 64>(p, dtable, s) : bwd_one<__half, 128>(p, dtable, s);
+    return type == kBF16 ? bwd_type<__nv_bfloat16>(p, dtable, s) : bwd_type<__half>(p, dtable, s);
 }
 
 cudaError_t attn_timeouts_bwd(unsigned int* count) {

@@ -36,9 +36,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, int parity) {
 }
 
 // ---- cp.async ----------------------------------------------------------------
-// 16 bytes, zeros where !live.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -117,16 +116,29 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// a b^T over dim16 columns: both K-major panels of `rows_a` and `rows_b` rows.
-__device__ __forceinline__ void mma_nt(uint32_t d, uint32_t a, int rows_a, uint32_t b, int rows_b, int dim16, uint32_t id) {
-    for (int k = 0; k < dim16; k += 16) {
-        const uint32_t at = static_cast<uint32_t>(k & 63) * 2;
-        mma_ss(d, desc(a + (k >> 6) * rows_a * 128 + at, 16), desc(b + (k >> 6) * rows_b * 128 + at, 16), id, k > 0);
-    }
+// a b^T over dim16 <= DP columns: both K-major panels of ROWS_A and ROWS_B rows.
+template <int DP, int ROWS_A, int ROWS_B>
+__device__ __forceinline__ void mma_nt(uint32_t d, uint32_t a, uint32_t b, int dim16, uint32_t id) {
+    const uint64_t da = desc(a, 16), db = desc(b, 16);
+#pragma unroll
+    for (int k = 0; k < DP; k += 16)
+        if (k < dim16)
+            mma_ss(d, da + ((k >> 6) * ROWS_A * 128 + (k & 63) * 2) / 16, db + ((k >> 6) * ROWS_B * 128 + (k & 63) * 2) / 16, id, k > 0);
 }
-// a b over k16 rows of b, a in tensor memory (two 16-bit values a column).
-__device__ __forceinline__ void mma_tn(uint32_t d, uint32_t a, uint32_t b, int rows_b, int k16, uint32_t id, bool add) {
-    for (int k = 0; k < k16; k += 16) mma_ts(d, a + k / 2, desc(b + k * 128, rows_b * 128), id, add || k > 0);
+// a b over k16 <= K rows of b (MN-major panels of K rows), a in tensor memory (two 16-bit values a column).
+template <int K>
+__device__ __forceinline__ void mma_tn(uint32_t d, uint32_t a, uint32_t b, int k16, uint32_t id, bool add) {
+    const uint64_t db = desc(b, K * 128);
+#pragma unroll
+    for (int k = 0; k < K; k += 16)
+        if (k < k16) mma_ts(d, a + k / 2, db + k * 128 / 16, id, add || k > 0);
+}
+
+// a^T b over K rows of MN-major panels, given their descriptors.
+template <int K>
+__device__ __forceinline__ void mma_tt(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
+#pragma unroll
+    for (int k = 0; k < K; k += 16) mma_ss(d, a + k * 128 / 16, b + k * 128 / 16, id, add || k > 0);
 }
 
 }  // namespace tc
