@@ -676,7 +676,7 @@ OSS_API int oss_window_attention_timeouts(uint32_t* count);
 /* buckets: rows of the table whose gradient is wanted, else 0; 0 bytes where an argument is out of range. */
 OSS_API int64_t oss_window_attention_backward_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows,
                                                             int64_t heads, int64_t kv_heads, int64_t dim,
-                                                            int64_t entries, int64_t buckets);
+                                                            int32_t causal, int64_t entries, int64_t buckets);
 /* d_table[buckets][heads] in the table's dtype, null: not wanted.  Every gradient is the same
  * on every run: sums have a fixed order, those of d_table are 64-bit integers. */
 OSS_API int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,

@@ -47,6 +47,7 @@ struct AttnParams {
     AttnBias bias;
     void* out;        // [tq][heads][dim]
     float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
+    int tiny_max;     // windows of 1 to so many keys go to the warp-level kernels (attention_tiny.cu)
     // forward only
     int pack;         // query heads of one key head that share a tile's rows (1 or the group)
     int splits;       // parts that a window's keys are cut into
@@ -63,12 +64,15 @@ struct AttnParams {
     // backward of 16-bit types only
     int short_max;      // windows of up to so many keys go to the kernel for short windows
     int qsplits;        // parts that the queries of a tile of keys are cut into
-    int short_blocks, dq_blocks, dkv_blocks;  // blocks for each (key) head of the three kernels
-    int* flags;         // [0]: nonzero where some window has more than short_max keys
+    int tiny_blocks, short_blocks, dq_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
+    int* flags;         // [0]: kSomeLong, kSomeShort
     float *part_dk, *part_dv;    // [qsplits][tk][kv_heads][dim], qsplits > 1 only
-    double* bias_part;           // [heads][bias_short + bias_long][entries]; null: no gradient of the table
-    int bias_short, bias_long;   // blocks of a head that sum the bias gradient, of short windows and of others
+    double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
+    int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them
 };
+
+constexpr int kSomeLong = 1;   // a window with more than short_max keys
+constexpr int kSomeShort = 2;  // one with more than tiny_max, up to short_max
 
 __host__ __device__ __forceinline__ int bias_entries(const AttnBias& b) {
     return b.table == nullptr ? 0 : (2 * b.ry + 1) * (2 * b.rx + 1);
@@ -134,13 +138,15 @@ __device__ __forceinline__ bool attn_tile(const int32_t* off, int t, const int32
 struct AttnWalk {
     const int32_t *off, *other;
     int t, ot, windows, per, rows;
+    int skip;  // windows with 1 to `skip` tokens on the other side are passed by
     int slot, end, w;
     AttnTile tile;
 
     // Called by whole warps. False: no tile.
     __device__ __forceinline__ bool start(const int32_t* off_, int t_, const int32_t* other_, int ot_, int windows_, int per_,
-                                          int rows_, int slot_, int end_) {
+                                          int rows_, int slot_, int end_, int skip_ = 0) {
         off = off_, t = t_, other = other_, ot = ot_, windows = windows_, per = per_, rows = rows_, slot = slot_, end = end_;
+        skip = skip_;
         const int lane = threadIdx.x & 31;
         int lo = 0, hi = windows + 2;
         while (hi - lo > 1) {
@@ -177,12 +183,28 @@ struct AttnWalk {
     __device__ __forceinline__ bool settle() {
         while (slot < end) {
             const int64_t first = static_cast<int64_t>(slot - slot_of(w)) * rows;
-            if (first >= 0 && first < static_cast<int64_t>(tile.len) * per) {
+            if (first >= 0 && first < static_cast<int64_t>(tile.len) * per && (tile.olen == 0 || tile.olen > skip)) {
                 tile.first = static_cast<int>(first);
                 return true;
             }
-            if (w >= windows + 1) return false;
-            enter(w + 1);
+            // the next window to stop at, 32 at a time
+            const int lane = threadIdx.x & 31;
+            int at = w + 1;
+            for (;; at += 32) {
+                const int c = at + lane;
+                bool stop = c > windows + 1;
+                if (!stop) {
+                    const int n = c >= 1 && c <= windows ? attn_offset(other, windows, ot, c + 1) - attn_offset(other, windows, ot, c) : 0;
+                    stop = attn_offset(off, windows, t, c + 1) > attn_offset(off, windows, t, c) && (n <= 0 || n > skip);
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, stop);
+                if (hit != 0u) {
+                    at += __ffs(hit) - 1;
+                    break;
+                }
+            }
+            if (at > windows + 1) return false;
+            enter(at);
             slot = max(slot, slot_of(w));
         }
         return false;
@@ -293,6 +315,10 @@ cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, in
 cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s);
 // attention_mma.cu, attention_mma_bwd.cu: bf16 and fp16, the forward without the join of split keys.
 cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s);
+// Windows of 1 to p.tiny_max keys, not causal, dim <= 64 (backward: 32, p.tiny_max <= 32).
+cudaError_t launch_attn_forward_tiny(const AttnParams& p, int type, cudaStream_t s);
+cudaError_t launch_attn_backward_tiny(const AttnParams& p, int type, cudaStream_t s);
+int attn_tiny_backward_blocks(const AttnParams& p);
 cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
 // Waits of the tensor-core kernels that ran out of their limit since the library was loaded.
 cudaError_t attn_timeouts(unsigned int* count);

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
     // causal windows: the last tiles see the most keys and go first
     const int slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
     AttnWalk walk;
-    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk)); more;
+    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk), p.tiny_max); more;
          more = walk.next()) {
         const AttnTile& t = walk.tile;
         const int rows = min(kRows, t.len * p.pack - t.first);

@@ -33,6 +33,7 @@ struct Loader {
     int dim, c, r0, step, shift;
     bool on, zero;  // on: the chunk belongs to the 16-column steps; zero: it lies past dim
     bool vec;       // every row starts on 16 bytes and ends on them
+    bool pairs;     // on 4 bytes
 
     __device__ __forceinline__ Loader(const void* q, int64_t st_, int64_t sh, int dim_, int head) : st(st_), dim(dim_) {
         const int chunks = ((dim + 15) / 16) * 2;
@@ -44,6 +45,7 @@ struct Loader {
         zero = c * 8 >= dim;
         p = static_cast<const T*>(q) + head * sh + (zero ? 0 : c * 8);
         vec = ((reinterpret_cast<uintptr_t>(q) & 15) | ((st_ | sh | dim) & 7)) == 0;
+        pairs = ((reinterpret_cast<uintptr_t>(q) & 3) | ((st_ | sh | dim) & 1)) == 0;
     }
     __device__ __forceinline__ uint32_t place(uint32_t dst, int panel_rows) const {
         return dst + (c >> 3) * panel_rows * 128 + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
@@ -83,10 +85,16 @@ struct Loader {
     }
     __device__ __forceinline__ void store_some(uint32_t to, const T* from) const {
         uint32_t w[4] = {0, 0, 0, 0};
-        const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
+        if (pairs) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(__ldg(s + e)) << (16 * (e & 1));
+            for (int e = 0; e < 4; ++e)
+                if (c * 8 + 2 * e < dim) w[e] = __ldg(reinterpret_cast<const uint32_t*>(from) + e);
+        } else {
+            const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(__ldg(s + e)) << (16 * (e & 1));
+        }
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
 };
@@ -189,6 +197,7 @@ __device__ __forceinline__ void store_panel(uint32_t src0, void* out, int heads,
     const int c = threadIdx.x & ((1 << shift) - 1), step = THREADS >> shift;
     if (c >= chunks) return;
     const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && dim % 8 == 0;
+    const bool pairs = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && dim % 2 == 0;
     for (int r = threadIdx.x >> shift; r < rows; r += step) {
         const int64_t row = pack == 1 ? (token0 + first + r) * heads + head0
                                       : (token0 + (first + r) / pack) * heads + head0 + (first + r) % pack;
@@ -198,6 +207,10 @@ __device__ __forceinline__ void store_panel(uint32_t src0, void* out, int heads,
         unsigned short* dst = static_cast<unsigned short*>(out) + row * dim + c * 8;
         if (vec) {
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if (pairs) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c * 8 + 2 * e < dim) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -215,6 +228,18 @@ __device__ __forceinline__ void write_part(float* to, const float* o, int c, int
         for (int i = 0; i < 16; ++i)
             if (c + i < dim) to[c + i] = o[i];
     }
+}
+
+template <typename T>
+constexpr int kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+
+// Power of two that dS is kept times.
+template <typename T>
+__device__ __forceinline__ float ds_scale(const AttnParams& p) {
+    if constexpr (kIsBf16<T>) return 1.0f;
+    const float bound = 2.0f * p.dim * __uint_as_float(p.bias_max[0]) * __uint_as_float(p.bias_max[1]);
+    if (!(bound > 0.0f)) return 1.0f;
+    return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
 }  // namespace

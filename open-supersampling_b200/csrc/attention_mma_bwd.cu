@@ -27,18 +27,6 @@ namespace {
 
 constexpr int kShortKeys = 64;
 
-template <typename T>
-constexpr int kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-
-// Power of two that dS is kept times.
-template <typename T>
-__device__ __forceinline__ float ds_scale(const AttnParams& p) {
-    if constexpr (kIsBf16<T>) return 1.0f;
-    const float bound = 2.0f * p.dim * __uint_as_float(p.bias_max[0]) * __uint_as_float(p.bias_max[1]);
-    if (!(bound > 0.0f)) return 1.0f;
-    return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
-}
-
 struct BiasSum {      // of a tile, uniform over the block
     BiasMode mode;
     float fixed;      // 0: nothing to add
@@ -320,12 +308,14 @@ __device__ __forceinline__ void finish_key_row(const AttnParams& p, uint32_t at,
 }
 
 // ---- which windows there are -----------------------------------------------------------------
-// flags[0]: some window has more than short_max keys.
 __global__ void __launch_bounds__(256) k_attn_flags(AttnParams p, int* flags) {
-    bool longer = false;
-    for (int w = blockIdx.x * 256 + threadIdx.x; w < p.windows; w += gridDim.x * 256)
-        longer |= attn_offset(p.k_off, p.windows, p.tk, w + 2) - attn_offset(p.k_off, p.windows, p.tk, w + 1) > p.short_max;
-    if (__syncthreads_or(longer) && threadIdx.x == 0) atomicOr(flags, 1);
+    int some = 0;
+    for (int w = blockIdx.x * 256 + threadIdx.x; w < p.windows; w += gridDim.x * 256) {
+        const int n = attn_offset(p.k_off, p.windows, p.tk, w + 2) - attn_offset(p.k_off, p.windows, p.tk, w + 1);
+        some |= n > p.short_max ? kSomeLong : n > p.tiny_max ? kSomeShort : 0;
+    }
+    some = __reduce_or_sync(0xffffffffu, some);
+    if (some != 0 && (threadIdx.x & 31) == 0) atomicOr(flags, some);
 }
 
 // ---- short windows ---------------------------------------------------------------------------
@@ -362,6 +352,39 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     const int dim16 = (p.dim + 15) & ~15;
     const Loader<T, kRows> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
         oq(p.q, p.q_st, p.q_sh, p.dim, kvh * group), og(p.dout, p.do_st, p.do_sh, p.dim, kvh * group);
+    // rows outside every window
+    if (z == 0) {
+        const int q_lo = attn_offset(p.q_off, p.windows, p.tq, 1), q_hi = attn_offset(p.q_off, p.windows, p.tq, p.windows + 1);
+        const int k_lo = attn_offset(p.k_off, p.windows, p.tk, 1), k_hi = attn_offset(p.k_off, p.windows, p.tk, p.windows + 1);
+        const int nq = q_lo + max(p.tq - q_hi, 0), nk = k_lo + max(p.tk - k_hi, 0);
+        for (int r = blockIdx.x; r < nq + nk; r += gridDim.x) {
+            const bool of_q = r < nq;
+            const int i = of_q ? r : r - nq, lo = of_q ? q_lo : k_lo, hi = of_q ? q_hi : k_hi;
+            const int64_t token = i < lo ? i : hi + (i - lo);
+            for (int c = tid; c < p.dim * (of_q ? group : 2); c += kRows) {
+                if (of_q) {
+                    static_cast<T*>(p.dq)[(token * p.heads + kvh * group) * p.dim + c] = from_f<T>(0.0f);
+                } else if (p.qsplits == 1) {
+                    static_cast<T*>(c < p.dim ? p.dk : p.dv)[(token * p.kv_heads + kvh) * p.dim + c % p.dim] = from_f<T>(0.0f);
+                } else {
+                    for (int s = 0; s < p.qsplits; ++s)
+                        (c < p.dim ? p.part_dk : p.part_dv)[((static_cast<int64_t>(s) * p.tk + token) * p.kv_heads + kvh) * p.dim + c % p.dim] = 0.0f;
+                }
+            }
+        }
+    }
+
+    // and windows without keys
+    if (z == 0)
+        for (int w = blockIdx.x; w < p.windows; w += gridDim.x) {
+            const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0;
+            if (attn_offset(p.k_off, p.windows, p.tk, w + 2) > attn_offset(p.k_off, p.windows, p.tk, w + 1)) continue;
+            const int per = group * p.dim;
+            for (int64_t i = tid; i < static_cast<int64_t>(lq) * per; i += kRows)
+                static_cast<T*>(p.dq)[((q0 + i / per) * p.heads + kvh * group) * p.dim + i % per] = from_f<T>(0.0f);
+        }
+    if ((*p.flags & kSomeShort) == 0) return;
+
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
@@ -385,39 +408,10 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     int par_s = 0, par_o = 0;
     bool alive = true;
 
-    // rows outside every window
-    if (z == 0) {
-        const int q_lo = attn_offset(p.q_off, p.windows, p.tq, 1), q_hi = attn_offset(p.q_off, p.windows, p.tq, p.windows + 1);
-        const int k_lo = attn_offset(p.k_off, p.windows, p.tk, 1), k_hi = attn_offset(p.k_off, p.windows, p.tk, p.windows + 1);
-        const int nq = q_lo + max(p.tq - q_hi, 0), nk = k_lo + max(p.tk - k_hi, 0);
-        for (int r = blockIdx.x; r < nq + nk; r += gridDim.x) {
-            const bool of_q = r < nq;
-            const int i = of_q ? r : r - nq, lo = of_q ? q_lo : k_lo, hi = of_q ? q_hi : k_hi;
-            const int64_t token = i < lo ? i : hi + (i - lo);
-            for (int c = tid; c < p.dim * (of_q ? group : 2); c += kRows) {
-                if (of_q) {
-                    static_cast<T*>(p.dq)[(token * p.heads + kvh * group) * p.dim + c] = from_f<T>(0.0f);
-                } else if (p.qsplits == 1) {
-                    static_cast<T*>(c < p.dim ? p.dk : p.dv)[(token * p.kv_heads + kvh) * p.dim + c % p.dim] = from_f<T>(0.0f);
-                } else {
-                    for (int s = 0; s < p.qsplits; ++s)
-                        (c < p.dim ? p.part_dk : p.part_dv)[((static_cast<int64_t>(s) * p.tk + token) * p.kv_heads + kvh) * p.dim + c % p.dim] = 0.0f;
-                }
-            }
-        }
-    }
-
     for (int w = blockIdx.x; w < p.windows; w += gridDim.x) {
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), lk = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
-        if (lk > p.short_max) continue;
-        if (lk == 0) {
-            const int64_t n = static_cast<int64_t>(lq) * group * p.dim;
-            if (z == 0)
-                for (int64_t i = tid; i < n; i += kRows)
-                    static_cast<T*>(p.dq)[((q0 + i / (group * p.dim)) * p.heads + kvh * group) * p.dim + i % (group * p.dim)] = from_f<T>(0.0f);
-            continue;
-        }
+        if (lk > p.short_max || lk <= p.tiny_max) continue;  // other kernels', and windows without keys
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
         const int i0 = min(z * per, total), i1 = min(i0 + per, total);
         const int n = lk, n16 = (n + 15) & ~15;
@@ -531,7 +525,7 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     if constexpr (BIAS) if (grad_bias) {
         __syncthreads();
         for (int e = tid; e < entries * group; e += kRows)
-            p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * (p.bias_short + p.bias_long) + z * gridDim.x + blockIdx.x) * entries +
+            p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * p.bias_parts + p.bias_tiny + z * gridDim.x + blockIdx.x) * entries +
                         e % entries] = acc[e];
     }
     if (!alive && tid == 0) count_timeout();
@@ -552,7 +546,7 @@ struct LongSmem {
 
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_constant__ AttnParams p) {
-    if (*p.flags == 0) return;
+    if ((*p.flags & kSomeLong) == 0) return;
     using L = LongSmem<DP>;
     constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -594,9 +588,13 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     int par_s = 0, par_o = 0;
     bool alive = true;
 
-    const int chunk = (slots + gridDim.x - 1) / gridDim.x, slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
+    // Tiles back and forth over the blocks, the last ones (of causal windows the longest) first, so that
+    // every block gets long and short ones.
     AttnWalk walk;
-    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, slot0, min(slots, slot0 + chunk)); more; more = walk.next()) {
+    for (int round = 0;; ++round) {
+        const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (at >= slots) break;
+        if (!walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, slots - 1 - at, slots - at)) continue;
         const AttnTile& t = walk.tile;
         if (t.window < 0 || t.olen <= p.short_max) continue;
         const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
@@ -732,7 +730,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     if (grad_bias) {
         __syncthreads();
         for (int e = tid; e < entries; e += kThreads)
-            p.bias_part[(static_cast<int64_t>(head) * (p.bias_short + p.bias_long) + p.bias_short + blockIdx.x) * entries + e] = acc[e];
+            p.bias_part[(static_cast<int64_t>(head) * p.bias_parts + p.bias_tiny + p.bias_short + blockIdx.x) * entries + e] = acc[e];
     }
     if (!alive && tid == 0) count_timeout();
     tc::fence_before();
@@ -743,7 +741,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
 // ---- long windows: dk, dv --------------------------------------------------------------------
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
-    if (*p.flags == 0) return;
+    if ((*p.flags & kSomeLong) == 0) return;
     using L = LongSmem<DP>;
     constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -778,9 +776,11 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
 
-    const int chunk = (slots + gridDim.x - 1) / gridDim.x, slot0 = blockIdx.x * chunk;
     AttnWalk walk;
-    for (bool more = walk.start(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, slot0, min(slots, slot0 + chunk)); more; more = walk.next()) {
+    for (int round = 0;; ++round) {
+        const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (at >= slots) break;
+        if (!walk.start(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, at, at + 1)) continue;
         const AttnTile& t = walk.tile;
         if (t.window < 0 || t.len <= p.short_max) continue;
         const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;
@@ -903,14 +903,24 @@ __global__ void __launch_bounds__(256) k_attn_join_dkv(AttnParams p) {
     static_cast<T*>(p.dv)[i] = from_f<T>(v);
 }
 
-// The parts of each entry, in order, into the first part.
+// The parts of each entry into the first part: thread (part lane, entry) adds every eighth part, the
+// eight sums are added in order.
 __global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
-    const int entries = bias_entries(p.bias), e = blockIdx.x * 256 + threadIdx.x;
-    if (e >= entries) return;
-    const int parts = p.bias_short + p.bias_long, used = *p.flags != 0 ? parts : p.bias_short;
-    double* at = p.bias_part + static_cast<int64_t>(blockIdx.y) * parts * entries + e;
+    __shared__ double sums[8][32];
+    const int entries = bias_entries(p.bias), lane = threadIdx.x & 31, row = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int flags = *p.flags, first_long = p.bias_tiny + p.bias_short;
+    double* at = p.bias_part + static_cast<int64_t>(blockIdx.y) * p.bias_parts * entries + e;
     double sum = 0.0;
-    for (int s = 0; s < used; ++s) sum += at[static_cast<int64_t>(s) * entries];
+    if (e < entries) {
+        for (int s = row; s < p.bias_parts; s += 8) {
+            const bool filled = s < p.bias_tiny || (s < first_long ? (flags & kSomeShort) != 0 : (flags & kSomeLong) != 0);
+            if (filled) sum += at[static_cast<int64_t>(s) * entries];
+        }
+    }
+    sums[row][lane] = sum;
+    __syncthreads();
+    if (row != 0 || e >= entries) return;
+    for (int r = 1; r < 8; ++r) sum += sums[r][lane];
     at[0] = sum;
 }
 
@@ -918,7 +928,7 @@ __global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
 // entries of one row add up the same in any order. A block a head.
 __global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dtable) {
     const int entries = bias_entries(p.bias), head = blockIdx.x, tid = threadIdx.x;
-    const double* sum = p.bias_part + static_cast<int64_t>(head) * (p.bias_short + p.bias_long) * entries;
+    const double* sum = p.bias_part + static_cast<int64_t>(head) * p.bias_parts * entries;
     __shared__ unsigned long long top;
     if (tid == 0) top = 0ull;
     __syncthreads();
@@ -953,6 +963,7 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
     const int entries = bias_entries(p.bias), group = p.heads / p.kv_heads, sum = p.bias_part != nullptr;
     cudaError_t err;
     const int b_short = 1024 + ShortSmem<DP>::kBytes + entries * group * (4 + 8 * sum) + entries * 4 * sum;
+    if (p.tiny_blocks > 0 && (err = launch_attn_backward_tiny(p, std::is_same<T, __half>::value ? kF16 : kBF16, s)) != cudaSuccess) return err;
     if (p.short_max == 0) {
         // only rows and windows without partners: no bias is looked up
         const int bytes = 1024 + ShortSmem<DP>::kBytes;
@@ -977,7 +988,7 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
         if ((err = cudaGetLastError()) != cudaSuccess) return err;
     }
     if (dtable != nullptr) {
-        k_attn_bias_parts<<<dim3((entries + 255) / 256, p.heads), 256, 0, s>>>(p);
+        k_attn_bias_parts<<<dim3((entries + 31) / 32, p.heads), 256, 0, s>>>(p);
         if ((err = cudaGetLastError()) != cudaSuccess) return err;
         k_attn_bias_table<<<p.heads, 1024, 0, s>>>(p, dtable);
         err = cudaGetLastError();

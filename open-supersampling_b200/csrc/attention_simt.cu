@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
 // gradient's fixed point, and fp16's range). A warp a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* delta, uint32_t* bias_max) {
-    if (p.flags != nullptr && *p.flags == 0 && bias_max == nullptr) return;  // short windows find their own
+    if (p.flags != nullptr && (*p.flags & kSomeLong) == 0 && bias_max == nullptr) return;  // short windows find their own
     const int lane = threadIdx.x & 31;
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads;
     const int64_t vrows = bias_max == nullptr ? 0 : static_cast<int64_t>(p.tk) * p.kv_heads;
@@ -598,7 +598,9 @@ cudaError_t delta_type(const AttnParams& p, cudaStream_t s, int sms) {
 }  // namespace
 
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s) {
-    const cudaError_t err = type == kF32 ? fwd_f32(p, s) : launch_attn_forward_mma(p, type, s);
+    cudaError_t err = cudaSuccess;
+    if (p.tiny_max > 0) err = launch_attn_forward_tiny(p, type, s);
+    if (err == cudaSuccess) err = type == kF32 ? fwd_f32(p, s) : launch_attn_forward_mma(p, type, s);
     if (err != cudaSuccess || p.splits == 1) return err;
     return type == kF32 ? join_parts<float>(p, s) : type == kBF16 ? join_parts<__nv_bfloat16>(p, s) : join_parts<__half>(p, s);
 }

@@ -1330,11 +1330,19 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
         const int64_t per = (resident + heads - 1) / heads;
         return static_cast<int>(tiles < per ? (tiles < 1 ? 1 : tiles) : per);
     };
+    // The warp-level kernel: up to 32 columns and keys, where windows that short are likely, and the
+    // biases and sums of its warps leave room for two blocks on an SM.
+    const int64_t side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
+    const bool tiny = !p.causal && p.dim <= 32 && p.tk <= 128 * windows &&
+                      entries * group * (4 * side + (sums ? 48 : 0)) <= 110 * 1024;
+    p.tiny_max = tiny ? 32 : 0;
+    p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;
     p.short_blocks = blocks(windows, (p.dim <= 64 ? 2 : 1) * kSms, p.kv_heads * p.qsplits);
     p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (sums ? 1 : 4) * kSms, p.heads);
     p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, 128), 4 * kSms, p.kv_heads * p.qsplits);
+    p.bias_tiny = p.tiny_blocks * p.qsplits;
     p.bias_short = p.short_max > 0 ? p.short_blocks * p.qsplits : 0;
-    p.bias_long = p.dq_blocks;
+    p.bias_parts = p.bias_tiny + p.bias_short + p.dq_blocks;
 }
 
 // Lays the backward's scratch out; without a base, counts its bytes. `zeroed`: the bytes from
@@ -1349,7 +1357,7 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
         const int64_t keys = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
         p.part_dk = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
         p.part_dv = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
-        p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * (p.bias_short + p.bias_long) * entries) : nullptr;
+        p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * p.bias_parts * entries) : nullptr;
     }
     const int64_t from = arena.used;
     p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
@@ -1402,6 +1410,12 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     p.pack = attention_pack(tq, windows, heads, kv_heads, entries);
     OSS_CHECK(tq * p.pack <= INT_MAX, OSS_ERR_RANGE, "token count times heads of a group exceeds int32 range");
     p.splits = attention_splits(tq, tk, windows, heads, p.pack);
+    // The warp-level kernel takes windows of up to 64 keys (32 with more than 32 columns) where the
+    // average one is no longer; its blocks hold the biases of up to 4 key heads.
+    const int64_t most = dim <= 32 ? 64 : 32, side = kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1;
+    if (dtype != oss::kF32 && !p.causal && dim <= 64 && windows > 0 && tk <= most * windows &&
+        side * (heads / kv_heads) * entries <= 16384)
+        p.tiny_max = static_cast<int>(most);
     if (p.splits > 1) {
         OSS_CHECK(scratch != nullptr && scratch_bytes >= attention_split_bytes(tq, heads, dim, p.splits), OSS_ERR_SCRATCH,
                   "scratch smaller than oss_window_attention_scratch_bytes");
@@ -1423,13 +1437,15 @@ int oss_window_attention_timeouts(uint32_t* count) {
 }
 
 int64_t oss_window_attention_backward_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
-                                                    int64_t kv_heads, int64_t dim, int64_t entries, int64_t buckets) {
+                                                    int64_t kv_heads, int64_t dim, int32_t causal, int64_t entries,
+                                                    int64_t buckets) {
     if (check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim) != OSS_OK || entries < 0 ||
         entries > oss::kMaxBiasEntries || buckets < 0 || buckets * heads > INT_MAX)
         return 0;
     oss::AttnParams p{};
     p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
     p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
+    p.causal = causal != 0;
     return attention_backward_scratch(p, dtype, entries, buckets, nullptr, 0, nullptr, nullptr);
 }
 
@@ -1458,7 +1474,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
     OSS_CHECK(q_offsets != nullptr && k_offsets != nullptr, OSS_ERR_INVALID, "offsets must be non-null");
     const int64_t sums = d_table == nullptr ? 0 : buckets;
     OSS_CHECK(scratch != nullptr &&
-                  scratch_bytes >= oss_window_attention_backward_scratch_bytes(dtype, tq, tk, windows, heads, kv_heads, dim,
+                  scratch_bytes >= oss_window_attention_backward_scratch_bytes(dtype, tq, tk, windows, heads, kv_heads, dim, causal,
                                                                                oss::bias_entries(p.bias), sums),
               OSS_ERR_SCRATCH, "scratch smaller than oss_window_attention_backward_scratch_bytes");
     p.q = q, p.k = k, p.v = v;

@@ -75,7 +75,7 @@ def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buck
         dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
         dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if want_table else None
         windows = q_offsets.numel() - 1
-        nbytes = lib.oss_window_attention_backward_scratch_bytes(DTYPES[q.dtype], tq, tk, windows, h, kv, d,
+        nbytes = lib.oss_window_attention_backward_scratch_bytes(DTYPES[q.dtype], tq, tk, windows, h, kv, d, int(causal),
                                                                  0 if table is None else buckets.numel(),
                                                                  table.size(0) if want_table else 0)
         scratch = torch.empty((max(1, nbytes),), device=q.device, dtype=torch.uint8)

@@ -94,6 +94,37 @@ def test_grouped_heads(cuda_device, dtype, heads, kv):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [7, 16, 30, 32, 48, 64])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2), (6, 3), (5, 5)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_few_keys(cuda_device, dtype, dim, heads, kv, biased):
+    """Tiles with few Gaussians, some with none, and one crowded: every kernel in one call."""
+    from oss_cuda import window_position_buckets
+
+    kl = [0, 1, 7, 8, 9, 16, 17, 31, 32, 33, 5, 0, 2, 12, 64, 3, 65, 140, 1, 20]
+    ql = [16, 1, 33, 0, 256, 100, 15, 17, 64, 47, 64, 0, 130, 16, 70, 40, 80, 90, 31, 32]
+    (q, k, v, do), qo, ko, g = inputs(ql, kl, heads, kv, dim, TYPES[dtype], seed=dim, qfirst=3, ktail=5)
+    kw = {}
+    if biased:
+        kw = dict(table=torch.randn(81, heads, generator=g).to(TYPES[dtype]), buckets=window_position_buckets(4, 4),
+                  q_pos=torch.randint(0, 5, (q.size(0), 2), generator=g).int(),
+                  k_pos=torch.randint(0, 5 if dim % 3 else 12, (k.size(0), 2), generator=g).int())
+    both(cuda_device, q, k, v, qo, ko, do, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lk", [20, 50, 100])
+def test_many_queries_of_few_keys(cuda_device, dtype, lk):
+    """One window's rows shared out over blocks, its key gradients joined."""
+    from oss_cuda import window_position_buckets
+
+    (q, k, v, do), qo, ko, g = inputs([6000, 4097], [lk, lk], 2, 1, 32, TYPES[dtype], seed=lk)
+    kw = dict(table=torch.randn(25, 2, generator=g).to(TYPES[dtype]), buckets=window_position_buckets(2, 2),
+              q_pos=torch.randint(0, 3, (q.size(0), 2), generator=g).int(), k_pos=torch.randint(0, 3, (k.size(0), 2), generator=g).int())
+    both(cuda_device, q, k, v, qo, ko, do, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lq,lk,causal", [(1, 3000, True), (2, 5001, False), (17, 2100, True)])
 def test_long_axis_is_split_and_joined(cuda_device, dtype, lq, lk, causal):
     from oss_cuda import _lib
