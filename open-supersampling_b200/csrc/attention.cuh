@@ -192,7 +192,7 @@ struct AttnWalk {
             int at = w + 1;
             for (;; at += 32) {
                 const int c = at + lane;
-                bool stop = c > windows + 1;
+                bool stop = c > windows + 1 || slot_of(c) >= end;
                 if (!stop) {
                     const int n = c >= 1 && c <= windows ? attn_offset(other, windows, ot, c + 1) - attn_offset(other, windows, ot, c) : 0;
                     stop = attn_offset(off, windows, t, c + 1) > attn_offset(off, windows, t, c) && (n <= 0 || n > skip);

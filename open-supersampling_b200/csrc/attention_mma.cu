@@ -77,6 +77,14 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
         lv(p.v, p.v_st, p.v_sh, p.dim, kvh);
     const float c2 = p.scale * kLog2e;
 
+    const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
+    const int chunk = (slots + gridDim.x - 1) / gridDim.x;
+    // causal windows: the last tiles see the most keys and go first
+    const int slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
+    AttnWalk walk;
+    bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk), p.tiny_max);
+    if (!more) return;
+
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
@@ -94,13 +102,7 @@ __global__ void __launch_bounds__(kRows, KT == 64 ? 4 : 2) k_attn_fwd_mma(const 
     int par_s = 0, par_o = 0;  // parities of the next wait
     bool alive = true;
 
-    const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
-    const int chunk = (slots + gridDim.x - 1) / gridDim.x;
-    // causal windows: the last tiles see the most keys and go first
-    const int slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
-    AttnWalk walk;
-    for (bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk), p.tiny_max); more;
-         more = walk.next()) {
+    for (; more; more = walk.next()) {
         const AttnTile& t = walk.tile;
         const int rows = min(kRows, t.len * p.pack - t.first);
         const int row = t.first + tid;

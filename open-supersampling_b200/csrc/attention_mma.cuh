@@ -84,17 +84,21 @@ struct Loader {
         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0) : "memory");
     }
     __device__ __forceinline__ void store_some(uint32_t to, const T* from) const {
-        uint32_t w[4] = {0, 0, 0, 0};
         if (pairs) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c * 8 + 2 * e < dim) w[e] = __ldg(reinterpret_cast<const uint32_t*>(from) + e);
-        } else {
-            const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(__ldg(s + e)) << (16 * (e & 1));
+            for (int e = 0; e < 4; ++e) {
+                if (c * 8 + 2 * e < dim)
+                    tc::cp_async4(to + 4 * e, from + 2 * e);
+                else
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + 4 * e), "r"(0) : "memory");
+            }
+            return;
         }
+        uint32_t w[4] = {0, 0, 0, 0};
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(from);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c * 8 + e < dim) w[e >> 1] |= static_cast<uint32_t>(__ldg(s + e)) << (16 * (e & 1));
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
 };

@@ -1,6 +1,6 @@
 // Window attention of 16-bit types on the tensor cores (tcgen05): backward.
 //
-// Per tile of 128 queries x keys, with thread = query row (two threads a row where a tile has 128 keys):
+// Per tile of 128 queries x keys, with 32 keys of a query row for each thread:
 //   S = Q K^T, dP = dO V^T          into tensor memory
 //   P = 2^(S - lse), dS = P (dP - delta)   in registers, written to shared memory as 16-bit values
 //   dV += P^T dO, dK += dS^T Q, dQ += dS K from shared memory: a row-major P is a K-major operand for
@@ -65,35 +65,44 @@ __device__ __forceinline__ BiasSum bias_sum(BiasMode mode, const float* wsize) {
     return b;
 }
 
-// Adds a thread's 64 terms of keys j0 .. to the block's integers (wsum: a warp's sum where the tile
+// Adds a thread's terms of keys j0 .. to the block's integers (wsum: a warp's sum where the tile
 // has one entry).
-template <int KT>
-__device__ __forceinline__ void bias_add(const AttnParams& p, const BiasSum& b, const float (&ds)[64], int n16, int head,
+template <int KT, int N>
+__device__ __forceinline__ void bias_add(const AttnParams& p, const BiasSum& b, const float (&ds)[N], int n16, int head,
                                          const KeyPos<KT>* k, int j0, int2 qp, int* I, float* wsum) {
     if (b.mode == kOne) {
         float sum = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-            if (j0 + c < n16) sum += ds[c];
+        for (int c = 0; c < N; ++c) sum += ds[c];  // 0 past the last key
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         if ((threadIdx.x & 31) == 0) *wsum = sum;
         return;
     }
+    if (b.bad || b.mode == kClamp) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            if (j0 + c >= n16) break;
+            const int e = bias_index(p.bias, qp, make_int2(k->y[j0 + c], k->x[j0 + c]));
+            if (!is_finite(ds[c]))
+                bias_mark_bad(p, head, e);
+            else
+                atomicAdd(I + e, __float2int_rn(ds[c] * b.fixed));
+        }
+        return;
+    }
     const int w = 2 * p.bias.rx + 1;
     const int* code = b.mode == kLinear ? k->code + j0 : k->x + j0;
     const int dy = b.mode == kLinear ? -qp.x : min(max(k->y[0] - qp.x, -p.bias.ry), p.bias.ry);
-    const int off = (dy + p.bias.ry) * w + p.bias.rx - qp.y;
+    int* at = I + (dy + p.bias.ry) * w + p.bias.rx - qp.y;
 #pragma unroll
-    for (int c = 0; c < 64; ++c) {
+    for (int c = 0; c < N; c += 4) {
         if (j0 + c >= n16) break;
-        const float x = ds[c];
-        if (x == 0.0f) continue;
-        const int e = b.mode == kClamp ? bias_index(p.bias, qp, make_int2(k->y[j0 + c], k->x[j0 + c])) : code[c] + off;
-        if (b.bad && !is_finite(x))
-            bias_mark_bad(p, head, e);
-        else
-            atomicAdd(I + e, __float2int_rn(x * b.fixed));
+        const int4 q = *reinterpret_cast<const int4*>(code + c);
+        atomicAdd(at + q.x, __float2int_rn(ds[c] * b.fixed));
+        atomicAdd(at + q.y, __float2int_rn(ds[c + 1] * b.fixed));
+        atomicAdd(at + q.z, __float2int_rn(ds[c + 2] * b.fixed));
+        atomicAdd(at + q.w, __float2int_rn(ds[c + 3] * b.fixed));
     }
 }
 
@@ -125,15 +134,16 @@ __device__ __forceinline__ void bias_join(const AttnParams& p, const BiasSum& b,
     }
 }
 
-// A row of 64 values as 16-bit into a panel.
-template <typename T>
-__device__ __forceinline__ void write_row(uint32_t panel, int row, const float (&x)[64], float by) {
+// N values of a row, columns j0 .., as 16-bit into panels.
+template <typename T, int N>
+__device__ __forceinline__ void write_row(uint32_t panels, int row, int j0, const float (&x)[N], float by) {
+    const uint32_t panel = panels + (j0 >> 6) * kRows * 128, chunk0 = (j0 & 63) >> 3;
 #pragma unroll
-    for (int c = 0; c < 64; c += 8) {
+    for (int c = 0; c < N; c += 8) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack2(x[c + 2 * i] * by, x[c + 2 * i + 1] * by, T{});
-        const uint32_t to = panel + row * 128 + ((((c >> 3)) ^ (row & 7)) << 4);
+        const uint32_t to = panel + row * 128 + (((chunk0 + (c >> 3)) ^ (row & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
 }
@@ -157,15 +167,15 @@ __device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim,
     }
 }
 
-// Scores and dP of a thread's 64 keys from tensor memory, and the weights: s becomes p, dp stays.
+// Scores and dP of a thread's N keys from tensor memory, and the weights: s becomes p, dp stays.
 // Zero where the mask is, whatever stands there.
-template <int KT, bool BIAS>
-__device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], float (&dp)[64], uint32_t ts, uint32_t tdp, int n16,
+template <int KT, bool BIAS, int N>
+__device__ __forceinline__ void weights(const AttnParams& p, float (&s)[N], float (&dp)[N], uint32_t ts, uint32_t tdp, int n16,
                                         int j0, bool whole, int see, float lse, BiasMode mode, const float* E,
                                         const KeyPos<KT>* kp, int2 qp) {
     const float c2 = p.scale * kLog2e;
 #pragma unroll
-    for (int c = 0; c < 64; c += 16) {
+    for (int c = 0; c < N; c += 16) {
         if (j0 + c < n16) {
             tc::tmem_ld16(ts + j0 + c, s + c);
             tc::tmem_ld16(tdp + j0 + c, dp + c);
@@ -177,7 +187,7 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], flo
     tc::wait_ld();
     const float2 by = make_float2(BIAS ? 1.0f : c2, BIAS ? 1.0f : c2), off = make_float2(-lse, -lse);
 #pragma unroll
-    for (int c = 0; c < 64; c += 16) {
+    for (int c = 0; c < N; c += 16) {
         if (j0 + c >= n16) continue;
         if constexpr (BIAS) add_bias<KT, 16>(*reinterpret_cast<float(*)[16]>(s + c), c2, p.bias, mode, E, kp, j0 + c, qp);
 #pragma unroll
@@ -189,7 +199,7 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], flo
     }
     if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
+        for (int c = 0; c < N; ++c) {
             const bool on = j0 + c < see;
             s[c] = on ? s[c] : 0.0f;
             dp[c] = on ? dp[c] : 0.0f;
@@ -198,10 +208,11 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[64], flo
 }
 
 // dp becomes p (dp - delta).
-__device__ __forceinline__ void score_gradients(const float (&s)[64], float (&dp)[64], float delta) {
+template <int N>
+__device__ __forceinline__ void score_gradients(const float (&s)[N], float (&dp)[N], float delta) {
     const float2 off = make_float2(-delta, -delta);
 #pragma unroll
-    for (int c = 0; c < 64; c += 2) {
+    for (int c = 0; c < N; c += 2) {
         const float2 d = __fmul2_rn(make_float2(s[c], s[c + 1]), __fadd2_rn(make_float2(dp[c], dp[c + 1]), off));
         dp[c] = d.x;
         dp[c + 1] = d.y;
@@ -325,13 +336,13 @@ struct ShortSmem {
     // dS, P, Q, dO, K, V; dS and P end before 16 KB that may be read past them (rows of keys 64 and on,
     // which nothing uses)
     static constexpr int kTiles = 2 * kP + 2 * kT + 2 * kK;
-    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<kShortKeys>)) + 64 + 64 + 32;
+    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<kShortKeys>)) + 64 + 128 + 2 * kRows * 4;
 };
 
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(const __grid_constant__ AttnParams p) {
     using L = ShortSmem<DP>;
-    constexpr int kCols = DP == 64 ? 256 : 512, KT = kShortKeys;
+    constexpr int kCols = DP == 64 ? 256 : 512, KT = kShortKeys, kThreads = 2 * kRows, N = KT / 2;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sd = tc::smem_addr(base), sp = sd + L::kP, sq = sp + L::kP, sg = sq + L::kT, sk = sg + L::kT, sv = sk + L::kK;
@@ -339,8 +350,9 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     Range* qrange = reinterpret_cast<Range*>(kp + 1);
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
-    float* wsize = reinterpret_cast<float*>(slot_tmem + 4);
-    float* wsum = wsize + 4;
+    float* wsize = reinterpret_cast<float*>(bars + 4);
+    float* wsum = wsize + 8;
+    float* half_delta = reinterpret_cast<float*>(bars + 16);  // [2][kRows]
     const int group = p.heads / p.kv_heads, entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y;
     const bool grad_bias = BIAS && p.bias_part != nullptr;
     double* acc = reinterpret_cast<double*>(base + L::kBytes);
@@ -348,9 +360,9 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
     const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
 
-    const int tid = threadIdx.x, warp = tid >> 5, z = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N, z = blockIdx.z;
     const int dim16 = (p.dim + 15) & ~15;
-    const Loader<T, kRows> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
+    const Loader<T, kThreads> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
         oq(p.q, p.q_st, p.q_sh, p.dim, kvh * group), og(p.dout, p.do_st, p.do_sh, p.dim, kvh * group);
     // rows outside every window
     if (z == 0) {
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             const bool of_q = r < nq;
             const int i = of_q ? r : r - nq, lo = of_q ? q_lo : k_lo, hi = of_q ? q_hi : k_hi;
             const int64_t token = i < lo ? i : hi + (i - lo);
-            for (int c = tid; c < p.dim * (of_q ? group : 2); c += kRows) {
+            for (int c = tid; c < p.dim * (of_q ? group : 2); c += kThreads) {
                 if (of_q) {
                     static_cast<T*>(p.dq)[(token * p.heads + kvh * group) * p.dim + c] = from_f<T>(0.0f);
                 } else if (p.qsplits == 1) {
@@ -380,7 +392,7 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0;
             if (attn_offset(p.k_off, p.windows, p.tk, w + 2) > attn_offset(p.k_off, p.windows, p.tk, w + 1)) continue;
             const int per = group * p.dim;
-            for (int64_t i = tid; i < static_cast<int64_t>(lq) * per; i += kRows)
+            for (int64_t i = tid; i < static_cast<int64_t>(lq) * per; i += kThreads)
                 static_cast<T*>(p.dq)[((q0 + i / per) * p.heads + kvh * group) * p.dim + i % per] = from_f<T>(0.0f);
         }
     if ((*p.flags & kSomeShort) == 0) return;
@@ -392,16 +404,16 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     }
     if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
     if constexpr (BIAS)
-    for (int e = tid; e < entries * group; e += kRows) {
+    for (int e = tid; e < entries * group; e += kThreads) {
         E[e] = bias_entry(p.bias, p.heads, kvh * group + e / entries, e % entries);
         if (grad_bias) acc[e] = 0.0;
     }
     if (grad_bias)
-        for (int e = tid; e < entries; e += kRows) I[e] = 0;
+        for (int e = tid; e < entries; e += kThreads) I[e] = 0;
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_dv = 2 * KT, t_dk = 2 * KT + DP;  // columns; S at 0, dP at 64, dQ over both
     const uint32_t id_grad = tc::idesc(kIsBf16<T>, dim16, true, true), id_q = tc::idesc(kIsBf16<T>, dim16, false, true);
     const float up = ds_scale<T>(p);
@@ -423,8 +435,8 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             oq.load(sq, kRows, q0 + first, rows, kRows, (it / qtiles) * p.q_sh);
             og.load(sg, kRows, q0 + first, rows, kRows, (it / qtiles) * p.do_sh);
             tc::cp_async_commit();
-            lse = tid < rows ? p.lse[static_cast<int64_t>(head) * p.tq + q0 + first + tid] : INFINITY;
-            if (BIAS) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(tid, rows - 1));
+            lse = row < rows ? p.lse[static_cast<int64_t>(head) * p.tq + q0 + first + row] : INFINITY;
+            if (BIAS) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(row, rows - 1));
         };
         __syncthreads();  // the window before has read its keys
         if (i0 < i1) {
@@ -437,7 +449,7 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             const int g = it / qtiles, head = kvh * group + g, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
             if (BIAS) {
                 const Range r = warp_range(qp);
-                if ((tid & 31) == 0) qrange[warp] = r;
+                if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
             }
             tc::cp_async_wait<0>();
             tc::fence_async();
@@ -450,30 +462,32 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
                 tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv, dim16, id);
                 tc::commit(bar_s);
             }
-            const int see = tid >= rows ? 0 : p.causal ? min(max(first + tid + lk - lq + 1, 0), lk) : lk;
+            const int see = row >= rows ? 0 : p.causal ? min(max(first + row + lk - lq + 1, 0), lk) : lk;
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= n);
             BiasMode mode = kOne;
             if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
-            float s[64], dp[64];
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, 0, whole, see, lse, mode, E + g * entries, kp, qp);
+            float s[N], dp[N];
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see, lse, mode, E + g * entries, kp, qp);
             float2 d0 = make_float2(0.0f, 0.0f), d1 = d0;
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
+            for (int c = 0; c < N; c += 4) {
                 d0 = __ffma2_rn(make_float2(s[c], s[c + 1]), make_float2(dp[c], dp[c + 1]), d0);
                 d1 = __ffma2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(dp[c + 2], dp[c + 3]), d1);
             }
-            const float delta = (d0.x + d0.y) + (d1.x + d1.y);
-            write_row<T>(sp, tid, s, 1.0f);
+            half_delta[tid] = (d0.x + d0.y) + (d1.x + d1.y);
+            write_row<T>(sp, row, j0, s, 1.0f);
+            __syncthreads();  // the other half of the row's keys
+            const float delta = half_delta[row] + half_delta[kRows + row];
             score_gradients(s, dp, delta);
-            write_row<T>(sd, tid, dp, up);
+            write_row<T>(sd, row, j0, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
                 if ((tid & 31) == 0) wsize[warp] = m;
             }
-            if (p.causal && tid < rows) p.delta[static_cast<int64_t>(head) * p.tq + q0 + first + tid] = delta;
+            if (p.causal && tid < rows) p.delta[static_cast<int64_t>(head) * p.tq + q0 + first + tid] = delta;  // tid: one of the two
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
@@ -489,8 +503,8 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             }
             BiasSum bs{kOne, 0.0f, false};
             if (grad_bias) {
-                bs = bias_sum<4>(mode, wsize);
-                if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, 0, qp, I, wsum + warp);
+                bs = bias_sum<8>(mode, wsize);
+                if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, j0, qp, I, wsum + warp);
             }
             alive = tc::mbar_wait(bar_o, par_o) && alive;
             par_o ^= 1;
@@ -498,33 +512,42 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
             const int2 qp_now = qp;
             const float lse_now = lse;
             if (it + 1 < i1) fetch(it + 1);
+            // columns of dQ in turn between the two threads of a row
             bool fine = true;
 #pragma unroll
             for (int c = 0; c < DP; c += 16) {
-                if (c >= dim16) continue;
+                if (c >= dim16 || ((c >> 4) & 1) != tid / kRows) continue;
                 float o[16];
                 tc::tmem_ld16(ts + c, o);
                 tc::wait_ld();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
-                stage16<T>(sd, tid, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
+                stage16<T>(sd, row, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
             }
-            if (p.causal && tid < rows && !fine && alive) query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, delta, up, sd);
+            if (p.causal) {
+                if (__syncthreads_or(!fine)) {  // some row of the tile: whoever holds one of its threads
+                    half_delta[tid] = fine ? 0.0f : 1.0f;
+                    __syncthreads();
+                    if (tid < rows && half_delta[row] + half_delta[kRows + row] != 0.0f && alive)
+                        query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, delta, up, sd);
+                }
+            }
             tc::fence_before();
             __syncthreads();
             if (grad_bias && (bs.fixed != 0.0f || bs.bad))
-                bias_join<kRows, 4, KT>(p, bs, entries, head, kp, qp_now, I, wsum, acc + g * entries);
-            store_panel<T, kRows>(sd, p.dq, p.heads, p.dim, q0, head, 1, first, rows);
+                bias_join<kThreads, 8, KT>(p, bs, entries, head, kp, qp_now, I, wsum, acc + g * entries);
+            store_panel<T, kThreads>(sd, p.dq, p.heads, p.dim, q0, head, 1, first, rows);
         }
-        if (warp < 2) {
-            finish_key_row<T, DP>(p, ts + t_dv, tid < n, i0 < i1, k0 + min(tid, n - 1), tid, kvh, q0, lq, lk, i0, i1, z, up, true, alive);
-            finish_key_row<T, DP>(p, ts + t_dk, tid < n, i0 < i1, k0 + min(tid, n - 1), tid, kvh, q0, lq, lk, i0, i1, z, up, false, alive);
+        if ((warp & 3) < 2) {
+            const bool of_v = tid < kRows;
+            finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, i0 < i1, k0 + min(row, n - 1), row, kvh, q0, lq, lk, i0, i1, z, up, of_v,
+                                  alive);
         }
         tc::fence_before();
     }
     if constexpr (BIAS) if (grad_bias) {
         __syncthreads();
-        for (int e = tid; e < entries * group; e += kRows)
+        for (int e = tid; e < entries * group; e += kThreads)
             p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * p.bias_parts + p.bias_tiny + z * gridDim.x + blockIdx.x) * entries +
                         e % entries] = acc[e];
     }
@@ -534,38 +557,81 @@ __global__ void __launch_bounds__(kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(cons
     if (warp == 0) tc::tmem_free<kCols>(tmem);
 }
 
+// The tiles of a block. Where windows have many tiles (1024 queries on average): back and forth over
+// the blocks, so that each gets tiles of many keys and of few (the last tiles of a causal window see
+// all of it, its first ones nearly nothing). Otherwise an even range of slots, whose empty ones even out.
+struct LongWalk {
+    AttnWalk walk;
+    const AttnParams& p;
+    int slots, round;
+    bool spread;
+    const int32_t *off, *other;
+    int t, ot, rows;
+    __device__ __forceinline__ LongWalk(int slots_, const AttnParams& p_) : p(p_), slots(slots_), round(-1) {
+        spread = static_cast<int64_t>(p.windows) * 1024 <= p.tq;
+    }
+    __device__ __forceinline__ bool first(const int32_t* off_, int t_, const int32_t* other_, int ot_, int rows_) {
+        off = off_, t = t_, other = other_, ot = ot_, rows = rows_;
+        if (spread) return next();
+        const int64_t n = slots;
+        return walk.start(off, t, other, ot, p.windows, 1, rows, static_cast<int>(n * blockIdx.x / gridDim.x),
+                          static_cast<int>(n * (blockIdx.x + 1) / gridDim.x));
+    }
+    __device__ __forceinline__ bool next() {
+        if (!spread) return walk.next();
+        for (;;) {
+            ++round;
+            const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            if (at >= slots) return false;
+            if (walk.start(off, t, other, ot, p.windows, 1, rows, slots - 1 - at, slots - at)) return true;
+        }
+    }
+};
+
 // ---- long windows: dq ------------------------------------------------------------------------
+// dq: with up to 64 columns 64 keys a tile and two blocks on an SM, which fill each other's waits;
+// with more, tensor memory holds one block, of 512 threads.
 template <int DP>
-struct LongSmem {
-    static constexpr int kT = kRows * DP * 2, kP = kRows * kRows * 2;
-    static constexpr int kBuf = DP == 64 ? 2 : 1;  // of what the kernel walks
-    static constexpr int kMisc = static_cast<int>(sizeof(KeyPos<kRows>)) * kBuf + 64 + 64 + 64;
-    static constexpr int kDq = 2 * kT + 2 * kBuf * kT + kP;
-    static constexpr int kDkv = 2 * kT + 2 * kBuf * kT + 2 * kP;
+struct DqShape {
+    static constexpr int KT = DP == 64 ? 64 : 128, kThreads = 4 * KT, N = 32;
+    static constexpr int kBuf = DP == 64 ? 2 : 1;  // of the keys and values
+    static constexpr int kT = kRows * DP * 2, kK = KT * DP * 2, kP = kRows * KT * 2;
+    static constexpr int kTiles = 2 * kT + 2 * kBuf * kK + kP;
+    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<KT>)) * kBuf + 64 + 64 + 128;
+    static constexpr int kCols = DP == 64 ? 256 : 512;  // S, dP, dQ
+};
+// dk, dv: 128 keys, so that the products fill their 128 rows; one block of 512 threads.
+template <int DP>
+struct DkvShape {
+    static constexpr int KT = 128, kThreads = 512, N = 32;
+    static constexpr int kBuf = DP == 64 ? 2 : 1;  // of the queries
+    static constexpr int kT = kRows * DP * 2, kP = kRows * KT * 2;
+    static constexpr int kTiles = 2 * kT + 2 * kBuf * kT + 2 * kP;
+    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<KT>)) + 64 + 64;
 };
 
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_attn_dq_long(const __grid_constant__ AttnParams p) {
     if ((*p.flags & kSomeLong) == 0) return;
-    using L = LongSmem<DP>;
-    constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
+    using L = DqShape<DP>;
+    constexpr int KT = L::KT, kBuf = L::kBuf, kThreads = L::kThreads, N = L::N, kWarps = kThreads / 32;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t sq = tc::smem_addr(base), sg = sq + L::kT, sk = sg + L::kT, sv = sk + kBuf * L::kT, sd = sv + kBuf * L::kT;
-    KeyPos<KT>* kps = reinterpret_cast<KeyPos<KT>*>(base + L::kDq);
+    const uint32_t sq = tc::smem_addr(base), sg = sq + L::kT, sk = sg + L::kT, sv = sk + kBuf * L::kK, sd = sv + kBuf * L::kK;
+    KeyPos<KT>* kps = reinterpret_cast<KeyPos<KT>*>(base + L::kTiles);
     Range* qrange = reinterpret_cast<Range*>(kps + kBuf);
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
     float* wsize = reinterpret_cast<float*>(bars + 8);
-    float* wsum = wsize + 8;
+    float* wsum = wsize + 16;
     const int entries = BIAS ? bias_entries(p.bias) : 0, head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
     const bool grad_bias = BIAS && p.bias_part != nullptr;
-    double* acc = reinterpret_cast<double*>(base + L::kDq + L::kMisc);
+    double* acc = reinterpret_cast<double*>(base + L::kBytes);
     int* I = reinterpret_cast<int*>(acc + (grad_bias ? entries : 0));
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
     const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
 
-    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
+    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tq, p.windows, kRows);
     const Loader<T, kThreads> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
         oq(p.q, p.q_st, p.q_sh, p.dim, head), og(p.dout, p.do_st, p.do_sh, p.dim, head);
@@ -574,7 +640,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
         tc::mbar_init(bar_o, 1);
         tc::mbar_init_fence();
     }
-    if (warp == 0) tc::tmem_alloc<512>(tc::smem_addr(slot_tmem));
+    if (warp == 0) tc::tmem_alloc<L::kCols>(tc::smem_addr(slot_tmem));
     for (int e = tid; e < entries; e += kThreads) {
         E[e] = bias_entry(p.bias, p.heads, head, e);
         if (grad_bias) acc[e] = 0.0, I[e] = 0;
@@ -588,14 +654,9 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     int par_s = 0, par_o = 0;
     bool alive = true;
 
-    // Tiles back and forth over the blocks, the last ones (of causal windows the longest) first, so that
-    // every block gets long and short ones.
-    AttnWalk walk;
-    for (int round = 0;; ++round) {
-        const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        if (at >= slots) break;
-        if (!walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, 1, kRows, slots - 1 - at, slots - at)) continue;
-        const AttnTile& t = walk.tile;
+    LongWalk walk(slots, p);
+    for (bool more = walk.first(p.q_off, p.tq, p.k_off, p.tk, kRows); more; more = walk.next()) {
+        const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.olen <= p.short_max) continue;
         const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
         const bool live = row < rows;
@@ -609,8 +670,8 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
         const int2 qp = entries > 0 ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0);
         auto fetch = [&](int kt) {
             const int b = kBuf == 2 ? kt & 1 : 0, n = min(KT, most - kt * KT), n16 = (n + 15) & ~15;
-            ok.load(sk + b * L::kT, KT, t.obegin + kt * KT, n, n16);
-            ov.load(sv + b * L::kT, KT, t.obegin + kt * KT, n, n16);
+            ok.load(sk + b * L::kK, KT, t.obegin + kt * KT, n, n16);
+            ov.load(sv + b * L::kK, KT, t.obegin + kt * KT, n, n16);
             if (BIAS) load_key_pos<KT>(kps + b, p.bias, t.obegin + kt * KT, n);
         };
         __syncthreads();  // the tile before has been read
@@ -635,12 +696,12 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
             if (tid == 0) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
-                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk + b * L::kT, dim16, id);
-                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv + b * L::kT, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk + b * L::kK, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv + b * L::kK, dim16, id);
                 tc::commit(bar_s);
             }
             if (grad_bias && kt > 0 && (bs.fixed != 0.0f || bs.bad))  // of the tile before
-                bias_join<kThreads, 8, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (kt - 1) & 1 : 0), qp, I, wsum, acc);
+                bias_join<kThreads, kWarps, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (kt - 1) & 1 : 0), qp, I, wsum, acc);
             if (kBuf == 2) {
                 if (kt > 0) {  // dQ of the tile before: its keys and dS are free
                     alive = tc::mbar_wait(bar_o, par_o) && alive;
@@ -655,10 +716,10 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
-            float s[64], dp[64];
+            float s[N], dp[N];
             weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, kp, qp);
             score_gradients(s, dp, delta);
-            write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
+            write_row<T>(sd, row, j0, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
                 if ((tid & 31) == 0) wsize[warp] = m;
@@ -668,7 +729,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after();
-                const uint64_t dd = tc::desc(sd, 16), dk = tc::desc(sk + b * L::kT, KT * 128);
+                const uint64_t dd = tc::desc(sd, 16), dk = tc::desc(sk + b * L::kK, KT * 128);
 #pragma unroll
                 for (int k = 0; k < KT; k += 16)
                     if (k < n16)
@@ -676,7 +737,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
                 tc::commit(bar_o);
             }
             if (grad_bias) {
-                bs = bias_sum<8>(mode, wsize);
+                bs = bias_sum<kWarps>(mode, wsize);
                 if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, j0, qp, I, wsum + warp);
             }
             if (kBuf == 1) {
@@ -685,7 +746,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
                 if (kt + 1 < tiles) {
                     if (grad_bias) {
                         __syncthreads();
-                        if (bs.fixed != 0.0f || bs.bad) bias_join<kThreads, 8, KT>(p, bs, entries, head, kp, qp, I, wsum, acc);
+                        if (bs.fixed != 0.0f || bs.bad) bias_join<kThreads, kWarps, KT>(p, bs, entries, head, kp, qp, I, wsum, acc);
                         bs = BiasSum{kOne, 0.0f, false};
                         __syncthreads();
                     } else if (BIAS) {
@@ -703,7 +764,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
         tc::fence_after();
         __syncthreads();
         if (grad_bias && tiles > 0 && (bs.fixed != 0.0f || bs.bad))
-            bias_join<kThreads, 8, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (tiles - 1) & 1 : 0), qp, I, wsum, acc);
+            bias_join<kThreads, kWarps, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (tiles - 1) & 1 : 0), qp, I, wsum, acc);
         if (tid < kRows) {
             bool fine = true;
 #pragma unroll
@@ -735,28 +796,28 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dq_long(const __grid_cons
     if (!alive && tid == 0) count_timeout();
     tc::fence_before();
     __syncthreads();
-    if (warp == 0) tc::tmem_free<512>(tmem);
+    if (warp == 0) tc::tmem_free<L::kCols>(tmem);
 }
 
 // ---- long windows: dk, dv --------------------------------------------------------------------
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
     if ((*p.flags & kSomeLong) == 0) return;
-    using L = LongSmem<DP>;
-    constexpr int KT = kRows, kBuf = L::kBuf, kThreads = 2 * kRows;
+    using L = DkvShape<DP>;
+    constexpr int KT = L::KT, kBuf = L::kBuf, kThreads = L::kThreads, N = L::N;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sk = tc::smem_addr(base), sv = sk + L::kT, sq = sv + L::kT, sg = sq + kBuf * L::kT, sp = sg + kBuf * L::kT,
                    sd = sp + L::kP;
-    KeyPos<KT>* kp = reinterpret_cast<KeyPos<KT>*>(base + L::kDkv);
+    KeyPos<KT>* kp = reinterpret_cast<KeyPos<KT>*>(base + L::kTiles);
     Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of both buffers' queries: 4 warps each, written in turn
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
     const int entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
-    float* E = reinterpret_cast<float*>(base + L::kDkv + L::kMisc);
+    float* E = reinterpret_cast<float*>(base + L::kBytes);
     const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
 
-    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * 64;
+    const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tk, p.windows, KT);
     const Loader<T, kThreads> ok(p.k, p.k_st, p.k_sh, p.dim, kvh), ov(p.v, p.v_st, p.v_sh, p.dim, kvh),
         oq(p.q, p.q_st, p.q_sh, p.dim, kvh * group), og(p.dout, p.do_st, p.do_sh, p.dim, kvh * group);
@@ -776,12 +837,9 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
 
-    AttnWalk walk;
-    for (int round = 0;; ++round) {
-        const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        if (at >= slots) break;
-        if (!walk.start(p.k_off, p.tk, p.q_off, p.tq, p.windows, 1, KT, at, at + 1)) continue;
-        const AttnTile& t = walk.tile;
+    LongWalk walk(slots, p);
+    for (bool more = walk.first(p.k_off, p.tk, p.q_off, p.tq, KT); more; more = walk.next()) {
+        const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.len <= p.short_max) continue;
         const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
@@ -847,11 +905,11 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
             alive = tc::mbar_wait(bar_s, par_s) && alive;
             par_s ^= 1;
             tc::fence_after();
-            float s[64], dp[64];
+            float s[N], dp[N];
             weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, lse, mode, E, kp, qp);
-            write_row<T>(sp + (j0 >> 6) * kRows * 128, row, s, 1.0f);
+            write_row<T>(sp, row, j0, s, 1.0f);
             score_gradients(s, dp, delta);
-            write_row<T>(sd + (j0 >> 6) * kRows * 128, row, dp, up);
+            write_row<T>(sd, row, j0, dp, up);
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
@@ -878,7 +936,7 @@ __global__ void __launch_bounds__(2 * kRows, 1) k_attn_dkv_long(const __grid_con
         }
         tc::fence_after();
         const bool of_v = tid < kRows;
-        finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, t.begin + t.first + min(row, n - 1), t.first + row, kvh, t.obegin, lq,
+        if (tid < 2 * kRows) finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, t.begin + t.first + min(row, n - 1), t.first + row, kvh, t.obegin, lq,
                               lk, i0, i1, z, up, of_v, alive);
         tc::fence_before();
     }
@@ -968,19 +1026,19 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
         // only rows and windows without partners: no bias is looked up
         const int bytes = 1024 + ShortSmem<DP>::kBytes;
         if ((err = smem_of(k_attn_bwd_short<T, DP, false>, bytes)) != cudaSuccess) return err;
-        k_attn_bwd_short<T, DP, false><<<dim3(p.short_blocks, p.kv_heads, 1), kRows, bytes, s>>>(p);
+        k_attn_bwd_short<T, DP, false><<<dim3(p.short_blocks, p.kv_heads, 1), 2 * kRows, bytes, s>>>(p);
     } else {
         if ((err = smem_of(k_attn_bwd_short<T, DP, BIAS>, b_short)) != cudaSuccess) return err;
-        k_attn_bwd_short<T, DP, BIAS><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), kRows, b_short, s>>>(p);
+        k_attn_bwd_short<T, DP, BIAS><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_short, s>>>(p);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    const int b_dq = 1024 + LongSmem<DP>::kDq + LongSmem<DP>::kMisc + entries * (4 + 12 * sum);
+    const int b_dq = 1024 + DqShape<DP>::kBytes + entries * (4 + 12 * sum);
     if ((err = smem_of(k_attn_dq_long<T, DP, BIAS>, b_dq)) != cudaSuccess) return err;
-    k_attn_dq_long<T, DP, BIAS><<<dim3(p.dq_blocks, p.heads), 2 * kRows, b_dq, s>>>(p);
+    k_attn_dq_long<T, DP, BIAS><<<dim3(p.dq_blocks, p.heads), DqShape<DP>::kThreads, b_dq, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    const int b_kv = 1024 + LongSmem<DP>::kDkv + LongSmem<DP>::kMisc + entries * 4;
+    const int b_kv = 1024 + DkvShape<DP>::kBytes + entries * 4;
     if ((err = smem_of(k_attn_dkv_long<T, DP, BIAS>, b_kv)) != cudaSuccess) return err;
-    k_attn_dkv_long<T, DP, BIAS><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_kv, s>>>(p);
+    k_attn_dkv_long<T, DP, BIAS><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), DkvShape<DP>::kThreads, b_kv, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     if (p.qsplits > 1) {
         const int64_t n = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;

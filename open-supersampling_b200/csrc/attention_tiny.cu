@@ -108,6 +108,21 @@ __device__ __forceinline__ void store_row16(T* row, int dim, const float (&o)[DB
     }
 }
 
+// Brings rows of an operand that are due in a few steps into L2: without it the loads in flight (16
+// rows a warp) cover a third of what HBM delivers in their latency. Lane i < 16: row r + i of this walk, or,
+// past its end, of the next one.
+constexpr int kAhead = 64;
+struct Ahead {
+    const char *now, *then;  // row 0 of this walk, and of the next (null: none)
+    int64_t step, end;       // bytes to the next row; rows of this walk
+    int then_end;
+    __device__ __forceinline__ void touch(int r) const {
+        const int i = r + (threadIdx.x & 15);
+        const char* at = i < end ? now + i * step : then != nullptr && i - end < then_end ? then + (i - end) * step : nullptr;
+        if (at != nullptr && (threadIdx.x & 31) < 16) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+    }
+};
+
 __device__ __forceinline__ float quad_sum(float x) {
     x += __shfl_xor_sync(0xffffffffu, x, 1);
     return x + __shfl_xor_sync(0xffffffffu, x, 2);
@@ -188,11 +203,21 @@ __device__ __forceinline__ Share share_of(int kv_heads) {
             static_cast<int>(gridDim.x) * (kWarps / side)};
 }
 
+// The rows of head gh of a window, then of the window's next head, or of the warp's next window.
+template <typename T>
+__device__ __forceinline__ Ahead ahead_of(const void* q, int64_t st, int64_t sh, int head0, int gh, int group, int64_t token, int rows, int next_q,
+                                          int next_rows) {
+    const T* p = static_cast<const T*>(q) + (head0 + gh) * sh;
+    const T* then = gh + 1 < group ? p + sh + token * st : next_rows > 0 ? p - gh * sh + next_q * st : nullptr;
+    return {reinterpret_cast<const char*>(p + token * st), reinterpret_cast<const char*>(then), st * static_cast<int64_t>(sizeof(T)), rows,
+            gh + 1 < group ? rows : next_rows};
+}
+
 // ---- forward --------------------------------------------------------------------------------
 // One window and key head, rows [r_begin, r_end), with NK blocks of 8 keys (the lower half of them full).
 template <typename T, int DB, int NK, bool BIAS>
 __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int group, int q0, int lq, int k0, int n, int r_begin,
-                                             int r_end, TinyPos<NK>* kp, const float* E, int entries) {
+                                             int r_end, TinyPos<NK>* kp, const float* E, int entries, int next_q, int next_rows) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float c2 = p.scale * kLog2e;
     uint32_t kr[NK][DB][4], vt[NK][DB][4];
@@ -224,6 +249,7 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
         uint32_t qa[DB][4], qb[DB][4];
         rq.load_at(qa, from, r_begin + g < r_end);
         rq.load_at(qb, from + 8 * p.q_st, r_begin + g + 8 < r_end);
+        const Ahead ahead = ahead_of<T>(p.q, p.q_st, p.q_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
         for (int r0 = r_begin; r0 < r_end; r0 += 16, to += 2 * to_step) {
             float s[NK][4];
 #pragma unroll
@@ -238,6 +264,7 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
                                  kr[kb][b][2 * h + 1]);
             }
             // the next rows are on their way meanwhile
+            ahead.touch(r0 - r_begin + kAhead);
             from += 16 * p.q_st;
             rq.load_at(qa, from, r0 + 16 + g < r_end);
             rq.load_at(qb, from + 8 * p.q_st, r0 + 24 + g < r_end);
@@ -334,12 +361,18 @@ __global__ void __launch_bounds__(32 * kWarps, DB == 1 ? 3 : 2) k_attn_fwd_tiny(
         const int per = ((lq + 15) / 16 + gridDim.z - 1) / gridDim.z * 16;
         const int r_begin = min(static_cast<int>(blockIdx.z) * per, lq), r_end = min(r_begin + per, lq);
         if (r_begin >= r_end) continue;
+        // the warp's next window, if it is of this kernel
+        int next_q = 0, next_rows = 0;
+        if (w + sh.step < p.windows) {
+            next_q = attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 1);
+            next_rows = gridDim.z > 1 ? 0 : attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 2) - next_q;
+        }
         if (n <= 16)
-            tiny_forward<T, DB, 2, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries);
+            tiny_forward<T, DB, 2, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, next_q, next_rows);
         else if (NB == 4 || n <= 32)
-            tiny_forward<T, DB, 4, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<4>*>(kp), Eh, entries);
+            tiny_forward<T, DB, 4, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<4>*>(kp), Eh, entries, next_q, next_rows);
         else
-            tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries);
+            tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, next_q, next_rows);
     }
 }
 
@@ -377,7 +410,8 @@ struct TinySums {
 // One window and key head, rows [r_begin, r_end), with NK blocks of 8 keys.
 template <typename T, int NK, bool BIAS>
 __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int group, int q0, int lq, int k0, int n, int r_begin, int r_end,
-                                              TinyPos<NK < 2 ? 2 : NK>* kp, const float* E, int entries, float up, TinySums& ts) {
+                                              TinyPos<NK < 2 ? 2 : NK>* kp, const float* E, int entries, float up, TinySums& ts, int next_q,
+                                              int next_rows) {
     constexpr int NP = NK < 2 ? 2 : NK;  // blocks of positions
     constexpr int NM = (NK + 1) / 2;     // 16-key steps
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -424,11 +458,15 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
             lse_at += 16;
         };
         fetch(r_begin);
+        const Ahead ahead_q = ahead_of<T>(p.q, p.q_st, p.q_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
+        const Ahead ahead_g = ahead_of<T>(p.dout, p.do_st, p.do_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
         for (int r0 = r_begin; r0 < r_end; r0 += 16, to += 2 * to_step) {
             uint32_t qa[4], qb[4], ga[4], gb[4];
             const float lse[2] = {nl[0], nl[1]};
 #pragma unroll
             for (int j = 0; j < 4; ++j) qa[j] = nqa[0][j], qb[j] = nqb[0][j], ga[j] = nga[0][j], gb[j] = ngb[0][j];
+            ahead_q.touch(r0 - r_begin + kAhead);
+            ahead_g.touch(r0 - r_begin + kAhead);
             fetch(r0 + 16);
             float s[NK][4], dp[NK][4];
 #pragma unroll
@@ -597,12 +635,18 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_attn_bwd_tiny(const __grid_c
         if (n > p.tiny_max || n == 0) continue;  // other kernels'
         const int per = ((lq + 15) / 16 + p.qsplits - 1) / p.qsplits * 16;
         const int r_begin = min(static_cast<int>(blockIdx.z) * per, lq), r_end = min(r_begin + per, lq);
+        // the warp's next window, if it is of this kernel
+        int next_q = 0, next_rows = 0;
+        if (w + sh.step < p.windows) {
+            next_q = attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 1);
+            next_rows = p.qsplits > 1 ? 0 : attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 2) - next_q;
+        }
         if (n <= 8)
-            tiny_backward<T, 1, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts);
+            tiny_backward<T, 1, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts, next_q, next_rows);
         else if (n <= 16)
-            tiny_backward<T, 2, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts);
+            tiny_backward<T, 2, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts, next_q, next_rows);
         else
-            tiny_backward<T, 4, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts);
+            tiny_backward<T, 4, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts, next_q, next_rows);
     }
     if constexpr (BIAS)
         if (grad_bias) {

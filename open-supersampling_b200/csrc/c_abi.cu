@@ -1325,9 +1325,10 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     const int64_t want = 2 * kSms / items, most = p.tq / windows * group / 512;
     const int64_t n = want < most ? want : most;
     p.qsplits = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
-    // resident blocks, or as many as there are tiles
+    // resident blocks (no more: a few blocks left over would take as long as all others again), or as
+    // many as there are tiles
     auto blocks = [](int64_t tiles, int64_t resident, int64_t heads) {
-        const int64_t per = (resident + heads - 1) / heads;
+        const int64_t per = resident / heads < 1 ? 1 : resident / heads;
         return static_cast<int>(tiles < per ? (tiles < 1 ? 1 : tiles) : per);
     };
     // The warp-level kernel: up to 32 columns and keys, where windows that short are likely, and the
@@ -1338,7 +1339,7 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     p.tiny_max = tiny ? 32 : 0;
     p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;
     p.short_blocks = blocks(windows, (p.dim <= 64 ? 2 : 1) * kSms, p.kv_heads * p.qsplits);
-    p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (sums ? 1 : 4) * kSms, p.heads);
+    p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (p.dim <= 64 ? 2 : 1) * (sums ? 1 : 4) * kSms, p.heads);
     p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, 128), 4 * kSms, p.kv_heads * p.qsplits);
     p.bias_tiny = p.tiny_blocks * p.qsplits;
     p.bias_short = p.short_max > 0 ? p.short_blocks * p.qsplits : 0;
