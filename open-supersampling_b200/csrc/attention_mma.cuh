@@ -39,7 +39,7 @@ struct Loader {
         const int chunks = ((dim + 15) / 16) * 2;
         shift = 32 - __clz(chunks - 1);  // lanes a row: the next power of two
         c = threadIdx.x & ((1 << shift) - 1);
-        r0 = threadIdx.x >> shift;
+        r0 = (threadIdx.x & (THREADS - 1)) >> shift;
         step = THREADS >> shift;  // 8 at least, so a chunk keeps its place in the swizzle from row to row
         on = c < chunks;
         zero = c * 8 >= dim;
@@ -144,6 +144,20 @@ __device__ __forceinline__ void load_key_pos(KeyPos<KT>* s, const AttnBias& b, i
     s->code[j] = p.x * (2 * b.rx + 1) + p.y;
     const Range r = warp_range(p);
     if ((j & 31) == 0) s->range[j >> 5] = r;
+}
+// The same by one warp.
+template <int KT>
+__device__ __forceinline__ void load_key_pos_warp(KeyPos<KT>* s, const AttnBias& b, int64_t token, int n) {
+#pragma unroll
+    for (int w = 0; w < KT / 32; ++w) {
+        const int j = 32 * w + (threadIdx.x & 31);
+        const int2 p = bias_pos(b.k_pos, b.axes, token + min(j, n - 1));
+        s->y[j] = p.x;
+        s->x[j] = p.y;
+        s->code[j] = p.x * (2 * b.rx + 1) + p.y;
+        const Range r = warp_range(p);
+        if ((j & 31) == 0) s->range[w] = r;
+    }
 }
 template <int KT>
 __device__ __forceinline__ Range key_range(const KeyPos<KT>* s) {

@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
     Range* qrange = reinterpret_cast<Range*>(kp + 1);
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     float* wsize = reinterpret_cast<float*>(bars + 4);
     float* wsum = wsize + 8;
     float* half_delta = reinterpret_cast<float*>(bars + 16);  // [2][kRows]
@@ -401,6 +402,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
         tc::mbar_init_fence();
+        *dead = 0;
     }
     if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
     if constexpr (BIAS)
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
                 tc::mma_nt<DP, kRows, KT>(tmem, sq, sk, dim16, id);
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= n);
             BiasMode mode = kOne;
             if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
-            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            alive = tc::mbar_wait(bar_s, par_s, dead) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
@@ -491,7 +493,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, L::kP), tc::desc(sg, kRows * 128), id_grad, it > i0);
                 tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, L::kP), tc::desc(sq, kRows * 128), id_grad, it > i0);
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
                 bs = bias_sum<8>(mode, wsize);
                 if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, j0, qp, I, wsum + warp);
             }
-            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
             par_o ^= 1;
             tc::fence_after();
             const int2 qp_now = qp;
@@ -622,6 +624,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     Range* qrange = reinterpret_cast<Range*>(kps + kBuf);
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     float* wsize = reinterpret_cast<float*>(bars + 8);
     float* wsum = wsize + 16;
     const int entries = BIAS ? bias_entries(p.bias) : 0, head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
@@ -639,6 +642,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
         tc::mbar_init_fence();
+        *dead = 0;
     }
     if (warp == 0) tc::tmem_alloc<L::kCols>(tc::smem_addr(slot_tmem));
     for (int e = tid; e < entries; e += kThreads) {
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
                 tc::mma_nt<DP, kRows, KT>(tmem, sq, sk + b * L::kK, dim16, id);
@@ -704,7 +708,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 bias_join<kThreads, kWarps, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (kt - 1) & 1 : 0), qp, I, wsum, acc);
             if (kBuf == 2) {
                 if (kt > 0) {  // dQ of the tile before: its keys and dS are free
-                    alive = tc::mbar_wait(bar_o, par_o) && alive;
+                    alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
                     par_o ^= 1;
                 }
                 if (grad_bias) __syncthreads();  // its key positions have been read
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             }
             BiasMode mode = kOne;
             if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
-            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            alive = tc::mbar_wait(bar_s, par_s, dead) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
@@ -727,7 +731,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint64_t dd = tc::desc(sd, 16), dk = tc::desc(sk + b * L::kK, KT * 128);
 #pragma unroll
@@ -741,7 +745,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 if (bs.fixed != 0.0f || bs.bad) bias_add<KT>(p, bs, dp, n16, head, kp, j0, qp, I, wsum + warp);
             }
             if (kBuf == 1) {
-                alive = tc::mbar_wait(bar_o, par_o) && alive;
+                alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
                 par_o ^= 1;
                 if (kt + 1 < tiles) {
                     if (grad_bias) {
@@ -758,7 +762,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             }
         }
         if (tiles > 0 && kBuf == 2) {
-            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
             par_o ^= 1;
         }
         tc::fence_after();
@@ -813,6 +817,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
     Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of both buffers' queries: 4 warps each, written in turn
     uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
+    volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     const int entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
     float* E = reinterpret_cast<float*>(base + L::kBytes);
     const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
@@ -825,6 +830,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
         tc::mbar_init_fence();
+        *dead = 0;
     }
     if (warp == 0) tc::tmem_alloc<512>(tc::smem_addr(slot_tmem));
     tc::fence_before();
@@ -883,7 +889,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
                 tc::mma_nt<DP, kRows, KT>(tmem, sq + b * L::kT, sk, dim16, id);
@@ -892,7 +898,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             }
             if (kBuf == 2) {
                 if (begun) {
-                    alive = tc::mbar_wait(bar_o, par_o) && alive;
+                    alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
                     par_o ^= 1;
                 }
                 if (after < i1) fetch(after, b ^ 1);
@@ -902,7 +908,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= t.first + n);
             BiasMode mode = kOne;
             if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
-            alive = tc::mbar_wait(bar_s, par_s) && alive;
+            alive = tc::mbar_wait(bar_s, par_s, dead) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
@@ -913,14 +919,14 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
-            if (tid == 0) {
+            if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, kRows * 128), tc::desc(sg + b * L::kT, kRows * 128), id_grad, begun);
                 tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, kRows * 128), tc::desc(sq + b * L::kT, kRows * 128), id_grad, begun);
                 tc::commit(bar_o);
             }
             if (kBuf == 1) {
-                alive = tc::mbar_wait(bar_o, par_o) && alive;
+                alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
                 par_o ^= 1;
                 if (after < i1) fetch(after, 0);
                 tc::cp_async_commit();
@@ -931,7 +937,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             it = after;
         }
         if (begun && kBuf == 2) {
-            alive = tc::mbar_wait(bar_o, par_o) && alive;
+            alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
             par_o ^= 1;
         }
         tc::fence_after();

@@ -28,11 +28,40 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, int parity) {
         : "memory");
     return done != 0;
 }
-// Bounded: a tile takes microseconds, the limit is seconds. False: it ran out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, int parity) {
-    for (int i = 0; i < (1 << 22); ++i)
+// Bounded: a tile takes microseconds, the limit is seconds. Once a wait of the block has run out
+// (*dead), the others give up as well. False: it ran out.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, int parity, volatile int* dead) {
+    for (int i = 0; i < (1 << 20); ++i) {
         if (mbar_try(bar, parity)) return true;
+        if ((i & 255) == 255 && *dead != 0) return false;
+    }
+    *dead = 1;
     return false;
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// One lane of a whole warp, always the same. Products are issued under it: with a plain test of the lane
+// the descriptors that reached them (they are warp-uniform registers) were not the ones computed.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
+}
+// Barrier `id` among `threads` threads of the block.
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// ---- tensor copies -------------------------------------------------------------
+// A box of a tensor of three axes into shared memory; completes `bar` by its bytes. x: a multiple of 8
+// 16-bit elements.
+__device__ __forceinline__ void tma_load(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
 }
 
 // ---- cp.async ----------------------------------------------------------------
