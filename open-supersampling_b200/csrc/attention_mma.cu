@@ -1,20 +1,17 @@
 // Window attention of 16-bit types on the tensor cores (tcgen05): forward.
 //
-// A block holds 128 query rows and walks its window's keys KT at a time. Four warps do the softmax
-// (thread = row = tensor-memory lane), a fifth moves the keys and values and issues the products:
+// A block holds 128 query rows and walks its window's keys 64 at a time. Four warps do the softmax
+// (thread = row = tensor-memory lane), one issues the products, one moves keys and values:
 //   S = Q K^T into tensor memory (both operands from shared memory)
 //   each thread reads its row of S, keeps the running maximum and sum in registers, and writes
 //   the weights back over S as 16-bit values
 //   O += P V, P from tensor memory
-// K of the next tile is on its way while the softmax runs, V while S is computed (a tensor copy each;
-// 16- or 4-byte copies or plain loads where strides or alignment allow none). Two or three blocks
-// share an SM and fill each other's waits. Tiles end at the window's last key rounded up to 16,
-// whatever KT is: N of S and K of P V are set by it.
+// S of the next tile is computed into a second buffer while the softmax runs, and two blocks share an
+// SM, so that the exponentials (16 a clock and SM) hardly pause. Keys and values arrive by tensor
+// copies, two tiles ahead; 16- or 4-byte copies or plain loads where strides or alignment allow none.
+// Tiles end at the window's last key rounded up to 16: N of S and K of P V are set by it.
 // The running maximum that the weights are taken against moves only when a row exceeds it by
 // 2^8: O has to be scaled in tensor memory then, which after the first tiles hardly happens.
-// With head dims up to 64 the exponentials (16 a clock and SM) bound long windows: 64-key tiles
-// leave room for three blocks. With 128 the products do, and 128-key tiles feed them from shared
-// memory at the full rate.
 #include <cuda.h>
 
 #include "attention_mma.cuh"
@@ -52,12 +49,12 @@ __device__ __noinline__ void forward_row(const AttnParams& p, int64_t token, int
 }
 
 // ---- forward ---------------------------------------------------------------------------
-template <int KT, int DP>
+template <int DP>
 struct FwdSmem {
-    static constexpr int kBuf = DP == 64 ? 2 : 1;  // tiles of keys, and of values
+    static constexpr int KT = 64;
     static constexpr int kQ = kRows * DP * 2, kK = KT * DP * 2;
-    static constexpr int kTiles = kQ + 2 * kBuf * kK;
-    static constexpr int kBytes = kTiles + kBuf * static_cast<int>(sizeof(KeyPos<KT>)) + 128;
+    static constexpr int kTiles = kQ + 4 * kK;  // two of keys, two of values
+    static constexpr int kBytes = kTiles + 2 * static_cast<int>(sizeof(KeyPos<KT>)) + 192;
 };
 
 // Keys or values by tensor copies: the map's axes are (column, head, token) or (column, token, head).
@@ -85,26 +82,24 @@ __device__ __forceinline__ void warp_load(uint32_t dst, int panel_rows, const vo
     }
 }
 
-template <typename T, int KT, int DP, bool BIAS>
-__global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps) {
-    using L = FwdSmem<KT, DP>;
-    constexpr int kCols = KT + DP, kBuf = L::kBuf;  // 128 or 256 columns: S (P over it), then O
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps) {
+    using L = FwdSmem<DP>;
+    constexpr int KT = L::KT, kCols = 256, kS = 64, kO = 128;  // columns: S (P over it) twice, then O
+    constexpr int kThreads = kRows + 64;
     constexpr int kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t sq = tc::smem_addr(base), sk = sq + L::kQ, sv = sk + kBuf * L::kK;
+    const uint32_t sq = tc::smem_addr(base), sk = sq + L::kQ, sv = sk + 2 * L::kK;
     KeyPos<KT>* kps = reinterpret_cast<KeyPos<KT>*>(base + L::kTiles);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(kps + kBuf);
-    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 14);
-    volatile int* dead = reinterpret_cast<volatile int*>(bars + 15);
-    float* E = reinterpret_cast<float*>(bars + 16);
-    const uint32_t bar0 = tc::smem_addr(bars);
-    // barriers: Q there, S done, P there, O done, then for each buffer K there, V there, positions there, positions read
-    const uint32_t bar_q = bar0, bar_s = bar0 + 8, bar_p = bar0 + 16, bar_o = bar0 + 24;
-    auto bar_k = [&](int b) { return bar0 + 32 + 8 * b; };
-    auto bar_v = [&](int b) { return bar0 + 48 + 8 * b; };
-    auto bar_pos = [&](int b) { return bar0 + 64 + 8 * b; };
-    auto bar_pos_read = [&](int b) { return bar0 + 80 + 8 * b; };
+    uint64_t* bars = reinterpret_cast<uint64_t*>(kps + 2);
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 20);
+    volatile int* dead = reinterpret_cast<volatile int*>(bars + 21);
+    float* E = reinterpret_cast<float*>(bars + 24);
+    // Barriers. One each: Q there, O done. For each buffer: P there (a softmax warp may be a tile ahead of
+    // another), S done, keys there and read, values there and read, key positions there and read.
+    const uint32_t bar0 = tc::smem_addr(bars), bar_q = bar0, bar_o = bar0 + 8, bar_p = bar0 + 16, bar_s = bar0 + 32, bar_k = bar0 + 48,
+                   bar_k_read = bar0 + 64, bar_v = bar0 + 80, bar_v_read = bar0 + 96, bar_pos = bar0 + 112, bar_pos_read = bar0 + 128;
 
     const int tid = threadIdx.x, warp = tid >> 5;
     const int head0 = blockIdx.y * p.pack, kvh = head0 / (p.heads / p.kv_heads);
@@ -120,15 +115,13 @@ __global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(c
     if (!more) return;
 
     if (tid == 0) {
-        for (int b = 0; b < 10; ++b) tc::mbar_init(bar0 + 8 * b, b == 0 || b == 2 ? kRows : 1);
-        tc::mbar_init(bar_pos_read(0), kRows);
-        tc::mbar_init(bar_pos_read(1), kRows);
+        for (int b = 0; b < 18; ++b) tc::mbar_init(bar0 + 8 * b, b == 0 || b == 2 || b == 3 || b >= 16 ? kRows : 1);
         tc::mbar_init_fence();
         *dead = 0;
     }
     if (warp == 0) tc::tmem_alloc<kCols>(tc::smem_addr(slot_tmem));
     if constexpr (BIAS)
-        for (int e = tid; e < entries * p.pack; e += kRows + 32) E[e] = bias_entry(p.bias, p.heads, head0 + e / entries, e % entries);
+        for (int e = tid; e < entries * p.pack; e += kThreads) E[e] = bias_entry(p.bias, p.heads, head0 + e / entries, e % entries);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -156,100 +149,101 @@ __global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(c
         return k;
     };
 
-    if (warp == 4) {
-        // ---- keys, values and products
-        const int lane = tid & 31;
-        const uint32_t id_o = tc::idesc(kBf16, dim16, false, true);
-        int par_q = 0, par_s = 0, par_p = 0, par_o = 0, count = 0;  // count: tiles of keys so far
+    // Every role counts the tiles of keys that it has passed: tile number u is in buffer u & 1, its barriers in
+    // their phase u >> 1.
+    int u = 0;
+    if (warp == 5) {
+        // ---- keys and values
+        const int lane = tid & 31, panels = dim16 > 64 ? 2 : 1;
         for (; more; more = walk.next()) {
             const AttnTile& t = walk.tile;
             const Keys kk = keys_of(t);
-            if (kk.tile0 >= kk.tile1) continue;
-            const int before = count - kk.tile0;  // tiles of keys before tile 0 of this one
-            auto tile_keys = [&](int kt) { return min(KT, kk.most - kt * KT); };
-            auto load = [&](bool values, int kt) {  // tile kt of K or V
-                const int b = kBuf == 2 ? (before + kt) & 1 : 0, n = tile_keys(kt);
-                const uint32_t dst = (values ? sv : sk) + b * L::kK;
-                const int token = t.obegin + kt * KT;
+            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++u) {
+                const int b = u & 1, parity = (u >> 1) & 1, n = min(KT, kk.most - kt * KT), token = t.obegin + kt * KT;
+                tc::mbar_wait(bar_k_read + 8 * b, parity ^ 1, dead);  // of two tiles before: passes at once at first
                 if (maps.use) {
                     if (tc::elect_one()) {
-                        const uint32_t bar = values ? bar_v(b) : bar_k(b);
-                        const int panels = dim16 > 64 ? 2 : 1;
-                        const bool ty = values ? maps.v_tokens_y : maps.k_tokens_y;
-                        tc::mbar_expect(bar, panels * KT * 128);
+                        tc::mbar_expect(bar_k + 8 * b, panels * KT * 128);
                         for (int h = 0; h < panels; ++h)
-                            tc::tma_load(dst + h * KT * 128, values ? &maps.v : &maps.k, bar, 64 * h, ty ? token : kvh, ty ? kvh : token);
+                            tc::tma_load(sk + b * L::kK + h * KT * 128, &maps.k, bar_k + 8 * b, 64 * h, maps.k_tokens_y ? token : kvh,
+                                         maps.k_tokens_y ? kvh : token);
                     }
-                } else if (values) {
-                    warp_load<T>(dst, KT, p.v, p.v_st, p.v_sh, p.dim, kvh, token, n, (n + 15) & ~15);
-                    tc::cp_async_commit();
                 } else {
-                    warp_load<T>(dst, KT, p.k, p.k_st, p.k_sh, p.dim, kvh, token, n, (n + 15) & ~15);
-                    tc::cp_async_commit();
+                    warp_load<T>(sk + b * L::kK, KT, p.k, p.k_st, p.k_sh, p.dim, kvh, token, n, (n + 15) & ~15);
                 }
-                if (BIAS && !values) {
-                    const int parity = ((before + kt) / kBuf) & 1;
-                    tc::mbar_wait(bar_pos_read(b), parity ^ 1, dead);  // passes at once the first time
+                tc::mbar_wait(bar_v_read + 8 * b, parity ^ 1, dead);
+                if (maps.use) {
+                    if (tc::elect_one()) {
+                        tc::mbar_expect(bar_v + 8 * b, panels * KT * 128);
+                        for (int h = 0; h < panels; ++h)
+                            tc::tma_load(sv + b * L::kK + h * KT * 128, &maps.v, bar_v + 8 * b, 64 * h, maps.v_tokens_y ? token : kvh,
+                                         maps.v_tokens_y ? kvh : token);
+                    }
+                } else {
+                    warp_load<T>(sv + b * L::kK, KT, p.v, p.v_st, p.v_sh, p.dim, kvh, token, n, (n + 15) & ~15);
+                    tc::cp_async_commit();
+                    tc::cp_async_wait<0>();
+                    tc::fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc::mbar_arrive(bar_k + 8 * b);
+                        tc::mbar_arrive(bar_v + 8 * b);
+                    }
+                }
+                if (BIAS) {
+                    tc::mbar_wait(bar_pos_read + 8 * b, parity ^ 1, dead);
                     load_key_pos_warp<KT>(kps + b, p.bias, token, n);
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(bar_pos(b));
+                    if (lane == 0) tc::mbar_arrive(bar_pos + 8 * b);
                 }
-            };
-            load(false, kk.tile0);
-            load(true, kk.tile0);
-            if (kBuf == 2 && kk.tile0 + 1 < kk.tile1) load(false, kk.tile0 + 1);
-            tc::mbar_wait(bar_q, par_q, dead);
-            par_q ^= 1;
-            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++count) {
-                const int b = kBuf == 2 ? count & 1 : 0, parity = (count / kBuf) & 1;
-                const int n = tile_keys(kt), n16 = (n + 15) & ~15;
-                if (kt > kk.tile0) {  // O of the tile before: P and its values are free
-                    tc::mbar_wait(bar_o, par_o, dead);
-                    par_o ^= 1;
-                    if (kBuf == 1) load(true, kt);
-                }
-                if (maps.use) {
-                    tc::mbar_wait(bar_k(b), parity, dead);
-                } else {
-                    tc::cp_async_wait<0>();
-                    tc::fence_async();
-                    __syncwarp();
-                }
+            }
+        }
+    } else if (warp == 4) {
+        // ---- products
+        const int lane = tid & 31;
+        const uint32_t id_o = tc::idesc(kBf16, dim16, false, true);
+        int par_q = 0, par_o = 0;
+        for (; more; more = walk.next()) {
+            const Keys kk = keys_of(walk.tile);
+            if (kk.tile0 >= kk.tile1) continue;
+            // S of tile kt, number v
+            auto scores = [&](int kt, int v) {
+                const int b = v & 1, n16 = (min(KT, kk.most - kt * KT) + 15) & ~15;
+                tc::mbar_wait(bar_k + 8 * b, (v >> 1) & 1, dead);
                 if (tc::elect_one()) {
                     tc::fence_after();
-                    tc::mma_nt<DP, kRows, KT>(tmem, sq, sk + b * L::kK, dim16, tc::idesc(kBf16, n16, false, false));
-                    tc::commit(bar_s);
+                    tc::mma_nt<DP, kRows, KT>(tmem + b * kS, sq, sk + b * L::kK, dim16, tc::idesc(kBf16, n16, false, false));
+                    tc::commit(bar_s + 8 * b);
+                    tc::commit(bar_k_read + 8 * b);
                 }
                 __syncwarp();
-                if (kBuf == 2 && kt + 1 < kk.tile1) {
-                    // the other buffers: of values since O above, of keys since the S before
-                    load(true, kt + 1);
+            };
+            tc::mbar_wait(bar_q, par_q, dead);
+            par_q ^= 1;
+            scores(kk.tile0, u);
+            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++u) {
+                const int b = u & 1, n = min(KT, kk.most - kt * KT), n16 = (n + 15) & ~15;
+                if (kt > kk.tile0) {  // P of the tile before has been read: its buffer takes the next S
+                    tc::mbar_wait(bar_o, par_o, dead);
+                    par_o ^= 1;
                 }
-                tc::mbar_wait(bar_s, par_s, dead);
-                par_s ^= 1;
-                if (kt + kBuf < kk.tile1) load(false, kt + kBuf);
-                tc::mbar_wait(bar_p, par_p, dead);
-                par_p ^= 1;
-                if (maps.use) {
-                    tc::mbar_wait(bar_v(b), parity, dead);
-                    if (n < n16) {  // what follows the window's last value meets weights of 0: it must not be NaN
-                        const int chunks = dim16 / 8;
-                        for (int i = lane; i < (n16 - n) * chunks; i += 32) {
-                            const int r = n + i / chunks, c = i % chunks;
-                            Loader<T, 32>::store_zero(sv + b * L::kK + (c >> 3) * KT * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                        }
-                        tc::fence_async();
-                        __syncwarp();
+                if (kt + 1 < kk.tile1) scores(kt + 1, u + 1);
+                tc::mbar_wait(bar_v + 8 * b, (u >> 1) & 1, dead);
+                if (maps.use && n < n16) {  // what follows the window's last value meets weights of 0: it must not be NaN
+                    const int chunks = dim16 / 8;
+                    for (int i = lane; i < (n16 - n) * chunks; i += 32) {
+                        const int r = n + i / chunks, c = i % chunks;
+                        Loader<T, 32>::store_zero(sv + b * L::kK + (c >> 3) * KT * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
                     }
-                } else {
-                    tc::cp_async_wait<0>();
                     tc::fence_async();
                     __syncwarp();
                 }
+                tc::mbar_wait(bar_p + 8 * b, (u >> 1) & 1, dead);
                 if (tc::elect_one()) {
                     tc::fence_after();
-                    tc::mma_tn<KT>(tmem + KT, tmem, sv + b * L::kK, n16, id_o, kt > kk.tile0);
+                    tc::mma_tn<KT>(tmem + kO, tmem + b * kS, sv + b * L::kK, n16, id_o, kt > kk.tile0);
                     tc::commit(bar_o);
+                    tc::commit(bar_v_read + 8 * b);
                 }
                 __syncwarp();
             }
@@ -258,9 +252,9 @@ __global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(c
         }
     } else {
         // ---- softmax
-        const uint32_t lane_at = static_cast<uint32_t>(warp * 32) << 16, ts = tmem + lane_at, to = ts + KT;
+        const uint32_t lane_at = static_cast<uint32_t>(warp * 32) << 16, to = tmem + lane_at + kO;
         const Loader<T, kRows> lq(p.q, p.q_st, p.q_sh, p.dim, head0);
-        int par_s = 0, par_o = 0, count = 0;
+        int par_o = 0;  // phase of O of the tile before
         bool alive = true;
         for (; more; more = walk.next()) {
             const AttnTile& t = walk.tile;
@@ -291,60 +285,46 @@ __global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(c
                 tc::fence_async();
                 tc::mbar_arrive(bar_q);
             }
-            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++count) {
-                const int k0 = kt * KT, n = min(KT, kk.most - k0), n16 = (n + 15) & ~15;
-                const KeyPos<KT>* kp = kps + (kBuf == 2 ? count & 1 : 0);
+            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++u) {
+                const int b = u & 1, k0 = kt * KT, n = min(KT, kk.most - k0), n16 = (n + 15) & ~15;
+                const uint32_t ts = tmem + lane_at + b * kS;
+                const KeyPos<KT>* kp = kps + b;
                 BiasMode mode = kOne;
                 if (BIAS) {
-                    alive = tc::mbar_wait(bar_pos(kBuf == 2 ? count & 1 : 0), (count / kBuf) & 1, dead) && alive;
+                    alive = tc::mbar_wait(bar_pos + 8 * b, (u >> 1) & 1, dead) && alive;
                     mode = bias_mode(p.bias, qr, key_range(kp));
                 }
-                alive = tc::mbar_wait(bar_s, par_s, dead) && alive;
-                par_s ^= 1;
+                alive = tc::mbar_wait(bar_s + 8 * b, (u >> 1) & 1, dead) && alive;
                 tc::fence_after();
-                // The row's scores, 64 at a time; with more, they are read twice (and, where the bias or the mask
-                // changed them, written back between), so that four warps' registers hold them.
-                constexpr int kPart = 64, kParts = KT / kPart;
-                const bool cut = n != n16 || k0 + n > kk.least;  // some rows see less of the tile
-                const int see = live ? (p.causal ? min(qt + kk.shift + 1, t.olen) : t.olen) - k0 : 0;
-                float s[kPart];
+                float s[KT];
+#pragma unroll
+                for (int c = 0; c < KT; c += 16)
+                    if (c < n16) tc::tmem_ld16(ts + c, s + c);
+                tc::wait_ld();
+                if (BIAS) {
+                    add_bias<KT>(s, c2, p.bias, mode, E + (live ? qh : 0) * entries, kp, 0, n16, qp);
+                    tc::mbar_arrive(bar_pos_read + 8 * b);
+                }
+                if (n != KT || k0 + n > kk.least) {  // some rows see less of the tile
+                    const int see = live ? (p.causal ? min(qt + kk.shift + 1, t.olen) : t.olen) - k0 : 0;
+#pragma unroll
+                    for (int c = 0; c < KT; ++c) s[c] = c < see ? s[c] : -INFINITY;
+                }
                 float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < kParts; ++h) {
-                    const int h0 = h * kPart;
-#pragma unroll
-                    for (int c = 0; c < kPart; c += 16)
-                        if (h0 + c < n16) tc::tmem_ld16(ts + h0 + c, s + c);
-                    tc::wait_ld();
-                    if (BIAS) {
-#pragma unroll
-                        for (int c = 0; c < kPart; c += 16)
-                            if (h0 + c < n16)
-                                add_bias<KT, 16>(*reinterpret_cast<float(*)[16]>(s + c), c2, p.bias, mode, E + (live ? qh : 0) * entries, kp, h0 + c, qp);
-                    }
-                    if (cut) {
-#pragma unroll
-                        for (int c = 0; c < kPart; ++c) s[c] = h0 + c < see ? s[c] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int c = 0; c < kPart; c += 16) {
-                        if (h0 + c >= n16) continue;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            top0 = fmaxf(top0, fmaxf(s[c + i], s[c + i + 1]));
-                            top1 = fmaxf(top1, fmaxf(s[c + i + 2], s[c + i + 3]));
-                        }
-                        if (kParts > 1 && (BIAS || cut)) tc::tmem_st16(ts + h0 + c, s + c);
-                    }
+                for (int c = 0; c < KT; c += 4) {
+                    top0 = fmaxf(top0, fmaxf(s[c], s[c + 1]));
+                    top1 = fmaxf(top1, fmaxf(s[c + 2], s[c + 3]));
                 }
-                if (kParts > 1 && (BIAS || cut)) tc::wait_st();
-                if (BIAS) tc::mbar_arrive(bar_pos_read(kBuf == 2 ? count & 1 : 0));
                 // the maximum passes NaN scores by: their weights are NaN whatever m is, and so is the row
                 const float top = fmaxf(top0, top1) * (BIAS ? 1.0f : c2);
                 const bool rise = top > m + 8.0f || (m == -INFINITY && top > m);
                 const float keep = rise ? ex2(m - top) : 1.0f;
                 if (rise) m = top;
-                if (kt > kk.tile0 && __any_sync(0xffffffffu, rise)) {  // O of the tiles before is there: S came after it
+                const bool scaled = kt > kk.tile0 && __any_sync(0xffffffffu, rise);
+                if (scaled) {
+                    alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
+                    tc::fence_after();
 #pragma unroll
                     for (int c = 0; c < DP; c += 16) {
                         if (c >= dim16) continue;
@@ -361,37 +341,32 @@ __global__ void __launch_bounds__(kRows + 32, KT == 64 ? 3 : 2) k_attn_fwd_mma(c
                 const float2 by = make_float2(BIAS ? 1.0f : c2, BIAS ? 1.0f : c2), off2 = make_float2(off, off);
                 float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
-                for (int h = 0; h < kParts; ++h) {
-                    const int h0 = h * kPart;
-                    if (kParts > 1) {
+                for (int c = 0; c < KT; c += 16) {
+                    if (c >= n16) continue;
+                    uint32_t w[8];
 #pragma unroll
-                        for (int c = 0; c < kPart; c += 16)
-                            if (h0 + c < n16) tc::tmem_ld16(ts + h0 + c, s + c);
-                        tc::wait_ld();
+                    for (int i = 0; i < 16; i += 4) {
+                        float2 x = make_float2(s[c + i], s[c + i + 1]), y = make_float2(s[c + i + 2], s[c + i + 3]);
+                        x = BIAS ? __fadd2_rn(x, off2) : __ffma2_rn(x, by, off2);
+                        y = BIAS ? __fadd2_rn(y, off2) : __ffma2_rn(y, by, off2);
+                        x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
+                        sum0 = __fadd2_rn(sum0, x);
+                        sum1 = __fadd2_rn(sum1, y);
+                        w[i / 2] = pack2(x.x, x.y, T{});
+                        w[i / 2 + 1] = pack2(y.x, y.y, T{});
                     }
-#pragma unroll
-                    for (int c = 0; c < kPart; c += 16) {
-                        if (h0 + c >= n16) continue;
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            float2 a = make_float2(s[c + i], s[c + i + 1]), b = make_float2(s[c + i + 2], s[c + i + 3]);
-                            a = BIAS ? __fadd2_rn(a, off2) : __ffma2_rn(a, by, off2);
-                            b = BIAS ? __fadd2_rn(b, off2) : __ffma2_rn(b, by, off2);
-                            a.x = ex2(a.x), a.y = ex2(a.y), b.x = ex2(b.x), b.y = ex2(b.y);
-                            sum0 = __fadd2_rn(sum0, a);
-                            sum1 = __fadd2_rn(sum1, b);
-                            w[i / 2] = pack2(a.x, a.y, T{});
-                            w[i / 2 + 1] = pack2(b.x, b.y, T{});
-                        }
-                        tc::tmem_st8(ts + (h0 + c) / 2, w);
-                    }
+                    tc::tmem_st8(ts + c / 2, w);
                 }
                 tc::wait_st();
+                if (kt > kk.tile0) {
+                    // O of the tile before. S runs ahead of O: seen only after this tile's weights are announced, its
+                    // phase could be told neither from the one before nor from the next.
+                    if (!scaled) alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
+                    par_o ^= 1;
+                }
                 tc::fence_before();
-                tc::mbar_arrive(bar_p);
+                tc::mbar_arrive(bar_p + 8 * b);
                 l = l * keep + ((sum0.x + sum0.y) + (sum1.x + sum1.y));
-                if (kt + 1 < kk.tile1) par_o ^= 1;  // the warp of the products waits for these
             }
             if (kk.tile0 < kk.tile1) {
                 alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
@@ -482,28 +457,28 @@ bool tile_map(CUtensorMap* map, int* tokens_y, const void* p, int64_t st, int64_
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int KT, int DP, bool BIAS>
+template <typename T, int DP, bool BIAS>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int entries = bias_entries(p.bias);
-    const int bytes = 1024 + FwdSmem<KT, DP>::kBytes + 4 * entries * p.pack;
-    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, KT, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = 1024 + FwdSmem<DP>::kBytes + 4 * entries * p.pack;
+    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
+    const int type = kIsBf16<T> ? kBF16 : kF16;
     TileMaps maps;
-    maps.use = p.dim % 8 == 0 &&
-               tile_map(&maps.k, &maps.k_tokens_y, p.k, p.k_st, p.k_sh, p.dim, p.kv_heads, p.tk, KT, kIsBf16<T> ? kBF16 : kF16) &&
-               tile_map(&maps.v, &maps.v_tokens_y, p.v, p.v_st, p.v_sh, p.dim, p.kv_heads, p.tk, KT, kIsBf16<T> ? kBF16 : kF16);
+    maps.use = p.dim % 8 == 0 && tile_map(&maps.k, &maps.k_tokens_y, p.k, p.k_st, p.k_sh, p.dim, p.kv_heads, p.tk, 64, type) &&
+               tile_map(&maps.v, &maps.v_tokens_y, p.v, p.v_st, p.v_sh, p.dim, p.kv_heads, p.tk, 64, type);
     // Blocks stay for several tiles of one head; four rounds of them even out tiles of unequal
     // length, one where each has to expand a bias first.
-    const int groups = p.heads / p.pack, resident = 148 * (KT == 64 ? 3 : 2) * (BIAS ? 1 : 4);
+    const int groups = p.heads / p.pack, resident = 148 * 2 * (BIAS ? 1 : 4);
     const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
     const int per_head = (resident + groups * p.splits - 1) / (groups * p.splits);
-    k_attn_fwd_mma<T, KT, DP, BIAS><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows + 32, bytes, s>>>(p, maps);
+    k_attn_fwd_mma<T, DP, BIAS><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows + 64, bytes, s>>>(p, maps);
     return cudaGetLastError();
 }
 template <typename T>
 cudaError_t fwd_type(const AttnParams& p, cudaStream_t s) {
-    if (p.bias.table != nullptr) return p.dim <= 64 ? fwd_one<T, 64, 64, true>(p, s) : fwd_one<T, 128, 128, true>(p, s);
-    return p.dim <= 64 ? fwd_one<T, 64, 64, false>(p, s) : fwd_one<T, 128, 128, false>(p, s);
+    if (p.bias.table != nullptr) return p.dim <= 64 ? fwd_one<T, 64, true>(p, s) : fwd_one<T, 128, true>(p, s);
+    return p.dim <= 64 ? fwd_one<T, 64, false>(p, s) : fwd_one<T, 128, false>(p, s);
 }
 
 }  // namespace

@@ -167,24 +167,31 @@ __device__ __forceinline__ Range key_range(const KeyPos<KT>* s) {
     return r;
 }
 
-// x[c] = x[c] c2 + bias of keys j0 + c, for a row at qp.
+// x[c] = x[c] c2 + bias of keys j0 + c, for a row at qp; keys up to n16 of the tile.
 template <int KT, int N>
 __device__ __forceinline__ void add_bias(float (&x)[N], float c2, const AttnBias& b, BiasMode mode, const float* E,
-                                         const KeyPos<KT>* k, int j0, int2 qp) {
+                                         const KeyPos<KT>* k, int j0, int n16, int2 qp) {
     const int w = 2 * b.rx + 1;
     if (mode == kOne) {
-        const float e = E[bias_index(b, qp, make_int2(k->y[j0], k->x[j0]))];
+        const float e = E[bias_index(b, qp, make_int2(k->y[0], k->x[0]))];
+        const float2 by = make_float2(c2, c2), add = make_float2(e, e);
 #pragma unroll
-        for (int c = 0; c < N; ++c) x[c] = fmaf(x[c], c2, e);
+        for (int c = 0; c < N; c += 2) {
+            const float2 y = __ffma2_rn(make_float2(x[c], x[c + 1]), by, add);
+            x[c] = y.x;
+            x[c + 1] = y.y;
+        }
     } else if (mode == kClamp) {
 #pragma unroll
-        for (int c = 0; c < N; ++c) x[c] = fmaf(x[c], c2, E[bias_index(b, qp, make_int2(k->y[j0 + c], k->x[j0 + c]))]);
+        for (int c = 0; c < N; ++c)
+            if (j0 + (c & ~15) < n16) x[c] = fmaf(x[c], c2, E[bias_index(b, qp, make_int2(k->y[j0 + c], k->x[j0 + c]))]);
     } else {
         const int* code = mode == kLinear ? k->code + j0 : k->x + j0;
-        const int dy = mode == kLinear ? -qp.x : min(max(k->y[j0] - qp.x, -b.ry), b.ry);
+        const int dy = mode == kLinear ? -qp.x : min(max(k->y[0] - qp.x, -b.ry), b.ry);
         const float* at = E + (dy + b.ry) * w + b.rx - qp.y;
 #pragma unroll
         for (int c = 0; c < N; c += 4) {
+            if (j0 + (c & ~15) >= n16) continue;
             const int4 q = *reinterpret_cast<const int4*>(code + c);
             x[c] = fmaf(x[c], c2, at[q.x]);
             x[c + 1] = fmaf(x[c + 1], c2, at[q.y]);

@@ -186,10 +186,14 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[N], floa
     }
     tc::wait_ld();
     const float2 by = make_float2(BIAS ? 1.0f : c2, BIAS ? 1.0f : c2), off = make_float2(-lse, -lse);
+    if constexpr (BIAS) add_bias<KT>(s, c2, p.bias, mode, E, kp, j0, n16, qp);
 #pragma unroll
     for (int c = 0; c < N; c += 16) {
-        if (j0 + c >= n16) continue;
-        if constexpr (BIAS) add_bias<KT, 16>(*reinterpret_cast<float(*)[16]>(s + c), c2, p.bias, mode, E, kp, j0 + c, qp);
+        if (j0 + c >= n16) {  // nothing of the bias stays there
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[c + i] = 0.0f;
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const float2 x = make_float2(s[c + i], s[c + i + 1]), y = BIAS ? __fadd2_rn(x, off) : __ffma2_rn(x, by, off);

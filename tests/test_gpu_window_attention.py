@@ -420,6 +420,24 @@ def test_many_windows(cuda_device):
     both(cuda_device, q, k, v, qo, ko, do)
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("lk", [60, 70, 130, 190])
+def test_blocks_that_walk_many_tiles(cuda_device, dim, lk):
+    """Far more tiles than blocks, of one to three tiles of keys, and of both parities in turn."""
+    g = torch.Generator().manual_seed(lk)
+    kl = (lk + torch.randint(-6, 7, (700,), generator=g)).tolist()
+    (q, k, v, do), qo, ko, _ = inputs([140] * 700, kl, 8, 4, dim, torch.bfloat16, seed=lk)
+    got = run(cuda_device, q, k, v, qo, ko, do)
+    again = run(cuda_device, q, k, v, qo, ko, do)
+    for n in got:
+        assert torch.equal(got[n], again[n])
+    for w in (0, 1, 2, 3, 350, 351, 697, 698, 699):  # the windows that are compared with the formula
+        a, b, c, e = qo[w], qo[w + 1], ko[w], ko[w + 1]
+        want = window_attention(q[a:b], k[c:e], v[c:e], [0, b - a], [0, e - c], dout=do[a:b])
+        for n, (lo, hi) in (("out", (a, b)), ("dq", (a, b)), ("dk", (c, e)), ("dv", (c, e))):
+            check(got[n][lo:hi], want[n], f"{n} of window {w}")
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_capture_and_replay(cuda_device, dtype):
     """Two graphs of a forward and backward each, replayed in turn with other inputs and offsets, on their own stream."""
@@ -493,3 +511,14 @@ def test_one_tensor_as_keys_and_values(cuda_device):
     want = window_attention(q, k, k, qo, ko, dout=do)
     check(dq, want["dq"])
     check(dk, tuple(a + b for a, b in zip(want["dk"], want["dv"])))
+
+
+def test_no_wait_ran_out(cuda_device):
+    """The waits inside the kernels are bounded; none of the calls above may have come to a bound."""
+    import ctypes
+
+    from oss_cuda import _lib
+
+    count = ctypes.c_uint32(7)
+    _lib.check(_lib.lib().oss_window_attention_timeouts(ctypes.addressof(count)), "oss_window_attention_timeouts")
+    assert count.value == 0
