@@ -3,12 +3,13 @@
 // and the backward of the three. norm(u) = (u - mean) r (layer) or u r (rms).
 //
 // Each row belongs to a group of lanes (8, 16 or 32 of a warp, or a whole block for rows of
-// more than 256 channels, of up to 256 threads or 1024); a lane keeps its 8 columns of the row and of the parameters in
-// registers, so that a call reads every activation once and writes every result once: HBM
-// bounds it. The backward takes x, h and the gate again and recomputes n and y in fp32 (y as
-// written would carry its rounding into every gradient), with the means and deviations of the
-// forward. Sums over rows go lane by lane in fp32 (one lane adds at most rows / groups terms),
-// then over the groups in double, always in the same order.
+// more than 256 channels, of up to 256 threads or 1024); a lane keeps its 8 columns of the row and
+// of the parameters in registers, so that a call reads every activation once and writes every
+// result once: HBM bounds it. Blocks stay and walk rows; the next row's values are on their way
+// while one is worked on. The backward takes x, h and the gate again and recomputes n and y in
+// fp32 (y as written would carry its rounding into every gradient), with the means and deviations
+// of the forward. Sums over rows go lane by lane in fp32 (one lane adds at most rows / groups terms),
+// over the groups of a block in order, then over the blocks in double, always in the same order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,27 +40,34 @@ __device__ __forceinline__ int col_of(int lane, int lanes, int i) {
     return ((i / V) * lanes + lane) * V + (i % V);
 }
 
+// A row's values as loaded. FULL: the lanes' columns end with the row.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(float (&out)[kElems], const T* p, int lane, int lanes, int c) {
+struct Raw {
+    Pack<T, V> v[kElems / V];
+};
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void fetch_row(Raw<T, V>& r, const T* p, bool live, int lane, int lanes, int c) {
 #pragma unroll
     for (int i = 0; i < kElems; i += V) {
         const int col = col_of<V>(lane, lanes, i);
-        if (col < c) {
-            const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(p + col);
-#pragma unroll
-            for (int v = 0; v < V; ++v) out[i + v] = up(t.v[v]);
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) out[i + v] = 0.0f;
-        }
+        if (live && (FULL || col < c)) r.v[i / V] = *reinterpret_cast<const Pack<T, V>*>(p + col);
     }
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_row(T* p, const float (&in)[kElems], int lane, int lanes, int c) {
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void unpack_row(float (&out)[kElems], const Raw<T, V>& r, bool live, int lane, int lanes, int c) {
+#pragma unroll
+    for (int i = 0; i < kElems; i += V) {
+        const bool on = live && (FULL || col_of<V>(lane, lanes, i) < c);
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[i + v] = on ? up(r.v[i / V].v[v]) : 0.0f;
+    }
+}
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void store_row(T* p, const float (&in)[kElems], bool live, int lane, int lanes, int c) {
 #pragma unroll
     for (int i = 0; i < kElems; i += V) {
         const int col = col_of<V>(lane, lanes, i);
-        if (col < c) {
+        if (live && (FULL || col < c)) {
             Pack<T, V> t;
 #pragma unroll
             for (int v = 0; v < V; ++v) down(t.v[v], in[i + v]);
@@ -83,9 +91,11 @@ __device__ __forceinline__ void load_param(float (&out)[kElems], const void* p, 
     }
 }
 
-// Sums of K values over the lanes of a row, the same in each of them.
+// Sums of K values over the lanes of a row, the same in each of them. `turn` alternates between the
+// two halves of `shared` (of 32 K_MAX floats each), so that one barrier a sum is enough.
+constexpr int kMostSums = 3;
 template <int TPR, int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], float* shared) {
+__device__ __forceinline__ void row_sum(float (&v)[K], float* shared, int& turn) {
     constexpr int W = TPR <= 0 ? 32 : TPR;
 #pragma unroll
     for (int x = W / 2; x > 0; x >>= 1)
@@ -93,15 +103,16 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* shared) {
         for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], x);
     if constexpr (TPR <= 0) {  // the whole block
         const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        __syncthreads();
+        float* at = shared + turn * 32 * kMostSums;
+        turn ^= 1;
         if ((threadIdx.x & 31) == 0)
 #pragma unroll
-            for (int k = 0; k < K; ++k) shared[k * 32 + warp] = v[k];
+            for (int k = 0; k < K; ++k) at[k * 32 + warp] = v[k];
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float s = 0.0f;
-            for (int w = 0; w < warps; ++w) s += shared[k * 32 + w];
+            for (int w = 0; w < warps; ++w) s += at[k * 32 + w];
             v[k] = s;
         }
     }
@@ -109,194 +120,237 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* shared) {
 
 // mean and 1 / deviation of a row; the deviation from centred values (a lane's absent columns
 // are left out).
-template <int TPR, int V>
-__device__ __forceinline__ float2 row_stats(const float (&u)[kElems], const GatedNorm& p, int lane, int lanes, float* shared) {
+template <int TPR, int V, bool FULL, bool LAYER>
+__device__ __forceinline__ float2 row_stats(const float (&u)[kElems], const GatedNorm& p, int lane, int lanes, float* shared, int& turn) {
     float mean = 0.0f;
-    if (p.layer) {
+    if (LAYER) {
         float s[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < kElems; ++i) s[0] += u[i];
-        row_sum<TPR>(s, shared);
+        row_sum<TPR>(s, shared, turn);
         mean = s[0] * p.inv_c;
     }
     float q[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < kElems; ++i) {
-        const float d = col_of<V>(lane, lanes, i) < p.c ? u[i] - mean : 0.0f;
+        const float d = !LAYER ? u[i] : FULL || col_of<V>(lane, lanes, i) < p.c ? u[i] - mean : 0.0f;
         q[0] = fmaf(d, d, q[0]);
     }
-    row_sum<TPR>(q, shared);
+    row_sum<TPR>(q, shared, turn);
     return make_float2(mean, rsqrtf(q[0] * p.inv_c + p.eps));
 }
 
-__device__ __forceinline__ float gate_value(float g, int act, float& slope) {
+// The gate's values to their activations, and with SLOPE to its slopes as well.
+template <bool SLOPE>
+__device__ __forceinline__ void activate(float (&g)[kElems], float (&slope)[kElems], int act) {
     if (act == 0) {
-        slope = 1.0f;
-        return g;
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) slope[i] = 1.0f;
+        return;
     }
-    const float s = 1.0f / (1.0f + __expf(-g));
-    if (act == 1) {
-        slope = s * (1.0f - s);
-        return s;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) {
+        const float s = __fdividef(1.0f, 1.0f + __expf(-g[i]));
+        if (act == 1) {
+            if (SLOPE) slope[i] = s * (1.0f - s);
+            g[i] = s;
+        } else {
+            if (SLOPE) slope[i] = s * (1.0f + g[i] * (1.0f - s));
+            g[i] *= s;
+        }
     }
-    slope = s * (1.0f + g * (1.0f - s));
-    return g * s;
 }
 
-template <typename T, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup) k_gated_norm_fwd(GatedNorm p) {
-    __shared__ float shared[TPR <= 0 ? 32 : 1];
+template <typename T, int TPR, int V, bool FULL, bool LAYER>
+__global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup, TPR < 0 ? 1 : 3) k_gated_norm_fwd(GatedNorm p) {
+    __shared__ float shared[TPR <= 0 ? 2 * 32 * kMostSums : 1];
     const int lanes = TPR <= 0 ? static_cast<int>(blockDim.x) : TPR, groups = static_cast<int>(blockDim.x) / lanes;
     const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-    float w[kElems], b[kElems], s[kElems], w2[kElems], b2[kElems];
+    int turn = 0;
+    float w[kElems], b[kElems] = {}, s[kElems], w2[kElems], b2[kElems] = {};
     load_param<V>(w, p.weight, p.param_type, 1.0f, lane, lanes, p.c);
-    load_param<V>(b, p.bias, p.param_type, 0.0f, lane, lanes, p.c);
+    if (LAYER) load_param<V>(b, p.bias, p.param_type, 0.0f, lane, lanes, p.c);
     load_param<V>(s, p.scale, p.param_type, 1.0f, lane, lanes, p.c);
     load_param<V>(w2, p.next_weight, p.param_type, 1.0f, lane, lanes, p.c);
-    load_param<V>(b2, p.next_bias, p.param_type, 0.0f, lane, lanes, p.c);
+    if (LAYER) load_param<V>(b2, p.next_bias, p.param_type, 0.0f, lane, lanes, p.c);
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) {  // scale (n w + b), the gate to come
+        w[i] *= s[i];
+        if (LAYER) b[i] *= s[i];
+    }
+    Raw<T, V> rx, rh, rg;
+    float one = 1.0f;
+    auto fetch = [&](int64_t row) {
+        const bool on = row < p.rows;
+        fetch_row<T, V, FULL>(rh, static_cast<const T*>(p.h) + row * p.h_st, on, lane, lanes, p.c);
+        fetch_row<T, V, FULL>(rx, static_cast<const T*>(p.x) + row * p.x_st, on, lane, lanes, p.c);
+        if (p.gate_kind == 2) fetch_row<T, V, FULL>(rg, static_cast<const T*>(p.gate) + row * p.g_st, on, lane, lanes, p.c);
+        if (p.gate_kind == 1) one = on ? up(static_cast<const T*>(p.gate)[row * p.g_st]) : 1.0f;
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group;
+    fetch(row);
     // whole blocks stay in the loop: the shuffles name every lane
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < p.rows; row0 += static_cast<int64_t>(gridDim.x) * groups) {
-        const int64_t row = row0 + group;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < p.rows; row0 += step, row += step) {
         const bool live = row < p.rows;
-        const int c = live ? p.c : 0;
-        float x[kElems], h[kElems], g[kElems];
-        load_row<T, V>(h, static_cast<const T*>(p.h) + (live ? row * p.h_st : 0), lane, lanes, c);
-        load_row<T, V>(x, static_cast<const T*>(p.x) + (live ? row * p.x_st : 0), lane, lanes, c);
+        float x[kElems], h[kElems], g[kElems], slope[kElems];
+        unpack_row<T, V, FULL>(h, rh, live, lane, lanes, p.c);
+        unpack_row<T, V, FULL>(x, rx, live, lane, lanes, p.c);
         if (p.gate_kind == 2) {
-            load_row<T, V>(g, static_cast<const T*>(p.gate) + (live ? row * p.g_st : 0), lane, lanes, c);
+            unpack_row<T, V, FULL>(g, rg, live, lane, lanes, p.c);
         } else {
-            const float one = p.gate_kind == 1 && live ? up(static_cast<const T*>(p.gate)[row * p.g_st]) : 1.0f;
 #pragma unroll
             for (int i = 0; i < kElems; ++i) g[i] = one;
         }
-        const float2 st1 = row_stats<TPR, V>(h, p, lane, lanes, shared);
+        fetch(row + step);
+        activate<false>(g, slope, p.act);
+        const float2 st1 = row_stats<TPR, V, FULL, LAYER>(h, p, lane, lanes, shared, turn);
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) {
-            float slope;
-            const float a = p.gate_kind == 0 ? 1.0f : gate_value(g[i], p.act, slope);
-            x[i] += s[i] * a * ((h[i] - st1.x) * st1.y * w[i] + b[i]);
-        }
-        store_row<T, V>(static_cast<T*>(p.y) + (live ? row * p.c : 0), x, lane, lanes, c);
+        for (int i = 0; i < kElems; ++i) x[i] = fmaf(g[i], LAYER ? fmaf((h[i] - st1.x) * st1.y, w[i], b[i]) : h[i] * st1.y * w[i], x[i]);
+        store_row<T, V, FULL>(static_cast<T*>(p.y) + row * p.c, x, live, lane, lanes, p.c);
         float2 st2 = make_float2(0.0f, 0.0f);
         if (p.z != nullptr) {
-            st2 = row_stats<TPR, V>(x, p, lane, lanes, shared);
+            st2 = row_stats<TPR, V, FULL, LAYER>(x, p, lane, lanes, shared, turn);
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) x[i] = (x[i] - st2.x) * st2.y * w2[i] + b2[i];
-            store_row<T, V>(static_cast<T*>(p.z) + (live ? row * p.c : 0), x, lane, lanes, c);
+            for (int i = 0; i < kElems; ++i) x[i] = LAYER ? fmaf((x[i] - st2.x) * st2.y, w2[i], b2[i]) : x[i] * st2.y * w2[i];
+            store_row<T, V, FULL>(static_cast<T*>(p.z) + row * p.c, x, live, lane, lanes, p.c);
         }
         if (p.stats != nullptr && live && lane == 0) p.stats[row] = make_float4(st1.x, st1.y, st2.x, st2.y);
     }
 }
 
-template <typename T, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup) k_gated_norm_bwd(GatedNorm p) {
-    __shared__ float shared[TPR <= 0 ? 96 : 1];
+template <typename T, int TPR, int V, bool FULL, bool LAYER>
+__global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup, TPR < 0 ? 1 : 2) k_gated_norm_bwd(GatedNorm p) {
+    __shared__ float shared[TPR <= 0 ? 2 * 32 * kMostSums : kGroup * kElems];
     const int lanes = TPR <= 0 ? static_cast<int>(blockDim.x) : TPR, groups = static_cast<int>(blockDim.x) / lanes;
     const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-    float w[kElems], b[kElems], s[kElems], w2[kElems];
+    int turn = 0;
+    float w[kElems], b[kElems] = {}, s[kElems], w2[kElems];
     load_param<V>(w, p.weight, p.param_type, 1.0f, lane, lanes, p.c);
-    load_param<V>(b, p.bias, p.param_type, 0.0f, lane, lanes, p.c);
+    if (LAYER) load_param<V>(b, p.bias, p.param_type, 0.0f, lane, lanes, p.c);
     load_param<V>(s, p.scale, p.param_type, 1.0f, lane, lanes, p.c);
     load_param<V>(w2, p.next_weight, p.param_type, 1.0f, lane, lanes, p.c);
     float dw[kElems] = {}, db[kElems] = {}, ds[kElems] = {}, dw2[kElems] = {}, db2[kElems] = {};
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < p.rows; row0 += static_cast<int64_t>(gridDim.x) * groups) {
-        const int64_t row = row0 + group;
+    Raw<T, V> rx, rh, rg, ry, rz;
+    float one = 1.0f;
+    float4 rst;
+    auto fetch = [&](int64_t row) {
+        const bool on = row < p.rows;
+        fetch_row<T, V, FULL>(rh, static_cast<const T*>(p.h) + row * p.h_st, on, lane, lanes, p.c);
+        fetch_row<T, V, FULL>(rx, static_cast<const T*>(p.x) + row * p.x_st, on, lane, lanes, p.c);
+        if (p.gate_kind == 2) fetch_row<T, V, FULL>(rg, static_cast<const T*>(p.gate) + row * p.g_st, on, lane, lanes, p.c);
+        if (p.gate_kind == 1) one = on ? up(static_cast<const T*>(p.gate)[row * p.g_st]) : 1.0f;
+        if (p.dz != nullptr) fetch_row<T, V, FULL>(rz, static_cast<const T*>(p.dz) + row * p.dz_st, on, lane, lanes, p.c);
+        if (p.dy != nullptr) fetch_row<T, V, FULL>(ry, static_cast<const T*>(p.dy) + row * p.dy_st, on, lane, lanes, p.c);
+        rst = on ? p.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group;
+    fetch(row);
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < p.rows; row0 += step, row += step) {
         const bool live = row < p.rows;
-        const int c = live ? p.c : 0;
-        float n[kElems], y[kElems], g[kElems], d[kElems];
-        load_row<T, V>(n, static_cast<const T*>(p.h) + (live ? row * p.h_st : 0), lane, lanes, c);
-        load_row<T, V>(y, static_cast<const T*>(p.x) + (live ? row * p.x_st : 0), lane, lanes, c);
+        float n[kElems], y[kElems], g[kElems], d[kElems], slope[kElems];
+        const float4 st = rst;
+        unpack_row<T, V, FULL>(n, rh, live, lane, lanes, p.c);
+        unpack_row<T, V, FULL>(y, rx, live, lane, lanes, p.c);
         if (p.gate_kind == 2) {
-            load_row<T, V>(g, static_cast<const T*>(p.gate) + (live ? row * p.g_st : 0), lane, lanes, c);
+            unpack_row<T, V, FULL>(g, rg, live, lane, lanes, p.c);
         } else {
-            const float one = p.gate_kind == 1 && live ? up(static_cast<const T*>(p.gate)[row * p.g_st]) : 1.0f;
 #pragma unroll
             for (int i = 0; i < kElems; ++i) g[i] = one;
         }
-        const float4 st = live ? p.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-        // y again, then its norm, from the forward's statistics
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) {
-            float slope;
-            const float a = p.gate_kind == 0 ? 1.0f : gate_value(g[i], p.act, slope);
-            n[i] = (n[i] - st.x) * st.y;
-            y[i] += s[i] * a * (n[i] * w[i] + b[i]);
-        }
-        if (p.dz != nullptr) {
-            float u[kElems];
-            load_row<T, V>(u, static_cast<const T*>(p.dz) + (live ? row * p.dz_st : 0), lane, lanes, c);
-            float m[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) {
-                y[i] = (y[i] - st.z) * st.w;  // absent columns: u is 0
-                dw2[i] = fmaf(u[i], y[i], dw2[i]);
-                db2[i] += u[i];
-                u[i] *= w2[i];
-                m[0] = fmaf(u[i], y[i], m[0]);
-                m[1] += u[i];
-            }
-            row_sum<TPR>(m, shared);
-            m[0] *= p.inv_c;
-            m[1] = p.layer ? m[1] * p.inv_c : 0.0f;
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) d[i] = (u[i] - y[i] * m[0] - m[1]) * st.w;
+        if (p.dy != nullptr) {
+            unpack_row<T, V, FULL>(d, ry, live, lane, lanes, p.c);
         } else {
 #pragma unroll
             for (int i = 0; i < kElems; ++i) d[i] = 0.0f;
         }
-        if (p.dy != nullptr) {
-            float u[kElems];
-            load_row<T, V>(u, static_cast<const T*>(p.dy) + (live ? row * p.dy_st : 0), lane, lanes, c);
+        float u[kElems];
+        if (p.dz != nullptr) unpack_row<T, V, FULL>(u, rz, live, lane, lanes, p.c);
+        fetch(row + step);
+        activate<true>(g, slope, p.act);
+        // y again, then its norm, from the forward's statistics
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) d[i] += u[i];
+        for (int i = 0; i < kElems; ++i) {
+            n[i] = (LAYER ? n[i] - st.x : n[i]) * st.y;
+            y[i] = fmaf(g[i] * s[i], LAYER ? fmaf(n[i], w[i], b[i]) : n[i] * w[i], y[i]);
         }
-        if (p.dx != nullptr) store_row<T, V>(static_cast<T*>(p.dx) + (live ? row * p.c : 0), d, lane, lanes, c);
+        if (p.dz != nullptr) {
+            float m[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                y[i] = (LAYER ? y[i] - st.z : y[i]) * st.w;  // absent columns: u is 0
+                dw2[i] = fmaf(u[i], y[i], dw2[i]);
+                if (LAYER) db2[i] += u[i];
+                u[i] *= w2[i];
+                m[0] = fmaf(u[i], y[i], m[0]);
+                if (LAYER) m[1] += u[i];
+            }
+            row_sum<TPR>(m, shared, turn);
+            m[0] *= p.inv_c;
+            m[1] *= p.inv_c;
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) d[i] = fmaf(LAYER ? u[i] - y[i] * m[0] - m[1] : u[i] - y[i] * m[0], st.w, d[i]);
+        }
+        if (p.dx != nullptr) store_row<T, V, FULL>(static_cast<T*>(p.dx) + row * p.c, d, live, lane, lanes, p.c);
         float m[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
-            if (col_of<V>(lane, lanes, i) >= c) d[i] = 0.0f;
-            float slope = 0.0f;
-            const float a = p.gate_kind == 0 ? 1.0f : gate_value(g[i], p.act, slope);
-            const float t = n[i] * w[i] + b[i];
-            const float da = d[i] * s[i] * t * slope;
-            ds[i] = fmaf(d[i] * a, t, ds[i]);
-            d[i] *= s[i] * a;  // dn
+            if (!live || (!FULL && col_of<V>(lane, lanes, i) >= p.c)) d[i] = 0.0f;
+            const float t = LAYER ? fmaf(n[i], w[i], b[i]) : n[i] * w[i], e = d[i] * g[i];
+            const float da = d[i] * slope[i] * (s[i] * t);
+            ds[i] = fmaf(e, t, ds[i]);
+            d[i] = e * s[i];  // dn
             dw[i] = fmaf(d[i], n[i], dw[i]);
-            db[i] += d[i];
+            if (LAYER) db[i] += d[i];
             d[i] *= w[i];
             m[0] = fmaf(d[i], n[i], m[0]);
-            m[1] += d[i];
+            if (LAYER) m[1] += d[i];
             m[2] += da;
             g[i] = da;
         }
-        row_sum<TPR>(m, shared);
+        row_sum<TPR>(m, shared, turn);
         if (p.dgate != nullptr) {
             if (p.gate_kind == 2)
-                store_row<T, V>(static_cast<T*>(p.dgate) + (live ? row * p.c : 0), g, lane, lanes, c);
+                store_row<T, V, FULL>(static_cast<T*>(p.dgate) + row * p.c, g, live, lane, lanes, p.c);
             else if (live && lane == 0)
                 down(static_cast<T*>(p.dgate)[row], m[2]);
         }
         if (p.dh != nullptr) {
             m[0] *= p.inv_c;
-            m[1] = p.layer ? m[1] * p.inv_c : 0.0f;
+            m[1] *= p.inv_c;
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) d[i] = (d[i] - n[i] * m[0] - m[1]) * st.y;
-            store_row<T, V>(static_cast<T*>(p.dh) + (live ? row * p.c : 0), d, lane, lanes, c);
+            for (int i = 0; i < kElems; ++i) d[i] = (LAYER ? d[i] - n[i] * m[0] - m[1] : d[i] - n[i] * m[0]) * st.y;
+            store_row<T, V, FULL>(static_cast<T*>(p.dh) + row * p.c, d, live, lane, lanes, p.c);
         }
     }
-    // a row of partial sums for each group: [5][gridDim.x groups][c]
-    const int64_t part = static_cast<int64_t>(blockIdx.x) * groups + group, parts = static_cast<int64_t>(gridDim.x) * groups;
+    // a row of partial sums for each block: [5][gridDim.x][c]
+    auto finish = [&](const float (&sum)[kElems], int which) {
+        float* to = p.partial + (static_cast<int64_t>(which) * gridDim.x + blockIdx.x) * p.c;
+        if constexpr (TPR <= 0) {
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-        const int col = col_of<V>(lane, lanes, i);
-        if (col >= p.c) continue;
-        p.partial[(0 * parts + part) * p.c + col] = dw[i];
-        p.partial[(1 * parts + part) * p.c + col] = ds[i];
-        p.partial[(2 * parts + part) * p.c + col] = dw2[i];
-        if (p.layer) {
-            p.partial[(3 * parts + part) * p.c + col] = db[i];
-            p.partial[(4 * parts + part) * p.c + col] = db2[i];
+            for (int i = 0; i < kElems; ++i) {
+                const int col = col_of<V>(lane, lanes, i);
+                if (col < p.c) to[col] = sum[i];
+            }
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) shared[group * lanes * kElems + col_of<V>(lane, lanes, i)] = sum[i];
+            __syncthreads();
+            for (int col = threadIdx.x; col < p.c; col += kGroup) {
+                float total = 0.0f;
+                for (int k = 0; k < groups; ++k) total += shared[k * lanes * kElems + col];
+                to[col] = total;
+            }
         }
+    };
+    finish(dw, 0);
+    finish(ds, 1);
+    finish(dw2, 2);
+    if (LAYER) {
+        finish(db, 3);
+        finish(db2, 4);
     }
 }
 
@@ -310,6 +364,7 @@ __global__ void __launch_bounds__(1024) k_gated_norm_reduce(GatedNorm p, int64_t
     double sum = 0.0;
     if (col < p.c) {
         const float* at = p.partial + static_cast<int64_t>(blockIdx.y) * parts * p.c + col;
+        #pragma unroll 4
         for (int64_t r = warp; r < parts; r += 32) sum += static_cast<double>(at[r * p.c]);
     }
     sums[warp][lane] = sum;
@@ -342,41 +397,55 @@ Shape shape_of(int64_t rows, int c, int most) {
     s.blocks = want < resident ? want : resident;
     return s;
 }
-constexpr int kFwdThreads = 1024, kBwdThreads = 768;
+constexpr int kFwdThreads = 3 * kGroup, kBwdThreads = 2 * kGroup;
 
+template <typename T, int V, bool FULL, bool LAYER>
+void fwd_full(const GatedNorm& p, const Shape& sh, cudaStream_t s) {
+    const unsigned g = static_cast<unsigned>(sh.blocks);
+    if (sh.tpr == 8)
+        k_gated_norm_fwd<T, 8, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
+    else if (sh.tpr == 16)
+        k_gated_norm_fwd<T, 16, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
+    else if (sh.tpr == 32)
+        k_gated_norm_fwd<T, 32, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
+    else if (sh.tpr == 0)
+        k_gated_norm_fwd<T, 0, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
+    else
+        k_gated_norm_fwd<T, -1, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
+}
 template <typename T, int V>
 cudaError_t fwd_vec(const GatedNorm& p, cudaStream_t s) {
     const Shape sh = shape_of(p.rows, p.c, kFwdThreads);
+    if (V > 1 && (sh.tpr > 0 ? sh.tpr : sh.threads) * kElems == p.c)
+        p.layer ? fwd_full<T, V, V != 1, true>(p, sh, s) : fwd_full<T, V, V != 1, false>(p, sh, s);
+    else
+        p.layer ? fwd_full<T, V, false, true>(p, sh, s) : fwd_full<T, V, false, false>(p, sh, s);
+    return cudaGetLastError();
+}
+template <typename T, int V, bool FULL, bool LAYER>
+void bwd_full(const GatedNorm& p, const Shape& sh, cudaStream_t s) {
     const unsigned g = static_cast<unsigned>(sh.blocks);
     if (sh.tpr == 8)
-        k_gated_norm_fwd<T, 8, V><<<g, sh.threads, 0, s>>>(p);
+        k_gated_norm_bwd<T, 8, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
     else if (sh.tpr == 16)
-        k_gated_norm_fwd<T, 16, V><<<g, sh.threads, 0, s>>>(p);
+        k_gated_norm_bwd<T, 16, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
     else if (sh.tpr == 32)
-        k_gated_norm_fwd<T, 32, V><<<g, sh.threads, 0, s>>>(p);
+        k_gated_norm_bwd<T, 32, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
     else if (sh.tpr == 0)
-        k_gated_norm_fwd<T, 0, V><<<g, sh.threads, 0, s>>>(p);
+        k_gated_norm_bwd<T, 0, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
     else
-        k_gated_norm_fwd<T, -1, V><<<g, sh.threads, 0, s>>>(p);
-    return cudaGetLastError();
+        k_gated_norm_bwd<T, -1, V, FULL, LAYER><<<g, sh.threads, 0, s>>>(p);
 }
 template <typename T, int V>
 cudaError_t bwd_vec(const GatedNorm& p, cudaStream_t s) {
     const Shape sh = shape_of(p.rows, p.c, kBwdThreads);
-    const unsigned g = static_cast<unsigned>(sh.blocks);
-    if (sh.tpr == 8)
-        k_gated_norm_bwd<T, 8, V><<<g, sh.threads, 0, s>>>(p);
-    else if (sh.tpr == 16)
-        k_gated_norm_bwd<T, 16, V><<<g, sh.threads, 0, s>>>(p);
-    else if (sh.tpr == 32)
-        k_gated_norm_bwd<T, 32, V><<<g, sh.threads, 0, s>>>(p);
-    else if (sh.tpr == 0)
-        k_gated_norm_bwd<T, 0, V><<<g, sh.threads, 0, s>>>(p);
+    if (V > 1 && (sh.tpr > 0 ? sh.tpr : sh.threads) * kElems == p.c)
+        p.layer ? bwd_full<T, V, V != 1, true>(p, sh, s) : bwd_full<T, V, V != 1, false>(p, sh, s);
     else
-        k_gated_norm_bwd<T, -1, V><<<g, sh.threads, 0, s>>>(p);
+        p.layer ? bwd_full<T, V, false, true>(p, sh, s) : bwd_full<T, V, false, false>(p, sh, s);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
-    k_gated_norm_reduce<<<dim3((p.c + 31) / 32, p.layer ? 5 : 3), 1024, 0, s>>>(p, sh.blocks * sh.groups);
+    k_gated_norm_reduce<<<dim3((p.c + 31) / 32, p.layer ? 5 : 3), 1024, 0, s>>>(p, sh.blocks);
     return cudaGetLastError();
 }
 
@@ -395,7 +464,7 @@ bool vectors(const GatedNorm& p, int elem) {
 
 int64_t gated_norm_partial_floats(int64_t rows, int c) {
     const Shape s = shape_of(rows, c, kBwdThreads);
-    return 5 * s.blocks * s.groups * c;
+    return 5 * s.blocks * c;
 }
 
 cudaError_t launch_gated_norm_forward(const GatedNorm& p, int type, cudaStream_t s) {
