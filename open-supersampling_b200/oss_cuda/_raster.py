@@ -37,6 +37,24 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+class on_device_of:
+    """torch.cuda.device(t.device) for a launch, at the cost of one comparison where that device is current already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, t: torch.Tensor):
+        index = t.device.index
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def check_float_cuda(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be CUDA")

@@ -17,7 +17,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._raster import check_int_cuda, stream_of
+from ._raster import check_int_cuda, on_device_of, stream_of
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_DIM = 128
@@ -30,37 +30,41 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
-def _strided(t: torch.Tensor):
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
 def _bias_args(table, buckets, q_pos, k_pos):
     if table is None:
-        return (None, 0, 0, None, 0, 0, None, None, 1)
-    return (table.data_ptr(), DTYPES[table.dtype], table.size(0), buckets.data_ptr(), (buckets.size(0) - 1) // 2,
-            (buckets.size(1) - 1) // 2, q_pos.data_ptr(), k_pos.data_ptr(), q_pos.dim())
+        return _NO_BIAS
+    ny, nx = buckets.shape
+    return (table.data_ptr(), DTYPES[table.dtype], table.size(0), buckets.data_ptr(), (ny - 1) // 2, (nx - 1) // 2,
+            q_pos.data_ptr(), k_pos.data_ptr(), q_pos.dim())
+
+
+_NO_BIAS = (None, 0, 0, None, 0, 0, None, None, 1)
+
+
+def _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos):
+    """The arguments that the forward and the backward entry points begin with."""
+    tq, h, d = q.shape
+    tk, kv, _ = k.shape
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return (DTYPES[q.dtype], tq, tk, q_offsets.size(0) - 1, h, kv, d, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+            v.data_ptr(), vs[0], vs[1], q_offsets.data_ptr(), k_offsets.data_ptr(), scale, causal,
+            *_bias_args(table, buckets, q_pos, k_pos))
 
 
 def attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos, want_lse):
     """(out, lse or None); arguments as checked by fused_window_cross_attention."""
     lib = _lib.lib()
-    with torch.cuda.device(q.device):
+    with on_device_of(q):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        tq, h, d = q.shape
-        tk, kv = k.size(0), k.size(1)
-        windows = q_offsets.numel() - 1
-        out = torch.empty((tq, h, d), device=q.device, dtype=q.dtype)
-        lse = torch.empty((h, tq), device=q.device, dtype=torch.float32) if want_lse else None
-        entries = 0 if table is None else buckets.numel()
-        nbytes = lib.oss_window_attention_scratch_bytes(tq, tk, windows, h, kv, d, entries)
-        scratch = torch.empty((nbytes,), device=q.device, dtype=torch.uint8) if nbytes else None
-        _lib.check(
-            lib.oss_window_attention_forward(DTYPES[q.dtype], tq, tk, windows, h, kv, d, *_strided(q), *_strided(k),
-                                             *_strided(v), q_offsets.data_ptr(), k_offsets.data_ptr(), scale, int(causal),
-                                             *_bias_args(table, buckets, q_pos, k_pos), out.data_ptr(), _lib.ptr(lse),
-                                             _lib.ptr(scratch), nbytes, stream_of(q)),
-            "oss_window_attention_forward",
-        )
+        args = _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos)
+        dev = q.device
+        out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        lse = torch.empty((q.size(1), q.size(0)), device=dev, dtype=torch.float32) if want_lse else None
+        nbytes = lib.oss_window_attention_scratch_bytes(*args[1:7], 0 if table is None else buckets.numel())
+        scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+        rc = lib.oss_window_attention_forward(*args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(scratch), nbytes, stream_of(q))
+        if rc:
+            _lib.check(rc, "oss_window_attention_forward")
     return out, lse
 
 
@@ -68,26 +72,23 @@ def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buck
                        want_table):
     """(d_q, d_k, d_v, d_table or None)."""
     lib = _lib.lib()
-    with torch.cuda.device(q.device):
+    with on_device_of(q):
         q, k, v, grad = _rows(q), _rows(k), _rows(v), _rows(grad)
-        tq, h, d = q.shape
-        tk, kv = k.size(0), k.size(1)
-        dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
-        dtable = torch.empty_like(table, memory_format=torch.contiguous_format) if want_table else None
-        windows = q_offsets.numel() - 1
-        nbytes = lib.oss_window_attention_backward_scratch_bytes(DTYPES[q.dtype], tq, tk, windows, h, kv, d, int(causal),
-                                                                 0 if table is None else buckets.numel(),
+        args = _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos)
+        dev, dtype = q.device, q.dtype
+        dq = torch.empty(q.shape, device=dev, dtype=dtype)
+        dk = torch.empty(k.shape, device=dev, dtype=dtype)
+        dv = torch.empty(k.shape, device=dev, dtype=dtype)
+        dtable = torch.empty(table.shape, device=dev, dtype=table.dtype) if want_table else None
+        nbytes = lib.oss_window_attention_backward_scratch_bytes(*args[:7], causal, 0 if table is None else buckets.numel(),
                                                                  table.size(0) if want_table else 0)
-        scratch = torch.empty((max(1, nbytes),), device=q.device, dtype=torch.uint8)
-        _lib.check(
-            lib.oss_window_attention_backward(DTYPES[q.dtype], tq, tk, windows, h, kv, d, *_strided(q),
-                                              *_strided(k), *_strided(v), q_offsets.data_ptr(), k_offsets.data_ptr(),
-                                              scale, int(causal), *_bias_args(table, buckets, q_pos, k_pos),
-                                              out.data_ptr(), lse.data_ptr(), *_strided(grad), dq.data_ptr(),
-                                              dk.data_ptr(), dv.data_ptr(), _lib.ptr(dtable), scratch.data_ptr(),
-                                              scratch.numel(), stream_of(q)),
-            "oss_window_attention_backward",
-        )
+        scratch = torch.empty(max(1, nbytes), device=dev, dtype=torch.uint8)
+        gs = grad.stride()
+        rc = lib.oss_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), gs[0], gs[1],
+                                               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dtable),
+                                               scratch.data_ptr(), nbytes, stream_of(q))
+        if rc:
+            _lib.check(rc, "oss_window_attention_backward")
     return dq, dk, dv, dtable
 
 
@@ -165,36 +166,40 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
     inputs the weights are rounded to their type before they meet v.  A value that is not finite reaches only
     the rows whose window and mask show it.  To capture a backward into a graph, drop earlier eager graphs of
     the same leaves first."""
+    dtype, dev, qs, ks = q.dtype, q.device, q.shape, k.shape
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be CUDA")
         if t.dim() != 3:
             raise RuntimeError(f"{name} must be (tokens, heads, head dim)")
-        if t.dtype not in DTYPES:
-            raise RuntimeError(f"{name} must be fp32, bf16 or fp16")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise RuntimeError("q, k and v must have one type and device")
-    if k.shape != v.shape or k.size(2) != q.size(2):
+        if t.dtype is not dtype or t.device != dev or dtype not in DTYPES:
+            raise RuntimeError("q, k and v must be fp32, bf16 or fp16, of one type and device")
+    if ks != v.shape or ks[2] != qs[2]:
         raise RuntimeError("k and v must have the same shape and q's head dim")
-    if not 1 <= q.size(2) <= MAX_HEAD_DIM:
+    if not 1 <= qs[2] <= MAX_HEAD_DIM:
         raise RuntimeError(f"head dim must be in [1, {MAX_HEAD_DIM}]")
-    if k.size(1) < 1 or q.size(1) < 1 or q.size(1) % k.size(1) != 0:
+    if ks[1] < 1 or qs[1] < 1 or qs[1] % ks[1] != 0:
         raise RuntimeError("the heads of q must be a multiple of those of k")
-    if max(q.size(0), k.size(0)) >= MAX_TOKENS:
+    if qs[0] >= MAX_TOKENS or ks[0] >= MAX_TOKENS:
         raise RuntimeError("at most 2**30 - 1 tokens")
     for t, name in ((q_offsets, "q_offsets"), (k_offsets, "k_offsets")):
         check_int_cuda(t, name)
-        if t.dim() != 1 or t.numel() < 1 or t.device != q.device:
+        if t.dim() != 1 or t.size(0) < 1 or t.device != dev:
             raise RuntimeError(f"{name} must be (windows + 1,) on q's device")
-    if q_offsets.numel() != k_offsets.numel():
+    if q_offsets.size(0) != k_offsets.size(0):
         raise RuntimeError("q_offsets and k_offsets must have the same length")
-    _check_bias(q, k, bias_table, buckets, q_pos, k_pos)
-    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    if bias_table is not None or buckets is not None or q_pos is not None or k_pos is not None:
+        _check_bias(q, k, bias_table, buckets, q_pos, k_pos)
+    scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
     if not 0.0 < scale < 3.0e38:
         raise ValueError("scale must be positive and finite")
     if bias_table is not None:
         bias_table = bias_table.contiguous()
-    return _WindowAttention.apply(q, k, v, q_offsets, k_offsets, scale, bool(causal), bias_table, buckets, q_pos, k_pos)
+    args = (q, k, v, q_offsets, k_offsets, scale, int(bool(causal)), bias_table, buckets, q_pos, k_pos)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (bias_table is not None and bias_table.requires_grad)):
+        return _WindowAttention.apply(*args)
+    return attention_forward(*args, False)[0]
 
 
 def window_position_buckets(reach_y: int, reach_x: int, device=None) -> torch.Tensor:

@@ -11,7 +11,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._raster import stream_of
+from ._raster import on_device_of, stream_of
 from .attention import DTYPES
 
 KINDS = ("rms", "layer")
@@ -21,35 +21,42 @@ MAX_CHANNELS = 8192
 
 def _rows(t: torch.Tensor, c: int) -> torch.Tensor:
     """t as (rows, c) with unit last stride: a view where its strides allow one."""
-    t = t.reshape(-1, c)
+    if t.dim() != 2:
+        t = t.reshape(-1, c)
     return t if t.stride(1) == 1 or c == 1 else t.contiguous()
 
 
-def _ptr_stride(t):
-    return (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+def _call_args(x, h, gate, params, layer, act, eps):
+    """The arguments that the forward and the backward entry points begin with."""
+    rows, c = x.shape
+    ptr = _lib.ptr
+    weight, bias, scale, next_weight, next_bias = params
+    if gate is None:
+        g = (None, 0, 0)
+    else:
+        g = (gate.data_ptr(), gate.stride(0), 2 if gate.size(1) == c and c > 1 else 1)
+    return (DTYPES[x.dtype], rows, c, x.data_ptr(), x.stride(0), h.data_ptr(), h.stride(0), *g, act, layer, eps,
+            DTYPES[weight.dtype], weight.data_ptr(), ptr(bias), ptr(scale), ptr(next_weight), ptr(next_bias))
 
 
-def _gate_kind(gate, c):
-    return 0 if gate is None else 2 if gate.size(1) == c and c > 1 else 1
+def norm_forward(x, h, gate, params, layer, act, eps, want_stats):
+    """(y, z or None, stats or None) of rows."""
+    with on_device_of(x):
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        z = torch.empty(x.shape, device=x.device, dtype=x.dtype) if params[3] is not None else None
+        stats = torch.empty((x.size(0), 4), device=x.device, dtype=torch.float32) if want_stats else None
+        rc = _lib.lib().oss_gated_norm_forward(*_call_args(x, h, gate, params, layer, act, eps), y.data_ptr(), _lib.ptr(z),
+                                               _lib.ptr(stats), stream_of(x))
+        if rc:
+            _lib.check(rc, "oss_gated_norm_forward")
+    return y, z, stats
 
 
 class _GatedNorm(Function):
     @staticmethod
     def forward(ctx, x, h, gate, weight, bias, scale, next_weight, next_bias, layer, act, eps):
-        lib = _lib.lib()
-        rows, c = x.shape
         params = (weight, bias, scale, next_weight, next_bias)
-        with torch.cuda.device(x.device):
-            y = torch.empty((rows, c), device=x.device, dtype=x.dtype)
-            z = torch.empty_like(y) if next_weight is not None else None
-            stats = torch.empty((rows, 4), device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
-            _lib.check(
-                lib.oss_gated_norm_forward(DTYPES[x.dtype], rows, c, *_ptr_stride(x), *_ptr_stride(h), *_ptr_stride(gate),
-                                           _gate_kind(gate, c), act, layer, eps, DTYPES[weight.dtype],
-                                           *(_lib.ptr(t) for t in params), y.data_ptr(), _lib.ptr(z), _lib.ptr(stats),
-                                           stream_of(x)),
-                "oss_gated_norm_forward",
-            )
+        y, z, stats = norm_forward(x, h, gate, params, layer, act, eps, True)
         ctx.save_for_backward(x, h, gate, *params, stats)
         ctx.meta = (layer, act, eps)
         ctx.set_materialize_grads(False)
@@ -60,31 +67,30 @@ class _GatedNorm(Function):
     def backward(ctx, dy, dz):
         if dy is None and dz is None:
             return (None,) * 11
-        lib = _lib.lib()
+        lib, ptr = _lib.lib(), _lib.ptr
         x, h, gate, *params, stats = ctx.saved_tensors
-        layer, act, eps = ctx.meta
         rows, c = x.shape
         need = ctx.needs_input_grad
-        with torch.cuda.device(x.device):
+        with on_device_of(x):
+            dev, dtype = x.device, x.dtype
             dy, dz = (None if t is None else _rows(t, c) for t in (dy, dz))
-            dx, dh = (torch.empty((rows, c), device=x.device, dtype=x.dtype) if n else None for n in need[:2])
-            dgate = torch.empty(gate.shape, device=x.device, dtype=x.dtype) if need[2] else None
-            dparams = [torch.empty_like(t) if n else None for t, n in zip(params, need[3:8])]
-            # without dz the second norm takes no part
-            zeros = [i for i in (3, 4) if dz is None and dparams[i] is not None]
-            for i in zeros:
-                dparams[i].zero_()
+            dx = torch.empty((rows, c), device=dev, dtype=dtype) if need[0] else None
+            dh = torch.empty((rows, c), device=dev, dtype=dtype) if need[1] else None
+            dgate = torch.empty(gate.shape, device=dev, dtype=dtype) if need[2] else None
+            dparams = [torch.empty(c, device=dev, dtype=t.dtype) if n else None for t, n in zip(params, need[3:8])]
+            wanted = [ptr(t) for t in dparams]
+            if dz is None:  # the second norm takes no part
+                for i in (3, 4):
+                    if dparams[i] is not None:
+                        dparams[i].zero_()
+                        wanted[i] = None
             nbytes = lib.oss_gated_norm_backward_scratch_bytes(rows, c)
-            scratch = torch.empty((max(16, nbytes),), device=x.device, dtype=torch.uint8)
-            _lib.check(
-                lib.oss_gated_norm_backward(DTYPES[x.dtype], rows, c, *_ptr_stride(x), *_ptr_stride(h), *_ptr_stride(gate),
-                                            _gate_kind(gate, c), act, layer, eps, DTYPES[params[0].dtype],
-                                            *(_lib.ptr(t) for t in params), stats.data_ptr(), *_ptr_stride(dy),
-                                            *_ptr_stride(dz), _lib.ptr(dx), _lib.ptr(dh), _lib.ptr(dgate),
-                                            *(None if i in zeros else _lib.ptr(t) for i, t in enumerate(dparams)),
-                                            scratch.data_ptr(), scratch.numel(), stream_of(x)),
-                "oss_gated_norm_backward",
-            )
+            scratch = torch.empty(max(16, nbytes), device=dev, dtype=torch.uint8)
+            rc = lib.oss_gated_norm_backward(*_call_args(x, h, gate, params, *ctx.meta), stats.data_ptr(), ptr(dy),
+                                             0 if dy is None else dy.stride(0), ptr(dz), 0 if dz is None else dz.stride(0),
+                                             ptr(dx), ptr(dh), ptr(dgate), *wanted, scratch.data_ptr(), nbytes, stream_of(x))
+            if rc:
+                _lib.check(rc, "oss_gated_norm_backward")
         return dx, dh, dgate, *dparams, None, None, None
 
 
@@ -114,31 +120,45 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
         raise ValueError("biases are for kind='layer'")
     if next_bias is not None and next_weight is None:
         raise ValueError("next_bias needs next_weight")
+    dtype, dev, shape = x.dtype, x.device, x.shape
     for t, name in ((x, "x"), (h, "h"), (gate, "gate")):
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be CUDA")
-        if t.dtype not in DTYPES or t.dtype != x.dtype or t.device != x.device:
+        if t.dtype is not dtype or t.device != dev or dtype not in DTYPES:
             raise RuntimeError("x, h and gate must be fp32, bf16 or fp16, of one type and device")
-    if x.dim() < 1 or not 1 <= x.size(-1) <= MAX_CHANNELS:
+    if len(shape) < 1 or not 1 <= shape[-1] <= MAX_CHANNELS:
         raise RuntimeError(f"x must be (..., C) with C in [1, {MAX_CHANNELS}]")
-    if h.shape != x.shape:
+    if h.shape != shape:
         raise RuntimeError("h must have x's shape")
-    c = x.size(-1)
-    if gate is not None and (gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1] or gate.size(-1) not in (1, c)):
+    c = shape[-1]
+    if gate is not None and (gate.dim() != len(shape) or gate.shape[:-1] != shape[:-1] or gate.shape[-1] not in (1, c)):
         raise RuntimeError("gate must be (..., C) or (..., 1)")
-    for t, name in ((weight, "weight"), (next_weight, "next_weight"), (scale, "scale"), (bias, "bias"),
-                    (next_bias, "next_bias")):
-        if t is None:
-            if name == "weight":
-                raise RuntimeError("weight must be given")
-            continue
-        if t.device != x.device or t.dim() != 1 or t.size(0) != c:
-            raise RuntimeError(f"{name} must be (C,) on x's device")
-        if t.dtype not in (torch.float32, x.dtype) or t.dtype != weight.dtype:
-            raise RuntimeError("parameters must be of one type, fp32 or x's")
-    g = None if gate is None else _rows(gate, gate.size(-1))
-    params = [None if t is None else t.contiguous() for t in (weight, bias, scale, next_weight, next_bias)]
-    y, z = _GatedNorm.apply(_rows(x, c), _rows(h, c), g, *params, int(kind == "layer"), ACTS[gate_act], eps)
-    return (y.view(x.shape), z.view(x.shape)) if z is not None else y.view(x.shape)
+    if weight is None:
+        raise RuntimeError("weight must be given")
+    wtype = weight.dtype
+    if wtype is not torch.float32 and wtype is not dtype:
+        raise RuntimeError("parameters must be of one type, fp32 or x's")
+    grad = torch.is_grad_enabled() and (x.requires_grad or h.requires_grad or (gate is not None and gate.requires_grad))
+    want_grad = torch.is_grad_enabled()
+    params = []
+    for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale"), (next_weight, "next_weight"), (next_bias, "next_bias")):
+        if t is not None:
+            if t.device != dev or t.dim() != 1 or t.size(0) != c:
+                raise RuntimeError(f"{name} must be (C,) on x's device")
+            if t.dtype is not wtype:
+                raise RuntimeError("parameters must be of one type, fp32 or x's")
+            grad = grad or (want_grad and t.requires_grad)
+            t = t.contiguous()
+        params.append(t)
+    x2, h2 = _rows(x, c), _rows(h, c)
+    g2 = None if gate is None else _rows(gate, gate.shape[-1])
+    layer, act = int(kind == "layer"), ACTS[gate_act]
+    if grad:
+        y, z = _GatedNorm.apply(x2, h2, g2, *params, layer, act, eps)
+    else:
+        y, z, _ = norm_forward(x2, h2, g2, params, layer, act, eps, False)
+    if len(shape) != 2:
+        y, z = y.view(shape), None if z is None else z.view(shape)
+    return y if z is None else (y, z)
