@@ -2,8 +2,8 @@
 //
 // Tiles of BM queries x 64 keys. 256 threads as 16 x 16: thread (ty, tx) holds rows ty RM + i and
 // keys tx + 16 c of a tile of scores, and rows ty RM + i, columns tx CN + c of an output tile.
-// Every product runs on FFMA from shared memory, 16 RM FMAs for RM + 4 16-byte loads, so that
-// the FP32 pipe (128 lanes a clock and SM) bounds it and not shared memory.
+// Every product runs on the FP32 pipe from shared memory, 16 RM FMAs for RM + 4 16-byte loads, two
+// FMAs an instruction, so that the pipe (128 lanes a clock and SM) bounds it and not shared memory.
 #include "attention.cuh"
 #include "internal.h"
 
@@ -50,59 +50,78 @@ __device__ __forceinline__ void load_rows(float* dst, const void* src, int64_t s
     }
 }
 
-// acc[i][c] += A[ty RM + i] . B[tx + 16 c] over DP
-template <int DP, int RM>
-__device__ __forceinline__ void dot_rows(float (&acc)[RM][4], const float* A, const float* B, int ty, int tx) {
+// acc[i][c] = A[ty RM + i] . B[tx + 16 c] over DP for c < NC: even and odd columns are two sums, so
+// that one instruction does both.
+template <int DP, int RM, int NC>
+__device__ __forceinline__ void dot_cols(float (&acc)[RM][4], const float* A, const float* B, int ty, int tx) {
     constexpr int LD = DP + 4;
+    float2 t[RM][NC] = {};
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-        float4 a[RM], b[4];
+        float4 a[RM], b[NC];
 #pragma unroll
         for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4*>(A + (ty * RM + i) * LD + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * LD + d);
+        for (int c = 0; c < NC; ++c) b[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * LD + d);
 #pragma unroll
         for (int i = 0; i < RM; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                acc[i][c] = fmaf(a[i].x, b[c].x, acc[i][c]);
-                acc[i][c] = fmaf(a[i].y, b[c].y, acc[i][c]);
-                acc[i][c] = fmaf(a[i].z, b[c].z, acc[i][c]);
-                acc[i][c] = fmaf(a[i].w, b[c].w, acc[i][c]);
+            for (int c = 0; c < NC; ++c) {
+                t[i][c] = __ffma2_rn(make_float2(a[i].x, a[i].y), make_float2(b[c].x, b[c].y), t[i][c]);
+                t[i][c] = __ffma2_rn(make_float2(a[i].z, a[i].w), make_float2(b[c].z, b[c].w), t[i][c]);
             }
     }
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][c] = c < NC ? t[i][c < NC ? c : 0].x + t[i][c < NC ? c : 0].y : 0.0f;
+}
+// The same for the first n rows of B (the others' products are 0): 16 of them at a time.
+template <int DP, int RM>
+__device__ __forceinline__ void dot_rows(float (&acc)[RM][4], const float* A, const float* B, int n, int ty, int tx) {
+    if (n > 48)
+        dot_cols<DP, RM, 4>(acc, A, B, ty, tx);
+    else if (n > 32)
+        dot_cols<DP, RM, 3>(acc, A, B, ty, tx);
+    else if (n > 16)
+        dot_cols<DP, RM, 2>(acc, A, B, ty, tx);
+    else
+        dot_cols<DP, RM, 1>(acc, A, B, ty, tx);
 }
 
-// acc[i][c] += sum_j P[ty RM + i][j] V[j][tx CN + c], j < kKeys. MASKED: a zero weight takes
+// acc[i][c] += sum_j P[ty RM + i][j] V[j][tx CN + c], j < n. MASKED: a zero weight takes
 // nothing from its row, whatever stands there (a NaN behind a mask stays there).
 template <int DP, int RM, int CN, bool MASKED>
-__device__ __forceinline__ void weigh_rows(float (&acc)[RM][CN], const float* P, int ldp, const float* V, int ty, int tx) {
+__device__ __forceinline__ void weigh_rows(float (&acc)[RM][CN], const float* P, int ldp, const float* V, int n, int ty, int tx) {
     constexpr int LD = DP + 4;
 #pragma unroll 2
-    for (int j = 0; j < kKeys; j += 4) {
+    for (int j = 0; j < n; j += 4) {
         float4 w[RM];
 #pragma unroll
         for (int i = 0; i < RM; ++i) w[i] = *reinterpret_cast<const float4*>(P + (ty * RM + i) * ldp + j);
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             float v[CN];
-            if constexpr (CN == 1) {
-                v[0] = V[(j + jj) * LD + tx];
-            } else if constexpr (CN == 2) {
+            if constexpr (CN == 2) {
                 const float2 t = *reinterpret_cast<const float2*>(V + (j + jj) * LD + tx * 2);
                 v[0] = t.x, v[1] = t.y;
             } else {
 #pragma unroll
-                for (int n = 0; n < CN / 4; ++n) {
-                    const float4 t = *reinterpret_cast<const float4*>(V + (j + jj) * LD + n * 64 + tx * 4);
-                    v[4 * n] = t.x, v[4 * n + 1] = t.y, v[4 * n + 2] = t.z, v[4 * n + 3] = t.w;
+                for (int n4 = 0; n4 < CN / 4; ++n4) {
+                    const float4 t = *reinterpret_cast<const float4*>(V + (j + jj) * LD + n4 * 64 + tx * 4);
+                    v[4 * n4] = t.x, v[4 * n4 + 1] = t.y, v[4 * n4 + 2] = t.z, v[4 * n4 + 3] = t.w;
                 }
             }
 #pragma unroll
             for (int i = 0; i < RM; ++i) {
                 const float p = jj == 0 ? w[i].x : jj == 1 ? w[i].y : jj == 2 ? w[i].z : w[i].w;
 #pragma unroll
-                for (int c = 0; c < CN; ++c) acc[i][c] = fmaf(p, MASKED && p == 0.0f ? 0.0f : v[c], acc[i][c]);
+                for (int c = 0; c < CN; c += 2) {
+                    const float2 x = make_float2(MASKED && p == 0.0f ? 0.0f : v[c], MASKED && p == 0.0f ? 0.0f : v[c + 1]);
+                    const float2 y = __ffma2_rn(make_float2(p, p), x, make_float2(acc[i][c], acc[i][c + 1]));
+                    acc[i][c] = y.x;
+                    acc[i][c + 1] = y.y;
+                }
             }
         }
     }
@@ -162,8 +181,8 @@ __global__ void __launch_bounds__(kThreads) k_attn_fwd(AttnParams p) {
         load_rows<T, DP, kKeys>(Vs, p.v, p.v_st, p.v_sh, t.obegin, kvh, 1, k0, n, p.dim);
         if (entries > 0 && tid < n) kpos[tid] = bias_pos(p.bias.k_pos, p.bias.axes, t.obegin + k0 + tid);
         __syncthreads();
-        float s[RM][4] = {};
-        dot_rows<DP, RM>(s, Qs, Ks, ty, tx);
+        float s[RM][4];
+        dot_rows<DP, RM>(s, Qs, Ks, n, ty, tx);
         bool cut = false;
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
@@ -205,9 +224,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_fwd(AttnParams p) {
         }
         // every thread takes the same branch
         if (__syncthreads_or(cut))
-            weigh_rows<DP, RM, CN, true>(o, Ps, LDP, Vs, ty, tx);
+            weigh_rows<DP, RM, CN, true>(o, Ps, LDP, Vs, n, ty, tx);
         else
-            weigh_rows<DP, RM, CN, false>(o, Ps, LDP, Vs, ty, tx);
+            weigh_rows<DP, RM, CN, false>(o, Ps, LDP, Vs, n, ty, tx);
     }
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
@@ -384,8 +403,29 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
         load_rows<T, DP, BM>(Gs, p.dout, p.do_st, p.do_sh, t.begin, head, 1, t.first, rows, p.dim);
         for (int r = tid; r < rows; r += kThreads) {
             const int64_t at = static_cast<int64_t>(head) * p.tq + t.begin + t.first + r;
-            lse[r] = p.lse[at], delta[r] = p.delta[at];
+            lse[r] = p.lse[at];
             if (entries > 0) qpos[r] = bias_pos(p.bias.q_pos, p.bias.axes, t.begin + t.first + r);
+        }
+        __syncthreads();
+        // delta = dout . out of the rows, for the kernel of dk and dv as well
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+            const int r = ty * RM + i;
+            float sum = 0.0f;
+            if (r < rows) {
+                const T* out = static_cast<const T*>(p.out) + (static_cast<int64_t>(t.begin + t.first + r) * p.heads + head) * p.dim;
+#pragma unroll
+                for (int c = 0; c < CN; ++c) {
+                    const int col = out_col<CN>(tx, c);
+                    if (col < p.dim) sum = fmaf(Gs[r * LD + col], to_f(out[col]), sum);
+                }
+            }
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (tx == 0 && r < rows) {
+                delta[r] = sum;
+                p.delta[static_cast<int64_t>(head) * p.tq + t.begin + t.first + r] = sum;
+            }
         }
         const int most = p.causal ? min(max(t.first + rows + t.olen - t.len, 0), t.olen) : t.olen;
         float dq[RM][CN] = {};
@@ -396,9 +436,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
             load_rows<T, DP, kKeys>(Vs, p.v, p.v_st, p.v_sh, t.obegin, kvh, 1, k0, n, p.dim);
             if (entries > 0 && tid < n) kpos[tid] = bias_pos(p.bias.k_pos, p.bias.axes, t.obegin + k0 + tid);
             __syncthreads();
-            float s[RM][4] = {}, dp[RM][4] = {};
-            dot_rows<DP, RM>(s, Qs, Ks, ty, tx);
-            dot_rows<DP, RM>(dp, Gs, Vs, ty, tx);
+            float s[RM][4], dp[RM][4];
+            dot_rows<DP, RM>(s, Qs, Ks, n, ty, tx);
+            dot_rows<DP, RM>(dp, Gs, Vs, n, ty, tx);
             const bool cut = score_grads<RM>(p, s, dp, t.first, rows, t, true, k0, n, lse, delta, Es, entries, qpos, kpos, ty, tx);
 #pragma unroll
             for (int i = 0; i < RM; ++i)
@@ -415,9 +455,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
                     }
                 }
             if (__syncthreads_or(cut))
-                weigh_rows<DP, RM, CN, true>(dq, Ds, LDP, Ks, ty, tx);
+                weigh_rows<DP, RM, CN, true>(dq, Ds, LDP, Ks, n, ty, tx);
             else
-                weigh_rows<DP, RM, CN, false>(dq, Ds, LDP, Ks, ty, tx);
+                weigh_rows<DP, RM, CN, false>(dq, Ds, LDP, Ks, n, ty, tx);
         }
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
@@ -482,23 +522,21 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(AttnParams p) {
                 if (entries > 0) qpos[r] = bias_pos(p.bias.q_pos, p.bias.axes, t.obegin + q0 + r);
             }
             __syncthreads();
-            float s[RM][4] = {}, dp[RM][4] = {};
-            dot_rows<DP, RM>(s, Qs, Ks, ty, tx);
-            dot_rows<DP, RM>(dp, Gs, Vs, ty, tx);
+            float s[RM][4], dp[RM][4];
+            dot_rows<DP, RM>(s, Qs, Ks, n, ty, tx);
+            dot_rows<DP, RM>(dp, Gs, Vs, n, ty, tx);
             const bool cut = score_grads<RM>(p, s, dp, q0, rows, t, false, t.first, n, lse, delta, Es, entries, qpos, kpos, ty, tx);
 #pragma unroll
-            for (int i = 0; i < RM; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    Pt[(tx + 16 * c) * LDP + ty * RM + i] = s[i][c];
-                    Dt[(tx + 16 * c) * LDP + ty * RM + i] = dp[i][c];
-                }
+            for (int c = 0; c < 4; ++c) {  // RM = 4: a row's four values together
+                *reinterpret_cast<float4*>(Pt + (tx + 16 * c) * LDP + ty * RM) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+                *reinterpret_cast<float4*>(Dt + (tx + 16 * c) * LDP + ty * RM) = make_float4(dp[0][c], dp[1][c], dp[2][c], dp[3][c]);
+            }
             if (__syncthreads_or(cut)) {
-                weigh_rows<DP, RM, CN, true>(dv, Pt, LDP, Gs, ty, tx);
-                weigh_rows<DP, RM, CN, true>(dk, Dt, LDP, Qs, ty, tx);
+                weigh_rows<DP, RM, CN, true>(dv, Pt, LDP, Gs, rows, ty, tx);
+                weigh_rows<DP, RM, CN, true>(dk, Dt, LDP, Qs, rows, ty, tx);
             } else {
-                weigh_rows<DP, RM, CN, false>(dv, Pt, LDP, Gs, ty, tx);
-                weigh_rows<DP, RM, CN, false>(dk, Dt, LDP, Qs, ty, tx);
+                weigh_rows<DP, RM, CN, false>(dv, Pt, LDP, Gs, rows, ty, tx);
+                weigh_rows<DP, RM, CN, false>(dk, Dt, LDP, Qs, rows, ty, tx);
             }
         }
     }
@@ -611,8 +649,8 @@ cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream
 
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
     if (type != kF32) return launch_attn_backward_mma(p, type, dtable, sms, s);
-    cudaError_t err = delta_type<float>(p, s, sms);
-    if (err != cudaSuccess) return err;
+    cudaError_t err = cudaSuccess;
+    if (p.bias_max != nullptr && (err = delta_type<float>(p, s, sms)) != cudaSuccess) return err;
     err = p.dim <= 32 ? bwd_dim<float, 32>(p, s, sms) : p.dim <= 64 ? bwd_dim<float, 64>(p, s, sms) : bwd_dim<float, 128>(p, s, sms);
     if (err != cudaSuccess || dtable == nullptr) return err;
     k_attn_bias_grad<<<(p.bias.buckets * p.heads + kThreads - 1) / kThreads, kThreads, 0, s>>>(p, dtable);
