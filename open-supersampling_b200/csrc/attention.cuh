@@ -65,7 +65,8 @@ struct AttnParams {
     int short_max;      // windows of up to so many keys go to the kernel for short windows
     int qsplits;        // parts that the queries of a tile of keys are cut into
     int tiny_blocks, short_blocks, dq_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
-    int* flags;         // [0]: kSomeLong, kSomeShort
+    int* flags;         // [0]: kSomeLong, kSomeShort; [1], [2]: windows of up to 16 and of 17 to 32 keys
+    int* tiny_list;     // [2][windows]: those windows, in order
     float *part_dk, *part_dv;    // [qsplits][tk][kv_heads][dim], qsplits > 1 only
     double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
     int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them

@@ -333,6 +333,39 @@ __global__ void __launch_bounds__(256) k_attn_flags(AttnParams p, int* flags) {
     if (some != 0 && (threadIdx.x & 31) == 0) atomicOr(flags, some);
 }
 
+// The same, with the windows of the warp-level kernels listed in order: a block, 1024 windows at a time.
+__global__ void __launch_bounds__(1024) k_attn_lists(AttnParams p, int* flags) {
+    __shared__ int sums[2][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int some = 0, base[2] = {0, 0};
+    for (int w0 = 0; w0 < p.windows; w0 += 1024) {
+        const int w = w0 + threadIdx.x;
+        int cls = -1;
+        if (w < p.windows) {
+            const int n = attn_offset(p.k_off, p.windows, p.tk, w + 2) - attn_offset(p.k_off, p.windows, p.tk, w + 1);
+            some |= n > p.short_max ? kSomeLong : n > p.tiny_max ? kSomeShort : 0;
+            if (n > 0 && n <= p.tiny_max) cls = n <= 16 ? 0 : 1;
+        }
+        const unsigned in[2] = {__ballot_sync(0xffffffffu, cls == 0), __ballot_sync(0xffffffffu, cls == 1)};
+        if (lane < 2) sums[lane][warp] = __popc(lane == 0 ? in[0] : in[1]);
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            int before = base[c], all = 0;
+            for (int k = 0; k < 32; ++k) {
+                if (k == warp) before += all;
+                all += sums[c][k];
+            }
+            if (cls == c) p.tiny_list[c * p.windows + before + __popc(in[c] & ((1u << lane) - 1u))] = w;
+            base[c] += all;
+        }
+        __syncthreads();
+    }
+    some = __reduce_or_sync(0xffffffffu, some);
+    if (some != 0 && lane == 0) atomicOr(flags, some);
+    if (threadIdx.x < 2) flags[1 + threadIdx.x] = base[threadIdx.x];
+}
+
 // ---- short windows ---------------------------------------------------------------------------
 template <int DP>
 struct ShortSmem {
@@ -1073,7 +1106,10 @@ cudaError_t bwd_type(const AttnParams& p, void* dtable, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
-    k_attn_flags<<<p.windows < 16384 ? 1 + p.windows / 1024 : 16, 256, 0, s>>>(p, p.flags);
+    if (p.tiny_max > 0)
+        k_attn_lists<<<1, 1024, 0, s>>>(p, p.flags);
+    else
+        k_attn_flags<<<p.windows < 16384 ? 1 + p.windows / 1024 : 16, 256, 0, s>>>(p, p.flags);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     if ((err = launch_attn_delta(p, type, sms, s)) != cudaSuccess) return err;

@@ -291,41 +291,57 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
 
 // ---- backward ----------------------------------------------------------------
 // delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for the bias
-// gradient's fixed point, and fp16's range). A warp a row.
-template <typename T>
+// gradient's fixed point, and fp16's range). LANES lanes a row, two values at a time where its
+// address and strides allow it (PAIRS).
+template <typename T, int LANES, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* delta, uint32_t* bias_max) {
     if (p.flags != nullptr && (*p.flags & kSomeLong) == 0 && bias_max == nullptr) return;  // short windows find their own
-    const int lane = threadIdx.x & 31;
+    constexpr int V = PAIRS ? 2 : 1;
+    struct alignas(V * sizeof(T)) Pair {
+        T v[V];
+    };
+    const int lane = threadIdx.x % LANES;
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads;
     const int64_t vrows = bias_max == nullptr ? 0 : static_cast<int64_t>(p.tk) * p.kv_heads;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+    const int64_t per = kThreads / LANES, step = static_cast<int64_t>(gridDim.x) * per;
     float most_do = 0.0f, most_v = 0.0f;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); row < rows + vrows; row += step) {
+    // whole warps stay in the loop: the shuffles name every lane
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per; row0 < rows + vrows; row0 += step) {
+        const int64_t row = row0 + threadIdx.x / LANES;
+        float sum = 0.0f;
         if (row < rows) {
-            const int64_t token = row / p.heads, head = row % p.heads;
+            const int64_t token = row / p.heads, head = row - token * p.heads;
             const T* g = static_cast<const T*>(p.dout) + token * p.do_st + head * p.do_sh;
             const T* o = static_cast<const T*>(p.out) + row * p.dim;
-            float sum = 0.0f;
-            for (int c = lane; c < p.dim; c += 32) {
-                const float x = to_f(g[c]);
-                sum = fmaf(x, to_f(o[c]), sum);
-                if (is_finite(x)) most_do = fmaxf(most_do, fabsf(x));
+            for (int c = V * lane; c < p.dim; c += V * LANES) {
+                const Pair x = *reinterpret_cast<const Pair*>(g + c), y = *reinterpret_cast<const Pair*>(o + c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float f = to_f(x.v[i]);
+                    sum = fmaf(f, to_f(y.v[i]), sum);
+                    if (is_finite(f)) most_do = fmaxf(most_do, fabsf(f));
+                }
             }
-            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (lane == 0) delta[head * p.tq + token] = sum;
-        } else {
-            const int64_t token = (row - rows) / p.kv_heads, head = (row - rows) % p.kv_heads;
+        } else if (row < rows + vrows) {
+            const int64_t token = (row - rows) / p.kv_heads, head = row - rows - token * p.kv_heads;
             const T* v = static_cast<const T*>(p.v) + token * p.v_st + head * p.v_sh;
-            for (int c = lane; c < p.dim; c += 32) {
-                const float x = to_f(v[c]);
-                if (is_finite(x)) most_v = fmaxf(most_v, fabsf(x));
+            for (int c = V * lane; c < p.dim; c += V * LANES) {
+                const Pair x = *reinterpret_cast<const Pair*>(v + c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float f = to_f(x.v[i]);
+                    if (is_finite(f)) most_v = fmaxf(most_v, fabsf(f));
+                }
             }
         }
+#pragma unroll
+        for (int x = LANES / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (lane == 0 && row < rows) delta[(row % p.heads) * p.tq + row / p.heads] = sum;
     }
     if (bias_max == nullptr) return;
     const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(most_do));
     const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
-    if (lane == 0) {
+    if ((threadIdx.x & 31) == 0) {
         if (a != 0u) atomicMax(bias_max, a);
         if (b != 0u) atomicMax(bias_max + 1, b);
     }
@@ -623,14 +639,24 @@ cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s, int sms) {
     return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t delta_type(const AttnParams& p, cudaStream_t s, int sms) {
+template <typename T, int LANES>
+cudaError_t delta_lanes(const AttnParams& p, cudaStream_t s, int sms) {
     uint32_t* bias_max = const_cast<uint32_t*>(p.bias_max);
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads + (bias_max ? static_cast<int64_t>(p.tk) * p.kv_heads : 0);
-    const int64_t blocks = (rows + 7) / 8;
+    const int64_t blocks = (rows * LANES + kThreads - 1) / kThreads;
     if (blocks == 0) return cudaSuccess;
-    k_attn_delta<T><<<static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms), kThreads, 0, s>>>(p, p.delta, bias_max);
+    const unsigned grid = static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms);
+    const uintptr_t bytes = reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.v);
+    const bool pairs = bytes % (2 * sizeof(T)) == 0 && ((p.do_st | p.do_sh | p.v_st | p.v_sh | p.dim) & 1) == 0;
+    if (pairs)
+        k_attn_delta<T, LANES, true><<<grid, kThreads, 0, s>>>(p, p.delta, bias_max);
+    else
+        k_attn_delta<T, LANES, false><<<grid, kThreads, 0, s>>>(p, p.delta, bias_max);
     return cudaGetLastError();
+}
+template <typename T>
+cudaError_t delta_type(const AttnParams& p, cudaStream_t s, int sms) {
+    return p.dim <= 32 ? delta_lanes<T, 8>(p, s, sms) : delta_lanes<T, 16>(p, s, sms);
 }
 
 }  // namespace

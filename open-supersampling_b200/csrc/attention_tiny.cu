@@ -108,21 +108,6 @@ __device__ __forceinline__ void store_row16(T* row, int dim, const float (&o)[DB
     }
 }
 
-// Brings rows of an operand that are due in a few steps into L2: without it the loads in flight (16
-// rows a warp) cover a third of what HBM delivers in their latency. Lane i < 16: row r + i of this walk, or,
-// past its end, of the next one.
-constexpr int kAhead = 64;
-struct Ahead {
-    const char *now, *then;  // row 0 of this walk, and of the next (null: none)
-    int64_t step, end;       // bytes to the next row; rows of this walk
-    int then_end;
-    __device__ __forceinline__ void touch(int r) const {
-        const int i = r + (threadIdx.x & 15);
-        const char* at = i < end ? now + i * step : then != nullptr && i - end < then_end ? then + (i - end) * step : nullptr;
-        if (at != nullptr && (threadIdx.x & 31) < 16) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-    }
-};
-
 __device__ __forceinline__ float quad_sum(float x) {
     x += __shfl_xor_sync(0xffffffffu, x, 1);
     return x + __shfl_xor_sync(0xffffffffu, x, 2);
@@ -203,21 +188,17 @@ __device__ __forceinline__ Share share_of(int kv_heads) {
             static_cast<int>(gridDim.x) * (kWarps / side)};
 }
 
-// The rows of head gh of a window, then of the window's next head, or of the warp's next window.
-template <typename T>
-__device__ __forceinline__ Ahead ahead_of(const void* q, int64_t st, int64_t sh, int head0, int gh, int group, int64_t token, int rows, int next_q,
-                                          int next_rows) {
-    const T* p = static_cast<const T*>(q) + (head0 + gh) * sh;
-    const T* then = gh + 1 < group ? p + sh + token * st : next_rows > 0 ? p - gh * sh + next_q * st : nullptr;
-    return {reinterpret_cast<const char*>(p + token * st), reinterpret_cast<const char*>(then), st * static_cast<int64_t>(sizeof(T)), rows,
-            gh + 1 < group ? rows : next_rows};
-}
+// Warps of a forward block. Without a bias one, with one window and key head: windows differ in cost, and
+// the hardware hands blocks out as others end. With one four, that share the expanded biases.
+constexpr int tiny_fwd_warps(bool bias) { return bias ? kWarps : 1; }
+constexpr int tiny_fwd_blocks(int db, int nb) { return db == 1 && nb == 4 ? 5 : db == 1 || nb == 4 ? 3 : 2; }  // of four warps
+constexpr int tiny_bwd_blocks(int nb) { return nb == 2 ? 3 : 2; }
 
 // ---- forward --------------------------------------------------------------------------------
 // One window and key head, rows [r_begin, r_end), with NK blocks of 8 keys (the lower half of them full).
 template <typename T, int DB, int NK, bool BIAS>
 __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int group, int q0, int lq, int k0, int n, int r_begin,
-                                             int r_end, TinyPos<NK>* kp, const float* E, int entries, int next_q, int next_rows) {
+                                             int r_end, TinyPos<NK>* kp, const float* E, int entries) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float c2 = p.scale * kLog2e;
     uint32_t kr[NK][DB][4], vt[NK][DB][4];
@@ -249,7 +230,6 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
         uint32_t qa[DB][4], qb[DB][4];
         rq.load_at(qa, from, r_begin + g < r_end);
         rq.load_at(qb, from + 8 * p.q_st, r_begin + g + 8 < r_end);
-        const Ahead ahead = ahead_of<T>(p.q, p.q_st, p.q_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
         for (int r0 = r_begin; r0 < r_end; r0 += 16, to += 2 * to_step) {
             float s[NK][4];
 #pragma unroll
@@ -264,7 +244,6 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
                                  kr[kb][b][2 * h + 1]);
             }
             // the next rows are on their way meanwhile
-            ahead.touch(r0 - r_begin + kAhead);
             from += 16 * p.q_st;
             rq.load_at(qa, from, r0 + 16 + g < r_end);
             rq.load_at(qb, from + 8 * p.q_st, r0 + 24 + g < r_end);
@@ -336,12 +315,14 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
     }
 }
 
+// Windows of up to 32 keys (NB = 4), or of 33 to 64 (NB = 8): apart, so that the few keys' registers let more
+// warps hide each other's latency, which bounds this kernel.
 template <typename T, int DB, int NB, bool BIAS>
-__global__ void __launch_bounds__(32 * kWarps, DB == 1 ? 3 : 2) k_attn_fwd_tiny(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * tiny_fwd_warps(BIAS), tiny_fwd_blocks(DB, NB) * 4 / tiny_fwd_warps(BIAS)) k_attn_fwd_tiny(const __grid_constant__ AttnParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int warp = threadIdx.x >> 5;
     const int group = p.heads / p.kv_heads, entries = BIAS ? bias_entries(p.bias) : 0;
-    const Share sh = share_of(p.kv_heads);
+    const Share sh = BIAS ? share_of(p.kv_heads) : Share{static_cast<int>(blockIdx.x) % p.kv_heads, static_cast<int>(blockIdx.x) / p.kv_heads, p.windows};
     const int side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
     TinyPos<NB>* kp = reinterpret_cast<TinyPos<NB>*>(smem_raw) + warp;
     float* E = reinterpret_cast<float*>(smem_raw + sizeof(TinyPos<NB>) * kWarps);
@@ -357,27 +338,24 @@ __global__ void __launch_bounds__(32 * kWarps, DB == 1 ? 3 : 2) k_attn_fwd_tiny(
     for (int w = sh.first; w < p.windows; w += sh.step) {
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), n = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
-        if (n > p.tiny_max || n == 0) continue;  // other kernels'
+        if (n > 8 * NB || n <= (NB == 8 ? 32 : 0)) continue;  // other kernels'
         const int per = ((lq + 15) / 16 + gridDim.z - 1) / gridDim.z * 16;
         const int r_begin = min(static_cast<int>(blockIdx.z) * per, lq), r_end = min(r_begin + per, lq);
         if (r_begin >= r_end) continue;
-        // the warp's next window, if it is of this kernel
-        int next_q = 0, next_rows = 0;
-        if (w + sh.step < p.windows) {
-            next_q = attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 1);
-            next_rows = gridDim.z > 1 ? 0 : attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 2) - next_q;
+        if constexpr (NB == 8) {
+            tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries);
+        } else {
+            if (n <= 16)
+                tiny_forward<T, DB, 2, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries);
+            else
+                tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries);
         }
-        if (n <= 16)
-            tiny_forward<T, DB, 2, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, next_q, next_rows);
-        else if (NB == 4 || n <= 32)
-            tiny_forward<T, DB, 4, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<4>*>(kp), Eh, entries, next_q, next_rows);
-        else
-            tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, next_q, next_rows);
     }
 }
 
 // ---- backward -------------------------------------------------------------------------------
-// 32 columns and 32 keys at most: dk and dv of the window stay in registers. The bias gradient
+// 32 columns and 32 keys at most: dk and dv of the window stay in registers. Windows of up to 16 keys
+// (NB = 2) and of 17 to 32 (NB = 4) apart, as in the forward. The bias gradient
 // goes into the warp's own 32-bit integers, at a scale that leaves room for what was added since
 // they were last moved to its fp64 sums.
 // A warp's sums of the bias gradient.
@@ -410,8 +388,7 @@ struct TinySums {
 // One window and key head, rows [r_begin, r_end), with NK blocks of 8 keys.
 template <typename T, int NK, bool BIAS>
 __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int group, int q0, int lq, int k0, int n, int r_begin, int r_end,
-                                              TinyPos<NK < 2 ? 2 : NK>* kp, const float* E, int entries, float up, TinySums& ts, int next_q,
-                                              int next_rows) {
+                                              TinyPos<NK < 2 ? 2 : NK>* kp, const float* E, int entries, float up, TinySums& ts) {
     constexpr int NP = NK < 2 ? 2 : NK;  // blocks of positions
     constexpr int NM = (NK + 1) / 2;     // 16-key steps
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -458,15 +435,11 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
             lse_at += 16;
         };
         fetch(r_begin);
-        const Ahead ahead_q = ahead_of<T>(p.q, p.q_st, p.q_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
-        const Ahead ahead_g = ahead_of<T>(p.dout, p.do_st, p.do_sh, kvh * group, gh, group, q0 + r_begin, r_end - r_begin, next_q, next_rows);
         for (int r0 = r_begin; r0 < r_end; r0 += 16, to += 2 * to_step) {
             uint32_t qa[4], qb[4], ga[4], gb[4];
             const float lse[2] = {nl[0], nl[1]};
 #pragma unroll
             for (int j = 0; j < 4; ++j) qa[j] = nqa[0][j], qb[j] = nqb[0][j], ga[j] = nga[0][j], gb[j] = ngb[0][j];
-            ahead_q.touch(r0 - r_begin + kAhead);
-            ahead_g.touch(r0 - r_begin + kAhead);
             fetch(r0 + 16);
             float s[NK][4], dp[NK][4];
 #pragma unroll
@@ -599,9 +572,8 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
         }
 }
 
-template <typename T, bool BIAS>
-__global__ void __launch_bounds__(32 * kWarps, 2) k_attn_bwd_tiny(const __grid_constant__ AttnParams p) {
-    constexpr int NB = 4;
+template <typename T, int NB, bool BIAS>
+__global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_tiny(const __grid_constant__ AttnParams p, int first_part) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int warp = threadIdx.x >> 5;
     const int group = p.heads / p.kv_heads, entries = BIAS ? bias_entries(p.bias) : 0;
@@ -629,24 +601,23 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_attn_bwd_tiny(const __grid_c
     const float* Eh = E + (kvh % side) * group * entries;
     TinySums ts{acc, I, grad_bias ? group * entries : 0, 0.0f, 0.0f};
 
-    for (int w = mine ? sh.first : p.windows; w < p.windows; w += sh.step) {
+    // the windows of this kernel's class, as listed
+    const int* list = p.tiny_list + (NB == 4 ? p.windows : 0);
+    const int listed = p.flags[NB == 4 ? 2 : 1];
+    for (int item = mine ? sh.first : listed; item < listed; item += sh.step) {
+        const int w = list[item];
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), n = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
-        if (n > p.tiny_max || n == 0) continue;  // other kernels'
         const int per = ((lq + 15) / 16 + p.qsplits - 1) / p.qsplits * 16;
         const int r_begin = min(static_cast<int>(blockIdx.z) * per, lq), r_end = min(r_begin + per, lq);
-        // the warp's next window, if it is of this kernel
-        int next_q = 0, next_rows = 0;
-        if (w + sh.step < p.windows) {
-            next_q = attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 1);
-            next_rows = p.qsplits > 1 ? 0 : attn_offset(p.q_off, p.windows, p.tq, w + sh.step + 2) - next_q;
+        if constexpr (NB == 4) {
+            tiny_backward<T, 4, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts);
+        } else {
+            if (n <= 8)
+                tiny_backward<T, 1, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts);
+            else
+                tiny_backward<T, 2, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts);
         }
-        if (n <= 8)
-            tiny_backward<T, 1, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts, next_q, next_rows);
-        else if (n <= 16)
-            tiny_backward<T, 2, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, reinterpret_cast<TinyPos<2>*>(kp), Eh, entries, up, ts, next_q, next_rows);
-        else
-            tiny_backward<T, 4, BIAS>(p, kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries, up, ts, next_q, next_rows);
     }
     if constexpr (BIAS)
         if (grad_bias) {
@@ -658,7 +629,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) k_attn_bwd_tiny(const __grid_c
                 if (head >= p.heads) continue;
                 double sum = 0.0;
                 for (int v = s; v < kWarps; v += side) sum += acc_all[v * group * entries + e % (group * entries)];
-                p.bias_part[(static_cast<int64_t>(head) * p.bias_parts + blockIdx.z * gridDim.x + blockIdx.x) * entries + e % entries] = sum;
+                p.bias_part[(static_cast<int64_t>(head) * p.bias_parts + first_part + blockIdx.z * gridDim.x + blockIdx.x) * entries + e % entries] = sum;
             }
         }
 }
@@ -671,7 +642,7 @@ static int tiny_blocks(const AttnParams& p, int resident, int z) {
     const int per = (resident * 148 + sets * z - 1) / (sets * z), most = (p.windows + kWarps / side - 1) / (kWarps / side);
     return most < 1 ? 1 : most < per ? most : per;
 }
-int attn_tiny_backward_blocks(const AttnParams& p) { return tiny_blocks(p, 2, p.qsplits); }
+int attn_tiny_backward_blocks(const AttnParams& p) { return tiny_blocks(p, 2, p.qsplits); }  // of each of the two kernels
 
 namespace {
 int sets_of(const AttnParams& p) {
@@ -684,7 +655,7 @@ int heads_of_block(const AttnParams& p) {
 
 template <typename T, int DB, int NB, bool BIAS>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
-    const int bytes = static_cast<int>(sizeof(TinyPos<NB>)) * kWarps + 4 * (BIAS ? heads_of_block(p) * bias_entries(p.bias) : 0);
+    const int bytes = BIAS ? static_cast<int>(sizeof(TinyPos<NB>)) * kWarps + 4 * heads_of_block(p) * bias_entries(p.bias) : 0;
     cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_tiny<T, DB, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
     // few windows: their rows are shared out as well, 64 at least
@@ -692,28 +663,43 @@ cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     int64_t z = 148 * 12 / (items < 1 ? 1 : items);
     z = z < avg / 64 ? z : avg / 64;
     z = z < 1 ? 1 : z > 1024 ? 1024 : z;
-    const int blocks = tiny_blocks(p, DB == 1 ? 3 : 2, static_cast<int>(z));
-    k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(blocks, sets_of(p), static_cast<unsigned>(z)), 32 * kWarps, bytes, s>>>(p);
+    const unsigned uz = static_cast<unsigned>(z);
+    if (BIAS) {  // four rounds of blocks, each with several windows
+        const int blocks = tiny_blocks(p, 4 * tiny_fwd_blocks(DB, NB), static_cast<int>(z));
+        k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(blocks, sets_of(p), uz), 32 * kWarps, bytes, s>>>(p);
+    } else {
+        k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(static_cast<unsigned>(items), 1, uz), 32, bytes, s>>>(p);
+    }
+    return cudaGetLastError();
+}
+template <typename T, int NB, bool BIAS>
+cudaError_t bwd_one(const AttnParams& p, int first_part, cudaStream_t s) {
+    const int64_t entries = BIAS ? bias_entries(p.bias) : 0, group = p.heads / p.kv_heads;
+    const int bytes = static_cast<int>(sizeof(TinyPos<NB>) * kWarps + 4 * heads_of_block(p) * entries +
+                                       (p.bias_part != nullptr ? 12 * kWarps * group * entries : 0));
+    cudaError_t err = cudaFuncSetAttribute(k_attn_bwd_tiny<T, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err != cudaSuccess) return err;
+    k_attn_bwd_tiny<T, NB, BIAS><<<dim3(p.tiny_blocks, sets_of(p), p.qsplits), 32 * kWarps, bytes, s>>>(p, first_part);
     return cudaGetLastError();
 }
 template <typename T, bool BIAS>
-cudaError_t bwd_one(const AttnParams& p, cudaStream_t s) {
-    const int64_t entries = BIAS ? bias_entries(p.bias) : 0, group = p.heads / p.kv_heads;
-    const int bytes = static_cast<int>(sizeof(TinyPos<4>) * kWarps + 4 * heads_of_block(p) * entries +
-                                       (p.bias_part != nullptr ? 12 * kWarps * group * entries : 0));
-    cudaError_t err = cudaFuncSetAttribute(k_attn_bwd_tiny<T, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (err != cudaSuccess) return err;
-    k_attn_bwd_tiny<T, BIAS><<<dim3(p.tiny_blocks, sets_of(p), p.qsplits), 32 * kWarps, bytes, s>>>(p);
-    return cudaGetLastError();
+cudaError_t fwd_bias(const AttnParams& p, cudaStream_t s) {
+    if (p.dim > 32) return fwd_one<T, 2, 4, BIAS>(p, s);
+    const cudaError_t err = fwd_one<T, 1, 8, BIAS>(p, s);
+    return err != cudaSuccess ? err : fwd_one<T, 1, 4, BIAS>(p, s);
+}
+template <typename T, bool BIAS>
+cudaError_t bwd_bias(const AttnParams& p, cudaStream_t s) {
+    const cudaError_t err = bwd_one<T, 4, BIAS>(p, 0, s);
+    return err != cudaSuccess ? err : bwd_one<T, 2, BIAS>(p, p.tiny_blocks * p.qsplits, s);
 }
 template <typename T>
 cudaError_t fwd_type(const AttnParams& p, cudaStream_t s) {
-    if (p.bias.table != nullptr) return p.dim <= 32 ? fwd_one<T, 1, 8, true>(p, s) : fwd_one<T, 2, 4, true>(p, s);
-    return p.dim <= 32 ? fwd_one<T, 1, 8, false>(p, s) : fwd_one<T, 2, 4, false>(p, s);
+    return p.bias.table != nullptr ? fwd_bias<T, true>(p, s) : fwd_bias<T, false>(p, s);
 }
 template <typename T>
 cudaError_t bwd_type(const AttnParams& p, cudaStream_t s) {
-    return p.bias.table != nullptr ? bwd_one<T, true>(p, s) : bwd_one<T, false>(p, s);
+    return p.bias.table != nullptr ? bwd_bias<T, true>(p, s) : bwd_bias<T, false>(p, s);
 }
 
 }  // namespace

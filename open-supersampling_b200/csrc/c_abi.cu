@@ -1341,7 +1341,7 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     p.short_blocks = blocks(windows, (p.dim <= 64 ? 2 : 1) * kSms, p.kv_heads * p.qsplits);
     p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (p.dim <= 64 ? 2 : 1) * (sums ? 1 : 4) * kSms, p.heads);
     p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, 128), 4 * kSms, p.kv_heads * p.qsplits);
-    p.bias_tiny = p.tiny_blocks * p.qsplits;
+    p.bias_tiny = 2 * p.tiny_blocks * p.qsplits;  // of its two kernels
     p.bias_short = p.short_max > 0 ? p.short_blocks * p.qsplits : 0;
     p.bias_parts = p.bias_tiny + p.bias_short + p.dq_blocks;
 }
@@ -1359,13 +1359,14 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
         p.part_dk = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
         p.part_dv = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
         p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * p.bias_parts * entries) : nullptr;
+        p.tiny_list = p.tiny_max > 0 ? arena.take<int>(2ll * p.windows) : nullptr;
     }
     const int64_t from = arena.used;
     p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
     p.bias_bad = sums ? arena.take<uint32_t>(sum_rows * p.heads) : nullptr;
     p.bias_max = sums || dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
     if (dtype == oss::kBF16) p.bias_max = nullptr;
-    p.flags = dtype != oss::kF32 ? arena.take<int>(1) : nullptr;
+    p.flags = dtype != oss::kF32 ? arena.take<int>(3) : nullptr;
     if (zero_at != nullptr) *zero_at = base + from, *zeroed = arena.used - from;
     return arena.used;
 }
