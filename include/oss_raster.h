@@ -659,8 +659,9 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
  *   q_pos[tq][axes], k_pos[tk][axes]  int32 (y, x), or (x) with axes = 1; clamped to +-2^29
  * entries: (2 ry + 1)(2 rx + 1), 0 without a table.
  * ------------------------------------------------------------------------- */
-OSS_API int64_t oss_window_attention_scratch_bytes(int64_t tq, int64_t tk, int64_t windows, int64_t heads,
-                                                   int64_t kv_heads, int64_t dim, int64_t entries);
+OSS_API int64_t oss_window_attention_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows,
+                                                   int64_t heads, int64_t kv_heads, int64_t dim, int32_t causal,
+                                                   int64_t entries);
 OSS_API int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
                                          int64_t kv_heads, int64_t dim, const void* q, int64_t q_st, int64_t q_sh,
                                          const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,

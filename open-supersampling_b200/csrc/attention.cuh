@@ -47,7 +47,8 @@ struct AttnParams {
     AttnBias bias;
     void* out;        // [tq][heads][dim]
     float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
-    int tiny_max;     // windows of 1 to so many keys go to the warp-level kernels (attention_tiny.cu)
+    int tiny_max;     // windows of up to so many keys (backward: of 1 to so many) go to the warp-level kernels
+                      // (attention_tiny.cu); 0: none
     // forward only
     int pack;         // query heads of one key head that share a tile's rows (1 or the group)
     int splits;       // parts that a window's keys are cut into
@@ -65,8 +66,10 @@ struct AttnParams {
     int short_max;      // windows of up to so many keys go to the kernel for short windows
     int qsplits;        // parts that the queries of a tile of keys are cut into
     int tiny_blocks, short_blocks, dq_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
+    // (flags and tiny_list in the forward: the counters and the pieces of attention_tiny.cu)
     int* flags;         // [0]: kSomeLong, kSomeShort; [1], [2]: windows of up to 16 and of 17 to 32 keys
     int* tiny_list;     // [2][windows]: those windows, in order
+    int tiny_pieces;    // forward: most pieces of a class
     float *part_dk, *part_dv;    // [qsplits][tk][kv_heads][dim], qsplits > 1 only
     double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
     int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them
@@ -136,17 +139,18 @@ __device__ __forceinline__ bool attn_tile(const int32_t* off, int t, const int32
 
 // The tiles of slots [slot, end) one after the other: a search for the first, then window by
 // window (neighbouring offsets share cache lines).
+template <int ROWS>
 struct AttnWalk {
     const int32_t *off, *other;
-    int t, ot, windows, per, rows;
-    int skip;  // windows with 1 to `skip` tokens on the other side are passed by
+    int t, ot, windows, per;
+    int skip;  // where not 0: windows with up to so many tokens on the other side are passed by
     int slot, end, w;
     AttnTile tile;
 
     // Called by whole warps. False: no tile.
     __device__ __forceinline__ bool start(const int32_t* off_, int t_, const int32_t* other_, int ot_, int windows_, int per_,
-                                          int rows_, int slot_, int end_, int skip_ = 0) {
-        off = off_, t = t_, other = other_, ot = ot_, windows = windows_, per = per_, rows = rows_, slot = slot_, end = end_;
+                                          int slot_, int end_, int skip_ = 0) {
+        off = off_, t = t_, other = other_, ot = ot_, windows = windows_, per = per_, slot = slot_, end = end_;
         skip = skip_;
         const int lane = threadIdx.x & 31;
         int lo = 0, hi = windows + 2;
@@ -162,13 +166,13 @@ struct AttnWalk {
     }
     __device__ __forceinline__ bool next() {
         ++slot;
-        const int64_t first = static_cast<int64_t>(tile.first) + rows;
+        const int64_t first = static_cast<int64_t>(tile.first) + ROWS;
         if (slot >= end || first >= static_cast<int64_t>(tile.len) * per) return settle();
         tile.first = static_cast<int>(first);
         return true;
     }
     __device__ __forceinline__ int slot_of(int at) const {
-        return static_cast<int>(static_cast<int64_t>(attn_offset(off, windows, t, at)) * per / rows) + at;
+        return static_cast<int>(static_cast<uint64_t>(attn_offset(off, windows, t, at)) * static_cast<unsigned>(per) / ROWS) + at;
     }
     __device__ __forceinline__ void enter(int at) {
         w = at;
@@ -183,8 +187,8 @@ struct AttnWalk {
     }
     __device__ __forceinline__ bool settle() {
         while (slot < end) {
-            const int64_t first = static_cast<int64_t>(slot - slot_of(w)) * rows;
-            if (first >= 0 && first < static_cast<int64_t>(tile.len) * per && (tile.olen == 0 || tile.olen > skip)) {
+            const int64_t first = static_cast<int64_t>(slot - slot_of(w)) * ROWS;
+            if (first >= 0 && first < static_cast<int64_t>(tile.len) * per && (tile.olen > skip || (tile.olen == 0 && (skip == 0 || tile.window < 0)))) {
                 tile.first = static_cast<int>(first);
                 return true;
             }
@@ -196,7 +200,8 @@ struct AttnWalk {
                 bool stop = c > windows + 1 || slot_of(c) >= end;
                 if (!stop) {
                     const int n = c >= 1 && c <= windows ? attn_offset(other, windows, ot, c + 1) - attn_offset(other, windows, ot, c) : 0;
-                    stop = attn_offset(off, windows, t, c + 1) > attn_offset(off, windows, t, c) && (n <= 0 || n > skip);
+                    stop = attn_offset(off, windows, t, c + 1) > attn_offset(off, windows, t, c) &&
+                           (n > skip || (n <= 0 && (skip == 0 || c < 1 || c > windows)));
                 }
                 const unsigned hit = __ballot_sync(0xffffffffu, stop);
                 if (hit != 0u) {
@@ -316,10 +321,13 @@ cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, in
 cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s);
 // attention_mma.cu, attention_mma_bwd.cu: bf16 and fp16, the forward without the join of split keys.
 cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s);
-// Windows of 1 to p.tiny_max keys, not causal, dim <= 64 (backward: 32, p.tiny_max <= 32).
+// Windows of up to p.tiny_max keys (backward: of 1 to 32), not causal, dim <= 64 (backward: 32).
 cudaError_t launch_attn_forward_tiny(const AttnParams& p, int type, cudaStream_t s);
 cudaError_t launch_attn_backward_tiny(const AttnParams& p, int type, cudaStream_t s);
 int attn_tiny_backward_blocks(const AttnParams& p);
+int attn_tiny_pieces(int tq, int windows);
+int attn_tiny_forward_counters(int kv_heads);
+int attn_tiny_lists();
 cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
 // Waits of the tensor-core kernels that ran out of their limit since the library was loaded.
 cudaError_t attn_timeouts(unsigned int* count);

@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
     const int chunk = (slots + gridDim.x - 1) / gridDim.x;
     // causal windows: the last tiles see the most keys and go first
     const int slot0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * chunk;
-    AttnWalk walk;
-    bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, kRows, slot0, min(slots, slot0 + chunk), p.tiny_max);
+    AttnWalk<kRows> walk;
+    bool more = walk.start(p.q_off, p.tq, p.k_off, p.tk, p.windows, p.pack, slot0, min(slots, slot0 + chunk), p.tiny_max);
     if (!more) return;
 
     if (tid == 0) {

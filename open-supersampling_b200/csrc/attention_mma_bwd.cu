@@ -599,21 +599,22 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
 // The tiles of a block. Where windows have many tiles (1024 queries on average): back and forth over
 // the blocks, so that each gets tiles of many keys and of few (the last tiles of a causal window see
 // all of it, its first ones nearly nothing). Otherwise an even range of slots, whose empty ones even out.
+template <int ROWS>
 struct LongWalk {
-    AttnWalk walk;
+    AttnWalk<ROWS> walk;
     const AttnParams& p;
     int slots, round;
     bool spread;
     const int32_t *off, *other;
-    int t, ot, rows;
+    int t, ot;
     __device__ __forceinline__ LongWalk(int slots_, const AttnParams& p_) : p(p_), slots(slots_), round(-1) {
         spread = static_cast<int64_t>(p.windows) * 1024 <= p.tq;
     }
-    __device__ __forceinline__ bool first(const int32_t* off_, int t_, const int32_t* other_, int ot_, int rows_) {
-        off = off_, t = t_, other = other_, ot = ot_, rows = rows_;
+    __device__ __forceinline__ bool first(const int32_t* off_, int t_, const int32_t* other_, int ot_) {
+        off = off_, t = t_, other = other_, ot = ot_;
         if (spread) return next();
         const int64_t n = slots;
-        return walk.start(off, t, other, ot, p.windows, 1, rows, static_cast<int>(n * blockIdx.x / gridDim.x),
+        return walk.start(off, t, other, ot, p.windows, 1, static_cast<int>(n * blockIdx.x / gridDim.x),
                           static_cast<int>(n * (blockIdx.x + 1) / gridDim.x));
     }
     __device__ __forceinline__ bool next() {
@@ -622,7 +623,7 @@ struct LongWalk {
             ++round;
             const int at = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
             if (at >= slots) return false;
-            if (walk.start(off, t, other, ot, p.windows, 1, rows, slots - 1 - at, slots - at)) return true;
+            if (walk.start(off, t, other, ot, p.windows, 1, slots - 1 - at, slots - at)) return true;
         }
     }
 };
@@ -695,8 +696,8 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     int par_s = 0, par_o = 0;
     bool alive = true;
 
-    LongWalk walk(slots, p);
-    for (bool more = walk.first(p.q_off, p.tq, p.k_off, p.tk, kRows); more; more = walk.next()) {
+    LongWalk<kRows> walk(slots, p);
+    for (bool more = walk.first(p.q_off, p.tq, p.k_off, p.tk); more; more = walk.next()) {
         const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.olen <= p.short_max) continue;
         const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
@@ -880,8 +881,8 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
 
-    LongWalk walk(slots, p);
-    for (bool more = walk.first(p.k_off, p.tk, p.q_off, p.tq, KT); more; more = walk.next()) {
+    LongWalk<KT> walk(slots, p);
+    for (bool more = walk.first(p.k_off, p.tk, p.q_off, p.tq); more; more = walk.next()) {
         const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.len <= p.short_max) continue;
         const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;

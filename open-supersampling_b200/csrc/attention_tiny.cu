@@ -188,29 +188,29 @@ __device__ __forceinline__ Share share_of(int kv_heads) {
             static_cast<int>(gridDim.x) * (kWarps / side)};
 }
 
-// Warps of a forward block. Without a bias one, with one window and key head: windows differ in cost, and
-// the hardware hands blocks out as others end. With one four, that share the expanded biases.
-constexpr int tiny_fwd_warps(bool bias) { return bias ? kWarps : 1; }
-constexpr int tiny_fwd_blocks(int db, int nb) { return db == 1 && nb == 4 ? 5 : db == 1 || nb == 4 ? 3 : 2; }  // of four warps
+constexpr int tiny_fwd_blocks(int db, int nb) { return nb == 16 ? 2 : db == 1 && nb == 4 ? 4 : 3; }
 constexpr int tiny_bwd_blocks(int nb) { return nb == 2 ? 3 : 2; }
 
 // ---- forward --------------------------------------------------------------------------------
 // One window and key head, rows [r_begin, r_end), with NK blocks of 8 keys (the lower half of them full).
+// The values of 16 blocks do not fit the registers beside their keys: they are loaded again each step.
 template <typename T, int DB, int NK, bool BIAS>
 __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int group, int q0, int lq, int k0, int n, int r_begin,
                                              int r_end, TinyPos<NK>* kp, const float* E, int entries) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float c2 = p.scale * kLog2e;
-    uint32_t kr[NK][DB][4], vt[NK][DB][4];
+    constexpr bool kKeepV = NK <= 8;
+    uint32_t kr[NK][DB][4], vt[kKeepV ? NK : 2][DB][4];
+    const Rows<T, DB> rv(p.v, p.v_st, p.v_sh, p.dim, kvh);
     {
-        const Rows<T, DB> rk(p.k, p.k_st, p.k_sh, p.dim, kvh), rv(p.v, p.v_st, p.v_sh, p.dim, kvh);
+        const Rows<T, DB> rk(p.k, p.k_st, p.k_sh, p.dim, kvh);
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb) {
             rk.load(kr[kb], k0 + 8 * kb + g, 8 * kb + g < n);
-            rv.load(vt[kb], k0 + 8 * kb + g, 8 * kb + g < n);
+            if (kKeepV) rv.load(vt[kKeepV ? kb : 0], k0 + 8 * kb + g, 8 * kb + g < n);
         }
 #pragma unroll
-        for (int kb = 0; kb < NK; ++kb)
+        for (int kb = 0; kb < (kKeepV ? NK : 0); ++kb)
 #pragma unroll
             for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -219,18 +219,28 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
     Range krange{0, 0, 0, 0};
     if (BIAS) krange = tiny_key_pos<NK>(kp, p.bias, k0, n);
     const int left = n - 2 * t;  // key 8 kb + 2 t + i is there where 8 kb + i < left
-    for (int gh = 0; gh < group; ++gh) {
-        const int head = kvh * group + gh;
-        const Rows<T, DB> rq(p.q, p.q_st, p.q_sh, p.dim, head);
-        const float* Eh = E + gh * entries;
-        // of row g: the next rows to load, and the rows to write
-        const T* from = rq.p + static_cast<int64_t>(q0 + r_begin + g) * p.q_st;
-        T* to = static_cast<T*>(p.out) + (static_cast<int64_t>(q0 + r_begin + g) * p.heads + head) * p.dim;
-        const int64_t to_step = static_cast<int64_t>(8) * p.heads * p.dim;
-        uint32_t qa[DB][4], qb[DB][4];
-        rq.load_at(qa, from, r_begin + g < r_end);
-        rq.load_at(qb, from + 8 * p.q_st, r_begin + g + 8 < r_end);
-        for (int r0 = r_begin; r0 < r_end; r0 += 16, to += 2 * to_step) {
+    // Sixteen rows of one head a step, the heads of the group in turn (their rows lie side by side), the
+    // loads two steps ahead.
+    const Rows<T, DB> rq(p.q, p.q_st, p.q_sh, p.dim, kvh * group);
+    uint32_t qa[DB][4], qb[DB][4], na[DB][4], nb[DB][4];
+    const T* from = rq.p + static_cast<int64_t>(q0 + r_begin + g) * p.q_st;  // of row g: the next rows to load
+    int from_row = r_begin + g, from_head = 0;
+    auto fetch = [&](uint32_t (&x)[DB][4], uint32_t (&y)[DB][4]) {
+        const T* at = from + from_head * p.q_sh;
+        rq.load_at(x, at, from_row < r_end);
+        rq.load_at(y, at + 8 * p.q_st, from_row + 8 < r_end);
+        if (++from_head == group) from_head = 0, from_row += 16, from += 16 * p.q_st;
+    };
+    fetch(qa, qb);
+    fetch(na, nb);
+    T* to_row = static_cast<T*>(p.out) + (static_cast<int64_t>(q0 + r_begin + g) * p.heads + kvh * group) * p.dim;
+    const int64_t to_step = static_cast<int64_t>(8) * p.heads * p.dim;
+    for (int r0 = r_begin; r0 < r_end; r0 += 16, to_row += 2 * to_step) {
+        const TinyBias<NK> tb(p.bias, kp, krange, q0, lq - 1, r0, BIAS);
+        for (int gh = 0; gh < group; ++gh) {
+            const int head = kvh * group + gh;
+            const float* Eh = E + gh * entries;
+            T* to = to_row + gh * p.dim;
             float s[NK][4];
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb) {
@@ -243,12 +253,12 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
                         mma16<T>(s[kb], qa[b][2 * h], qb[b][2 * h], qa[b][2 * h + 1], qb[b][2 * h + 1], kr[kb][b][2 * h],
                                  kr[kb][b][2 * h + 1]);
             }
-            // the next rows are on their way meanwhile
-            from += 16 * p.q_st;
-            rq.load_at(qa, from, r0 + 16 + g < r_end);
-            rq.load_at(qb, from + 8 * p.q_st, r0 + 24 + g < r_end);
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) qa[b][j] = na[b][j], qb[b][j] = nb[b][j];
+            fetch(na, nb);
             if (BIAS) {
-                const TinyBias<NK> tb(p.bias, kp, krange, q0, lq - 1, r0, true);
                 if (tb.linear) {
 #pragma unroll
                     for (int kb = 0; kb < NK; ++kb)
@@ -295,13 +305,26 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
             }
             float o[DB][4][4] = {};
 #pragma unroll
-            for (int kk = 0; kk < NK / 2; ++kk)
+            for (int kk = 0; kk < NK / 2; ++kk) {
+                const int v0 = kKeepV ? 2 * kk : 0;
+                if (!kKeepV) {
+                    if (16 * kk >= n) break;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        rv.load(vt[h], k0 + 16 * kk + 8 * h + g, 16 * kk + 8 * h + g < n);
+#pragma unroll
+                        for (int b = 0; b < DB; ++b)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) vt[h][b][j] = transpose8(vt[h][b][j]);
+                    }
+                }
 #pragma unroll
                 for (int b = 0; b < DB; ++b)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma16<T>(o[b][j], pk[2 * kk][0], pk[2 * kk][1], pk[2 * kk + 1][0], pk[2 * kk + 1][1], vt[2 * kk][b][j],
-                                 vt[2 * kk + 1][b][j]);
+                        mma16<T>(o[b][j], pk[2 * kk][0], pk[2 * kk][1], pk[2 * kk + 1][0], pk[2 * kk + 1][1], vt[v0][b][j],
+                                 vt[v0 + 1][b][j]);
+            }
             sum.x = quad_sum(sx.x + sx.y);
             sum.y = quad_sum(sy.x + sy.y);
             if (r0 + g < r_end) store_row16<T, DB>(to, p.dim, o, 0, sum.x == 0.0f ? 0.0f : __fdividef(1.0f, sum.x));
@@ -315,14 +338,49 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
     }
 }
 
-// Windows of up to 32 keys (NB = 4), or of 33 to 64 (NB = 8): apart, so that the few keys' registers let more
-// warps hide each other's latency, which bounds this kernel.
+// The walk of the forward kernels: pieces of up to kPiece rows of a window, listed by class (up to 32 keys,
+// 33 to 64, 65 to 128) and taken from a queue for each key head, since windows differ in cost.
+constexpr int kPiece = 64;
+constexpr int kClasses = 3;
+__host__ __device__ constexpr int class_of(int nb) { return nb == 4 ? 0 : nb == 8 ? 1 : 2; }
+
+__global__ void __launch_bounds__(256) k_attn_pieces(const __grid_constant__ AttnParams p) {
+    const int w = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 31;
+    int cls = -1, pieces = 0;
+    if (w < p.windows) {
+        const int n = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - attn_offset(p.k_off, p.windows, p.tk, w + 1), 0);
+        const int lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - attn_offset(p.q_off, p.windows, p.tq, w + 1), 0);
+        if (n <= p.tiny_max) cls = n <= 32 ? 0 : n <= 64 ? 1 : 2;
+        pieces = (lq + kPiece - 1) / kPiece;
+    }
+#pragma unroll
+    for (int c = 0; c < kClasses; ++c) {
+        const int mine = cls == c ? pieces : 0;
+        int upto = mine;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += v;
+        }
+        int at = 0;
+        if (lane == 31 && upto > 0) at = atomicAdd(p.flags + c, upto);
+        at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
+        int2* list = reinterpret_cast<int2*>(p.tiny_list) + static_cast<int64_t>(c) * p.tiny_pieces;
+        for (int i = 0; i < mine; ++i)
+            if (at + i < p.tiny_pieces) list[at + i] = make_int2(w, i * kPiece);
+    }
+}
+
+// Windows of up to 32 keys (NB = 4), of 33 to 64 (NB = 8) or of 65 to 128 (NB = 16): apart, so that the few
+// keys' registers let more warps hide each other's latency, which bounds this kernel.
 template <typename T, int DB, int NB, bool BIAS>
-__global__ void __launch_bounds__(32 * tiny_fwd_warps(BIAS), tiny_fwd_blocks(DB, NB) * 4 / tiny_fwd_warps(BIAS)) k_attn_fwd_tiny(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * kWarps, tiny_fwd_blocks(DB, NB)) k_attn_fwd_tiny(const __grid_constant__ AttnParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.heads / p.kv_heads, entries = BIAS ? bias_entries(p.bias) : 0;
-    const Share sh = BIAS ? share_of(p.kv_heads) : Share{static_cast<int>(blockIdx.x) % p.kv_heads, static_cast<int>(blockIdx.x) / p.kv_heads, p.windows};
+    const int listed = min(p.flags[class_of(NB)], p.tiny_pieces);
+    if (listed == 0) return;
+    const Share sh = share_of(p.kv_heads);
     const int side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
     TinyPos<NB>* kp = reinterpret_cast<TinyPos<NB>*>(smem_raw) + warp;
     float* E = reinterpret_cast<float*>(smem_raw + sizeof(TinyPos<NB>) * kWarps);
@@ -335,14 +393,29 @@ __global__ void __launch_bounds__(32 * tiny_fwd_warps(BIAS), tiny_fwd_blocks(DB,
     }
     if (sh.kvh >= p.kv_heads) return;
     const float* Eh = E + (sh.kvh % side) * group * entries;
-    for (int w = sh.first; w < p.windows; w += sh.step) {
+    const int2* list = reinterpret_cast<const int2*>(p.tiny_list) + static_cast<int64_t>(class_of(NB)) * p.tiny_pieces;
+    int* queue = p.flags + kClasses + class_of(NB) * p.kv_heads + sh.kvh;
+    int item = 0;
+    if (lane == 0) item = atomicAdd(queue, 1);
+    for (;;) {
+        const int now = __shfl_sync(0xffffffffu, item, 0);
+        if (now >= listed) break;
+        if (lane == 0) item = atomicAdd(queue, 1);  // the next one, known by the time it is wanted
+        const int2 piece = list[now];
+        const int w = piece.x;
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), n = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
-        if (n > 8 * NB || n <= (NB == 8 ? 32 : 0)) continue;  // other kernels'
-        const int per = ((lq + 15) / 16 + gridDim.z - 1) / gridDim.z * 16;
-        const int r_begin = min(static_cast<int>(blockIdx.z) * per, lq), r_end = min(r_begin + per, lq);
-        if (r_begin >= r_end) continue;
-        if constexpr (NB == 8) {
+        const int r_begin = piece.y, r_end = min(r_begin + kPiece, lq);
+        if (n == 0) {  // nothing to see: zeros
+            for (int r = r_begin * group + lane; r < r_end * group; r += 32) {
+                const int64_t token = q0 + r / group, head = sh.kvh * group + r % group;
+                T* out = static_cast<T*>(p.out) + (token * p.heads + head) * p.dim;
+                for (int c = 0; c < p.dim; ++c) out[c] = from_f<T>(0.0f);
+                if (p.lse != nullptr) p.lse[head * p.tq + token] = INFINITY;
+            }
+            continue;
+        }
+        if constexpr (NB >= 8) {
             tiny_forward<T, DB, NB, BIAS>(p, sh.kvh, group, q0, lq, k0, n, r_begin, r_end, kp, Eh, entries);
         } else {
             if (n <= 16)
@@ -642,6 +715,9 @@ static int tiny_blocks(const AttnParams& p, int resident, int z) {
     const int per = (resident * 148 + sets * z - 1) / (sets * z), most = (p.windows + kWarps / side - 1) / (kWarps / side);
     return most < 1 ? 1 : most < per ? most : per;
 }
+int attn_tiny_pieces(int tq, int windows) { return tq / kPiece + windows; }
+int attn_tiny_forward_counters(int kv_heads) { return kClasses * (1 + kv_heads); }
+int attn_tiny_lists() { return kClasses; }
 int attn_tiny_backward_blocks(const AttnParams& p) { return tiny_blocks(p, 2, p.qsplits); }  // of each of the two kernels
 
 namespace {
@@ -658,18 +734,10 @@ cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int bytes = BIAS ? static_cast<int>(sizeof(TinyPos<NB>)) * kWarps + 4 * heads_of_block(p) * bias_entries(p.bias) : 0;
     cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_tiny<T, DB, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
-    // few windows: their rows are shared out as well, 64 at least
-    const int64_t items = static_cast<int64_t>(p.windows) * p.kv_heads, avg = p.tq / (p.windows < 1 ? 1 : p.windows);
-    int64_t z = 148 * 12 / (items < 1 ? 1 : items);
-    z = z < avg / 64 ? z : avg / 64;
-    z = z < 1 ? 1 : z > 1024 ? 1024 : z;
-    const unsigned uz = static_cast<unsigned>(z);
-    if (BIAS) {  // four rounds of blocks, each with several windows
-        const int blocks = tiny_blocks(p, 4 * tiny_fwd_blocks(DB, NB), static_cast<int>(z));
-        k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(blocks, sets_of(p), uz), 32 * kWarps, bytes, s>>>(p);
-    } else {
-        k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(static_cast<unsigned>(items), 1, uz), 32, bytes, s>>>(p);
-    }
+    // as many blocks as stay resident, or as there can be pieces
+    const int side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1, sets = sets_of(p);
+    const int per = (148 * tiny_fwd_blocks(DB, NB) + sets - 1) / sets, most = (p.tiny_pieces + kWarps / side - 1) / (kWarps / side);
+    k_attn_fwd_tiny<T, DB, NB, BIAS><<<dim3(most < per ? most : per, sets), 32 * kWarps, bytes, s>>>(p);
     return cudaGetLastError();
 }
 template <typename T, int NB, bool BIAS>
@@ -685,7 +753,8 @@ cudaError_t bwd_one(const AttnParams& p, int first_part, cudaStream_t s) {
 template <typename T, bool BIAS>
 cudaError_t fwd_bias(const AttnParams& p, cudaStream_t s) {
     if (p.dim > 32) return fwd_one<T, 2, 4, BIAS>(p, s);
-    const cudaError_t err = fwd_one<T, 1, 8, BIAS>(p, s);
+    cudaError_t err = fwd_one<T, 1, 16, BIAS>(p, s);
+    if (err == cudaSuccess) err = fwd_one<T, 1, 8, BIAS>(p, s);
     return err != cudaSuccess ? err : fwd_one<T, 1, 4, BIAS>(p, s);
 }
 template <typename T, bool BIAS>
@@ -705,6 +774,10 @@ cudaError_t bwd_type(const AttnParams& p, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_attn_forward_tiny(const AttnParams& p, int type, cudaStream_t s) {
+    cudaError_t err = cudaMemsetAsync(p.flags, 0, sizeof(int) * kClasses * (1 + p.kv_heads), s);
+    if (err != cudaSuccess) return err;
+    k_attn_pieces<<<(p.windows + 255) / 256, 256, 0, s>>>(p);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
     return type == kBF16 ? fwd_type<__nv_bfloat16>(p, s) : fwd_type<__half>(p, s);
 }
 cudaError_t launch_attn_backward_tiny(const AttnParams& p, int type, cudaStream_t s) {

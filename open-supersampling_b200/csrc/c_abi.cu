@@ -1308,9 +1308,43 @@ int attention_splits(int64_t tq, int64_t tk, int64_t windows, int64_t heads, int
     return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
 }
 
-int64_t attention_split_bytes(int64_t tq, int64_t heads, int64_t dim, int splits) {
-    if (splits == 1) return 0;
-    return oss::arena_bytes(splits * tq * heads * dim, 4) + oss::arena_bytes(splits * tq * heads * 2, 4);
+// Keys of the windows that the forward's warp-level kernels take, 0: none. They are for windows of up
+// to 128 keys (32 with more than 32 columns) where the average one has at most half of that; their
+// blocks hold the biases of up to 4 key heads.
+int attention_tiny(int32_t dtype, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads, int64_t dim, bool causal,
+                   int64_t entries) {
+    const int64_t most = dim <= 32 ? 128 : 32, side = kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1;
+    return dtype != oss::kF32 && !causal && dim <= 64 && windows > 0 && 2 * tk <= most * windows &&
+                   side * (heads / kv_heads) * entries <= 16384
+               ? static_cast<int>(most)
+               : 0;
+}
+
+// Lays the forward's scratch out; without a base, counts its bytes.
+int64_t attention_forward_scratch(oss::AttnParams& p, char* base, int64_t size) {
+    oss::Arena arena{base, size, 0};
+    if (p.splits > 1) {
+        const int64_t rows = static_cast<int64_t>(p.splits) * p.tq * p.heads;
+        p.part_o = arena.take<float>(rows * p.dim);
+        p.part_ml = arena.take<float>(rows * 2);
+    }
+    if (p.tiny_max > 0) {
+        p.tiny_pieces = oss::attn_tiny_pieces(p.tq, p.windows);
+        p.tiny_list = reinterpret_cast<int*>(arena.take<int2>(static_cast<int64_t>(oss::attn_tiny_lists()) * p.tiny_pieces));
+        p.flags = arena.take<int>(oss::attn_tiny_forward_counters(p.kv_heads));
+    }
+    return arena.used;
+}
+
+// The sizes of a call and what follows from them, in p.
+void attention_forward_plan(oss::AttnParams& p, int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                            int64_t kv_heads, int64_t dim, bool causal, int64_t entries) {
+    p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
+    p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
+    p.causal = causal;
+    p.pack = attention_pack(tq, windows, heads, kv_heads, entries);
+    p.splits = attention_splits(tq, tk, windows, heads, p.pack);
+    p.tiny_max = attention_tiny(dtype, tk, windows, heads, kv_heads, dim, causal, entries);
 }
 
 // How the backward of 16-bit types is cut: see oss::AttnParams.
@@ -1375,11 +1409,14 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
 
 extern "C" {
 
-int64_t oss_window_attention_scratch_bytes(int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
-                                           int64_t dim, int64_t entries) {
-    if (heads <= 0 || kv_heads <= 0) return 0;
-    const int pack = attention_pack(tq, windows, heads, kv_heads, entries);
-    return attention_split_bytes(tq, heads, dim, attention_splits(tq, tk, windows, heads, pack));
+int64_t oss_window_attention_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
+                                           int64_t kv_heads, int64_t dim, int32_t causal, int64_t entries) {
+    if (check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim) != OSS_OK || entries < 0 ||
+        entries > oss::kMaxBiasEntries)
+        return 0;
+    oss::AttnParams p{};
+    attention_forward_plan(p, dtype, tq, tk, windows, heads, kv_heads, dim, causal != 0, entries);
+    return attention_forward_scratch(p, nullptr, 0);
 }
 
 int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
@@ -1405,26 +1442,14 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     p.q = q, p.k = k, p.v = v;
     p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
     p.q_off = q_offsets, p.k_off = k_offsets;
-    p.windows = static_cast<int>(windows), p.tq = static_cast<int>(tq), p.tk = static_cast<int>(tk);
-    p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
-    p.scale = scale, p.causal = causal != 0;
+    p.scale = scale;
     p.out = out, p.lse = lse;
-    p.pack = attention_pack(tq, windows, heads, kv_heads, entries);
+    attention_forward_plan(p, dtype, tq, tk, windows, heads, kv_heads, dim, causal != 0, entries);
     OSS_CHECK(tq * p.pack <= INT_MAX, OSS_ERR_RANGE, "token count times heads of a group exceeds int32 range");
-    p.splits = attention_splits(tq, tk, windows, heads, p.pack);
-    // The warp-level kernel takes windows of up to 64 keys (32 with more than 32 columns) where the
-    // average one is no longer; its blocks hold the biases of up to 4 key heads.
-    const int64_t most = dim <= 32 ? 64 : 32, side = kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1;
-    if (dtype != oss::kF32 && !p.causal && dim <= 64 && windows > 0 && tk <= most * windows &&
-        side * (heads / kv_heads) * entries <= 16384)
-        p.tiny_max = static_cast<int>(most);
-    if (p.splits > 1) {
-        OSS_CHECK(scratch != nullptr && scratch_bytes >= attention_split_bytes(tq, heads, dim, p.splits), OSS_ERR_SCRATCH,
-                  "scratch smaller than oss_window_attention_scratch_bytes");
-        oss::Arena arena{static_cast<char*>(scratch), scratch_bytes, 0};
-        p.part_o = arena.take<float>(p.splits * tq * heads * dim);
-        p.part_ml = arena.take<float>(p.splits * tq * heads * 2);
-    }
+    const int64_t need = attention_forward_scratch(p, nullptr, 0);
+    OSS_CHECK(need == 0 || (scratch != nullptr && scratch_bytes >= need), OSS_ERR_SCRATCH,
+              "scratch smaller than oss_window_attention_scratch_bytes");
+    attention_forward_scratch(p, static_cast<char*>(scratch), scratch_bytes);
     OSS_CUDA_TRY(oss::launch_attn_forward(p, dtype, static_cast<cudaStream_t>(stream)));
     return OSS_OK;
 }

@@ -149,7 +149,7 @@ SIGNATURES = {
         ctypes.c_int, [_i64, _i64, _i64, _i64, _i32, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "oss_reduce_pair_grads_feathered": (
         ctypes.c_int, [_i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
-    "oss_window_attention_scratch_bytes": (_i64, [_i64] * 7),
+    "oss_window_attention_scratch_bytes": (_i64, [_i32, *[_i64] * 6, _i32, _i64]),
     "oss_window_attention_forward": (
         ctypes.c_int,
         [_i32, *[_i64] * 6, *[_p, _i64, _i64] * 3, _p, _p, ctypes.c_float, _i32, _p, _i32, _i64, _p, _i64, _i64, _p, _p,

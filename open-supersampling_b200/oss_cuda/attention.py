@@ -60,7 +60,7 @@ def attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, bucke
         dev = q.device
         out = torch.empty(q.shape, device=dev, dtype=q.dtype)
         lse = torch.empty((q.size(1), q.size(0)), device=dev, dtype=torch.float32) if want_lse else None
-        nbytes = lib.oss_window_attention_scratch_bytes(*args[1:7], 0 if table is None else buckets.numel())
+        nbytes = lib.oss_window_attention_scratch_bytes(*args[:7], causal, 0 if table is None else buckets.numel())
         scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
         rc = lib.oss_window_attention_forward(*args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(scratch), nbytes, stream_of(q))
         if rc:

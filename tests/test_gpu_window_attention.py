@@ -129,7 +129,7 @@ def test_many_queries_of_few_keys(cuda_device, dtype, lk):
 def test_long_axis_is_split_and_joined(cuda_device, dtype, lq, lk, causal):
     from oss_cuda import _lib
 
-    assert _lib.lib().oss_window_attention_scratch_bytes(2 * lq, lk + 700, 2, 4, 2, 64, 0) > 0
+    assert _lib.lib().oss_window_attention_scratch_bytes(0, 2 * lq, lk + 700, 2, 4, 2, 64, int(causal), 0) > 0
     (q, k, v, do), qo, ko, _ = inputs([lq, lq], [lk, 700], 4, 2, 64, TYPES[dtype], seed=lk)
     both(cuda_device, q, k, v, qo, ko, causal=causal)
     both(cuda_device, q, k, v, qo, ko, do, causal=causal)
