@@ -124,6 +124,22 @@ def test_many_queries_of_few_keys(cuda_device, dtype, lk):
     both(cuda_device, q, k, v, qo, ko, do, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,kv", [(8, 4, 4), (20, 6, 3), (31, 2, 1), (32, 5, 5), (64, 4, 2)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_windows_of_every_class(cuda_device, dtype, dim, heads, kv, biased):
+    """Windows of every class of the few-keys kernels and beyond in one call, with pieces of rows around 64."""
+    kl = [0, 1, 15, 16, 17, 32, 33, 48, 64, 65, 80, 96, 97, 127, 128, 129, 300] + [3] * 20
+    ql = [7, 64, 65, 1, 130, 3, 63, 128, 5, 66, 17, 129, 2, 64, 33, 70, 9] + [0, 1, 40, 2] * 5
+    (q, k, v, do), qo, ko, g = inputs(ql, kl, heads, kv, dim, TYPES[dtype], seed=dim, qfirst=2, ktail=3, qtail=70)
+    kw = {}
+    if biased:
+        kw = {"buckets": torch.arange(35, dtype=torch.int32).view(5, 7), "table": torch.randn(35, heads, generator=g),
+              "q_pos": torch.randint(0, 9, (q.shape[0], 2), generator=g).int(),
+              "k_pos": torch.randint(0, 9, (k.shape[0], 2), generator=g).int()}
+    both(cuda_device, q, k, v, qo, ko, do, **kw)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lq,lk,causal", [(1, 3000, True), (2, 5001, False), (17, 2100, True)])
 def test_long_axis_is_split_and_joined(cuda_device, dtype, lq, lk, causal):
