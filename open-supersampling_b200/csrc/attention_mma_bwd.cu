@@ -160,6 +160,10 @@ __device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim,
             for (int i = 0; i < 4; ++i) w[i] = pack2(o[8 * h + 2 * i] * by, o[8 * h + 2 * i + 1] * by, T{});
             *reinterpret_cast<uint4*>(to + c + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+    } else if (dim % 2 == 0 && (reinterpret_cast<uintptr_t>(to) & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+            if (c + i < dim) reinterpret_cast<uint32_t*>(to + c)[i / 2] = pack2(o[i] * by, o[i + 1] * by, T{});
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -259,7 +263,10 @@ __device__ __noinline__ void query_row(const AttnParams& p, int64_t q, int head,
 // dk (want_v: dv) of key k, the j-th of its window, over the query tiles [i0, i1) of its heads.
 template <typename T>
 __device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int kvh, int64_t q0, int lq, int lk, int i0, int i1, float up,
-                                     bool want_v, T* out, float* part) {
+                                     bool want_v, int z) {
+    const int64_t row = (k * p.kv_heads + kvh) * p.dim;
+    T* out = static_cast<T*>(want_v ? p.dv : p.dk) + row;
+    float* part = p.qsplits > 1 ? (want_v ? p.part_dv : p.part_dk) + static_cast<int64_t>(z) * p.tk * p.kv_heads * p.dim + row : nullptr;
     float o[kMaxHeadDim];
     const int group = p.heads / p.kv_heads, qtiles = (lq + kRows - 1) / kRows;
     for (int c = 0; c < kMaxHeadDim; ++c) o[c] = 0.0f;
@@ -288,10 +295,11 @@ __device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int 
     }
 }
 
-// A row of dk or dv out of tensor memory. Whole warps; rows of lanes with `live`.
+// A row of dk or dv out of tensor memory. Whole warps; rows of lanes with `live`. `staged`: to row r of the panel at
+// `to` instead of memory. True: the row has to be found by key_row.
 template <typename T, int DP>
-__device__ __forceinline__ void finish_key_row(const AttnParams& p, uint32_t at, bool live, bool any, int64_t k, int j, int kvh, int64_t q0,
-                                               int lq, int lk, int i0, int i1, int z, float up, bool want_v, bool alive) {
+__device__ __forceinline__ bool finish_key_row(const AttnParams& p, uint32_t at, bool live, bool any, int64_t k, int kvh, int z,
+                                               float up, bool want_v, bool alive, bool staged, uint32_t to, int r) {
     const int64_t row = (k * p.kv_heads + kvh) * p.dim;
     T* out = static_cast<T*>(want_v ? p.dv : p.dk) + row;
     float* part = p.qsplits > 1 ? (want_v ? p.part_dv : p.part_dk) + static_cast<int64_t>(z) * p.tk * p.kv_heads * p.dim + row : nullptr;
@@ -315,11 +323,13 @@ __device__ __forceinline__ void finish_key_row(const AttnParams& p, uint32_t at,
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= by;
             write_part(part, o, c, p.dim);
+        } else if (staged) {
+            stage16<T>(to, r, o, c, by);
         } else {
             write_out<T>(out, o, c, p.dim, by);
         }
     }
-    if (p.causal && live && !fine && alive) key_row<T>(p, k, j, kvh, q0, lq, lk, i0, i1, up, want_v, out, part);
+    return p.causal && live && !fine && alive;
 }
 
 // ---- which windows there are -----------------------------------------------------------------
@@ -579,8 +589,9 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         }
         if ((warp & 3) < 2) {
             const bool of_v = tid < kRows;
-            finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, i0 < i1, k0 + min(row, n - 1), row, kvh, q0, lq, lk, i0, i1, z, up, of_v,
-                                  alive);
+            const int64_t key = k0 + min(row, n - 1);
+            if (finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, i0 < i1, key, kvh, z, up, of_v, alive, false, 0, 0))
+                key_row<T>(p, key, row, kvh, q0, lq, lk, i0, i1, up, of_v, z);
         }
         tc::fence_before();
     }
@@ -643,11 +654,11 @@ struct DqShape {
 // dk, dv: 128 keys, so that the products fill their 128 rows; one block of 512 threads.
 template <int DP>
 struct DkvShape {
-    static constexpr int KT = 128, kThreads = 512, N = 32;
-    static constexpr int kBuf = DP == 64 ? 2 : 1;  // of the queries
-    static constexpr int kT = kRows * DP * 2, kP = kRows * KT * 2;
-    static constexpr int kTiles = 2 * kT + 2 * kBuf * kT + 2 * kP;
-    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<KT>)) + 64 + 64;
+    static constexpr int KT = DP == 64 ? 64 : 128, kThreads = 4 * KT, N = 32;
+    static constexpr int kT = kRows * DP * 2, kK = KT * DP * 2, kP = kRows * KT * 2;
+    static constexpr int kTiles = 2 * kP + 2 * kT + 2 * kK;
+    static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<KT>)) + 8 * static_cast<int>(sizeof(Range)) + 64;
+    static constexpr int kCols = DP == 64 ? 256 : 512;  // S, dP, dV, dK
 };
 
 template <typename T, int DP, bool BIAS>
@@ -843,17 +854,18 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
 
 // ---- long windows: dk, dv --------------------------------------------------------------------
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_attn_dkv_long(const __grid_constant__ AttnParams p) {
     if ((*p.flags & kSomeLong) == 0) return;
     using L = DkvShape<DP>;
-    constexpr int KT = L::KT, kBuf = L::kBuf, kThreads = L::kThreads, N = L::N;
+    constexpr int KT = L::KT, kThreads = L::kThreads, N = L::N;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t sk = tc::smem_addr(base), sv = sk + L::kT, sq = sv + L::kT, sg = sq + kBuf * L::kT, sp = sg + kBuf * L::kT,
-                   sd = sp + L::kP;
+    // P and dS first: with tiles of 64 keys the products still take 128 of their columns, the second half
+    // from what lies behind, for rows of dK and dV that nobody reads
+    const uint32_t sp = tc::smem_addr(base), sd = sp + L::kP, sq = sd + L::kP, sg = sq + L::kT, sk = sg + L::kT, sv = sk + L::kK;
     KeyPos<KT>* kp = reinterpret_cast<KeyPos<KT>*>(base + L::kTiles);
-    Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of both buffers' queries: 4 warps each, written in turn
-    uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 4);
+    Range* qrange = reinterpret_cast<Range*>(kp + 1);  // of a tile's queries, by warps; and of the next one's
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qrange + 8);
     uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(bars + 2);
     volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     const int entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
@@ -870,7 +882,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
         tc::mbar_init_fence();
         *dead = 0;
     }
-    if (warp == 0) tc::tmem_alloc<512>(tc::smem_addr(slot_tmem));
+    if (warp == 0) tc::tmem_alloc<L::kCols>(tc::smem_addr(slot_tmem));
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -880,6 +892,9 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
     const float up = ds_scale<T>(p);
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
+    // dk and dv through smem where their rows are not on 16 bytes (there, direct stores were 2% faster)
+    const bool staged = p.qsplits == 1 &&
+                        ((p.dim & 7) != 0 || ((reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv)) & 15) != 0);
 
     LongWalk<KT> walk(slots, p);
     for (bool more = walk.first(p.k_off, p.tk, p.q_off, p.tq); more; more = walk.next()) {
@@ -891,38 +906,31 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
         // causal: query tiles before this one see none of the tile's keys
         const int qt0 = p.causal ? min(max(t.first - (lk - lq), 0) / kRows, qtiles) : 0;
         auto next = [&](int it) { return it < i1 && it % qtiles < qt0 ? it - it % qtiles + qt0 : it; };
-        auto fetch = [&](int it, int b) {
+        auto fetch = [&](int it) {
             const int first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
-            oq.load(sq + b * L::kT, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.q_sh);
-            og.load(sg + b * L::kT, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.do_sh);
+            oq.load(sq, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.q_sh);
+            og.load(sg, kRows, t.obegin + first, rows, kRows, (it / qtiles) * p.do_sh);
         };
-        __syncthreads();
-        int it = next(i0), b = 0;
-        const bool any = it < i1;
-        if (any) {
-            ok.load(sk, KT, t.begin + t.first, n, n16);
-            ov.load(sv, KT, t.begin + t.first, n, n16);
-            fetch(it, 0);
-            if (BIAS) load_key_pos<KT>(kp, p.bias, t.begin + t.first, n);
-        }
-        tc::cp_async_commit();
-        bool begun = false;
-        while (it < i1) {
+        // What a thread knows of its query of a tile; asked for a tile ahead.
+        struct Row {
+            float lse, delta;
+            int2 qp;
+        };
+        auto row_of = [&](int it) {
             const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
-            const int after = next(it + 1);
-            const bool live = row < rows;
-            const int64_t token = t.obegin + first + min(row, rows - 1);
-            const float lse = live ? p.lse[static_cast<int64_t>(head) * p.tq + token] : INFINITY;
-            const float delta = live ? p.delta[static_cast<int64_t>(head) * p.tq + token] : 0.0f;
-            int2 qp = make_int2(0, 0);
-            if (BIAS) {
-                qp = bias_pos(p.bias.q_pos, p.bias.axes, token);
-                const Range r = warp_range(qp);
-                if (tid < kRows && (tid & 31) == 0) qrange[warp] = r;
-                if (head != head_of_E)  // everyone is past the last tile's lookups: its barrier before dV and dK
-                    for (int e = tid; e < entries; e += kThreads) E[e] = bias_entry(p.bias, p.heads, head, e);
-                head_of_E = head;
-            }
+            const int64_t token = t.obegin + first + min(row, rows - 1), at = static_cast<int64_t>(head) * p.tq + token;
+            return Row{p.lse[at], p.delta[at], BIAS ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0)};
+        };
+        auto post_range = [&](const Row& r, int half) {
+            const Range x = warp_range(r.qp);
+            if (tid < kRows && (tid & 31) == 0) qrange[4 * half + warp] = x;
+        };
+        auto load_E = [&](int it) {
+            head_of_E = kvh * group + it / qtiles;
+            for (int e = tid; e < entries; e += kThreads) E[e] = bias_entry(p.bias, p.heads, head_of_E, e);
+        };
+        // Of the queries in smem, once everyone's copies are there.
+        auto scores = [&] {
             tc::cp_async_wait<0>();
             tc::fence_async();
             tc::fence_before();
@@ -930,64 +938,88 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, 1) k_attn_dkv_long(con
             if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
-                tc::mma_nt<DP, kRows, KT>(tmem, sq + b * L::kT, sk, dim16, id);
-                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg + b * L::kT, sv, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem, sq, sk, dim16, id);
+                tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv, dim16, id);
                 tc::commit(bar_s);
             }
-            if (kBuf == 2) {
-                if (begun) {
-                    alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
-                    par_o ^= 1;
-                }
-                if (after < i1) fetch(after, b ^ 1);
-                tc::cp_async_commit();
+        };
+        __syncthreads();
+        int it = next(i0), half = 0;
+        const bool any = it < i1;
+        Row now{};
+        if (any) {
+            ok.load(sk, KT, t.begin + t.first, n, n16);
+            ov.load(sv, KT, t.begin + t.first, n, n16);
+            fetch(it);
+            tc::cp_async_commit();
+            now = row_of(it);
+            if (BIAS) {
+                load_key_pos<KT>(kp, p.bias, t.begin + t.first, n);
+                post_range(now, 0);
+                if (kvh * group + it / qtiles != head_of_E) load_E(it);
             }
+            scores();
+        }
+        bool begun = false;
+        while (it < i1) {
+            const int first = (it % qtiles) * kRows, rows = min(kRows, lq - first), after = next(it + 1);
+            const bool live = row < rows;
+            Row ahead{};
+            if (after < i1) ahead = row_of(after);
             const int see = !live ? 0 : p.causal ? min(max(first + row + lk - lq + 1, 0), lk) : lk;
             const bool whole = n == n16 && (!p.causal || first + lk - lq + 1 >= t.first + n);
             BiasMode mode = kOne;
-            if (BIAS) mode = bias_mode(p.bias, join(join(qrange[0], qrange[1]), join(qrange[2], qrange[3])), key_range(kp));
+            if (BIAS) {
+                const Range* r = qrange + 4 * half;
+                mode = bias_mode(p.bias, join(join(r[0], r[1]), join(r[2], r[3])), key_range(kp));
+            }
             alive = tc::mbar_wait(bar_s, par_s, dead) && alive;
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, lse, mode, E, kp, qp);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, live ? now.lse : INFINITY, mode, E, kp, now.qp);
             write_row<T>(sp, row, j0, s, 1.0f);
-            score_gradients(s, dp, delta);
+            score_gradients(s, dp, live ? now.delta : 0.0f);
             write_row<T>(sd, row, j0, dp, up);
+            if (BIAS && after < i1) post_range(ahead, half ^ 1);
             tc::fence_async();
             tc::fence_before();
             __syncthreads();
             if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
-                tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, kRows * 128), tc::desc(sg + b * L::kT, kRows * 128), id_grad, begun);
-                tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, kRows * 128), tc::desc(sq + b * L::kT, kRows * 128), id_grad, begun);
+                tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, kRows * 128), tc::desc(sg, kRows * 128), id_grad, begun);
+                tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, kRows * 128), tc::desc(sq, kRows * 128), id_grad, begun);
                 tc::commit(bar_o);
             }
-            if (kBuf == 1) {
-                alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
-                par_o ^= 1;
-                if (after < i1) fetch(after, 0);
-                tc::cp_async_commit();
-            } else {
-                b ^= 1;
-            }
-            begun = true;
-            it = after;
-        }
-        if (begun && kBuf == 2) {
+            if (BIAS && after < i1 && kvh * group + after / qtiles != head_of_E) load_E(after);  // everyone is past this head's lookups
             alive = tc::mbar_wait(bar_o, par_o, dead) && alive;
             par_o ^= 1;
+            begun = true;
+            if (after < i1) {
+                fetch(after);
+                tc::cp_async_commit();
+                scores();
+            }
+            it = after, now = ahead, half ^= 1;
         }
         tc::fence_after();
         const bool of_v = tid < kRows;
-        if (tid < 2 * kRows) finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, t.begin + t.first + min(row, n - 1), t.first + row, kvh, t.obegin, lq,
-                              lk, i0, i1, z, up, of_v, alive);
+        const int64_t key = t.begin + t.first + min(row, n - 1);
+        const bool slow = tid < 2 * kRows && finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, key, kvh, z, up,
+                                                                   of_v, alive, staged, of_v ? sp : sd, row);
+        if (staged) {
+            __syncthreads();
+            store_panel<T, kThreads>(sp, p.dv, p.kv_heads, p.dim, t.begin, kvh, 1, t.first, n);
+            store_panel<T, kThreads>(sd, p.dk, p.kv_heads, p.dim, t.begin, kvh, 1, t.first, n);
+            if (p.causal) __syncthreads();  // before rows that are written once more
+        }
+        if (slow) key_row<T>(p, key, t.first + row, kvh, t.obegin, lq, lk, i0, i1, up, of_v, z);
         tc::fence_before();
     }
     if (!alive && tid == 0) count_timeout();
     tc::fence_before();
     __syncthreads();
-    if (warp == 0) tc::tmem_free<512>(tmem);
+    if (warp == 0) tc::tmem_free<L::kCols>(tmem);
 }
 
 // ---- sums across blocks ------------------------------------------------------------------------

@@ -289,6 +289,12 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
         p.lse[(row % p.heads) * p.tq + row / p.heads] = l == 0.0f ? INFINITY : top + log2f(l);
 }
 
+// Of 64 bits where it must be: such a division costs some ninety instructions more.
+__device__ __forceinline__ int64_t divide(int64_t x, int by) {
+    return x >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(by)) : x / by;
+}
+
+
 // ---- backward ----------------------------------------------------------------
 // delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for the bias
 // gradient's fixed point, and fp16's range). LANES lanes a row, two values at a time where its
@@ -309,8 +315,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* de
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per; row0 < rows + vrows; row0 += step) {
         const int64_t row = row0 + threadIdx.x / LANES;
         float sum = 0.0f;
+        int64_t token = 0, head = 0;
         if (row < rows) {
-            const int64_t token = row / p.heads, head = row - token * p.heads;
+            token = divide(row, p.heads), head = row - token * p.heads;
             const T* g = static_cast<const T*>(p.dout) + token * p.do_st + head * p.do_sh;
             const T* o = static_cast<const T*>(p.out) + row * p.dim;
             for (int c = V * lane; c < p.dim; c += V * LANES) {
@@ -323,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* de
                 }
             }
         } else if (row < rows + vrows) {
-            const int64_t token = (row - rows) / p.kv_heads, head = row - rows - token * p.kv_heads;
+            token = divide(row - rows, p.kv_heads), head = row - rows - token * p.kv_heads;
             const T* v = static_cast<const T*>(p.v) + token * p.v_st + head * p.v_sh;
             for (int c = V * lane; c < p.dim; c += V * LANES) {
                 const Pair x = *reinterpret_cast<const Pair*>(v + c);
@@ -336,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* de
         }
 #pragma unroll
         for (int x = LANES / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        if (lane == 0 && row < rows) delta[(row % p.heads) * p.tq + row / p.heads] = sum;
+        if (lane == 0 && row < rows) delta[head * p.tq + token] = sum;
     }
     if (bias_max == nullptr) return;
     const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(most_do));

@@ -1355,8 +1355,9 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     // Parts of the queries, so that few tiles of keys still fill the card: at least 4 tiles of 128
     // queries in each on average.
     const int64_t windows = p.windows < 1 ? 1 : p.windows;
-    const int64_t items = (windows > p.tk / 128 ? windows : p.tk / 128) * p.kv_heads;
-    const int64_t want = 2 * kSms / items, most = p.tq / windows * group / 512;
+    const int64_t key_tile = p.dim <= 64 ? 64 : 128, resident = kSms * (p.dim <= 64 ? 2 : 1);
+    const int64_t items = (windows > p.tk / key_tile ? windows : p.tk / key_tile) * p.kv_heads;
+    const int64_t want = 2 * resident / items, most = p.tq / windows * group / 512;
     const int64_t n = want < most ? want : most;
     p.qsplits = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
     // resident blocks (no more: a few blocks left over would take as long as all others again), or as
@@ -1372,9 +1373,9 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
                       entries * group * (4 * side + (sums ? 48 : 0)) <= 110 * 1024;
     p.tiny_max = tiny ? 32 : 0;
     p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;
-    p.short_blocks = blocks(windows, (p.dim <= 64 ? 2 : 1) * kSms, p.kv_heads * p.qsplits);
-    p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (p.dim <= 64 ? 2 : 1) * (sums ? 1 : 4) * kSms, p.heads);
-    p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, 128), 4 * kSms, p.kv_heads * p.qsplits);
+    p.short_blocks = blocks(windows, resident, p.kv_heads * p.qsplits);
+    p.dq_blocks = blocks(oss::attn_slots(p.tq, p.windows, 128), (sums ? 1 : 4) * resident, p.heads);
+    p.dkv_blocks = blocks(oss::attn_slots(p.tk, p.windows, static_cast<int>(key_tile)), 4 * resident, p.kv_heads * p.qsplits);
     p.bias_tiny = 2 * p.tiny_blocks * p.qsplits;  // of its two kernels
     p.bias_short = p.short_max > 0 ? p.short_blocks * p.qsplits : 0;
     p.bias_parts = p.bias_tiny + p.bias_short + p.dq_blocks;
