@@ -102,7 +102,7 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
     weight, bias, scale, next_weight, next_bias
                  (C,) parameters of one type, fp32 or x's; only weight is required (scale 1, no biases)
     gate         (..., C) of x's type, or (..., 1): one for each row; None: 1
-    gate_act     "none", "sigmoid" or "silu" of the gate
+    gate_act     "none", "sigmoid" or "silu" of the gate; without a gate it changes nothing
     kind         "rms" (u / sqrt(mean(u^2) + eps)) or "layer" ((u - mean) / sqrt(var + eps)); biases are for "layer"
 
     Returns (y, z), or y alone without next_weight.  The arithmetic is fp32, each result rounded once (z is taken
@@ -111,8 +111,6 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
         raise ValueError(f"kind must be one of {KINDS}, got {kind!r}")
     if gate_act not in ACTS:
         raise ValueError(f"gate_act must be one of {sorted(ACTS)}, got {gate_act!r}")
-    if gate is None and gate_act != "none":
-        raise ValueError("gate_act applies with gate only")
     eps = float(eps)
     if not 0.0 <= eps < 3.0e38:
         raise ValueError("eps must be non-negative and finite")
@@ -154,7 +152,7 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
         params.append(t)
     x2, h2 = _rows(x, c), _rows(h, c)
     g2 = None if gate is None else _rows(gate, gate.shape[-1])
-    layer, act = int(kind == "layer"), ACTS[gate_act]
+    layer, act = int(kind == "layer"), ACTS[gate_act] if gate is not None else 0
     if grad:
         y, z = _GatedNorm.apply(x2, h2, g2, *params, layer, act, eps)
     else:

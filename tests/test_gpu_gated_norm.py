@@ -94,6 +94,13 @@ def test_gates(cuda_device, dtype, gate, act):
         check(run(cuda_device, a, act, "layer", dy=dy, dz=dz), want, a, "layer")
 
 
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_activation_without_gate_changes_nothing(cuda_device, act):
+    a, dy, dz = tensors(37, 72, torch.bfloat16, "none", "rms")
+    want, got = (run(cuda_device, a, x, dy=dy, dz=dz) for x in ("none", act))
+    assert all(torch.equal(got[n], want[n]) for n in want if want[n] is not None)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("leave", [["scale"], ["gate"], ["next_weight"], ["scale", "gate", "next_weight"]])
 def test_parts_left_out(cuda_device, dtype, leave):

@@ -94,7 +94,6 @@ def norm(**change):
 NORM = {
     "kind": (dict(kind="batch"), ValueError, "kind"),
     "activation": (dict(gate=lambda: fake((6, 48)), gate_act="relu"), ValueError, "gate_act"),
-    "activation without gate": (dict(gate_act="silu"), ValueError, "with gate only"),
     "eps negative": (dict(eps=-1e-6), ValueError, "eps"),
     "eps NaN": (dict(eps=math.nan), ValueError, "eps"),
     "eps infinite": (dict(eps=math.inf), ValueError, "eps"),
