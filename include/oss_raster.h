@@ -653,6 +653,9 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
  *   q[tq][heads][dim], k and v[tk][kv_heads][dim]  token and head strides in elements, unit last stride
  *   out[tq][heads][dim], d_q, d_k, d_v             contiguous
  *   lse[heads][tq]     fp32, base-2 log of the row's sum (null: not wanted); +inf for a row without keys
+ *   out_lo[tq][heads][dim]  what rounding took from out, of q's type, for the backward of 16-bit types (null: not
+ *                      wanted there, and in the backward not known, which costs its gradients a little precision).
+ *                      Rows that the backward does not need may stay unwritten.
  *   table[buckets][heads]  null: no bias.  bucket_map[2 ry + 1][2 rx + 1] maps the key's position less the
  *                      query's, clamped to +-ry and +-rx, to a row of the table; a value outside
  *                      [0, buckets) adds no bias.  At most 4096 entries.
@@ -668,8 +671,8 @@ OSS_API int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, 
                                          int64_t v_sh, const int32_t* q_offsets, const int32_t* k_offsets, float scale,
                                          int32_t causal, const void* table, int32_t table_dtype, int64_t buckets,
                                          const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
-                                         const int32_t* k_pos, int32_t axes, void* out, float* lse, void* scratch,
-                                         int64_t scratch_bytes, void* stream);
+                                         const int32_t* k_pos, int32_t axes, void* out, float* lse, void* out_lo,
+                                         void* scratch, int64_t scratch_bytes, void* stream);
 /* Waits inside the tensor-core kernels are bounded; one that runs out (which would be a fault of the
  * library) leaves NaN in its rows and is counted.  count: blocks that this happened to on the current
  * device since the library was loaded.  Synchronises. */
@@ -687,7 +690,7 @@ OSS_API int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk,
                                           int32_t causal, const void* table, int32_t table_dtype, int64_t buckets,
                                           const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
                                           const int32_t* k_pos, int32_t axes, const void* out, const float* lse,
-                                          const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
+                                          const void* out_lo, const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
                                           void* d_v, void* d_table, void* scratch, int64_t scratch_bytes, void* stream);
 
 /* n = norm(h) weight + bias,  y = x + scale act(gate) n,  z = norm(y) next_weight + next_bias.

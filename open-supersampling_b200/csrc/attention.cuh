@@ -47,6 +47,10 @@ struct AttnParams {
     AttnBias bias;
     void* out;        // [tq][heads][dim]
     float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
+    // What rounding took from out, [tq][heads][dim] of the same type, of windows with more keys than short_max (others'
+    // may stay unwritten): dout . out is then right to 16 bits more. With out alone the gradients of long windows were
+    // off by half as much again as rounding them makes them, and the bias table's by twice. May be null; 16-bit types.
+    void* out_lo;
     int tiny_max;     // windows of up to so many keys (backward: of 1 to so many) go to the warp-level kernels
                       // (attention_tiny.cu); 0: none
     // forward only
@@ -310,6 +314,12 @@ __device__ __forceinline__ void bias_mark_bad(const AttnParams& p, int head, int
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// What rounding x to T takes from it.
+template <typename T>
+__device__ __forceinline__ float lost_by(float x) {
+    const float d = x - to_f(from_f<T>(x));
+    return is_finite(d) ? d : 0.0f;
+}
 
 
 // ---- launchers -----------------------------------------------------------------

@@ -412,6 +412,26 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
             if (p.splits > 1) continue;
             tc::bar_sync(1, kRows);
             store_panel<T, kRows>(sq, p.out, p.heads, p.dim, t.begin, head0, p.pack, t.first, rows);
+            if (p.out_lo == nullptr) continue;
+            tc::bar_sync(1, kRows);  // the staging has been read
+#pragma unroll
+            for (int c = 0; c < DP; c += 16) {
+                if (c >= dim16) continue;
+                float o[16];
+                if (kk.tile0 < kk.tile1) {
+                    tc::tmem_ld16(to + c, o);
+                    tc::wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = fine ? lost_by<T>(o[i] * inv) : 0.0f;
+                stage16<T>(sq, tid, o, c, 1.0f);
+            }
+            tc::fence_before();
+            tc::bar_sync(1, kRows);
+            store_panel<T, kRows>(sq, p.out_lo, p.heads, p.dim, t.begin, head0, p.pack, t.first, rows);
         }
         if (!alive && tid == 0) count_timeout();
         tc::fence_before();

@@ -287,6 +287,12 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
 #pragma unroll
     for (int c = 0; c < kMaxHeadDim / 32; ++c)
         if (lane + 32 * c < p.dim) out[lane + 32 * c] = from_f<T>(o[c] * inv);
+    if (p.out_lo != nullptr) {
+        T* lo = static_cast<T*>(p.out_lo) + row * p.dim;
+#pragma unroll
+        for (int c = 0; c < kMaxHeadDim / 32; ++c)
+            if (lane + 32 * c < p.dim) lo[lane + 32 * c] = from_f<T>(lost_by<T>(o[c] * inv));
+    }
     if (p.lse != nullptr && lane == 0)
         p.lse[(row % p.heads) * p.tq + row / p.heads] = l == 0.0f ? INFINITY : top + log2f(l);
 }
@@ -323,12 +329,15 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* de
             token = divide(row, p.heads), head = row - token * p.heads;
             const T* g = static_cast<const T*>(p.dout) + token * p.do_st + head * p.do_sh;
             const T* o = static_cast<const T*>(p.out) + row * p.dim;
+            const T* lo = p.out_lo == nullptr ? nullptr : static_cast<const T*>(p.out_lo) + row * p.dim;
             for (int c = V * lane; c < p.dim; c += V * LANES) {
                 const Pair x = *reinterpret_cast<const Pair*>(g + c), y = *reinterpret_cast<const Pair*>(o + c);
+                Pair less{};
+                if (lo != nullptr) less = *reinterpret_cast<const Pair*>(lo + c);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float f = to_f(x.v[i]);
-                    sum = fmaf(f, to_f(y.v[i]), sum);
+                    sum = fmaf(f, to_f(y.v[i]) + (lo == nullptr ? 0.0f : to_f(less.v[i])), sum);
                     if (is_finite(f)) most_do = fmaxf(most_do, fabsf(f));
                 }
             }

@@ -332,6 +332,18 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
             sum.y = quad_sum(sy.x + sy.y);
             if (r0 + g < r_end) store_row16<T, DB>(to, p.dim, o, 0, sum.x == 0.0f ? 0.0f : __fdividef(1.0f, sum.x));
             if (r0 + g + 8 < r_end) store_row16<T, DB>(to + to_step, p.dim, o, 1, sum.y == 0.0f ? 0.0f : __fdividef(1.0f, sum.y));
+            if (NK == 16 && p.out_lo != nullptr) {  // windows of fewer keys find dout . out by themselves
+                const float ix = sum.x == 0.0f ? 0.0f : __fdividef(1.0f, sum.x), iy = sum.y == 0.0f ? 0.0f : __fdividef(1.0f, sum.y);
+#pragma unroll
+                for (int b = 0; b < DB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[b][j][i] = lost_by<T>(o[b][j][i] * (i < 2 ? ix : iy));
+                T* lo = static_cast<T*>(p.out_lo) + (to - static_cast<T*>(p.out));
+                if (r0 + g < r_end) store_row16<T, DB>(lo, p.dim, o, 0, 1.0f);
+                if (r0 + g + 8 < r_end) store_row16<T, DB>(lo + to_step, p.dim, o, 1, 1.0f);
+            }
             if (p.lse != nullptr && t == 0) {
                 float* lse = p.lse + static_cast<int64_t>(head) * p.tq + q0 + r0 + g;
                 if (r0 + g < r_end) lse[0] = sum.x == 0.0f ? INFINITY : top.x + log2f(sum.x);

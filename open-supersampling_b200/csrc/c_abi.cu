@@ -1427,7 +1427,7 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
                                  const int32_t* k_offsets, float scale, int32_t causal, const void* table,
                                  int32_t table_dtype, int64_t buckets, const int32_t* bucket_map, int64_t ry, int64_t rx,
                                  const int32_t* q_pos, const int32_t* k_pos, int32_t axes, void* out, float* lse,
-                                 void* scratch, int64_t scratch_bytes, void* stream) {
+                                 void* out_lo, void* scratch, int64_t scratch_bytes, void* stream) {
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
     OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
@@ -1445,8 +1445,10 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
     p.q_off = q_offsets, p.k_off = k_offsets;
     p.scale = scale;
-    p.out = out, p.lse = lse;
+    p.out = out, p.lse = lse, p.out_lo = dtype == oss::kF32 ? nullptr : out_lo;
     attention_forward_plan(p, dtype, tq, tk, windows, heads, kv_heads, dim, causal != 0, entries);
+    // without the backward's kernel for short windows, the warp-level kernels' would miss what it needs of them
+    if (p.out_lo != nullptr && entries * (heads / kv_heads) > oss::kMaxBiasEntries) p.tiny_max = 0;
     OSS_CHECK(tq * p.pack <= INT_MAX, OSS_ERR_RANGE, "token count times heads of a group exceeds int32 range");
     const int64_t need = attention_forward_scratch(p, nullptr, 0);
     OSS_CHECK(need == 0 || (scratch != nullptr && scratch_bytes >= need), OSS_ERR_SCRATCH,
@@ -1484,7 +1486,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
                                   const int32_t* k_offsets, float scale, int32_t causal, const void* table,
                                   int32_t table_dtype, int64_t buckets, const int32_t* bucket_map, int64_t ry, int64_t rx,
                                   const int32_t* q_pos, const int32_t* k_pos, int32_t axes, const void* out,
-                                  const float* lse, const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
+                                  const float* lse, const void* out_lo, const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
                                   void* d_v, void* d_table, void* scratch, int64_t scratch_bytes, void* stream) {
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
@@ -1513,6 +1515,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
     p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
     p.scale = scale, p.causal = causal != 0, p.pack = 1, p.splits = 1;
     p.out = const_cast<void*>(out), p.lse = const_cast<float*>(lse);
+    p.out_lo = dtype == oss::kF32 ? nullptr : const_cast<void*>(out_lo);
     p.dout = d_out, p.do_st = do_st, p.do_sh = do_sh, p.dq = d_q, p.dk = d_k, p.dv = d_v;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     char* zero_at = nullptr;

@@ -153,13 +153,13 @@ SIGNATURES = {
     "oss_window_attention_forward": (
         ctypes.c_int,
         [_i32, *[_i64] * 6, *[_p, _i64, _i64] * 3, _p, _p, ctypes.c_float, _i32, _p, _i32, _i64, _p, _i64, _i64, _p, _p,
-         _i32, _p, _p, _p, _i64, _p]),
+         _i32, _p, _p, _p, _p, _i64, _p]),
     "oss_window_attention_timeouts": (ctypes.c_int, [_p]),
     "oss_window_attention_backward_scratch_bytes": (_i64, [_i32, *[_i64] * 6, _i32, _i64, _i64]),
     "oss_window_attention_backward": (
         ctypes.c_int,
         [_i32, *[_i64] * 6, *[_p, _i64, _i64] * 3, _p, _p, ctypes.c_float, _i32, _p, _i32, _i64, _p, _i64, _i64, _p, _p,
-         _i32, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
+         _i32, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p]),
     "oss_gated_norm_forward": (
         ctypes.c_int,
         [_i32, _i64, _i64, *[_p, _i64] * 3, _i32, _i32, _i32, ctypes.c_float, _i32, *[_p] * 5, _p, _p, _p, _p]),

@@ -52,7 +52,7 @@ def _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_p
 
 
 def attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos, want_lse):
-    """(out, lse or None); arguments as checked by fused_window_cross_attention."""
+    """(out, and for the backward lse and what rounding took from out, or None); arguments as checked by fused_window_cross_attention."""
     lib = _lib.lib()
     with on_device_of(q):
         q, k, v = _rows(q), _rows(k), _rows(v)
@@ -60,16 +60,18 @@ def attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, bucke
         dev = q.device
         out = torch.empty(q.shape, device=dev, dtype=q.dtype)
         lse = torch.empty((q.size(1), q.size(0)), device=dev, dtype=torch.float32) if want_lse else None
+        lo = torch.empty_like(out) if want_lse and q.dtype is not torch.float32 else None
         nbytes = lib.oss_window_attention_scratch_bytes(*args[:7], causal, 0 if table is None else buckets.numel())
         scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-        rc = lib.oss_window_attention_forward(*args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(scratch), nbytes, stream_of(q))
+        rc = lib.oss_window_attention_forward(*args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(lo), _lib.ptr(scratch), nbytes,
+                                               stream_of(q))
         if rc:
             _lib.check(rc, "oss_window_attention_forward")
-    return out, lse
+    return out, lse, lo
 
 
-def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos, out, lse, grad,
-                       want_table):
+def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos, out, lse, lo,
+                       grad, want_table):
     """(d_q, d_k, d_v, d_table or None)."""
     lib = _lib.lib()
     with on_device_of(q):
@@ -84,7 +86,7 @@ def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buck
                                                                  table.size(0) if want_table else 0)
         scratch = torch.empty(max(1, nbytes), device=dev, dtype=torch.uint8)
         gs = grad.stride()
-        rc = lib.oss_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), grad.data_ptr(), gs[0], gs[1],
+        rc = lib.oss_window_attention_backward(*args, out.data_ptr(), lse.data_ptr(), _lib.ptr(lo), grad.data_ptr(), gs[0], gs[1],
                                                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dtable),
                                                scratch.data_ptr(), nbytes, stream_of(q))
         if rc:
@@ -95,20 +97,20 @@ def attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buck
 class _WindowAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos):
-        out, lse = attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos,
-                                     any(ctx.needs_input_grad))
-        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, table, buckets, q_pos, k_pos, out, lse)
+        out, lse, lo = attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos,
+                                         any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, table, buckets, q_pos, k_pos, out, lse, lo)
         ctx.meta = (scale, causal)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, q_offsets, k_offsets, table, buckets, q_pos, k_pos, out, lse = ctx.saved_tensors
+        q, k, v, q_offsets, k_offsets, table, buckets, q_pos, k_pos, out, lse, lo = ctx.saved_tensors
         scale, causal = ctx.meta
         need = ctx.needs_input_grad
         dq, dk, dv, dtable = attention_backward(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos,
-                                                out, lse, grad, table is not None and need[7])
+                                                out, lse, lo, grad, table is not None and need[7])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, dtable,
                 None, None, None)
 

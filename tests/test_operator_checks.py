@@ -152,7 +152,7 @@ def c_forward(dtype=1, tq=4, tk=5, windows=1, heads=4, kv=2, dim=32, q=64, scale
               ry=1, rx=1, pos=64, axes=2, out=64, offsets=64, scratch=None, nbytes=0):
     return _lib.lib().oss_window_attention_forward(
         dtype, tq, tk, windows, heads, kv, dim, q, heads * dim, dim, q, kv * dim, dim, q, kv * dim, dim, offsets, offsets, scale, 0,
-        table, tdtype, rows, bmap, ry, rx, pos, pos, axes, out, None, scratch, nbytes, None)
+        table, tdtype, rows, bmap, ry, rx, pos, pos, axes, out, None, None, scratch, nbytes, None)
 
 
 @pytest.mark.parametrize("change, rc, message", [
@@ -185,7 +185,7 @@ def test_c_attention_scratch():
         a.update(change)
         return lib.oss_window_attention_backward(
             1, 4, 5, 1, 4, 2, 32, 64, 128, 32, 64, 64, 32, 64, 64, 32, 64, 64, 1.0, 0, None, 0, 0, None, 0, 0, None, None, 1,
-            64, a["lse"], 64, 128, 32, a["dq"], a["dk"], 64, a["dtable"], a["scratch"], a["nbytes"], None)
+            64, a["lse"], None, 64, 128, 32, a["dq"], a["dk"], 64, a["dtable"], a["scratch"], a["nbytes"], None)
 
     assert backward(dtable=64) == 1 and "bias table" in last_error()
     assert backward(lse=None) == 1 and "lse" in last_error()
