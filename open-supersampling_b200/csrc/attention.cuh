@@ -48,7 +48,7 @@ struct AttnParams {
     void* out;        // [tq][heads][dim]
     float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
     // What rounding took from out, [tq][heads][dim] of the same type, of windows with more keys than short_max (others'
-    // may stay unwritten): dout . out is then right to 16 bits more. With out alone the gradients of long windows were
+    // may stay unwritten): dout . out is then right to fp32. With out alone the gradients of long windows were
     // off by half as much again as rounding them makes them, and the bias table's by twice. May be null; 16-bit types.
     void* out_lo;
     int tiny_max;     // windows of up to so many keys (backward: of 1 to so many) go to the warp-level kernels

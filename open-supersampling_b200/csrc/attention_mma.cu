@@ -85,7 +85,11 @@ __device__ __forceinline__ void warp_load(uint32_t dst, int panel_rows, const vo
     }
 }
 
-template <typename T, int DP, bool BIAS>
+// REST, for training: what rounding takes from the weights follows them as 16-bit values in the other half of
+// their buffer, O takes both, and what rounding takes from out is written too. dout . out of the backward is
+// then right to fp32: with rounded weights the table's gradient of packed causal histories was off by up to
+// 1.7 times what its own rounding makes it. 7 windows of up to 4095 tokens, forward and backward: 10% of the time.
+template <typename T, int DP, bool BIAS, bool REST>
 __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_constant__ AttnParams p, const __grid_constant__ TileMaps maps) {
     using L = FwdSmem<DP>;
     constexpr int KT = L::KT, kCols = 256, kS = 64, kO = 128;  // columns: S (P over it) twice, then O
@@ -245,6 +249,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 if (tc::elect_one()) {
                     tc::fence_after();
                     tc::mma_tn<KT>(tmem + kO, tmem + b * kS, sv + b * L::kK, n16, id_o, kt > kk.tile0);
+                    if (REST) tc::mma_tn<KT>(tmem + kO, tmem + b * kS + KT / 2, sv + b * L::kK, n16, id_o, true);
                     tc::commit(bar_o);
                     tc::commit(bar_v_read + 8 * b);
                 }
@@ -347,6 +352,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 for (int c = 0; c < KT; c += 16) {
                     if (c >= n16) continue;
                     uint32_t w[8];
+                    float rest[16];
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         float2 x = make_float2(s[c + i], s[c + i + 1]), y = make_float2(s[c + i + 2], s[c + i + 3]);
@@ -357,8 +363,17 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                         sum1 = __fadd2_rn(sum1, y);
                         w[i / 2] = pack2(x.x, x.y, T{});
                         w[i / 2 + 1] = pack2(y.x, y.y, T{});
+                        if (REST) {
+                            rest[i] = lost_by<T>(x.x), rest[i + 1] = lost_by<T>(x.y);
+                            rest[i + 2] = lost_by<T>(y.x), rest[i + 3] = lost_by<T>(y.y);
+                        }
                     }
                     tc::tmem_st8(ts + c / 2, w);
+                    if (REST) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = pack2(rest[2 * i], rest[2 * i + 1], T{});
+                        tc::tmem_st8(ts + KT / 2 + c / 2, w);
+                    }
                 }
                 tc::wait_st();
                 if (kt > kk.tile0) {
@@ -412,7 +427,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
             if (p.splits > 1) continue;
             tc::bar_sync(1, kRows);
             store_panel<T, kRows>(sq, p.out, p.heads, p.dim, t.begin, head0, p.pack, t.first, rows);
-            if (p.out_lo == nullptr) continue;
+            if (!REST) continue;
             tc::bar_sync(1, kRows);  // the staging has been read
 #pragma unroll
             for (int c = 0; c < DP; c += 16) {
@@ -480,11 +495,11 @@ bool tile_map(CUtensorMap* map, int* tokens_y, const void* p, int64_t st, int64_
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, bool BIAS>
+template <typename T, int DP, bool BIAS, bool REST>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int entries = bias_entries(p.bias);
     const int bytes = 1024 + FwdSmem<DP>::kBytes + 4 * entries * p.pack;
-    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, DP, BIAS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
     const int type = kIsBf16<T> ? kBF16 : kF16;
     TileMaps maps;
@@ -495,13 +510,17 @@ cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int groups = p.heads / p.pack, resident = 148 * 2 * (BIAS ? 1 : 4);
     const int slots = attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, kRows);
     const int per_head = (resident + groups * p.splits - 1) / (groups * p.splits);
-    k_attn_fwd_mma<T, DP, BIAS><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows + 64, bytes, s>>>(p, maps);
+    k_attn_fwd_mma<T, DP, BIAS, REST><<<dim3(slots < per_head ? slots : per_head, groups, p.splits), kRows + 64, bytes, s>>>(p, maps);
     return cudaGetLastError();
+}
+template <typename T, bool REST>
+cudaError_t fwd_rest(const AttnParams& p, cudaStream_t s) {
+    if (p.bias.table != nullptr) return p.dim <= 64 ? fwd_one<T, 64, true, REST>(p, s) : fwd_one<T, 128, true, REST>(p, s);
+    return p.dim <= 64 ? fwd_one<T, 64, false, REST>(p, s) : fwd_one<T, 128, false, REST>(p, s);
 }
 template <typename T>
 cudaError_t fwd_type(const AttnParams& p, cudaStream_t s) {
-    if (p.bias.table != nullptr) return p.dim <= 64 ? fwd_one<T, 64, true>(p, s) : fwd_one<T, 128, true>(p, s);
-    return p.dim <= 64 ? fwd_one<T, 64, false>(p, s) : fwd_one<T, 128, false>(p, s);
+    return p.out_lo != nullptr ? fwd_rest<T, true>(p, s) : fwd_rest<T, false>(p, s);
 }
 
 }  // namespace

@@ -148,21 +148,6 @@ __device__ __forceinline__ void write_row(uint32_t panels, int row, int j0, cons
     }
 }
 
-// What that rounding takes from them, again as 16-bit values, to tensor memory (two a column): dQ takes both.
-// Against 64 bits dQ of 135 fp16 windows of 256 under 576 keys is then off by 0.00022 (0.00021 is its own
-// rounding), without it by 0.00032; 2% of the time of forward and backward.
-template <typename T, int N>
-__device__ __forceinline__ void write_rest(uint32_t at, const float (&x)[N], float by) {
-#pragma unroll
-    for (int c = 0; c < N; c += 16) {
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = pack2(lost_by<T>(x[c + 2 * i] * by), lost_by<T>(x[c + 2 * i + 1] * by), T{});
-        tc::tmem_st8(at + c / 2, w);
-    }
-    tc::wait_st();
-}
-
 // 16 columns of a row of a gradient, straight to memory.
 template <typename T>
 __device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim, float by) {
@@ -665,7 +650,7 @@ struct DqShape {
     static constexpr int kT = kRows * DP * 2, kK = KT * DP * 2, kP = kRows * KT * 2;
     static constexpr int kTiles = 2 * kT + 2 * kBuf * kK + kP;
     static constexpr int kBytes = kTiles + static_cast<int>(sizeof(KeyPos<KT>)) * kBuf + 64 + 64 + 128;
-    static constexpr int kCols = DP == 64 ? 256 : 512;  // S, dP, dQ, what rounding took from dS
+    static constexpr int kCols = DP == 64 ? 256 : 512;  // S, dP, dQ
 };
 // dk, dv: the same. Products of 64 keys leave half of their 128 rows unused, but two blocks fill each other's
 // waits: 420 us for those windows, against 596 us with 128 keys and one block of 512 threads, and 486 us when
@@ -791,7 +776,6 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, kp, qp);
             score_gradients(s, dp, delta);
             write_row<T>(sd, row, j0, dp, up);
-            write_rest<T>(ts + 2 * KT + DP + j0 / 2, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
                 if ((tid & 31) == 0) wsize[warp] = m;
@@ -806,7 +790,6 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 for (int k = 0; k < KT; k += 16)
                     if (k < n16)
                         tc::mma_ss(tmem + 2 * KT, dd + ((k >> 6) * kRows * 128 + (k & 63) * 2) / 16, dk + k * 128 / 16, id_q, kt > 0 || k > 0);
-                tc::mma_tn<KT>(tmem + 2 * KT, tmem + 2 * KT + DP, sk + b * L::kK, n16, id_q, true);
                 tc::commit(bar_o);
             }
             if (grad_bias) {
