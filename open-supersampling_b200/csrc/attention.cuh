@@ -64,6 +64,7 @@ struct AttnParams {
     float* delta;        // [heads][tq], sum_j p_ij dp_ij
     void *dq, *dk, *dv;  // contiguous [tq][heads][dim], [tk][kv_heads][dim]
     unsigned long long* bias_acc;  // [buckets][heads], fixed point
+    unsigned long long* bias_top;  // [buckets][heads], largest magnitude of its entries' sums (bits of a double)
     uint32_t* bias_bad;            // [buckets][heads], nonzero where a term was not finite
     const uint32_t* bias_max;      // [2]: largest finite |dout|, |v| (bits of non-negative floats)
     // backward of 16-bit types only

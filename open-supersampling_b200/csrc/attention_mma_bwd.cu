@@ -1062,30 +1062,35 @@ __global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
 }
 
 // Entries to the rows of the table that they map to: in 64-bit fixed point, so that several
-// entries of one row add up the same in any order. A block a head.
+// entries of one row add up the same in any order, at a scale of the row's own (with one for all rows
+// of a head, a window of large gradients took the bits of the rows that only others reach). A block a head.
+__device__ __forceinline__ int table_shift(unsigned long long top) {
+    const double most = __longlong_as_double(static_cast<long long>(top));
+    return most > 0.0 ? 48 - ilogb(most) : 0;  // 4096 entries of at most 2^49
+}
 __global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dtable) {
     const int entries = bias_entries(p.bias), head = blockIdx.x, tid = threadIdx.x;
     const double* sum = p.bias_part + static_cast<int64_t>(head) * p.bias_parts * entries;
-    __shared__ unsigned long long top;
-    if (tid == 0) top = 0ull;
-    __syncthreads();
-    unsigned long long m = 0ull;
-    for (int e = tid; e < entries; e += 1024) m = max(m, static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
-    atomicMax(&top, m);
-    __syncthreads();
-    const double most = __longlong_as_double(static_cast<long long>(top));
-    const int shift = most > 0.0 ? 48 - ilogb(most) : 0;  // 4096 entries of at most 2^49
     for (int e = tid; e < entries; e += 1024) {
         const int bucket = __ldg(p.bias.map + e);
         if (bucket >= 0 && bucket < p.bias.buckets)
-            atomicAdd(p.bias_acc + static_cast<int64_t>(bucket) * p.heads + head,
-                      static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], shift))));
+            atomicMax(p.bias_top + static_cast<int64_t>(bucket) * p.heads + head,
+                      static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
+    }
+    __threadfence();
+    __syncthreads();
+    for (int e = tid; e < entries; e += 1024) {
+        const int bucket = __ldg(p.bias.map + e);
+        if (bucket >= 0 && bucket < p.bias.buckets) {
+            const int64_t i = static_cast<int64_t>(bucket) * p.heads + head;
+            atomicAdd(p.bias_acc + i, static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], table_shift(__ldcg(p.bias_top + i))))));
+        }
     }
     __threadfence();
     __syncthreads();
     for (int b = tid; b < p.bias.buckets; b += 1024) {
         const int64_t i = static_cast<int64_t>(b) * p.heads + head;
-        const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -shift);
+        const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -table_shift(__ldcg(p.bias_top + i)));
         store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
     }
 }

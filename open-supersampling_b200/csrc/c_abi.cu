@@ -1399,6 +1399,7 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
     }
     const int64_t from = arena.used;
     p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
+    p.bias_top = sums && dtype != oss::kF32 ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
     p.bias_bad = sums ? arena.take<uint32_t>(sum_rows * p.heads) : nullptr;
     p.bias_max = sums || dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
     if (dtype == oss::kBF16) p.bias_max = nullptr;
