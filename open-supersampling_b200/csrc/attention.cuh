@@ -63,21 +63,22 @@ struct AttnParams {
     int64_t do_st, do_sh;
     float* delta;        // [heads][tq], sum_j p_ij dp_ij
     void *dq, *dk, *dv;  // contiguous [tq][heads][dim], [tk][kv_heads][dim]
-    unsigned long long* bias_acc;  // [buckets][heads], fixed point
+    unsigned long long* bias_acc;  // [buckets][heads], fixed point; zero at the start, as the next two
     unsigned long long* bias_top;  // [buckets][heads], largest magnitude of its entries' sums (bits of a double)
     uint32_t* bias_bad;            // [buckets][heads], nonzero where a term was not finite
     const uint32_t* bias_max;      // [2]: largest finite |dout|, |v| (bits of non-negative floats)
+    double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
+    int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them
+    int dq_blocks;               // blocks of the kernel for dq for each head
     // backward of 16-bit types only
     int short_max;      // windows of up to so many keys go to the kernel for short windows
     int qsplits;        // parts that the queries of a tile of keys are cut into
-    int tiny_blocks, short_blocks, dq_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
+    int tiny_blocks, short_blocks, dkv_blocks;  // blocks of the kernels for each (set of) head(s)
     // flags and tiny_list serve the forward of the few-keys kernels too: counters and queues, and pieces by class
     int* flags;         // [0]: kSomeLong, kSomeShort; [1], [2]: windows of up to 16 and of 17 to 32 keys
     int* tiny_list;     // [2][windows]: those windows, in order
     int tiny_pieces;    // forward: most pieces of a class
     float *part_dk, *part_dv;    // [qsplits][tk][kv_heads][dim], qsplits > 1 only
-    double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
-    int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them
 };
 
 constexpr int kSomeLong = 1;   // a window with more than short_max keys
@@ -281,16 +282,11 @@ __device__ __forceinline__ int bias_index(const AttnBias& b, int2 qp, int2 kp) {
     return dy * (2 * b.rx + 1) + dx;
 }
 
-// Gradient of the bias: sums of ds in 64-bit fixed point, which come out the same in any
-// order.  |ds| summed over a row is at most 2 |dout| |v| dim, so with the exponent below the
-// sum over all rows stays under 2^61.
-__device__ __forceinline__ float bias_fixed_scale(const uint32_t* bias_max, int dim, int tq) {
-    const double bound =
-        2.0 * static_cast<double>(__uint_as_float(bias_max[0])) * static_cast<double>(__uint_as_float(bias_max[1])) * dim;
-    int e = 126;
-    // a finite fp32 ds is below 2^128 whatever the bound says
-    if (bound > 0.0) e = 60 - (32 - __clz(tq)) - min(ilogb(bound), 128);
-    return exp2f(static_cast<float>(min(max(e, -126), 126)));
+// Gradient of the bias: a tile's terms join integer sums, which come out the same in any order, at a
+// power of two that keeps the tile's sum of magnitudes m below 2^bits. (A scale for the whole call
+// let one large value, even of a row that no window holds, take the bits of all others.)
+__device__ __forceinline__ float bias_scale(float m, int bits) {
+    return m > 0.0f ? exp2f(static_cast<float>(min(max(bits - 1 - ilogbf(fminf(m, 3.0e38f)), -126), 126))) : 0.0f;
 }
 
 // 64-bit add into two shared 32-bit words (native integer atomics; the carry goes by hand).
@@ -302,19 +298,30 @@ __device__ __forceinline__ void bias_add_shared(uint32_t* lo, uint32_t* hi, int 
     if (vh != 0u) atomicAdd(hi + e, vh);
 }
 
-// A block's sum of one entry joins the global sum of its bucket.
-__device__ __forceinline__ void bias_flush(const AttnParams& p, int head, int e, uint32_t lo, uint32_t hi) {
-    if ((lo | hi) == 0u) return;
-    const int bucket = __ldg(p.bias.map + e);
-    if (bucket >= 0 && bucket < p.bias.buckets)
-        atomicAdd(p.bias_acc + static_cast<int64_t>(bucket) * p.heads + head, (static_cast<unsigned long long>(hi) << 32) | lo);
-}
 __device__ __forceinline__ void bias_mark_bad(const AttnParams& p, int head, int e) {
     const int bucket = __ldg(p.bias.map + e);
     if (bucket >= 0 && bucket < p.bias.buckets) p.bias_bad[static_cast<int64_t>(bucket) * p.heads + head] = 1u;
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// The sum of finite |ds| of a warp's rows, negative where some is not finite.
+template <int N>
+__device__ __forceinline__ float warp_size(const float (&ds)[N]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) m += fabsf(ds[c]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
+    if (is_finite(m)) return m;
+    m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+        if (is_finite(ds[c])) m += fabsf(ds[c]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
+    return -fmaxf(fminf(m, 3.0e38f), 1.0e-38f);
+}
+
 // What rounding x to T takes from it.
 template <typename T>
 __device__ __forceinline__ float lost_by(float x) {
@@ -328,8 +335,9 @@ __device__ __forceinline__ float lost_by(float x) {
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
 // dtable (null: no gradient of the table).
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
-// attention_simt.cu: delta (p.flags null or set) and p.bias_max (where not null).
+// attention_simt.cu: delta (p.flags null or set) and p.bias_max (where not null); p.bias_part to dtable.
 cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s);
+cudaError_t launch_attn_bias_grad(const AttnParams& p, void* dtable, cudaStream_t s);
 // attention_mma.cu, attention_mma_bwd.cu: bf16 and fp16, the forward without the join of split keys.
 cudaError_t launch_attn_forward_mma(const AttnParams& p, int type, cudaStream_t s);
 // Windows of up to p.tiny_max keys (backward: of 1 to 32), not causal, dim <= 64 (backward: 32).

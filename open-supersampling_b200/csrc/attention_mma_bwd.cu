@@ -33,24 +33,6 @@ struct BiasSum {      // of a tile, uniform over the block
     bool bad;         // some terms are not finite
 };
 
-// The sum of finite |ds| of a warp's rows, negative where some is not finite.
-template <int N>
-__device__ __forceinline__ float warp_size(const float (&ds)[N]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int c = 0; c < N; ++c) m += fabsf(ds[c]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
-    if (is_finite(m)) return m;
-    m = 0.0f;
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-        if (is_finite(ds[c])) m += fabsf(ds[c]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) m += __shfl_xor_sync(0xffffffffu, m, x);
-    return -fmaxf(fminf(m, 3.0e38f), 1.0e-38f);
-}
-
 template <int WARPS>
 __device__ __forceinline__ BiasSum bias_sum(BiasMode mode, const float* wsize) {
     float m = 0.0f;
@@ -61,7 +43,7 @@ __device__ __forceinline__ BiasSum bias_sum(BiasMode mode, const float* wsize) {
         bad |= wsize[w] < 0.0f;
     }
     BiasSum b{mode, 0.0f, bad};
-    if (m > 0.0f) b.fixed = exp2f(static_cast<float>(min(max(29 - ilogbf(fminf(m, 3.0e38f)), -126), 126)));
+    b.fixed = bias_scale(m, 30);
     return b;
 }
 
@@ -1040,61 +1022,6 @@ __global__ void __launch_bounds__(256) k_attn_join_dkv(AttnParams p) {
     static_cast<T*>(p.dv)[i] = from_f<T>(v);
 }
 
-// The parts of each entry into the first part: thread (part lane, entry) adds every eighth part, the
-// eight sums are added in order.
-__global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
-    __shared__ double sums[8][32];
-    const int entries = bias_entries(p.bias), lane = threadIdx.x & 31, row = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
-    const int flags = *p.flags, first_long = p.bias_tiny + p.bias_short;
-    double* at = p.bias_part + static_cast<int64_t>(blockIdx.y) * p.bias_parts * entries + e;
-    double sum = 0.0;
-    if (e < entries) {
-        for (int s = row; s < p.bias_parts; s += 8) {
-            const bool filled = s < p.bias_tiny || (s < first_long ? (flags & kSomeShort) != 0 : (flags & kSomeLong) != 0);
-            if (filled) sum += at[static_cast<int64_t>(s) * entries];
-        }
-    }
-    sums[row][lane] = sum;
-    __syncthreads();
-    if (row != 0 || e >= entries) return;
-    for (int r = 1; r < 8; ++r) sum += sums[r][lane];
-    at[0] = sum;
-}
-
-// Entries to the rows of the table that they map to: in 64-bit fixed point, so that several
-// entries of one row add up the same in any order, at a scale of the row's own (with one for all rows
-// of a head, a window of large gradients took the bits of the rows that only others reach). A block a head.
-__device__ __forceinline__ int table_shift(unsigned long long top) {
-    const double most = __longlong_as_double(static_cast<long long>(top));
-    return most > 0.0 ? 48 - ilogb(most) : 0;  // 4096 entries of at most 2^49
-}
-__global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dtable) {
-    const int entries = bias_entries(p.bias), head = blockIdx.x, tid = threadIdx.x;
-    const double* sum = p.bias_part + static_cast<int64_t>(head) * p.bias_parts * entries;
-    for (int e = tid; e < entries; e += 1024) {
-        const int bucket = __ldg(p.bias.map + e);
-        if (bucket >= 0 && bucket < p.bias.buckets)
-            atomicMax(p.bias_top + static_cast<int64_t>(bucket) * p.heads + head,
-                      static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
-    }
-    __threadfence();
-    __syncthreads();
-    for (int e = tid; e < entries; e += 1024) {
-        const int bucket = __ldg(p.bias.map + e);
-        if (bucket >= 0 && bucket < p.bias.buckets) {
-            const int64_t i = static_cast<int64_t>(bucket) * p.heads + head;
-            atomicAdd(p.bias_acc + i, static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], table_shift(__ldcg(p.bias_top + i))))));
-        }
-    }
-    __threadfence();
-    __syncthreads();
-    for (int b = tid; b < p.bias.buckets; b += 1024) {
-        const int64_t i = static_cast<int64_t>(b) * p.heads + head;
-        const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -table_shift(__ldcg(p.bias_top + i)));
-        store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
-    }
-}
-
 template <typename K>
 cudaError_t smem_of(K kernel, int bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -1129,13 +1056,7 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
         k_attn_join_dkv<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
         if ((err = cudaGetLastError()) != cudaSuccess) return err;
     }
-    if (dtable != nullptr) {
-        k_attn_bias_parts<<<dim3((entries + 31) / 32, p.heads), 256, 0, s>>>(p);
-        if ((err = cudaGetLastError()) != cudaSuccess) return err;
-        k_attn_bias_table<<<p.heads, 1024, 0, s>>>(p, dtable);
-        err = cudaGetLastError();
-    }
-    return err;
+    return dtable != nullptr ? launch_attn_bias_grad(p, dtable, s) : cudaSuccess;
 }
 
 template <typename T>

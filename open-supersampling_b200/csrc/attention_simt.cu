@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kKeys = 64;  // keys of a tile
+constexpr int64_t kMaxSmem = 227 * 1024;  // of a block
 
 // ---- shared-memory layout ---------------------------------------------------
 struct Smem {
@@ -304,8 +305,7 @@ __device__ __forceinline__ int64_t divide(int64_t x, int by) {
 
 
 // ---- backward ----------------------------------------------------------------
-// delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for the bias
-// gradient's fixed point, and fp16's range). LANES lanes a row, two values at a time where its
+// delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for fp16's range). LANES lanes a row, two values at a time where its
 // address and strides allow it (PAIRS). Bound by the latency of its loads: 10.8 us for 4095 rows of 8 heads
 // of 64, 43 us for 34560 rows of 6 heads of 30 and 77760 keys.
 template <typename T, int LANES, bool PAIRS>
@@ -399,10 +399,12 @@ __device__ __forceinline__ bool score_grads(const AttnParams& p, float (&s)[RM][
 }
 
 // dq: a tile of queries walks its window's keys; the bias gradient is summed here too.
-// GRAD_BIAS: a block keeps its head and walks slots blockIdx.x, + gridDim.x, ..., so that its
-// shared sums are added to the global ones once.
+// GRAD_BIAS: a block keeps its head and walks slots blockIdx.x, + gridDim.x, .... A tile's terms are
+// summed in 64-bit integers at 2^-60 of their sum of magnitudes, then join the block's fp64 sums,
+// each by its entry's own thread; those stay in shared memory (`own_acc`), or where a large map leaves no
+// room for them in the block's part of p.bias_part.
 template <typename T, int DP, bool GRAD_BIAS>
-__global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
+__global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p, int own_acc) {
     constexpr int RM = 4, BM = 64, LD = DP + 4, CN = DP / 16, LDP = kKeys + 4;
     extern __shared__ __align__(16) float smem_f[];
     Smem sm{smem_f};
@@ -419,14 +421,24 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
     float* Es = sm.take(entries);
     uint32_t* lo = reinterpret_cast<uint32_t*>(sm.take(GRAD_BIAS ? entries : 0));
     uint32_t* hi = reinterpret_cast<uint32_t*>(sm.take(GRAD_BIAS ? entries : 0));
+    float* wsize = sm.take(GRAD_BIAS ? 8 : 0);
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int head = blockIdx.y, kvh = head / (p.heads / p.kv_heads);
     const int slots = attn_slots(p.tq, p.windows, BM);
-    float fixed = 0.0f;
-    if (GRAD_BIAS) {
-        fixed = bias_fixed_scale(p.bias_max, p.dim, p.tq);
-        for (int e = tid; e < entries; e += kThreads) lo[e] = hi[e] = 0u;
-    }
+    double* part = GRAD_BIAS ? p.bias_part + (static_cast<int64_t>(head) * p.bias_parts + blockIdx.x) * entries : nullptr;
+    double* acc = GRAD_BIAS && own_acc ? reinterpret_cast<double*>(sm.take(2 * entries)) : part;
+    float fixed = 0.0f;  // of the sums that have not joined yet
+    if (GRAD_BIAS)
+        for (int e = tid; e < entries; e += kThreads) lo[e] = hi[e] = 0u, acc[e] = 0.0;
+    auto join = [&] {  // after a barrier
+        if (fixed == 0.0f) return;
+        const double unit = 1.0 / static_cast<double>(fixed);
+        for (int e = tid; e < entries; e += kThreads) {
+            const long long sum = static_cast<long long>((static_cast<unsigned long long>(hi[e]) << 32) | lo[e]);
+            if (sum != 0) acc[e] += static_cast<double>(sum) * unit, lo[e] = hi[e] = 0u;
+        }
+        fixed = 0.0f;
+    };
     for (int e = tid; e < entries; e += kThreads) Es[e] = bias_entry(p.bias, p.heads, head, e);
 
     for (int slot = blockIdx.x; slot < slots; slot += gridDim.x) {
@@ -467,6 +479,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
         for (int k0 = 0; k0 < most; k0 += kKeys) {
             const int n = min(kKeys, t.olen - k0);
             __syncthreads();
+            if (GRAD_BIAS) join();
             load_rows<T, DP, kKeys>(Ks, p.k, p.k_st, p.k_sh, t.obegin, kvh, 1, k0, n, p.dim);
             load_rows<T, DP, kKeys>(Vs, p.v, p.v_st, p.v_sh, t.obegin, kvh, 1, k0, n, p.dim);
             if (entries > 0 && tid < n) kpos[tid] = bias_pos(p.bias.k_pos, p.bias.axes, t.obegin + k0 + tid);
@@ -481,15 +494,32 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
                 for (int c = 0; c < 4; ++c) {
                     const int r = ty * RM + i, j = tx + 16 * c;
                     Ds[r * LDP + j] = dp[i][c];
-                    if (GRAD_BIAS && dp[i][c] != 0.0f) {
-                        const int e = bias_index(p.bias, qpos[r], kpos[j]);
+                }
+            if (GRAD_BIAS) {
+                float flat[4 * RM];
+#pragma unroll
+                for (int i = 0; i < 4 * RM; ++i) flat[i] = dp[i / 4][i % 4];
+                const float m = fabsf(warp_size(flat));
+                if ((tid & 31) == 0) wsize[tid >> 5] = m;
+            }
+            const bool masked = __syncthreads_or(cut);
+            if (GRAD_BIAS) {
+                float m = 0.0f;
+                for (int w = 0; w < kThreads / 32; ++w) m += wsize[w];
+                fixed = bias_scale(m, 60);
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (dp[i][c] == 0.0f) continue;
+                        const int e = bias_index(p.bias, qpos[ty * RM + i], kpos[tx + 16 * c]);
                         if (is_finite(dp[i][c]))
                             bias_add_shared(lo, hi, e, __float2ll_rn(dp[i][c] * fixed));
                         else
                             bias_mark_bad(p, head, e);
                     }
-                }
-            if (__syncthreads_or(cut))
+            }
+            if (masked)
                 weigh_rows<DP, RM, CN, true>(dq, Ds, LDP, Ks, n, ty, tx);
             else
                 weigh_rows<DP, RM, CN, false>(dq, Ds, LDP, Ks, n, ty, tx);
@@ -506,7 +536,9 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p) {
     }
     if (GRAD_BIAS) {
         __syncthreads();
-        for (int e = tid; e < entries; e += kThreads) bias_flush(p, head, e, lo[e], hi[e]);
+        join();
+        if (own_acc)
+            for (int e = tid; e < entries; e += kThreads) part[e] = acc[e];
     }
 }
 
@@ -590,13 +622,60 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(AttnParams p) {
     }
 }
 
-// The bias gradient out of fixed point, rounded once.
-__global__ void __launch_bounds__(kThreads) k_attn_bias_grad(AttnParams p, void* dtable) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
-    if (i >= p.bias.buckets * p.heads) return;
-    const double fixed = static_cast<double>(bias_fixed_scale(p.bias_max, p.dim, p.tq));
-    const double x = static_cast<double>(static_cast<long long>(p.bias_acc[i])) / fixed;
-    store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
+// ---- the bias gradient of all blocks -----------------------------------------------
+// The parts of each entry into the first part: thread (part lane, entry) adds every eighth part, the
+// eight sums are added in order.
+__global__ void __launch_bounds__(256) k_attn_bias_parts(AttnParams p) {
+    __shared__ double sums[8][32];
+    const int entries = bias_entries(p.bias), lane = threadIdx.x & 31, row = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int flags = p.flags == nullptr ? kSomeLong : *p.flags, first_long = p.bias_tiny + p.bias_short;
+    double* at = p.bias_part + static_cast<int64_t>(blockIdx.y) * p.bias_parts * entries + e;
+    double sum = 0.0;
+    if (e < entries) {
+        for (int s = row; s < p.bias_parts; s += 8) {
+            const bool filled = s < p.bias_tiny || (s < first_long ? (flags & kSomeShort) != 0 : (flags & kSomeLong) != 0);
+            if (filled) sum += at[static_cast<int64_t>(s) * entries];
+        }
+    }
+    sums[row][lane] = sum;
+    __syncthreads();
+    if (row != 0 || e >= entries) return;
+    for (int r = 1; r < 8; ++r) sum += sums[r][lane];
+    at[0] = sum;
+}
+
+// Entries to the rows of the table that they map to: in 64-bit fixed point, so that several
+// entries of one row add up the same in any order, at a scale of the row's own (with one for all rows
+// of a head, a window of large gradients took the bits of the rows that only others reach). A block a head.
+__device__ __forceinline__ int table_shift(unsigned long long top) {
+    const double most = __longlong_as_double(static_cast<long long>(top));
+    return most > 0.0 ? 48 - ilogb(most) : 0;  // 4096 entries of at most 2^49
+}
+__global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dtable) {
+    const int entries = bias_entries(p.bias), head = blockIdx.x, tid = threadIdx.x;
+    const double* sum = p.bias_part + static_cast<int64_t>(head) * p.bias_parts * entries;
+    for (int e = tid; e < entries; e += 1024) {
+        const int bucket = __ldg(p.bias.map + e);
+        if (bucket >= 0 && bucket < p.bias.buckets)
+            atomicMax(p.bias_top + static_cast<int64_t>(bucket) * p.heads + head,
+                      static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
+    }
+    __threadfence();
+    __syncthreads();
+    for (int e = tid; e < entries; e += 1024) {
+        const int bucket = __ldg(p.bias.map + e);
+        if (bucket >= 0 && bucket < p.bias.buckets) {
+            const int64_t i = static_cast<int64_t>(bucket) * p.heads + head;
+            atomicAdd(p.bias_acc + i, static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], table_shift(__ldcg(p.bias_top + i))))));
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    for (int b = tid; b < p.bias.buckets; b += 1024) {
+        const int64_t i = static_cast<int64_t>(b) * p.heads + head;
+        const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -table_shift(__ldcg(p.bias_top + i)));
+        store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
+    }
 }
 
 int64_t floats(int64_t n) { return (n + 3) / 4 * 4; }
@@ -636,20 +715,21 @@ cudaError_t join_parts(const AttnParams& p, cudaStream_t s) {
 }
 
 template <typename T, int DP>
-cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s, int sms) {
+cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s) {
     const int64_t entries = bias_entries(p.bias);
-    const bool grad_bias = p.bias_acc != nullptr;
-    const int64_t dq_bytes = 4 * (4 * floats(64 * (DP + 4)) + floats(64 * 68) + 2 * 64 + 4 * 64 +
-                                  floats(entries) * (grad_bias ? 3 : 1));
+    const bool grad_bias = p.bias_part != nullptr;
+    int64_t dq_bytes = 4 * (4 * floats(64 * (DP + 4)) + floats(64 * 68) + 2 * 64 + 4 * 64 + floats(entries) * (grad_bias ? 3 : 1) +
+                            (grad_bias ? 8 : 0));
+    const int own_acc = grad_bias && dq_bytes + 4 * floats(2 * entries) <= kMaxSmem;
+    if (own_acc) dq_bytes += 4 * floats(2 * entries);
     const int slots = attn_slots(p.tq, p.windows, 64);
     cudaError_t err;
     if (grad_bias) {
         if ((err = set_smem(k_attn_dq<T, DP, true>, dq_bytes)) != cudaSuccess) return err;
-        const int per_head = (4 * sms + p.heads - 1) / p.heads;
-        k_attn_dq<T, DP, true><<<dim3(slots < per_head ? slots : per_head, p.heads), kThreads, dq_bytes, s>>>(p);
+        k_attn_dq<T, DP, true><<<dim3(p.dq_blocks, p.heads), kThreads, dq_bytes, s>>>(p, own_acc);
     } else {
         if ((err = set_smem(k_attn_dq<T, DP, false>, dq_bytes)) != cudaSuccess) return err;
-        k_attn_dq<T, DP, false><<<dim3(slots, p.heads), kThreads, dq_bytes, s>>>(p);
+        k_attn_dq<T, DP, false><<<dim3(slots, p.heads), kThreads, dq_bytes, s>>>(p, 0);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int64_t kv_bytes = 4 * (4 * floats(64 * (DP + 4)) + 2 * floats(64 * 68) + 2 * 64 + 4 * 64 + floats(entries));
@@ -689,17 +769,21 @@ cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s) {
 }
 
 cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s) {
-    return type == kF32 ? delta_type<float>(p, s, sms) : type == kBF16 ? delta_type<__nv_bfloat16>(p, s, sms) : delta_type<__half>(p, s, sms);
+    return type == kBF16 ? delta_type<__nv_bfloat16>(p, s, sms) : delta_type<__half>(p, s, sms);
+}
+
+cudaError_t launch_attn_bias_grad(const AttnParams& p, void* dtable, cudaStream_t s) {
+    k_attn_bias_parts<<<dim3((bias_entries(p.bias) + 31) / 32, p.heads), 256, 0, s>>>(p);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+    k_attn_bias_table<<<p.heads, 1024, 0, s>>>(p, dtable);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s) {
     if (type != kF32) return launch_attn_backward_mma(p, type, dtable, sms, s);
-    cudaError_t err = cudaSuccess;
-    if (p.bias_max != nullptr && (err = delta_type<float>(p, s, sms)) != cudaSuccess) return err;
-    err = p.dim <= 32 ? bwd_dim<float, 32>(p, s, sms) : p.dim <= 64 ? bwd_dim<float, 64>(p, s, sms) : bwd_dim<float, 128>(p, s, sms);
-    if (err != cudaSuccess || dtable == nullptr) return err;
-    k_attn_bias_grad<<<(p.bias.buckets * p.heads + kThreads - 1) / kThreads, kThreads, 0, s>>>(p, dtable);
-    return cudaGetLastError();
+    const cudaError_t err = p.dim <= 32 ? bwd_dim<float, 32>(p, s) : p.dim <= 64 ? bwd_dim<float, 64>(p, s) : bwd_dim<float, 128>(p, s);
+    return err != cudaSuccess || dtable == nullptr ? err : launch_attn_bias_grad(p, dtable, s);
 }
 
 }  // namespace oss

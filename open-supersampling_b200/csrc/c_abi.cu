@@ -1394,15 +1394,18 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
         const int64_t keys = static_cast<int64_t>(p.tk) * p.kv_heads * p.dim;
         p.part_dk = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
         p.part_dv = p.qsplits > 1 ? arena.take<float>(p.qsplits * keys) : nullptr;
-        p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * p.bias_parts * entries) : nullptr;
         p.tiny_list = p.tiny_max > 0 ? arena.take<int>(2ll * p.windows) : nullptr;
+    } else {
+        // four blocks an SM: the queries' tiles go to them in turn
+        const int slots = oss::attn_slots(p.tq, p.windows, 64), per_head = (4 * kSms + p.heads - 1) / p.heads;
+        p.bias_parts = p.dq_blocks = slots < per_head ? slots : per_head;
     }
+    p.bias_part = sums ? arena.take<double>(static_cast<int64_t>(p.heads) * p.bias_parts * entries) : nullptr;
     const int64_t from = arena.used;
     p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
-    p.bias_top = sums && dtype != oss::kF32 ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
+    p.bias_top = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
     p.bias_bad = sums ? arena.take<uint32_t>(sum_rows * p.heads) : nullptr;
-    p.bias_max = sums || dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
-    if (dtype == oss::kBF16) p.bias_max = nullptr;
+    p.bias_max = dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
     p.flags = dtype != oss::kF32 ? arena.take<int>(3) : nullptr;
     if (zero_at != nullptr) *zero_at = base + from, *zeroed = arena.used - from;
     return arena.used;
