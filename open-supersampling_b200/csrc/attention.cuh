@@ -66,7 +66,8 @@ struct AttnParams {
     unsigned long long* bias_acc;  // [buckets][heads], fixed point; zero at the start, as the next two
     unsigned long long* bias_top;  // [buckets][heads], largest magnitude of its entries' sums (bits of a double)
     uint32_t* bias_bad;            // [buckets][heads], nonzero where a term was not finite
-    const uint32_t* bias_max;      // [2]: largest finite |dout|, |v| (bits of non-negative floats)
+    uint32_t* win_max;             // fp16: [windows][kv_heads][2], largest finite |dout| and |v| of a window (bits of an
+                                   // fp16 value); zero at the start
     double* bias_part;           // [heads][bias_parts][entries]; null: no gradient of the table
     int bias_tiny, bias_short, bias_parts;  // parts of the tiny and the short windows' blocks, and all of them
     int dq_blocks;               // blocks of the kernel for dq for each head
@@ -335,7 +336,7 @@ __device__ __forceinline__ float lost_by(float x) {
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
 // dtable (null: no gradient of the table).
 cudaError_t launch_attn_backward(const AttnParams& p, int type, void* dtable, int sms, cudaStream_t s);
-// attention_simt.cu: delta (p.flags null or set) and p.bias_max (where not null); p.bias_part to dtable.
+// attention_simt.cu: delta of 16-bit types, where some window is long; p.bias_part to dtable.
 cudaError_t launch_attn_delta(const AttnParams& p, int type, int sms, cudaStream_t s);
 cudaError_t launch_attn_bias_grad(const AttnParams& p, void* dtable, cudaStream_t s);
 // attention_mma.cu, attention_mma_bwd.cu: bf16 and fp16, the forward without the join of split keys.

@@ -258,11 +258,15 @@ __device__ __forceinline__ void write_part(float* to, const float* o, int c, int
 template <typename T>
 constexpr int kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
 
-// Power of two that dS is kept times.
+// Power of two that dS of a window and key head is kept times. (One for the whole call let a large value
+// in another window, or in a row that no window holds, push dS below fp16's range.)
 template <typename T>
-__device__ __forceinline__ float ds_scale(const AttnParams& p) {
+__device__ __forceinline__ float ds_scale(const AttnParams& p, int window, int kvh) {
     if constexpr (kIsBf16<T>) return 1.0f;
-    const float bound = 2.0f * p.dim * __uint_as_float(p.bias_max[0]) * __uint_as_float(p.bias_max[1]);
+    const uint2 m = __ldg(reinterpret_cast<const uint2*>(p.win_max) + static_cast<int64_t>(window) * p.kv_heads + kvh);
+    const float most_do = __half2float(__ushort_as_half(static_cast<unsigned short>(m.x))),
+                most_v = __half2float(__ushort_as_half(static_cast<unsigned short>(m.y)));
+    const float bound = 2.0f * p.dim * most_do * most_v;
     if (!(bound > 0.0f)) return 1.0f;
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }

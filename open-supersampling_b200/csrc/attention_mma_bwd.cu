@@ -12,7 +12,7 @@
 // that walks keys for dQ and one that walks queries for dK and dV (seven products instead of five,
 // but no sums across blocks: every gradient has a fixed order of additions).
 //
-// fp16 keeps dS times a power of two that puts its bound 2 dim max|dout| max|v| at 2^15, so that
+// fp16 keeps dS times a power of two that puts the window's bound 2 dim max|dout| max|v| at 2^15, so that
 // gradients of any size stay within the type's range.
 //
 // The bias gradient is summed per tile in shared 32-bit integers (native atomics; the same in any
@@ -358,6 +358,47 @@ __global__ void __launch_bounds__(1024) k_attn_lists(AttnParams p, int* flags) {
     if (threadIdx.x < 2) flags[1 + threadIdx.x] = base[threadIdx.x];
 }
 
+// The largest finite |dout| and |v| of each window and key head, fp16. A block takes 128 rows of a window's queries, or
+// of its keys; its warps share out key heads and rows, eight lanes a row.
+__global__ void __launch_bounds__(256) k_attn_window_max(const __grid_constant__ AttnParams p, int q_slots) {
+    const bool of_q = static_cast<int>(blockIdx.x) < q_slots;
+    AttnTile t;
+    if (!attn_tile(of_q ? p.q_off : p.k_off, of_q ? p.tq : p.tk, of_q ? p.k_off : p.q_off, of_q ? p.tk : p.tq, p.windows, 1, kRows,
+                   of_q ? blockIdx.x : blockIdx.x - q_slots, t))
+        return;
+    if (t.window < 0 || t.olen == 0) return;
+    const int group = of_q ? p.heads / p.kv_heads : 1, rows = min(kRows, t.len - t.first), lane = threadIdx.x & 31;
+    const int64_t st = of_q ? p.do_st : p.v_st, sh = of_q ? p.do_sh : p.v_sh;
+    const unsigned short* base = static_cast<const unsigned short*>(of_q ? p.dout : p.v) + (static_cast<int64_t>(t.begin) + t.first) * st;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+    const bool vec = ((at & 15) | ((st | sh | p.dim) & 7)) == 0, pairs = ((at & 3) | ((st | sh | p.dim) & 1)) == 0;
+    const int parts = p.kv_heads < 8 ? 8 / p.kv_heads : 1;
+    auto of = [](uint32_t x) {  // of two values
+        const uint32_t a = x & 0x7fffu, b = (x >> 16) & 0x7fffu;
+        return max(a < 0x7c00u ? a : 0u, b < 0x7c00u ? b : 0u);
+    };
+    for (int unit = threadIdx.x >> 5; unit < p.kv_heads * parts; unit += 8) {
+        const int kvh = unit % p.kv_heads;
+        uint32_t m = 0u;
+        for (int r = unit / p.kv_heads * 4 + (lane >> 3); r < rows; r += 4 * parts)
+            for (int g = 0; g < group; ++g) {
+                const unsigned short* row = base + r * st + (kvh * group + g) * sh;
+                if (vec) {
+                    for (int c = 8 * (lane & 7); c < p.dim; c += 64) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + c));
+                        m = max(m, max(max(of(x.x), of(x.y)), max(of(x.z), of(x.w))));
+                    }
+                } else if (pairs) {
+                    for (int c = 2 * (lane & 7); c < p.dim; c += 16) m = max(m, of(__ldg(reinterpret_cast<const uint32_t*>(row + c))));
+                } else {
+                    for (int c = lane & 7; c < p.dim; c += 8) m = max(m, of(__ldg(row + c)));
+                }
+            }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0 && m != 0u) atomicMax(p.win_max + (static_cast<int64_t>(t.window) * p.kv_heads + kvh) * 2 + (of_q ? 0 : 1), m);
+    }
+}
+
 // ---- short windows ---------------------------------------------------------------------------
 template <int DP>
 struct ShortSmem {
@@ -447,7 +488,6 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
     const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_dv = 2 * KT, t_dk = 2 * KT + DP;  // columns; S at 0, dP at 64, dQ over both
     const uint32_t id_grad = tc::idesc(kIsBf16<T>, dim16, true, true), id_q = tc::idesc(kIsBf16<T>, dim16, false, true);
-    const float up = ds_scale<T>(p);
     int par_s = 0, par_o = 0;
     bool alive = true;
 
@@ -455,6 +495,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), lk = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
         if (lk > p.short_max || lk <= p.tiny_max) continue;  // other kernels', and windows without keys
+        const float up = ds_scale<T>(p, w, kvh);
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
         const int i0 = min(z * per, total), i1 = min(i0 + per, total);
         const int n = lk, n16 = (n + 15) & ~15;
@@ -688,7 +729,6 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     tc::fence_after();
     const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t id_q = tc::idesc(kIsBf16<T>, dim16, false, true);
-    const float up = ds_scale<T>(p);
     int par_s = 0, par_o = 0;
     bool alive = true;
 
@@ -696,6 +736,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     for (bool more = walk.first(p.q_off, p.tq, p.k_off, p.tk); more; more = walk.next()) {
         const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.olen <= p.short_max) continue;
+        const float up = ds_scale<T>(p, t.window, kvh);
         const int rows = min(kRows, t.len - t.first), shift = t.olen - t.len;
         const bool live = row < rows;
         const int see = !live ? 0 : p.causal ? min(max(t.first + row + shift + 1, 0), t.olen) : t.olen;
@@ -874,7 +915,6 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
     const uint32_t tmem = *slot_tmem, ts = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_dv = 2 * KT, t_dk = 2 * KT + DP;
     const uint32_t id_grad = tc::idesc(kIsBf16<T>, dim16, true, true);
-    const float up = ds_scale<T>(p);
     int par_s = 0, par_o = 0, head_of_E = -1;
     bool alive = true;
     // dk and dv through smem where their rows are not on 16 bytes (there, direct stores were 2% faster)
@@ -885,6 +925,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
     for (bool more = walk.first(p.k_off, p.tk, p.q_off, p.tq); more; more = walk.next()) {
         const AttnTile& t = walk.walk.tile;
         if (t.window < 0 || t.len <= p.short_max) continue;
+        const float up = ds_scale<T>(p, t.window, kvh);
         const int lq = t.olen, lk = t.len, n = min(KT, lk - t.first), n16 = (n + 15) & ~15;
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
         const int i0 = min(z * per, total), i1 = min(i0 + per, total);
@@ -1074,6 +1115,11 @@ cudaError_t launch_attn_backward_mma(const AttnParams& p, int type, void* dtable
         k_attn_flags<<<p.windows < 16384 ? 1 + p.windows / 1024 : 16, 256, 0, s>>>(p, p.flags);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
+    if (p.win_max != nullptr) {
+        const int q_slots = attn_slots(p.tq, p.windows, kRows), k_slots = attn_slots(p.tk, p.windows, kRows);
+        k_attn_window_max<<<q_slots + k_slots, 256, 0, s>>>(p, q_slots);
+        if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    }
     if ((err = launch_attn_delta(p, type, sms, s)) != cudaSuccess) return err;
     return type == kBF16 ? bwd_type<__nv_bfloat16>(p, dtable, s) : bwd_type<__half>(p, dtable, s);
 }

@@ -305,23 +305,21 @@ __device__ __forceinline__ int64_t divide(int64_t x, int by) {
 
 
 // ---- backward ----------------------------------------------------------------
-// delta[h][i] = dout . out of a row, and the largest finite |dout| and |v| (for fp16's range). LANES lanes a row, two values at a time where its
-// address and strides allow it (PAIRS). Bound by the latency of its loads: 10.8 us for 4095 rows of 8 heads
-// of 64, 43 us for 34560 rows of 6 heads of 30 and 77760 keys.
+// delta[h][i] = dout . out of a row. LANES lanes a row, two values at a time where its
+// address and strides allow it (PAIRS). Bound by the latency of its loads: TIME for 4095 rows of 8 heads
+// of 64, TIME for 34560 rows of 6 heads of 30.
 template <typename T, int LANES, bool PAIRS>
-__global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* delta, uint32_t* bias_max) {
-    if (p.flags != nullptr && (*p.flags & kSomeLong) == 0 && bias_max == nullptr) return;  // short windows find their own
+__global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p) {
+    if ((*p.flags & kSomeLong) == 0) return;  // short windows find their own
     constexpr int V = PAIRS ? 2 : 1;
     struct alignas(V * sizeof(T)) Pair {
         T v[V];
     };
     const int lane = threadIdx.x % LANES;
     const int64_t rows = static_cast<int64_t>(p.tq) * p.heads;
-    const int64_t vrows = bias_max == nullptr ? 0 : static_cast<int64_t>(p.tk) * p.kv_heads;
     const int64_t per = kThreads / LANES, step = static_cast<int64_t>(gridDim.x) * per;
-    float most_do = 0.0f, most_v = 0.0f;
     // whole warps stay in the loop: the shuffles name every lane
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per; row0 < rows + vrows; row0 += step) {
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per; row0 < rows; row0 += step) {
         const int64_t row = row0 + threadIdx.x / LANES;
         float sum = 0.0f;
         int64_t token = 0, head = 0;
@@ -335,34 +333,13 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p, float* de
                 Pair less{};
                 if (lo != nullptr) less = *reinterpret_cast<const Pair*>(lo + c);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float f = to_f(x.v[i]);
-                    sum = fmaf(f, to_f(y.v[i]) + (lo == nullptr ? 0.0f : to_f(less.v[i])), sum);
-                    if (is_finite(f)) most_do = fmaxf(most_do, fabsf(f));
-                }
-            }
-        } else if (row < rows + vrows) {
-            token = divide(row - rows, p.kv_heads), head = row - rows - token * p.kv_heads;
-            const T* v = static_cast<const T*>(p.v) + token * p.v_st + head * p.v_sh;
-            for (int c = V * lane; c < p.dim; c += V * LANES) {
-                const Pair x = *reinterpret_cast<const Pair*>(v + c);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float f = to_f(x.v[i]);
-                    if (is_finite(f)) most_v = fmaxf(most_v, fabsf(f));
-                }
+                for (int i = 0; i < V; ++i)
+                    sum = fmaf(to_f(x.v[i]), to_f(y.v[i]) + (lo == nullptr ? 0.0f : to_f(less.v[i])), sum);
             }
         }
 #pragma unroll
         for (int x = LANES / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        if (lane == 0 && row < rows) delta[head * p.tq + token] = sum;
-    }
-    if (bias_max == nullptr) return;
-    const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(most_do));
-    const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
-    if ((threadIdx.x & 31) == 0) {
-        if (a != 0u) atomicMax(bias_max, a);
-        if (b != 0u) atomicMax(bias_max + 1, b);
+        if (lane == 0 && row < rows) p.delta[head * p.tq + token] = sum;
     }
 }
 
@@ -740,17 +717,15 @@ cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s) {
 
 template <typename T, int LANES>
 cudaError_t delta_lanes(const AttnParams& p, cudaStream_t s, int sms) {
-    uint32_t* bias_max = const_cast<uint32_t*>(p.bias_max);
-    const int64_t rows = static_cast<int64_t>(p.tq) * p.heads + (bias_max ? static_cast<int64_t>(p.tk) * p.kv_heads : 0);
-    const int64_t blocks = (rows * LANES + kThreads - 1) / kThreads;
+    const int64_t blocks = (static_cast<int64_t>(p.tq) * p.heads * LANES + kThreads - 1) / kThreads;
     if (blocks == 0) return cudaSuccess;
     const unsigned grid = static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms);
-    const uintptr_t bytes = reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.v);
-    const bool pairs = bytes % (2 * sizeof(T)) == 0 && ((p.do_st | p.do_sh | p.v_st | p.v_sh | p.dim) & 1) == 0;
+    const uintptr_t bytes = reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out);
+    const bool pairs = bytes % (2 * sizeof(T)) == 0 && ((p.do_st | p.do_sh | p.dim) & 1) == 0;
     if (pairs)
-        k_attn_delta<T, LANES, true><<<grid, kThreads, 0, s>>>(p, p.delta, bias_max);
+        k_attn_delta<T, LANES, true><<<grid, kThreads, 0, s>>>(p);
     else
-        k_attn_delta<T, LANES, false><<<grid, kThreads, 0, s>>>(p, p.delta, bias_max);
+        k_attn_delta<T, LANES, false><<<grid, kThreads, 0, s>>>(p);
     return cudaGetLastError();
 }
 template <typename T>

@@ -687,7 +687,6 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_t
     }
     const bool mine = sh.kvh < p.kv_heads;
     const int kvh = mine ? sh.kvh : 0;
-    const float up = ds_scale<T>(p);
     const float* Eh = E + (kvh % side) * group * entries;
     TinySums ts{acc, I, grad_bias ? group * entries : 0, 0.0f, 0.0f};
 
@@ -696,6 +695,7 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_t
     const int listed = p.flags[NB == 4 ? 2 : 1];
     for (int item = mine ? sh.first : listed; item < listed; item += sh.step) {
         const int w = list[item];
+        const float up = ds_scale<T>(p, w, kvh);
         const int q0 = attn_offset(p.q_off, p.windows, p.tq, w + 1), lq = max(attn_offset(p.q_off, p.windows, p.tq, w + 2) - q0, 0);
         const int k0 = attn_offset(p.k_off, p.windows, p.tk, w + 1), n = max(attn_offset(p.k_off, p.windows, p.tk, w + 2) - k0, 0);
         const int per = ((lq + 15) / 16 + p.qsplits - 1) / p.qsplits * 16;

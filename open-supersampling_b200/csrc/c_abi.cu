@@ -1405,7 +1405,7 @@ int64_t attention_backward_scratch(oss::AttnParams& p, int32_t dtype, int64_t en
     p.bias_acc = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
     p.bias_top = sums ? arena.take<unsigned long long>(sum_rows * p.heads) : nullptr;
     p.bias_bad = sums ? arena.take<uint32_t>(sum_rows * p.heads) : nullptr;
-    p.bias_max = dtype == oss::kF16 ? arena.take<uint32_t>(2) : nullptr;
+    p.win_max = dtype == oss::kF16 ? arena.take<uint32_t>(2ll * p.windows * p.kv_heads) : nullptr;
     p.flags = dtype != oss::kF32 ? arena.take<int>(3) : nullptr;
     if (zero_at != nullptr) *zero_at = base + from, *zeroed = arena.used - from;
     return arena.used;

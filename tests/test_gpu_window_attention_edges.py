@@ -41,7 +41,7 @@ def large_case(dtype, dim):
     return q, k, v, do, qo, ko, kw
 
 
-@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [32, 64, 72])
 @pytest.mark.parametrize("where", ["padding", "neighbour"])
 def test_large_values_elsewhere_change_nothing(cuda_device, dtype, dim, where):
