@@ -306,8 +306,8 @@ __device__ __forceinline__ int64_t divide(int64_t x, int by) {
 
 // ---- backward ----------------------------------------------------------------
 // delta[h][i] = dout . out of a row. LANES lanes a row, two values at a time where its
-// address and strides allow it (PAIRS). Bound by the latency of its loads: TIME for 4095 rows of 8 heads
-// of 64, TIME for 34560 rows of 6 heads of 30.
+// address and strides allow it (PAIRS). Bound by the latency of its loads: 13 us for 34560 rows of
+// 6 heads of 30.
 template <typename T, int LANES, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p) {
     if ((*p.flags & kSomeLong) == 0) return;  // short windows find their own
