@@ -1360,7 +1360,7 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     const int64_t items = (windows > p.tk / key_tile ? windows : p.tk / key_tile) * p.kv_heads;
     const int64_t want = 2 * resident / items, most = p.tq / windows * group / 512;
     const int64_t n = want < most ? want : most;
-    p.qsplits = static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+    p.qsplits = static_cast<int>(n < 1 || p.tk == 0 ? 1 : n > 64 ? 64 : n);  // without keys there is nothing to join
     // resident blocks (no more: a few blocks left over would take as long as all others again), or as
     // many as there are tiles
     auto blocks = [](int64_t tiles, int64_t resident, int64_t heads) {

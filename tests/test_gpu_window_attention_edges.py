@@ -62,3 +62,19 @@ def test_large_values_elsewhere_change_nothing(cuda_device, dtype, dim, where):
         check_window(got, want, w, qo, ko)
         mine = (column >= (5 * w - 1 if w else 0)) & (column <= 5 * w + 3)
         check(got["dtable"][mine.to(cuda_device)], tuple(t[mine] for t in want["dtable"]), f"dtable of window {w}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries,heads,kv,dim", [([1024], 2, 2, 32), ([1024] * 4, 4, 2, 64), ([3000], 8, 1, 128)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_no_keys_at_all(cuda_device, dtype, queries, heads, kv, dim, biased):
+    """Enough queries that they are shared out over blocks, and nothing for them to see."""
+    (q, k, v, do), qo, ko, g = inputs(queries, [0] * len(queries), heads, kv, dim, TYPES[dtype])
+    kw = {}
+    if biased:
+        kw = dict(table=torch.randn(3, heads, generator=g).to(TYPES[dtype]), buckets=torch.tensor([[0, 1, 2]], dtype=torch.int32),
+                  q_pos=torch.zeros(q.shape[0], dtype=torch.int32), k_pos=torch.zeros(0, dtype=torch.int32))
+    got = run(cuda_device, q, k, v, qo, ko, do, **kw)
+    assert got["dk"].shape == k.shape and got["dv"].shape == v.shape
+    for n in got:
+        assert not got[n].any(), n
