@@ -446,19 +446,33 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_fwd_blocks(DB, NB)) k_attn_f
 // ---- backward -------------------------------------------------------------------------------
 // 32 columns and 32 keys at most: dk and dv of the window stay in registers. Windows of up to 16 keys
 // (NB = 2) and of 17 to 32 (NB = 4) apart, as in the forward. The bias gradient
-// goes into the warp's own 32-bit integers, at a scale that leaves room for what was added since
-// they were last moved to its fp64 sums.
+// goes into the warp's own 32-bit integers, at a scale of each head's that leaves room for what was added
+// since they were last moved to its fp64 sums. A step of 16 rows stands at 2^20 at least: a scale kept from
+// a window, or a head, of larger gradients would round the smaller ones away (entries that only these
+// reach lost 24% at 2^-16 of the larger ones).
 // A warp's sums of the bias gradient.
 struct TinySums {
-    double* acc;  // [n]
-    int* I;       // [n], times `fixed`
-    int n;        // 0: no gradient is wanted
+    double* acc;   // [group][n]
+    int* I;        // [group][n], times the head's `fixed`
+    float* state;  // [group][2], `fixed` and `used` of the heads that are not worked on
+    int n;         // entries; 0: no gradient is wanted
+    int head;      // of the group
     float fixed, used;
-    // the integers to the fp64 sums
+    __device__ __forceinline__ void enter(int head_) {
+        head = head_;
+        fixed = state[2 * head];
+        used = state[2 * head + 1];
+    }
+    __device__ __forceinline__ void leave() {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) state[2 * head] = fixed, state[2 * head + 1] = used;
+        __syncwarp();
+    }
+    // the head's integers to the fp64 sums
     __device__ __forceinline__ void flush() {
         __syncwarp();
         const double unit = fixed > 0.0f ? 1.0 / static_cast<double>(fixed) : 0.0;
-        for (int e = threadIdx.x & 31; e < n; e += 32) {
+        for (int e = head * n + (threadIdx.x & 31); e < (head + 1) * n; e += 32) {
             const int v = I[e];
             if (v != 0) acc[e] += static_cast<double>(v) * unit, I[e] = 0;
         }
@@ -467,9 +481,12 @@ struct TinySums {
     }
     // Room for terms of this size altogether, in up to 512 roundings of half a step.
     __device__ __forceinline__ void reserve(float size) {
-        if (size > 0.0f && !(fixed > 0.0f && used + size * fixed + 512.0f < 1073741824.0f)) {
-            flush();
-            fixed = exp2f(static_cast<float>(min(max(23 - ilogbf(size), -126), 126)));
+        if (size > 0.0f && !(size * fixed >= 1048576.0f && used + size * fixed + 512.0f < 1073741824.0f)) {
+            const float to = exp2f(static_cast<float>(min(max(23 - ilogbf(size), -126), 126)));
+            if (to != fixed || used + size * fixed + 512.0f >= 1073741824.0f) {
+                flush();
+                fixed = to;
+            }
         }
         used += size * fixed + 512.0f;
     }
@@ -502,6 +519,7 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
     const int left = n - 2 * t;  // key 8 kb + 2 t + i is there where 8 kb + i < left
     for (int gh = 0; gh < group; ++gh) {
         const int head = kvh * group + gh;
+        if (BIAS && ts.n > 0) ts.enter(gh);
         const Rows<T, 1> rq(p.q, p.q_st, p.q_sh, p.dim, head), rg(p.dout, p.do_st, p.do_sh, p.dim, head);
         const float* Eh = E + gh * entries;
         // of row g: the next rows to load, and the rows to write
@@ -636,6 +654,7 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
             if (r0 + g < r_end) store_row16<T, 1>(to, p.dim, dq, 0, p.scale / up);
             if (r0 + g + 8 < r_end) store_row16<T, 1>(to + to_step, p.dim, dq, 1, p.scale / up);
         }
+        if (BIAS && ts.n > 0) ts.leave();
     }
 #pragma unroll
     for (int m = 0; m < NM; ++m)
@@ -674,8 +693,7 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_t
     double* acc_all = reinterpret_cast<double*>(smem_raw + sizeof(TinyPos<NB>) * kWarps);
     int* I_all = reinterpret_cast<int*>(acc_all + (grad_bias ? kWarps * group * entries : 0));
     float* E = reinterpret_cast<float*>(I_all + (grad_bias ? kWarps * group * entries : 0));
-    double* acc = acc_all + warp * group * entries;
-    int* I = I_all + warp * group * entries;
+    float* state = E + side * group * entries;  // of the warps' sums
     if constexpr (BIAS) {
         for (int e = threadIdx.x; e < side * group * entries; e += 32 * kWarps) {
             const int head = blockIdx.y * side * group + e / entries;
@@ -683,12 +701,14 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_t
         }
         if (grad_bias)
             for (int e = threadIdx.x; e < kWarps * group * entries; e += 32 * kWarps) acc_all[e] = 0.0, I_all[e] = 0;
+        if (grad_bias)
+            for (int e = threadIdx.x; e < kWarps * group * 2; e += 32 * kWarps) state[e] = 0.0f;
         __syncthreads();
     }
     const bool mine = sh.kvh < p.kv_heads;
     const int kvh = mine ? sh.kvh : 0;
     const float* Eh = E + (kvh % side) * group * entries;
-    TinySums ts{acc, I, grad_bias ? group * entries : 0, 0.0f, 0.0f};
+    TinySums ts{acc_all + warp * group * entries, I_all + warp * group * entries, state + warp * group * 2, grad_bias ? entries : 0, 0, 0.0f, 0.0f};
 
     // the windows of this kernel's class, as listed
     const int* list = p.tiny_list + (NB == 4 ? p.windows : 0);
@@ -711,7 +731,10 @@ __global__ void __launch_bounds__(32 * kWarps, tiny_bwd_blocks(NB)) k_attn_bwd_t
     }
     if constexpr (BIAS)
         if (grad_bias) {
-            ts.flush();
+            for (int gh = 0; gh < group; ++gh) {
+                ts.enter(gh);
+                ts.flush();
+            }
             // the warps of one key head, in order, make one part
             __syncthreads();
             for (int e = threadIdx.x; e < side * group * entries; e += 32 * kWarps) {
@@ -761,7 +784,7 @@ template <typename T, int NB, bool BIAS>
 cudaError_t bwd_one(const AttnParams& p, int first_part, cudaStream_t s) {
     const int64_t entries = BIAS ? bias_entries(p.bias) : 0, group = p.heads / p.kv_heads;
     const int bytes = static_cast<int>(sizeof(TinyPos<NB>) * kWarps + 4 * heads_of_block(p) * entries +
-                                       (p.bias_part != nullptr ? 12 * kWarps * group * entries : 0));
+                                       (p.bias_part != nullptr ? kWarps * group * (12 * entries + 8) : 0));
     cudaError_t err = cudaFuncSetAttribute(k_attn_bwd_tiny<T, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return err;
     k_attn_bwd_tiny<T, NB, BIAS><<<dim3(p.tiny_blocks, sets_of(p), p.qsplits), 32 * kWarps, bytes, s>>>(p, first_part);

@@ -1371,7 +1371,7 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
     // biases and sums of its warps leave room for two blocks on an SM.
     const int64_t side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
     const bool tiny = !p.causal && p.dim <= 32 && p.tk <= 128 * windows &&
-                      entries * group * (4 * side + (sums ? 48 : 0)) <= 110 * 1024;
+                      (entries * (4 * side + (sums ? 48 : 0)) + (sums ? 32 : 0)) * group <= 110 * 1024;
     p.tiny_max = tiny ? 32 : 0;
     p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;
     p.short_blocks = blocks(windows, resident, p.kv_heads * p.qsplits);

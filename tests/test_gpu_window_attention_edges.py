@@ -78,3 +78,45 @@ def test_no_keys_at_all(cuda_device, dtype, queries, heads, kv, dim, biased):
     assert got["dk"].shape == k.shape and got["dv"].shape == v.shape
     for n in got:
         assert not got[n].any(), n
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("keys", [7, 16, 30])
+@pytest.mark.parametrize("size", [2.0**-8, 2.0**-14, 2.0**-20])
+def test_bias_gradient_of_small_windows(cuda_device, dtype, keys, size):
+    """Windows of ordinary gradients, then ones of far smaller gradients, each with rows of the table of their own; the
+    same for the heads of a group."""
+    windows = 1024  # more than the blocks' warps: each walks windows of both kinds
+    (q, k, v, do), qo, ko, g = inputs([64] * windows, [keys] * windows, 4, 1, 16, TYPES[dtype], seed=keys)
+    small = torch.arange(windows) >= windows // 2
+    rows_q, rows_k = small.repeat_interleave(64), small.repeat_interleave(keys)
+    scale = torch.where(rows_q, size, 1.0)[:, None, None].expand(-1, 4, 1).clone()
+    scale[:, 2] *= size  # and one head
+    do = (do.double() * scale).to(TYPES[dtype])
+    qp, kp = torch.randint(0, 2, (q.shape[0],), generator=g).int(), torch.randint(0, 2, (k.shape[0],), generator=g).int()
+    kp += torch.where(rows_k, 6, 0).int()
+    table = torch.randn(17, 4, generator=g)
+    buckets = torch.arange(17, dtype=torch.int32).view(1, 17)
+    kw = dict(table=table, buckets=buckets, q_pos=qp, k_pos=kp)
+    got = run(cuda_device, q, k, v, qo, ko, do, **kw)["dtable"]
+    # the formula, all windows at once
+    qd, kd, vd, dd = (t.double().view(windows, -1, t.shape[1], 16) for t in (q, k, v, do))
+    row = (kp.view(windows, 1, -1) - qp.view(windows, -1, 1) + 8).long()
+    s = torch.einsum("wihd,wjd->whij", qd, kd[:, :, 0]) / 4 + table.double()[row].permute(0, 3, 1, 2)
+    p = torch.softmax(s, -1)
+    dp = torch.einsum("wihd,wjd->whij", dd, vd[:, :, 0])
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    want, size_of = torch.zeros(17, 4, dtype=torch.float64), torch.zeros(17, 4, dtype=torch.float64)
+    # a pair's term is off by its score's, dp's and delta's errors (as the formula's, 24 = dim + 8, without out's rounding:
+    # these kernels take delta from p and dp), and by half a step of the sums, 2^-20 of the 16 rows' sum of magnitudes
+    f = 2.0**-24
+    score = 24 * f * (torch.einsum("wihd,wjd->whij", qd.abs(), kd[:, :, 0].abs()) / 4 + table.abs().max())
+    dpe = 24 * f * torch.einsum("wihd,wjd->whij", dd.abs(), vd[:, :, 0].abs())
+    rel = 2 * score.amax(-1, keepdim=True) + (16 + keys) * f
+    off = rel * ds.abs() + p * (dpe + (p * (dpe + rel * dp.abs())).sum(-1, keepdim=True) + 4 * f * dp.abs())
+    step = ds.abs().view(windows, 4, 4, 16 * keys).sum(-1)[..., None, None].expand(-1, -1, -1, 16, keys).reshape(ds.shape)
+    off = off + 2.0**-21 * step
+    flat = row.reshape(-1)
+    want.index_add_(0, flat, ds.permute(0, 2, 3, 1).reshape(-1, 4))
+    size_of.index_add_(0, flat, off.permute(0, 2, 3, 1).reshape(-1, 4))
+    check(got, (want, 1.05 * size_of + f * want.abs() + 1e-35), "dtable")
