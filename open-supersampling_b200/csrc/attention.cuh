@@ -332,6 +332,14 @@ __device__ __forceinline__ float lost_by(float x) {
 
 
 // ---- launchers -----------------------------------------------------------------
+constexpr int kMaxSmem = 227 * 1024;  // of a block
+// Lets a kernel take any shared memory there is. The limit is one for all host threads: set to what a call needs,
+// it made the launch of another thread fail that came with a larger map in between.
+template <typename K>
+cudaError_t allow_smem(K kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+}
+
 // type: AttnType of q, k, v and out.
 cudaError_t launch_attn_forward(const AttnParams& p, int type, cudaStream_t s);
 // dtable (null: no gradient of the table).

@@ -499,7 +499,7 @@ template <typename T, int DP, bool BIAS, bool REST>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int entries = bias_entries(p.bias);
     const int bytes = 1024 + FwdSmem<DP>::kBytes + 4 * entries * p.pack;
-    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_mma<T, DP, BIAS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t err = allow_smem(k_attn_fwd_mma<T, DP, BIAS, REST>);
     if (err != cudaSuccess) return err;
     const int type = kIsBf16<T> ? kBF16 : kF16;
     TileMaps maps;

@@ -1071,11 +1071,6 @@ __global__ void __launch_bounds__(256) k_attn_join_dkv(AttnParams p) {
     static_cast<T*>(p.dv)[i] = from_f<T>(v);
 }
 
-template <typename K>
-cudaError_t smem_of(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <typename T, int DP, bool BIAS>
 cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
     const int entries = bias_entries(p.bias), group = p.heads / p.kv_heads, sum = p.bias_part != nullptr;
@@ -1085,19 +1080,19 @@ cudaError_t bwd_one(const AttnParams& p, void* dtable, cudaStream_t s) {
     if (p.short_max == 0) {
         // only rows and windows without partners: no bias is looked up
         const int bytes = 1024 + ShortSmem<DP>::kBytes;
-        if ((err = smem_of(k_attn_bwd_short<T, DP, false>, bytes)) != cudaSuccess) return err;
+        if ((err = allow_smem(k_attn_bwd_short<T, DP, false>)) != cudaSuccess) return err;
         k_attn_bwd_short<T, DP, false><<<dim3(p.short_blocks, p.kv_heads, 1), 2 * kRows, bytes, s>>>(p);
     } else {
-        if ((err = smem_of(k_attn_bwd_short<T, DP, BIAS>, b_short)) != cudaSuccess) return err;
+        if ((err = allow_smem(k_attn_bwd_short<T, DP, BIAS>)) != cudaSuccess) return err;
         k_attn_bwd_short<T, DP, BIAS><<<dim3(p.short_blocks, p.kv_heads, p.qsplits), 2 * kRows, b_short, s>>>(p);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int b_dq = 1024 + DqShape<DP>::kBytes + entries * (4 + 12 * sum);
-    if ((err = smem_of(k_attn_dq_long<T, DP, BIAS>, b_dq)) != cudaSuccess) return err;
+    if ((err = allow_smem(k_attn_dq_long<T, DP, BIAS>)) != cudaSuccess) return err;
     k_attn_dq_long<T, DP, BIAS><<<dim3(p.dq_blocks, p.heads), DqShape<DP>::kThreads, b_dq, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int b_kv = 1024 + DkvShape<DP>::kBytes + entries * 4;
-    if ((err = smem_of(k_attn_dkv_long<T, DP, BIAS>, b_kv)) != cudaSuccess) return err;
+    if ((err = allow_smem(k_attn_dkv_long<T, DP, BIAS>)) != cudaSuccess) return err;
     k_attn_dkv_long<T, DP, BIAS><<<dim3(p.dkv_blocks, p.kv_heads, p.qsplits), DkvShape<DP>::kThreads, b_kv, s>>>(p);
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     if (p.qsplits > 1) {

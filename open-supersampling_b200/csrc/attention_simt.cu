@@ -14,7 +14,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kKeys = 64;  // keys of a tile
-constexpr int64_t kMaxSmem = 227 * 1024;  // of a block
 
 // ---- shared-memory layout ---------------------------------------------------
 struct Smem {
@@ -657,17 +656,12 @@ __global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dt
 
 int64_t floats(int64_t n) { return (n + 3) / 4 * 4; }
 
-template <typename K>
-cudaError_t set_smem(K kernel, int64_t bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-}
-
 template <typename T, int DP, int RM>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     constexpr int BM = 16 * RM;
     const int64_t bytes = 4 * (floats(BM * (DP + 4)) + 2 * floats(kKeys * (DP + 4)) + floats(BM * (kKeys + 4)) + BM * 2 +
                                kKeys * 2 + floats(static_cast<int64_t>(bias_entries(p.bias)) * p.pack));
-    cudaError_t err = set_smem(k_attn_fwd<T, DP, RM>, bytes);
+    cudaError_t err = allow_smem(k_attn_fwd<T, DP, RM>);
     if (err != cudaSuccess) return err;
     const dim3 grid(attn_slots(static_cast<int64_t>(p.tq) * p.pack, p.windows, BM), p.heads / p.pack, p.splits);
     k_attn_fwd<T, DP, RM><<<grid, kThreads, bytes, s>>>(p);
@@ -702,15 +696,15 @@ cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s) {
     const int slots = attn_slots(p.tq, p.windows, 64);
     cudaError_t err;
     if (grad_bias) {
-        if ((err = set_smem(k_attn_dq<T, DP, true>, dq_bytes)) != cudaSuccess) return err;
+        if ((err = allow_smem(k_attn_dq<T, DP, true>)) != cudaSuccess) return err;
         k_attn_dq<T, DP, true><<<dim3(p.dq_blocks, p.heads), kThreads, dq_bytes, s>>>(p, own_acc);
     } else {
-        if ((err = set_smem(k_attn_dq<T, DP, false>, dq_bytes)) != cudaSuccess) return err;
+        if ((err = allow_smem(k_attn_dq<T, DP, false>)) != cudaSuccess) return err;
         k_attn_dq<T, DP, false><<<dim3(slots, p.heads), kThreads, dq_bytes, s>>>(p, 0);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
     const int64_t kv_bytes = 4 * (4 * floats(64 * (DP + 4)) + 2 * floats(64 * 68) + 2 * 64 + 4 * 64 + floats(entries));
-    if ((err = set_smem(k_attn_dkv<T, DP>, kv_bytes)) != cudaSuccess) return err;
+    if ((err = allow_smem(k_attn_dkv<T, DP>)) != cudaSuccess) return err;
     k_attn_dkv<T, DP><<<dim3(attn_slots(p.tk, p.windows, kKeys), p.kv_heads), kThreads, kv_bytes, s>>>(p);
     return cudaGetLastError();
 }

@@ -772,7 +772,7 @@ int heads_of_block(const AttnParams& p) {
 template <typename T, int DB, int NB, bool BIAS>
 cudaError_t fwd_one(const AttnParams& p, cudaStream_t s) {
     const int bytes = BIAS ? static_cast<int>(sizeof(TinyPos<NB>)) * kWarps + 4 * heads_of_block(p) * bias_entries(p.bias) : 0;
-    cudaError_t err = cudaFuncSetAttribute(k_attn_fwd_tiny<T, DB, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t err = allow_smem(k_attn_fwd_tiny<T, DB, NB, BIAS>);
     if (err != cudaSuccess) return err;
     // as many blocks as stay resident, or as there can be pieces
     const int side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1, sets = sets_of(p);
@@ -785,7 +785,7 @@ cudaError_t bwd_one(const AttnParams& p, int first_part, cudaStream_t s) {
     const int64_t entries = BIAS ? bias_entries(p.bias) : 0, group = p.heads / p.kv_heads;
     const int bytes = static_cast<int>(sizeof(TinyPos<NB>) * kWarps + 4 * heads_of_block(p) * entries +
                                        (p.bias_part != nullptr ? kWarps * group * (12 * entries + 8) : 0));
-    cudaError_t err = cudaFuncSetAttribute(k_attn_bwd_tiny<T, NB, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaError_t err = allow_smem(k_attn_bwd_tiny<T, NB, BIAS>);
     if (err != cudaSuccess) return err;
     k_attn_bwd_tiny<T, NB, BIAS><<<dim3(p.tiny_blocks, sets_of(p), p.qsplits), 32 * kWarps, bytes, s>>>(p, first_part);
     return cudaGetLastError();

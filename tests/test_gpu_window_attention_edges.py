@@ -2,6 +2,8 @@
 (tests/attention_reference.py states the allowed errors)."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -120,3 +122,61 @@ def test_bias_gradient_of_small_windows(cuda_device, dtype, keys, size):
     want.index_add_(0, flat, ds.permute(0, 2, 3, 1).reshape(-1, 4))
     size_of.index_add_(0, flat, off.permute(0, 2, 3, 1).reshape(-1, 4))
     check(got, (want, 1.05 * size_of + f * want.abs() + 1e-35), "dtable")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("keys", [20, 100])
+def test_host_threads_with_other_maps(cuda_device, dtype, keys):
+    """Threads that call at once with bias maps of very different size, and so shared memory: no launch fails, no result
+    changes. The calls go to the C entry points, which hold no lock, so that many of them overlap."""
+    from oss_cuda import _lib, attention, window_position_buckets
+
+    dev, lib = cuda_device, _lib.lib()
+    calls = []
+    for reach in (0, 31, 2, 31):
+        (q, k, v, do), qo, ko, g = inputs([40, 30], [keys, keys], 1, 1, 32, TYPES[dtype], seed=reach)
+        i32 = dict(dtype=torch.int32, device=dev)
+        buckets = window_position_buckets(reach, reach).to(dev)
+        table = torch.randn(buckets.numel(), 1, generator=g).to(dev)
+        pos = [torch.randint(-20, 20, (t.shape[0], 2), generator=g).int().to(dev) for t in (q, k)]
+        q, k, v, do = (t.to(dev) for t in (q, k, v, do))
+        keep = (q, k, v, torch.tensor(qo, **i32), torch.tensor(ko, **i32), 0.2, 0, table, buckets, *pos)
+        args = attention._call_args(*keep)
+        out, dq, dk, dv, dt = (torch.empty_like(t) for t in (q, q, k, v, table))
+        lo, lse = torch.empty_like(q), torch.empty(1, q.shape[0], device=dev)
+        sizes = (lib.oss_window_attention_scratch_bytes(*args[:7], 0, buckets.numel()),
+                 lib.oss_window_attention_backward_scratch_bytes(*args[:7], 0, buckets.numel(), table.shape[0]))
+        scratch = [torch.empty(n + 16, dtype=torch.uint8, device=dev) for n in sizes]
+        stream = torch.cuda.Stream(dev)
+        forward = (*args, out.data_ptr(), lse.data_ptr(), lo.data_ptr(), scratch[0].data_ptr(), sizes[0], stream.cuda_stream)
+        backward = (*args, out.data_ptr(), lse.data_ptr(), lo.data_ptr(), do.data_ptr(), do.stride(0), do.stride(1), dq.data_ptr(),
+                    dk.data_ptr(), dv.data_ptr(), dt.data_ptr(), scratch[1].data_ptr(), sizes[1], stream.cuda_stream)
+        calls.append((forward, backward, (out, dq, dk, dv, dt), (keep, do, lo, lse, scratch, stream)))
+    torch.cuda.synchronize(dev)
+
+    def both_ways(i):
+        return lib.oss_window_attention_forward(*calls[i][0]) or lib.oss_window_attention_backward(*calls[i][1])
+
+    want = []
+    for i, (_, _, results, _) in enumerate(calls):
+        assert both_ways(i) == 0
+        torch.cuda.synchronize(dev)
+        want.append([t.clone() for t in results])
+    refused = []
+
+    def work(i):
+        for _ in range(400):
+            rc = both_ways(i)
+            if rc:
+                refused.append((i, rc, lib.oss_last_error().decode()))
+
+    with torch.cuda.device(dev):
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+        for x in threads:
+            x.start()
+        for x in threads:
+            x.join()
+    torch.cuda.synchronize(dev)
+    assert not refused, (len(refused), refused[:2])
+    for (_, _, results, _), w in zip(calls, want):
+        assert all(torch.equal(a, b) for a, b in zip(results, w))
