@@ -11,6 +11,7 @@ import os
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -53,6 +54,14 @@ class on_device_of:
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+def check_no_tangent(name: str, *tensors: torch.Tensor | None) -> None:
+    """An operator without forward-mode derivatives refuses a tangent: its kernels would drop it."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def check_float_cuda(t: torch.Tensor, name: str) -> None:

@@ -17,7 +17,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._raster import check_int_cuda, on_device_of, stream_of
+from ._raster import check_int_cuda, check_no_tangent, on_device_of, stream_of
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_DIM = 128
@@ -164,7 +164,7 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
                  q_pos (Tq, 2) and k_pos (Tk, 2) int32 (y, x), or (Tq,) and (Tk,) with a (1, 2 r + 1) map.
 
     A query that sees no key, or lies outside every window, gives zeros.  Differentiable once, in q, k, v and
-    bias_table, with the same bits on every run.  Scores, softmax and sums are held in fp32; with 16-bit
+    bias_table, in reverse mode, with the same bits on every run.  Scores, softmax and sums are held in fp32; with 16-bit
     inputs the weights are rounded to their type before they meet v.  A value that is not finite reaches only
     the rows whose window and mask show it.  To capture a backward into a graph, drop earlier eager graphs of
     the same leaves first."""
@@ -195,6 +195,7 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
     scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
     if not 0.0 < scale < 3.0e38:
         raise ValueError("scale must be positive and finite")
+    check_no_tangent("fused_window_cross_attention", q, k, v, bias_table)
     if bias_table is not None:
         bias_table = bias_table.contiguous()
     args = (q, k, v, q_offsets, k_offsets, scale, int(bool(causal)), bias_table, buckets, q_pos, k_pos)

@@ -11,7 +11,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._raster import on_device_of, stream_of
+from ._raster import check_no_tangent, on_device_of, stream_of
 from .attention import DTYPES
 
 KINDS = ("rms", "layer")
@@ -106,7 +106,7 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
     kind         "rms" (u / sqrt(mean(u^2) + eps)) or "layer" ((u - mean) / sqrt(var + eps)); biases are for "layer"
 
     Returns (y, z), or y alone without next_weight.  The arithmetic is fp32, each result rounded once (z is taken
-    from y before it is rounded).  Differentiable once, in every tensor, with the same bits on every run."""
+    from y before it is rounded).  Differentiable once, in every tensor, in reverse mode, with the same bits on every run."""
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {KINDS}, got {kind!r}")
     if gate_act not in ACTS:
@@ -150,6 +150,7 @@ def gated_residual_norm(x, h, weight, next_weight=None, *, gate=None, gate_act="
             grad = grad or (want_grad and t.requires_grad)
             t = t.contiguous()
         params.append(t)
+    check_no_tangent("gated_residual_norm", x, h, gate, *params)
     x2, h2 = _rows(x, c), _rows(h, c)
     g2 = None if gate is None else _rows(gate, gate.shape[-1])
     layer, act = int(kind == "layer"), ACTS[gate_act] if gate is not None else 0

@@ -180,3 +180,18 @@ def test_host_threads_with_other_maps(cuda_device, dtype, keys):
     assert not refused, (len(refused), refused[:2])
     for (_, _, results, _), w in zip(calls, want):
         assert all(torch.equal(a, b) for a, b in zip(results, w))
+
+
+def test_forward_mode_level_without_a_tangent(cuda_device):
+    """Inside a forward-mode level, calls without tangents give what they give outside."""
+    import torch.autograd.forward_ad as forward_ad
+
+    from oss_cuda import gated_residual_norm
+
+    (q, k, v, do), qo, ko, _ = inputs([20], [30], 2, 2, 16, torch.float32)
+    x, w = torch.randn(4, 8, device=cuda_device), torch.ones(8, device=cuda_device)
+    want, norm = run(cuda_device, q, k, v, qo, ko, do), gated_residual_norm(x, x, w)
+    with forward_ad.dual_level():
+        got = run(cuda_device, q, k, v, qo, ko, do)
+        assert torch.equal(gated_residual_norm(x, x, w), norm)
+    assert all(torch.equal(got[n], want[n]) for n in want)
