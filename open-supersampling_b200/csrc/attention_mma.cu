@@ -104,9 +104,10 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
     volatile int* dead = reinterpret_cast<volatile int*>(bars + 21);
     float* E = reinterpret_cast<float*>(bars + 24);
     // Barriers. One each: Q there, O done. For each buffer: P there (a softmax warp may be a tile ahead of
-    // another), S done, keys there and read, values there and read, key positions there and read.
+    // another), S done, keys there and read, values there and read, key positions there and read. The last one is
+    // for products in flight after a wait that ran out.
     const uint32_t bar0 = tc::smem_addr(bars), bar_q = bar0, bar_o = bar0 + 8, bar_p = bar0 + 16, bar_s = bar0 + 32, bar_k = bar0 + 48,
-                   bar_k_read = bar0 + 64, bar_v = bar0 + 80, bar_v_read = bar0 + 96, bar_pos = bar0 + 112, bar_pos_read = bar0 + 128;
+                   bar_k_read = bar0 + 64, bar_v = bar0 + 80, bar_v_read = bar0 + 96, bar_pos = bar0 + 112, bar_pos_read = bar0 + 128, bar_end = bar0 + 144;
 
     const int tid = threadIdx.x, warp = tid >> 5;
     const int head0 = blockIdx.y * p.pack, kvh = head0 / (p.heads / p.kv_heads);
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
     if (!more) return;
 
     if (tid == 0) {
-        for (int b = 0; b < 18; ++b) tc::mbar_init(bar0 + 8 * b, b == 0 || b == 2 || b == 3 || b >= 16 ? kRows : 1);
+        for (int b = 0; b < 19; ++b) tc::mbar_init(bar0 + 8 * b, b == 0 || b == 2 || b == 3 || b == 16 || b == 17 ? kRows : 1);
         tc::mbar_init_fence();
         *dead = 0;
     }
@@ -162,12 +163,15 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
     if (warp == 5) {
         // ---- keys and values
         const int lane = tid & 31, panels = dim16 > 64 ? 2 : 1;
-        for (; more; more = walk.next()) {
+        bool ok = true;
+        int k_sent = 0, v_sent = 0;  // tiles whose copies have been issued
+        for (; ok && more; more = walk.next()) {
             const AttnTile& t = walk.tile;
             const Keys kk = keys_of(t);
             for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++u) {
                 const int b = u & 1, parity = (u >> 1) & 1, n = min(KT, kk.most - kt * KT), token = t.obegin + kt * KT;
-                tc::mbar_wait(bar_k_read + 8 * b, parity ^ 1, dead);  // of two tiles before: passes at once at first
+                // of two tiles before: passes at once at first
+                if (!(ok = __all_sync(0xffffffffu, tc::mbar_wait(bar_k_read + 8 * b, parity ^ 1, dead)))) break;
                 if (maps.use) {
                     if (tc::elect_one()) {
                         tc::mbar_expect(bar_k + 8 * b, panels * KT * 128);
@@ -175,10 +179,11 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                             tc::tma_load(sk + b * L::kK + h * KT * 128, &maps.k, bar_k + 8 * b, 64 * h, maps.k_tokens_y ? token : kvh,
                                          maps.k_tokens_y ? kvh : token);
                     }
+                    ++k_sent;
                 } else {
                     warp_load<T>(sk + b * L::kK, KT, p.k, p.k_st, p.k_sh, p.dim, kvh, token, n, (n + 15) & ~15);
                 }
-                tc::mbar_wait(bar_v_read + 8 * b, parity ^ 1, dead);
+                if (!(ok = __all_sync(0xffffffffu, tc::mbar_wait(bar_v_read + 8 * b, parity ^ 1, dead)))) break;
                 if (maps.use) {
                     if (tc::elect_one()) {
                         tc::mbar_expect(bar_v + 8 * b, panels * KT * 128);
@@ -186,6 +191,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                             tc::tma_load(sv + b * L::kK + h * KT * 128, &maps.v, bar_v + 8 * b, 64 * h, maps.v_tokens_y ? token : kvh,
                                          maps.v_tokens_y ? kvh : token);
                     }
+                    ++v_sent;
                 } else {
                     warp_load<T>(sv + b * L::kK, KT, p.v, p.v_st, p.v_sh, p.dim, kvh, token, n, (n + 15) & ~15);
                     tc::cp_async_commit();
@@ -198,25 +204,34 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                     }
                 }
                 if (BIAS) {
-                    tc::mbar_wait(bar_pos_read + 8 * b, parity ^ 1, dead);
+                    if (!(ok = __all_sync(0xffffffffu, tc::mbar_wait(bar_pos_read + 8 * b, parity ^ 1, dead)))) break;
                     load_key_pos_warp<KT>(kps + b, p.bias, token, n);
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(bar_pos + 8 * b);
                 }
             }
+            if (!ok) break;
+        }
+        if (!ok) {  // the copies in flight, before the block may end
+            tc::cp_async_commit();
+            tc::cp_async_wait<0>();
+            for (int i = max(k_sent - 2, 0); i < k_sent; ++i) tc::mbar_settle(bar_k + 8 * (i & 1), (i >> 1) & 1);
+            for (int i = max(v_sent - 2, 0); i < v_sent; ++i) tc::mbar_settle(bar_v + 8 * (i & 1), (i >> 1) & 1);
         }
     } else if (warp == 4) {
         // ---- products
         const int lane = tid & 31;
         const uint32_t id_o = tc::idesc(kBf16, dim16, false, true);
         int par_q = 0, par_o = 0;
-        for (; more; more = walk.next()) {
+        bool ok = true;  // no wait has run out: whatever is issued has its operands
+        auto wait = [&](uint32_t bar, int parity) { return ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, dead)); };
+        for (; ok && more; more = walk.next()) {
             const Keys kk = keys_of(walk.tile);
             if (kk.tile0 >= kk.tile1) continue;
             // S of tile kt, number v
             auto scores = [&](int kt, int v) {
                 const int b = v & 1, n16 = (min(KT, kk.most - kt * KT) + 15) & ~15;
-                tc::mbar_wait(bar_k + 8 * b, (v >> 1) & 1, dead);
+                if (!wait(bar_k + 8 * b, (v >> 1) & 1)) return;
                 if (tc::elect_one()) {
                     tc::fence_after();
                     tc::mma_nt<DP, kRows, KT>(tmem + b * kS, sq, sk + b * L::kK, dim16, tc::idesc(kBf16, n16, false, false));
@@ -225,17 +240,17 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 }
                 __syncwarp();
             };
-            tc::mbar_wait(bar_q, par_q, dead);
+            if (!wait(bar_q, par_q)) break;
             par_q ^= 1;
             scores(kk.tile0, u);
-            for (int kt = kk.tile0; kt < kk.tile1; ++kt, ++u) {
+            for (int kt = kk.tile0; ok && kt < kk.tile1; ++kt, ++u) {
                 const int b = u & 1, n = min(KT, kk.most - kt * KT), n16 = (n + 15) & ~15;
                 if (kt > kk.tile0) {  // P of the tile before has been read: its buffer takes the next S
-                    tc::mbar_wait(bar_o, par_o, dead);
+                    if (!wait(bar_o, par_o)) break;
                     par_o ^= 1;
                 }
                 if (kt + 1 < kk.tile1) scores(kt + 1, u + 1);
-                tc::mbar_wait(bar_v + 8 * b, (u >> 1) & 1, dead);
+                if (!wait(bar_v + 8 * b, (u >> 1) & 1)) break;
                 if (maps.use && n < n16) {  // what follows the window's last value meets weights of 0: it must not be NaN
                     const int chunks = dim16 / 8;
                     for (int i = lane; i < (n16 - n) * chunks; i += 32) {
@@ -245,7 +260,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                     tc::fence_async();
                     __syncwarp();
                 }
-                tc::mbar_wait(bar_p + 8 * b, (u >> 1) & 1, dead);
+                if (!wait(bar_p + 8 * b, (u >> 1) & 1)) break;
                 if (tc::elect_one()) {
                     tc::fence_after();
                     tc::mma_tn<KT>(tmem + kO, tmem + b * kS, sv + b * L::kK, n16, id_o, kt > kk.tile0);
@@ -255,8 +270,13 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 }
                 __syncwarp();
             }
-            tc::mbar_wait(bar_o, par_o, dead);
+            if (!wait(bar_o, par_o)) break;
             par_o ^= 1;
+        }
+        if (!ok) {  // the products in flight, before their tensor memory is freed
+            if (tc::elect_one()) tc::commit(bar_end);
+            __syncwarp();
+            tc::mbar_settle(bar_end, 0);
         }
     } else {
         // ---- softmax
@@ -391,8 +411,12 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 par_o ^= 1;
                 tc::fence_after();
             }
+            // A wait of the block has run out: its rows become NaN. (The warps that load and issue stop at theirs,
+            // and every wait for them then runs out here too.)
+            alive = alive && *dead == 0;
+            if (!alive) l = __uint_as_float(0x7fffffffu);
             // O out of tensor memory, staged through the Q panels so that rows are written together
-            const float inv = p.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = p.splits > 1 ? (alive ? 1.0f : l) : l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t at = token * p.heads + head;
             const int64_t part = static_cast<int64_t>(blockIdx.z) * p.tq * p.heads + at;
             if (live && p.splits > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
@@ -413,13 +437,16 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
 #pragma unroll
                 for (int i = 0; i < 16; ++i) fine = fine && (!p.causal || is_finite(o[i]));  // columns past dim are 0
                 if (p.splits > 1) {
+                    if (!alive)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = l;
                     if (live) write_part(p.part_o + part * p.dim, o, c, p.dim);
                 } else {
-                    stage16<T>(sq, tid, o, c, alive ? inv : __uint_as_float(0x7fffffffu));
+                    stage16<T>(sq, tid, o, c, inv);
                 }
             }
             tc::fence_before();  // before the next tile's first P is announced, and so its O is written
-            if (p.causal && live && !fine) {
+            if (p.causal && live && !fine && alive) {
                 forward_row<T>(p, token, head, BIAS ? p.bias.k_pos : nullptr, t.obegin, kk.tile0 * KT,
                                min(min(qt + kk.shift + 1, t.olen), kk.tile1 * KT), m == -INFINITY ? 0.0f : m, E + qh * entries, qp, sq,
                                p.splits > 1 ? p.part_o + part * p.dim : nullptr, inv);
@@ -448,10 +475,10 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
             tc::bar_sync(1, kRows);
             store_panel<T, kRows>(sq, p.out_lo, p.heads, p.dim, t.begin, head0, p.pack, t.first, rows);
         }
-        if (!alive && tid == 0) count_timeout();
         tc::fence_before();
     }
     __syncthreads();
+    if (tid == 0 && *dead != 0) count_timeout();
     if (warp == 0) tc::tmem_free<kCols>(tmem);
 }
 

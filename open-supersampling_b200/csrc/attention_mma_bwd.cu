@@ -27,6 +27,22 @@ namespace {
 
 constexpr int kShortKeys = 64;
 
+constexpr float kNaN = __builtin_nanf("");
+
+// The end of a block. Where a wait has run out (`lost`): counted, and what is still in flight is waited for.
+__device__ __forceinline__ void finish_block(bool lost, uint32_t bar_end) {
+    if (lost) {
+        tc::cp_async_wait<0>();
+        if (threadIdx.x == 0) count_timeout();
+        if (threadIdx.x < 32) {
+            if (tc::elect_one()) tc::commit(bar_end);
+            __syncwarp();
+            tc::mbar_settle(bar_end, 0);
+        }
+    }
+    __syncthreads();
+}
+
 struct BiasSum {      // of a tile, uniform over the block
     BiasMode mode;
     float fixed;      // 0: nothing to add
@@ -285,7 +301,7 @@ __device__ __forceinline__ bool finish_key_row(const AttnParams& p, uint32_t at,
     const int64_t row = (k * p.kv_heads + kvh) * p.dim;
     T* out = static_cast<T*>(want_v ? p.dv : p.dk) + row;
     float* part = p.qsplits > 1 ? (want_v ? p.part_dv : p.part_dk) + static_cast<int64_t>(z) * p.tk * p.kv_heads * p.dim + row : nullptr;
-    const float by = !alive ? __uint_as_float(0x7fffffffu) : want_v ? 1.0f : p.scale / up;
+    const float by = !alive ? kNaN : want_v ? 1.0f : p.scale / up;
     bool fine = true;
 #pragma unroll
     for (int c = 0; c < DP; c += 16) {
@@ -437,7 +453,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
     double* acc = reinterpret_cast<double*>(base + L::kBytes);
     int* I = reinterpret_cast<int*>(acc + (grad_bias ? group * entries : 0));
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
-    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8, bar_end = bar_s + 24;
 
     const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N, z = blockIdx.z;
     const int dim16 = (p.dim + 15) & ~15;
@@ -479,6 +495,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
+        tc::mbar_init(bar_end, 1);
         tc::mbar_init_fence();
         *dead = 0;
     }
@@ -534,7 +551,12 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             tc::cp_async_wait<0>();
             tc::fence_async();
             tc::fence_before();
-            __syncthreads();
+            if (__syncthreads_or(!alive)) {  // a wait has run out: nothing more is issued, the rows become NaN
+                alive = false;
+                for (int i = tid; i < rows * p.dim; i += kThreads)
+                    static_cast<T*>(p.dq)[(static_cast<int64_t>(q0 + first + i / p.dim) * p.heads + head) * p.dim + i % p.dim] = from_f<T>(kNaN);
+                continue;
+            }
             if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
@@ -570,8 +592,8 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             if (p.causal && tid < rows) p.delta[static_cast<int64_t>(head) * p.tq + q0 + first + tid] = delta;  // tid: one of the two
             tc::fence_async();
             tc::fence_before();
-            __syncthreads();
-            if (warp == 0 && tc::elect_one()) {
+            if (__syncthreads_or(!alive)) alive = false;  // two threads share a row
+            if (alive && warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 tc::mma_tt<kRows>(tmem + t_dv, tc::desc(sp, L::kP), tc::desc(sg, kRows * 128), id_grad, it > i0);
                 tc::mma_tt<kRows>(tmem + t_dk, tc::desc(sd, L::kP), tc::desc(sq, kRows * 128), id_grad, it > i0);
@@ -602,7 +624,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
                 tc::wait_ld();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
-                stage16<T>(sd, row, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
+                stage16<T>(sd, row, o, c, alive ? p.scale / up : kNaN);
             }
             if (p.causal) {
                 if (__syncthreads_or(!fine)) {  // some row of the tile: whoever holds one of its threads
@@ -618,6 +640,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
                 bias_join<kThreads, 8, KT>(p, bs, entries, head, kp, qp_now, I, wsum, acc + g * entries);
             store_panel<T, kThreads>(sd, p.dq, p.heads, p.dim, q0, head, 1, first, rows);
         }
+        if (__syncthreads_or(!alive)) alive = false;  // one thread's weights are in every row
         if ((warp & 3) < 2) {
             const bool of_v = tid < kRows;
             const int64_t key = k0 + min(row, n - 1);
@@ -626,15 +649,14 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         }
         tc::fence_before();
     }
+    const bool lost = __syncthreads_or(!alive);
     if constexpr (BIAS) if (grad_bias) {
-        __syncthreads();
         for (int e = tid; e < entries * group; e += kThreads)
             p.bias_part[(static_cast<int64_t>(kvh * group + e / entries) * p.bias_parts + p.bias_tiny + z * gridDim.x + blockIdx.x) * entries +
-                        e % entries] = acc[e];
+                        e % entries] = lost ? kNaN : acc[e];
     }
-    if (!alive && tid == 0) count_timeout();
     tc::fence_before();
-    __syncthreads();
+    finish_block(lost, bar_end);
     if (warp == 0) tc::tmem_free<kCols>(tmem);
 }
 
@@ -715,7 +737,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     double* acc = reinterpret_cast<double*>(base + L::kBytes);
     int* I = reinterpret_cast<int*>(acc + (grad_bias ? entries : 0));
     float* E = reinterpret_cast<float*>(I + (grad_bias ? entries : 0));
-    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8, bar_end = bar_s + 24;
 
     const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tq, p.windows, kRows);
@@ -724,6 +746,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
+        tc::mbar_init(bar_end, 1);
         tc::mbar_init_fence();
         *dead = 0;
     }
@@ -779,7 +802,10 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             tc::cp_async_wait<0>();
             tc::fence_async();
             tc::fence_before();
-            __syncthreads();
+            if (__syncthreads_or(!alive)) {  // a wait has run out: nothing more is issued
+                alive = false;
+                break;
+            }
             if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
@@ -849,7 +875,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             par_o ^= 1;
         }
         tc::fence_after();
-        __syncthreads();
+        if (__syncthreads_or(!alive)) alive = false;  // one thread's part is in others' rows
         if (grad_bias && tiles > 0 && (bs.fixed != 0.0f || bs.bad))
             bias_join<kThreads, kWarps, KT>(p, bs, entries, head, kps + (kBuf == 2 ? (tiles - 1) & 1 : 0), qp, I, wsum, acc);
         if (tid < kRows) {
@@ -867,7 +893,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
-                stage16<T>(sq, row, o, c, alive ? p.scale / up : __uint_as_float(0x7fffffffu));
+                stage16<T>(sq, row, o, c, alive ? p.scale / up : kNaN);
             }
             if (p.causal && live && !fine && alive) query_row<T>(p, token, head, t.obegin, see, lse, delta, up, sq);
         }
@@ -875,14 +901,12 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
         __syncthreads();
         store_panel<T, kThreads>(sq, p.dq, p.heads, p.dim, t.begin, head, 1, t.first, rows);
     }
-    if (grad_bias) {
-        __syncthreads();
+    const bool lost = __syncthreads_or(!alive);
+    if (grad_bias)
         for (int e = tid; e < entries; e += kThreads)
-            p.bias_part[(static_cast<int64_t>(head) * p.bias_parts + p.bias_tiny + p.bias_short + blockIdx.x) * entries + e] = acc[e];
-    }
-    if (!alive && tid == 0) count_timeout();
+            p.bias_part[(static_cast<int64_t>(head) * p.bias_parts + p.bias_tiny + p.bias_short + blockIdx.x) * entries + e] = lost ? kNaN : acc[e];
     tc::fence_before();
-    __syncthreads();
+    finish_block(lost, bar_end);
     if (warp == 0) tc::tmem_free<L::kCols>(tmem);
 }
 
@@ -904,7 +928,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
     volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     const int entries = BIAS ? bias_entries(p.bias) : 0, kvh = blockIdx.y, group = p.heads / p.kv_heads, z = blockIdx.z;
     float* E = reinterpret_cast<float*>(base + L::kBytes);
-    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8;
+    const uint32_t bar_s = tc::smem_addr(bars), bar_o = bar_s + 8, bar_end = bar_s + 24;
 
     const int tid = threadIdx.x, warp = tid >> 5, row = tid & (kRows - 1), j0 = (tid / kRows) * N;
     const int dim16 = (p.dim + 15) & ~15, slots = attn_slots(p.tk, p.windows, KT);
@@ -913,6 +937,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
     if (tid == 0) {
         tc::mbar_init(bar_s, 1);
         tc::mbar_init(bar_o, 1);
+        tc::mbar_init(bar_end, 1);
         tc::mbar_init_fence();
         *dead = 0;
     }
@@ -963,12 +988,12 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
             head_of_E = kvh * group + it / qtiles;
             for (int e = tid; e < entries; e += kThreads) E[e] = bias_entry(p.bias, p.heads, head_of_E, e);
         };
-        // Of the queries in smem, once everyone's copies are there.
+        // Of the queries in smem, once everyone's copies are there. False: a wait has run out, nothing more is issued.
         auto scores = [&] {
             tc::cp_async_wait<0>();
             tc::fence_async();
             tc::fence_before();
-            __syncthreads();
+            if (__syncthreads_or(!alive)) return false;
             if (warp == 0 && tc::elect_one()) {
                 tc::fence_after();
                 const uint32_t id = tc::idesc(kIsBf16<T>, n16, false, false);
@@ -976,10 +1001,12 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
                 tc::mma_nt<DP, kRows, KT>(tmem + KT, sg, sv, dim16, id);
                 tc::commit(bar_s);
             }
+            return true;
         };
         __syncthreads();
         int it = next(i0), half = 0;
         const bool any = it < i1;
+        bool issued = false;  // the scores of `it`; the same in every thread
         Row now{};
         if (any) {
             ok.load(sk, KT, t.begin + t.first, n, n16);
@@ -992,10 +1019,10 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
                 post_range(now, 0);
                 if (kvh * group + it / qtiles != head_of_E) load_E(it);
             }
-            scores();
+            issued = scores();
         }
         bool begun = false;
-        while (it < i1) {
+        while (issued && it < i1) {
             const int first = (it % qtiles) * kRows, rows = min(kRows, lq - first), after = next(it + 1);
             const bool live = row < rows;
             Row ahead{};
@@ -1032,11 +1059,12 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
             if (after < i1) {
                 fetch(after);
                 tc::cp_async_commit();
-                scores();
+                issued = scores();
             }
             it = after, now = ahead, half ^= 1;
         }
         tc::fence_after();
+        if (__syncthreads_or(!alive)) alive = false;  // one thread's weights are in every row
         const bool of_v = tid < kRows;
         const int64_t key = t.begin + t.first + min(row, n - 1);
         const bool slow = tid < 2 * kRows && finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, key, kvh, z, up,
@@ -1050,9 +1078,9 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
         if (slow) key_row<T>(p, key, t.first + row, kvh, t.obegin, lq, lk, i0, i1, up, of_v, z);
         tc::fence_before();
     }
-    if (!alive && tid == 0) count_timeout();
+    const bool lost = __syncthreads_or(!alive);
     tc::fence_before();
-    __syncthreads();
+    finish_block(lost, bar_end);
     if (warp == 0) tc::tmem_free<L::kCols>(tmem);
 }
 

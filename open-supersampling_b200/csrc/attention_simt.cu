@@ -632,15 +632,18 @@ __global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dt
     const double* sum = p.bias_part + static_cast<int64_t>(head) * p.bias_parts * entries;
     for (int e = tid; e < entries; e += 1024) {
         const int bucket = __ldg(p.bias.map + e);
-        if (bucket >= 0 && bucket < p.bias.buckets)
-            atomicMax(p.bias_top + static_cast<int64_t>(bucket) * p.heads + head,
-                      static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
+        if (bucket < 0 || bucket >= p.bias.buckets) continue;
+        const int64_t i = static_cast<int64_t>(bucket) * p.heads + head;
+        if (isfinite(sum[e]))
+            atomicMax(p.bias_top + i, static_cast<unsigned long long>(__double_as_longlong(fabs(sum[e]))));
+        else
+            p.bias_bad[i] = 1u;
     }
     __threadfence();
     __syncthreads();
     for (int e = tid; e < entries; e += 1024) {
         const int bucket = __ldg(p.bias.map + e);
-        if (bucket >= 0 && bucket < p.bias.buckets) {
+        if (bucket >= 0 && bucket < p.bias.buckets && isfinite(sum[e])) {
             const int64_t i = static_cast<int64_t>(bucket) * p.heads + head;
             atomicAdd(p.bias_acc + i, static_cast<unsigned long long>(__double2ll_rn(ldexp(sum[e], table_shift(__ldcg(p.bias_top + i))))));
         }
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(1024) k_attn_bias_table(AttnParams p, void* dt
     for (int b = tid; b < p.bias.buckets; b += 1024) {
         const int64_t i = static_cast<int64_t>(b) * p.heads + head;
         const double x = ldexp(static_cast<double>(static_cast<long long>(__ldcg(p.bias_acc + i))), -table_shift(__ldcg(p.bias_top + i)));
-        store_typed(dtable, p.bias.table_type, i, p.bias_bad[i] ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
+        store_typed(dtable, p.bias.table_type, i, __ldcg(p.bias_bad + i) ? __uint_as_float(0x7fffffffu) : static_cast<float>(x));
     }
 }
 

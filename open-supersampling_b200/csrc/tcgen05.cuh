@@ -28,15 +28,25 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, int parity) {
         : "memory");
     return done != 0;
 }
-// Bounded: a tile takes microseconds, the limit is seconds. Once a wait of the block has run out
-// (*dead), the others give up as well. False: it ran out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, int parity, volatile int* dead) {
-    for (int i = 0; i < (1 << 20); ++i) {
+// Bounded: a tile takes microseconds, the limit is about ten seconds. Once a wait of the block has run out
+// (*dead), the others give up as well. False: it ran out; what it waited for is not there, and nothing may be
+// issued that relies on it.
+constexpr long long kWaitCycles = 20000000000ll;
+[[nodiscard]] __device__ __forceinline__ bool mbar_wait(uint32_t bar, int parity, volatile int* dead) {
+    if (mbar_try(bar, parity)) return true;
+    const long long start = clock64();
+    for (int i = 1; i < (1 << 30); ++i) {
         if (mbar_try(bar, parity)) return true;
-        if ((i & 255) == 255 && *dead != 0) return false;
+        if ((i & 63) == 1 && (*dead != 0 || clock64() - start > kWaitCycles)) break;
     }
     *dead = 1;
     return false;
+}
+// After a wait that ran out, for what is still on its way: a second at most, whatever *dead says.
+__device__ __forceinline__ void mbar_settle(uint32_t bar, int parity) {
+    const long long start = clock64();
+    for (int i = 0; i < (1 << 28) && !mbar_try(bar, parity) && clock64() - start < kWaitCycles / 10; ++i) {
+    }
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
