@@ -213,15 +213,19 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[N], floa
     }
 }
 
-// dp becomes p (dp - delta).
+// dp becomes p (dp - delta). Hidden pairs' are 0 even where delta is not finite.
 template <int N>
-__device__ __forceinline__ void score_gradients(const float (&s)[N], float (&dp)[N], float delta) {
+__device__ __forceinline__ void score_gradients(const float (&s)[N], float (&dp)[N], float delta, int j0, bool whole, int see) {
     const float2 off = make_float2(-delta, -delta);
 #pragma unroll
     for (int c = 0; c < N; c += 2) {
         const float2 d = __fmul2_rn(make_float2(s[c], s[c + 1]), __fadd2_rn(make_float2(dp[c], dp[c + 1]), off));
         dp[c] = d.x;
         dp[c + 1] = d.y;
+    }
+    if (!whole) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) dp[c] = j0 + c < see ? dp[c] : 0.0f;
     }
 }
 
@@ -583,7 +587,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             write_row<T>(sp, row, j0, s, 1.0f);
             __syncthreads();  // the other half of the row's keys
             const float delta = half_delta[row] + half_delta[kRows + row];
-            score_gradients(s, dp, delta);
+            score_gradients(s, dp, delta, j0, whole, see);
             write_row<T>(sd, row, j0, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
@@ -830,8 +834,9 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, n == n16 && kt * KT + n <= least, see - kt * KT, lse, mode, E, kp, qp);
-            score_gradients(s, dp, delta);
+            const bool whole = n == n16 && kt * KT + n <= least;
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - kt * KT, lse, mode, E, kp, qp);
+            score_gradients(s, dp, delta, j0, whole, see - kt * KT);
             write_row<T>(sd, row, j0, dp, up);
             if (grad_bias) {
                 const float m = warp_size(dp);
@@ -1040,7 +1045,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
             float s[N], dp[N];
             weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, live ? now.lse : INFINITY, mode, E, kp, now.qp);
             write_row<T>(sp, row, j0, s, 1.0f);
-            score_gradients(s, dp, live ? now.delta : 0.0f);
+            score_gradients(s, dp, live ? now.delta : 0.0f, j0, whole, see - t.first);
             write_row<T>(sd, row, j0, dp, up);
             if (BIAS && after < i1) post_range(ahead, half ^ 1);
             tc::fence_async();

@@ -195,3 +195,17 @@ def test_forward_mode_level_without_a_tangent(cuda_device):
         got = run(cuda_device, q, k, v, qo, ko, do)
         assert torch.equal(gated_residual_norm(x, x, w), norm)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [50, 300])
+def test_hidden_pairs_leave_the_table_alone(cuda_device, dtype, tokens):
+    """A gradient that is not finite reaches the rows of the table that its query sees; hidden pairs reach none."""
+    (q, k, v, do), qo, ko, g = inputs([tokens], [tokens], 2, 1, 32, TYPES[dtype], seed=tokens)
+    pos = torch.arange(tokens).int()
+    kw = dict(causal=True, table=torch.randn(7, 2, generator=g), buckets=torch.arange(7, dtype=torch.int32).view(1, 7),
+              q_pos=pos, k_pos=pos)
+    do[tokens // 2, 1, 3] = float("nan")
+    got = run(cuda_device, q, k, v, qo, ko, do, **kw)["dtable"].cpu()
+    assert torch.isnan(got[:4, 1]).all() and torch.isfinite(got[:, 0]).all()
+    assert not got[4:].any()
