@@ -24,8 +24,7 @@ namespace oss {
 namespace {
 
 // ---- a row again, where a product met what its mask hides --------------------------------
-// 0 times a NaN or an infinity behind the causal mask is NaN. A row that comes out not finite is
-// summed once more over the keys it sees (which leaves it not finite if one of those is).
+// Sums a row over the keys that it sees, in the order of its tiles.
 template <typename T>
 __device__ __noinline__ void forward_row(const AttnParams& p, int64_t token, int head, const int32_t* k_pos0, int64_t kt0, int k0,
                                          int k1, float m, const float* E, int2 qp, uint32_t stage, float* part, float inv) {
@@ -446,10 +445,16 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
                 }
             }
             tc::fence_before();  // before the next tile's first P is announced, and so its O is written
-            if (p.causal && live && !fine && alive) {
-                forward_row<T>(p, token, head, BIAS ? p.bias.k_pos : nullptr, t.obegin, kk.tile0 * KT,
-                               min(min(qt + kk.shift + 1, t.olen), kk.tile1 * KT), m == -INFINITY ? 0.0f : m, E + qh * entries, qp, sq,
-                               p.splits > 1 ? p.part_o + part * p.dim : nullptr, inv);
+            // Where l is finite, so is every weight: the values are at fault.
+            bool again = p.causal && live && alive && !fine && is_finite(l);
+            if (__any_sync(0xffffffffu, again)) {
+                const int lo = kk.tile0 * KT, hi = min(kk.most, kk.tile1 * KT), see = min(max(qt + kk.shift + 1, lo), hi);
+                const T* vb = static_cast<const T*>(p.v) + t.obegin * p.v_st + kvh * p.v_sh;
+                const int last = last_not_finite<T>(vb, p.v_st, __reduce_min_sync(0xffffffffu, again ? see : hi), hi, p.dim);
+                again = again && last >= see && hidden_spoils<T>(vb, p.v_st, see, last + 1, lo, see, p.dim);
+                if (again)
+                    forward_row<T>(p, token, head, BIAS ? p.bias.k_pos : nullptr, t.obegin, lo, see, m == -INFINITY ? 0.0f : m, E + qh * entries,
+                                   qp, sq, p.splits > 1 ? p.part_o + part * p.dim : nullptr, inv);
             }
             if (p.splits > 1) continue;
             tc::bar_sync(1, kRows);

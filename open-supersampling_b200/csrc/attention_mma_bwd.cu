@@ -262,6 +262,64 @@ __device__ __noinline__ void query_row(const AttnParams& p, int64_t q, int head,
     for (int c = 0; c < ((p.dim + 15) & ~15); c += 16) stage16<T>(stage, threadIdx.x & (kRows - 1), o + c, c, p.scale / up);
 }
 
+// Whether query_row has to find dq again: dq came out not finite (`odd`) with finite weights. Whole warps; row of the lane.
+template <typename T>
+__device__ __forceinline__ bool query_again(const AttnParams& p, bool odd, int64_t k0, int kvh, int see, int most, float lse, float delta) {
+    bool again = odd && (see == 0 || (is_finite(lse) && is_finite(delta)));
+    if (__any_sync(0xffffffffu, again)) {
+        const T* kb = static_cast<const T*>(p.k) + k0 * p.k_st + kvh * p.k_sh;
+        const int last = last_not_finite<T>(kb, p.k_st, __reduce_min_sync(0xffffffffu, again ? see : most), most, p.dim);
+        again = again && last >= see && hidden_spoils<T>(kb, p.k_st, see, last + 1, 0, see, p.dim);
+    }
+    return again;
+}
+
+// Whether key_row has to find dk (want_v: dv) of the j-th key again, whose products began with query tile qt0 of a
+// head. Whole warps; key of the lane.
+template <typename T>
+__device__ __noinline__ bool key_again(const AttnParams& p, bool odd, int j, int kvh, int64_t q0, int lq, int lk, int qt0, int i0, int i1,
+                                       bool want_v) {
+    if (!__any_sync(0xffffffffu, odd)) return false;
+    const int group = p.heads / p.kv_heads, qtiles = (lq + kRows - 1) / kRows, from = max(j - (lk - lq), 0);  // the first query that sees it
+    const int most = min(__reduce_max_sync(0xffffffffu, odd ? from : 0), lq);
+    const int64_t st = want_v ? p.do_st : p.q_st, sh = want_v ? p.do_sh : p.q_sh;
+    const T* x0 = static_cast<const T*>(want_v ? p.dout : p.q) + q0 * st;
+    // seen: a row of weights that are not finite makes all of the key so
+    auto rows_explain = [&] {
+        for (int it = i1 - 1; it >= i0; --it) {
+            const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows;
+            const float *lse = p.lse + static_cast<int64_t>(head) * p.tq + q0, *delta = p.delta + static_cast<int64_t>(head) * p.tq + q0;
+            for (int i = min(first + kRows, lq) - 1; i >= max(first, from); --i)
+                if (!is_finite(lse[i]) || (!want_v && !is_finite(delta[i]))) return true;
+        }
+        return false;
+    };
+    bool again = false, explained = false, asked = false;
+    for (int it = i0; it < i1; ++it) {
+        const int first = (it % qtiles) * kRows, end = min(min(first + kRows, lq), most);
+        if (it % qtiles < qt0 || first >= end) continue;
+        const T* x = x0 + (kvh * group + it / qtiles) * sh;
+        // hidden: rows of the tile before `from`
+        const bool some = last_not_finite<T>(x, st, first, end, p.dim) >= 0;
+        if (!some || !odd || again || explained) continue;
+        if (!asked) explained = rows_explain(), asked = true;
+        if (explained) continue;
+        const int h1 = min(end, from);
+        for (int c = 0; c < p.dim && !again; ++c) {
+            bool hidden = false, seen = false;
+            for (int r = first; r < h1 && !hidden; ++r) hidden = !is_finite(to_f(x[r * st + c]));
+            if (!hidden) continue;
+            for (int k = i1 - 1; k >= i0 && !seen; --k) {
+                const T* y = x0 + (kvh * group + k / qtiles) * sh;
+                const int f = (k % qtiles) * kRows;
+                for (int r = min(f + kRows, lq) - 1; r >= max(f, from) && !seen; --r) seen = !is_finite(to_f(y[r * st + c]));
+            }
+            again = !seen;
+        }
+    }
+    return again;
+}
+
 // dk (want_v: dv) of key k, the j-th of its window, over the query tiles [i0, i1) of its heads.
 template <typename T>
 __device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int kvh, int64_t q0, int lq, int lk, int i0, int i1, float up,
@@ -298,7 +356,7 @@ __device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int 
 }
 
 // A row of dk or dv out of tensor memory. Whole warps; rows of lanes with `live`. `staged`: to row r of the panel at
-// `to` instead of memory. True: the row has to be found by key_row.
+// `to` instead of memory. True: some value is not finite, in a causal window.
 template <typename T, int DP>
 __device__ __forceinline__ bool finish_key_row(const AttnParams& p, uint32_t at, bool live, bool any, int64_t k, int kvh, int z,
                                                float up, bool want_v, bool alive, bool staged, uint32_t to, int r) {
@@ -634,7 +692,8 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
                 if (__syncthreads_or(!fine)) {  // some row of the tile: whoever holds one of its threads
                     half_delta[tid] = fine ? 0.0f : 1.0f;
                     __syncthreads();
-                    if (tid < rows && half_delta[row] + half_delta[kRows + row] != 0.0f && alive)
+                    const bool odd = row < rows && half_delta[row] + half_delta[kRows + row] != 0.0f && alive;
+                    if (tid < kRows && query_again<T>(p, odd, k0, kvh, see, n, lse_now, delta))
                         query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, delta, up, sd);
                 }
             }
@@ -648,7 +707,8 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         if ((warp & 3) < 2) {
             const bool of_v = tid < kRows;
             const int64_t key = k0 + min(row, n - 1);
-            if (finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, i0 < i1, key, kvh, z, up, of_v, alive, false, 0, 0))
+            const bool odd = finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, i0 < i1, key, kvh, z, up, of_v, alive, false, 0, 0);
+            if (p.causal && key_again<T>(p, odd, row, kvh, q0, lq, lk, 0, i0, i1, of_v))
                 key_row<T>(p, key, row, kvh, q0, lq, lk, i0, i1, up, of_v, z);
         }
         tc::fence_before();
@@ -900,7 +960,8 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 for (int i = 0; i < 16; ++i) fine = fine && is_finite(o[i]);
                 stage16<T>(sq, row, o, c, alive ? p.scale / up : kNaN);
             }
-            if (p.causal && live && !fine && alive) query_row<T>(p, token, head, t.obegin, see, lse, delta, up, sq);
+            if (p.causal && query_again<T>(p, live && !fine && alive, t.obegin, kvh, see, most, lse, delta))
+                query_row<T>(p, token, head, t.obegin, see, lse, delta, up, sq);
         }
         tc::fence_before();
         __syncthreads();
@@ -1072,7 +1133,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
         if (__syncthreads_or(!alive)) alive = false;  // one thread's weights are in every row
         const bool of_v = tid < kRows;
         const int64_t key = t.begin + t.first + min(row, n - 1);
-        const bool slow = tid < 2 * kRows && finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, key, kvh, z, up,
+        const bool odd = tid < 2 * kRows && finish_key_row<T, DP>(p, ts + (of_v ? t_dv : t_dk), row < n, any, key, kvh, z, up,
                                                                    of_v, alive, staged, of_v ? sp : sd, row);
         if (staged) {
             __syncthreads();
@@ -1080,7 +1141,8 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
             store_panel<T, kThreads>(sd, p.dk, p.kv_heads, p.dim, t.begin, kvh, 1, t.first, n);
             if (p.causal) __syncthreads();  // before rows that are written once more
         }
-        if (slow) key_row<T>(p, key, t.first + row, kvh, t.obegin, lq, lk, i0, i1, up, of_v, z);
+        if (p.causal && tid < 2 * kRows && key_again<T>(p, odd, t.first + row, kvh, t.obegin, lq, lk, qt0, i0, i1, of_v))
+            key_row<T>(p, key, t.first + row, kvh, t.obegin, lq, lk, i0, i1, up, of_v, z);
         tc::fence_before();
     }
     const bool lost = __syncthreads_or(!alive);

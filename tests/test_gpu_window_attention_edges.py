@@ -2,6 +2,7 @@
 (tests/attention_reference.py states the allowed errors)."""
 from __future__ import annotations
 
+import math
 import threading
 
 import pytest
@@ -209,3 +210,85 @@ def test_hidden_pairs_leave_the_table_alone(cuda_device, dtype, tokens):
     got = run(cuda_device, q, k, v, qo, ko, do, **kw)["dtable"].cpu()
     assert torch.isnan(got[:4, 1]).all() and torch.isfinite(got[:, 0]).all()
     assert not got[4:].any()
+
+
+def long_case(dtype, tokens, dim, seed=1):
+    (q, k, v, do), qo, ko, _ = inputs([tokens], [tokens], 2, 1, dim, dtype, seed=seed)
+    return {"q": q, "k": k, "v": v, "dout": do}, qo
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bad", ["first key", "first value", "every value", "every key infinite", "last gradient", "last query"])
+def test_visible_values_that_are_not_finite_cost_little(cuda_device, dtype, bad):
+    """A NaN that a row sees is left alone: a causal call with one takes no more than some times the call without."""
+    dev = cuda_device
+    t, off = long_case(TYPES[dtype], 4096, 64)
+    clean = {n: x.to(dev) for n, x in t.items()}
+    if bad == "first key":
+        t["k"][0] = math.nan
+    elif bad == "first value":
+        t["v"][0, 0, 3] = math.inf
+    elif bad == "every value":
+        t["v"][:] = math.nan
+    elif bad == "every key infinite":
+        t["k"][:] = math.inf
+    elif bad == "last gradient":
+        t["dout"][-1] = math.inf
+    else:
+        t["q"][-1] = math.nan
+    spoilt = {n: x.to(dev) for n, x in t.items()}
+
+    def milliseconds(x):
+        best = math.inf
+        for _ in range(3):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            run(dev, x["q"], x["k"], x["v"], off, off, x["dout"], causal=True)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    without = milliseconds(clean)
+    assert milliseconds(spoilt) < 8 * without + 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,at", [(700, 350), (1500, 1023), (60, 31)])
+@pytest.mark.parametrize("dim", [32, 72])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_one_value_that_is_not_finite(cuda_device, dtype, tokens, at, dim, value):
+    """It reaches the rows that see it, and no others: clean ones are right to the last bit that is theirs."""
+    t, off = long_case(TYPES[dtype], tokens, dim)
+    want = window_attention(t["q"], t["k"], t["v"], off, off, causal=True, dout=t["dout"])
+
+    def go(name, index):
+        x = {n: y.clone() for n, y in t.items()}
+        x[name][index] = value
+        return run(cuda_device, x["q"], x["k"], x["v"], off, off, x["dout"], causal=True)
+
+    def clean(got, n, rows):
+        check(got[n][rows], tuple(y[rows] for y in want[n]), n)
+
+    before, after = slice(0, at), slice(at, tokens)
+    got = go("v", (at, 0, 5))
+    clean(got, "out", before)
+    assert not torch.isfinite(got["out"][after, :, 5]).any()
+    others = [c for c in range(dim) if c != 5]
+    check(got["out"][:, :, others], tuple(y[:, :, others] for y in want["out"]), "other columns of out")
+    clean(got, "dq", before)
+    clean(got, "dv", slice(0, tokens))
+    # delta of the rows that see it is NaN or an infinity, and so is every ds of theirs
+    assert not torch.isfinite(got["dq"][after]).any() and not torch.isfinite(got["dk"]).any()
+    got = go("k", (at, 0))
+    clean(got, "out", before)
+    clean(got, "dq", before)
+    got = go("dout", (at, 1, 7))
+    check(got["dv"][at + 1:], tuple(y[at + 1:] for y in want["dv"]), "dv")
+    check(got["dk"][at + 1:], tuple(y[at + 1:] for y in want["dk"]), "dk")
+    assert not torch.isfinite(got["dv"][:at + 1, :, 7]).any()
+    check(got["dv"][:, :, [c for c in range(dim) if c != 7]], tuple(y[:, :, [c for c in range(dim) if c != 7]] for y in want["dv"]), "dv")
+    got = go("q", (at, 1))
+    clean(got, "dk", slice(at + 1, tokens))
+    clean(got, "dv", slice(at + 1, tokens))
+    clean(got, "out", before)
