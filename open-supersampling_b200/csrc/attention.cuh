@@ -19,8 +19,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // gradient sums stay in shared memory beside the tiles (16 + 32 KB).
 constexpr int kMaxBiasEntries = 4096;
 constexpr int kMaxHeadDim = 128;
-// Positions are clamped to this magnitude on load, so that their differences and the linear
-// codes y (2 rx + 1) + x of positions that need no clamp stay within int32.
+// Positions are clamped to this magnitude on load, so that their differences stay within int32. Linear
+// codes count y from a key of the tile: (y - y0) (2 rx + 1) + x, which stays there too where no pair needs clamping.
 constexpr int kMaxPosition = 1 << 29;
 
 enum AttnType { kF32 = 0, kBF16 = 1, kF16 = 2 };

@@ -127,9 +127,14 @@ __device__ __forceinline__ Range join(const Range& a, const Range& b) {
     return {min(a.y0, b.y0), max(a.y1, b.y1), min(a.x0, b.x0), max(a.x1, b.x1)};
 }
 
+// y (2 rx + 1) + x; wraps where nobody uses it.
+__device__ __forceinline__ int linear_code(const AttnBias& b, int y, int x) {
+    return static_cast<int>(static_cast<unsigned>(y) * static_cast<unsigned>(2 * b.rx + 1) + static_cast<unsigned>(x));
+}
+
 template <int KT>
 struct KeyPos {  // of a tile, in shared memory
-    int y[KT], x[KT], code[KT];  // code: y (2 rx + 1) + x
+    int y[KT], x[KT], code[KT];  // code: (y - y[0]) (2 rx + 1) + x, of use where no pair needs clamping
     Range range[KT / 32];
 };
 
@@ -141,7 +146,7 @@ __device__ __forceinline__ void load_key_pos(KeyPos<KT>* s, const AttnBias& b, i
     const int2 p = bias_pos(b.k_pos, b.axes, token + min(j, n - 1));
     s->y[j] = p.x;
     s->x[j] = p.y;
-    s->code[j] = p.x * (2 * b.rx + 1) + p.y;
+    s->code[j] = linear_code(b, p.x - bias_pos(b.k_pos, b.axes, token).x, p.y);
     const Range r = warp_range(p);
     if ((j & 31) == 0) s->range[j >> 5] = r;
 }
@@ -150,11 +155,11 @@ template <int KT>
 __device__ __forceinline__ void load_key_pos_warp(KeyPos<KT>* s, const AttnBias& b, int64_t token, int n) {
 #pragma unroll
     for (int w = 0; w < KT / 32; ++w) {
-        const int j = 32 * w + (threadIdx.x & 31);
+        const int j = 32 * w + (threadIdx.x & 31), y0 = bias_pos(b.k_pos, b.axes, token).x;
         const int2 p = bias_pos(b.k_pos, b.axes, token + min(j, n - 1));
         s->y[j] = p.x;
         s->x[j] = p.y;
-        s->code[j] = p.x * (2 * b.rx + 1) + p.y;
+        s->code[j] = linear_code(b, p.x - y0, p.y);
         const Range r = warp_range(p);
         if ((j & 31) == 0) s->range[w] = r;
     }
@@ -187,7 +192,7 @@ __device__ __forceinline__ void add_bias(float (&x)[N], float c2, const AttnBias
             if (j0 + (c & ~15) < n16) x[c] = fmaf(x[c], c2, E[bias_index(b, qp, make_int2(k->y[j0 + c], k->x[j0 + c]))]);
     } else {
         const int* code = mode == kLinear ? k->code + j0 : k->x + j0;
-        const int dy = mode == kLinear ? -qp.x : min(max(k->y[0] - qp.x, -b.ry), b.ry);
+        const int dy = min(max(k->y[0] - qp.x, -b.ry), b.ry);
         const float* at = E + (dy + b.ry) * w + b.rx - qp.y;
 #pragma unroll
         for (int c = 0; c < N; c += 4) {

@@ -91,7 +91,7 @@ __device__ __forceinline__ void bias_add(const AttnParams& p, const BiasSum& b, 
     }
     const int w = 2 * p.bias.rx + 1;
     const int* code = b.mode == kLinear ? k->code + j0 : k->x + j0;
-    const int dy = b.mode == kLinear ? -qp.x : min(max(k->y[0] - qp.x, -p.bias.ry), p.bias.ry);
+    const int dy = min(max(k->y[0] - qp.x, -p.bias.ry), p.bias.ry);
     int* at = I + (dy + p.bias.ry) * w + p.bias.rx - qp.y;
 #pragma unroll
     for (int c = 0; c < N; c += 4) {

@@ -138,12 +138,12 @@ __device__ __forceinline__ Range tiny_key_pos(TinyPos<NB>* s, const AttnBias& b,
     __syncwarp();
 #pragma unroll
     for (int base = 0; base < 8 * NB; base += 32) {  // whole warps: the ranges name every lane
-        const int j = base + lane;
+        const int j = base + lane, y0 = bias_pos(b.k_pos, b.axes, token).x;
         const int2 p = bias_pos(b.k_pos, b.axes, token + min(j, n - 1));
         if (j < 8 * NB) {
             s->y[j] = p.x;
             s->x[j] = p.y;
-            s->code[j] = p.x * (2 * b.rx + 1) + p.y;
+            s->code[j] = linear_code(b, p.x - y0, p.y);
         }
         const Range r = warp_range(p);
         range = base == 0 ? r : join(range, r);
@@ -163,11 +163,11 @@ struct TinyBias {
     __device__ __forceinline__ TinyBias(const AttnBias& b_, const TinyPos<NB>* k_, const Range& kr, int64_t token, int last, int r0, bool on)
         : b(b_), k(k_), linear(false) {
         if (!on) return;
-        const int g = (threadIdx.x & 31) >> 2, w = 2 * b.rx + 1;
+        const int g = (threadIdx.x & 31) >> 2, y0 = k->y[0];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             q[h] = bias_pos(b.q_pos, b.axes, token + min(r0 + g + 8 * h, last));
-            off[h] = (b.ry - q[h].x) * w + b.rx - q[h].y;
+            off[h] = linear_code(b, b.ry + y0 - q[h].x, b.rx - q[h].y);
         }
         const Range qr = join(warp_range(q[0]), warp_range(q[1]));
         linear = bias_mode(b, qr, kr) == kLinear;

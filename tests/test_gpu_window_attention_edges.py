@@ -292,3 +292,22 @@ def test_one_value_that_is_not_finite(cuda_device, dtype, tokens, at, dim, value
     clean(got, "dk", slice(at + 1, tokens))
     clean(got, "dv", slice(at + 1, tokens))
     clean(got, "out", before)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("keys", [12, 50, 200])
+@pytest.mark.parametrize("where", [2**29 - 40, -(2**29) + 40, 2**31 - 2])
+@pytest.mark.parametrize("reach", [(2, 2), (9, 30)])
+def test_far_positions(cuda_device, dtype, keys, where, reach):
+    """Positions far from 0 along both axes, under maps of few and of many columns: only differences count (beyond 2^29
+    a position counts as 2^29)."""
+    (q, k, v, do), qo, ko, g = inputs([40, 70], [keys, keys], 4, 2, 32, TYPES[dtype], seed=keys)
+    buckets = torch.arange((2 * reach[0] + 1) * (2 * reach[1] + 1), dtype=torch.int32).view(2 * reach[0] + 1, -1)
+    table = torch.randn(buckets.numel(), 4, generator=g)
+    near = [torch.randint(0, 3, (x.shape[0], 2), generator=g) for x in (q, k)]
+    at = [(x + where).clamp(-(2**31), 2**31 - 1).int() for x in near]
+    ref = [x.clamp(-(2**29), 2**29) for x in at]
+    want = window_attention(q, k, v, qo, ko, dout=do, table=table, buckets=buckets, q_pos=ref[0], k_pos=ref[1])
+    got = run(cuda_device, q, k, v, qo, ko, do, table=table, buckets=buckets, q_pos=at[0], k_pos=at[1])
+    for n in want:
+        check(got[n], want[n], n)
