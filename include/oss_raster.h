@@ -652,7 +652,10 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
  * window.  A row that sees no key, and a row outside every window, is zero.
  *   q[tq][heads][dim], k and v[tk][kv_heads][dim]  token and head strides in elements, unit last stride
  *   out[tq][heads][dim], d_q, d_k, d_v             contiguous
- *   lse[heads][tq]     fp32, base-2 log of the row's sum (null: not wanted); +inf for a row without keys
+ *   lse[heads][tq]     fp32, base-2 log of the row's sum (null: not wanted); +inf for a row without keys.
+ *                      With OSS_ATTENTION_LSE_PAIR added to dtype, in both calls, lse[2][heads][tq]: what rounding
+ *                      took from it follows. Without it gradients of rows whose scores all lie far beyond +-1024
+ *                      (a bias of -1e9 on all keys) lose the log of the row's sum.
  *   out_lo[tq][heads][dim]  what rounding took from out, of q's type, for the backward of 16-bit types (null: not
  *                      wanted there, and in the backward not known, which costs its gradients a little precision).
  *                      Rows that the backward does not need may stay unwritten.
@@ -662,6 +665,7 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
  *   q_pos[tq][axes], k_pos[tk][axes]  int32 (y, x), or (x) with axes = 1; clamped to +-2^29
  * entries: (2 ry + 1)(2 rx + 1), 0 without a table.
  * ------------------------------------------------------------------------- */
+#define OSS_ATTENTION_LSE_PAIR 16
 OSS_API int64_t oss_window_attention_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows,
                                                    int64_t heads, int64_t kv_heads, int64_t dim, int32_t causal,
                                                    int64_t entries);

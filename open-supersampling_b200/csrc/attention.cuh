@@ -47,6 +47,7 @@ struct AttnParams {
     AttnBias bias;
     void* out;        // [tq][heads][dim]
     float* lse;       // [heads][tq], base 2, +inf for a row that sees no key; may be null
+    float* lse_rest;  // [heads][tq], what rounding took from lse where that is far from 0; may be null
     // What rounding took from out, [tq][heads][dim] of the same type, of windows with more keys than short_max (others'
     // may stay unwritten): dout . out is then right to fp32. With out alone the gradients of long windows were
     // off by half as much again as rounding them makes them, and the bias table's by twice. May be null; 16-bit types.
@@ -262,6 +263,24 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// ---- the log of a row's sum ------------------------------------------------------
+// A row whose every score is far from 0 (a bias of -1e9 on all its keys) loses the log of its sum beside the
+// maximum, and its weights in the backward would be too large by that. What rounding takes is kept there, and
+// weights are taken times 2^-rest; a closer row loses less than 2^-14.
+constexpr float kFar = 1024.0f;
+__device__ __forceinline__ bool is_far(float lse) { return fabsf(lse) > kFar && fabsf(lse) < INFINITY; }
+__device__ __forceinline__ void store_lse(const AttnParams& p, int64_t at, float m, float l) {
+    const float b = log2f(l), lse = l == 0.0f ? INFINITY : m + b;
+    p.lse[at] = lse;
+    if (p.lse_rest != nullptr && is_far(lse)) {
+        const float bb = lse - m;
+        p.lse_rest[at] = (m - (lse - bb)) + (b - bb);
+    }
+}
+__device__ __forceinline__ float far_factor(const AttnParams& p, int64_t at, float lse) {
+    return p.lse_rest != nullptr && is_far(lse) ? ex2(-p.lse_rest[at]) : 1.0f;
 }
 
 // ---- bias ------------------------------------------------------------------

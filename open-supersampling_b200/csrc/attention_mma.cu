@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kRows + 64, 2) k_attn_fwd_mma(const __grid_con
             const int64_t part = static_cast<int64_t>(blockIdx.z) * p.tq * p.heads + at;
             if (live && p.splits > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
             if (live && p.splits == 1 && p.lse != nullptr)
-                p.lse[static_cast<int64_t>(head) * p.tq + token] = l == 0.0f ? INFINITY : m + log2f(l);
+                store_lse(p, static_cast<int64_t>(head) * p.tq + token, m, l);
             bool fine = true;
 #pragma unroll
             for (int c = 0; c < DP; c += 16) {

@@ -173,7 +173,7 @@ __device__ __forceinline__ void write_out(T* to, const float* o, int c, int dim,
 // Zero where the mask is, whatever stands there.
 template <int KT, bool BIAS, int N>
 __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[N], float (&dp)[N], uint32_t ts, uint32_t tdp, int n16,
-                                        int j0, bool whole, int see, float lse, BiasMode mode, const float* E,
+                                        int j0, bool whole, int see, float lse, float far, BiasMode mode, const float* E,
                                         const KeyPos<KT>* kp, int2 qp) {
     const float c2 = p.scale * kLog2e;
 #pragma unroll
@@ -202,6 +202,10 @@ __device__ __forceinline__ void weights(const AttnParams& p, float (&s)[N], floa
             s[c + i] = ex2(y.x);
             s[c + i + 1] = ex2(y.y);
         }
+    }
+    if (__any_sync(0xffffffffu, far != 1.0f)) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) s[c] *= far;
     }
     if (!whole) {
 #pragma unroll
@@ -247,14 +251,14 @@ __device__ __forceinline__ float score_of(const AttnParams& p, int64_t q, int64_
 
 // dq of one row over the keys [k0, k0 + see) that it sees, staged in the panels at `stage`.
 template <typename T>
-__device__ __noinline__ void query_row(const AttnParams& p, int64_t q, int head, int64_t k0, int see, float lse, float delta, float up,
+__device__ __noinline__ void query_row(const AttnParams& p, int64_t q, int head, int64_t k0, int see, float lse, float far, float delta, float up,
                                        uint32_t stage) {
     float o[kMaxHeadDim];
     const int kvh = head / (p.heads / p.kv_heads);
     const T* g = static_cast<const T*>(p.dout) + q * p.do_st + head * p.do_sh;
     for (int c = 0; c < kMaxHeadDim; ++c) o[c] = 0.0f;
     for (int64_t k = k0; k < k0 + see; ++k) {
-        const float w = ex2(score_of<T>(p, q, k, head, kvh) - lse);
+        const float w = ex2(score_of<T>(p, q, k, head, kvh) - lse) * far;
         const float d = to_f(from_f<T>(w * (dot_row(g, static_cast<const T*>(p.v) + k * p.v_st + kvh * p.v_sh, p.dim) - delta) * up));
         const T* kk = static_cast<const T*>(p.k) + k * p.k_st + kvh * p.k_sh;
         for (int c = 0; c < p.dim; ++c) o[c] = fmaf(d, to_f(kk[c]), o[c]);
@@ -334,12 +338,13 @@ __device__ __noinline__ void key_row(const AttnParams& p, int64_t k, int j, int 
         const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows;
         for (int i = max(first, j - (lk - lq)); i < min(first + kRows, lq); ++i) {
             const int64_t q = q0 + i;
-            float w = ex2(score_of<T>(p, q, k, head, kvh) - p.lse[static_cast<int64_t>(head) * p.tq + q]);
+            const int64_t at = static_cast<int64_t>(head) * p.tq + q;
+            float w = ex2(score_of<T>(p, q, k, head, kvh) - p.lse[at]) * far_factor(p, at, p.lse[at]);
             const T* g = static_cast<const T*>(p.dout) + q * p.do_st + head * p.do_sh;
             const T* with = g;
             if (!want_v) {
                 w *= (dot_row(g, static_cast<const T*>(p.v) + k * p.v_st + kvh * p.v_sh, p.dim) -
-                      p.delta[static_cast<int64_t>(head) * p.tq + q]) * up;
+                      p.delta[at]) * up;
                 with = static_cast<const T*>(p.q) + q * p.q_st + head * p.q_sh;
             }
             w = to_f(from_f<T>(w));
@@ -586,7 +591,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
         const int qtiles = (lq + kRows - 1) / kRows, total = group * qtiles, per = (total + p.qsplits - 1) / p.qsplits;
         const int i0 = min(z * per, total), i1 = min(i0 + per, total);
         const int n = lk, n16 = (n + 15) & ~15;
-        float lse = INFINITY;
+        float lse = INFINITY, far = 1.0f;
         int2 qp = make_int2(0, 0);
         // Q, dO and the row's scalars of one tile
         auto fetch = [&](int it) {
@@ -594,7 +599,9 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             oq.load(sq, kRows, q0 + first, rows, kRows, (it / qtiles) * p.q_sh);
             og.load(sg, kRows, q0 + first, rows, kRows, (it / qtiles) * p.do_sh);
             tc::cp_async_commit();
-            lse = row < rows ? p.lse[static_cast<int64_t>(head) * p.tq + q0 + first + row] : INFINITY;
+            const int64_t at = static_cast<int64_t>(head) * p.tq + q0 + first + min(row, rows - 1);
+            lse = row < rows ? p.lse[at] : INFINITY;
+            far = far_factor(p, at, lse);
             if (BIAS) qp = bias_pos(p.bias.q_pos, p.bias.axes, q0 + first + min(row, rows - 1));
         };
         __syncthreads();  // the window before has read its keys
@@ -634,7 +641,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see, lse, mode, E + g * entries, kp, qp);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see, lse, far, mode, E + g * entries, kp, qp);
             float2 d0 = make_float2(0.0f, 0.0f), d1 = d0;
 #pragma unroll
             for (int c = 0; c < N; c += 4) {
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
             par_o ^= 1;
             tc::fence_after();
             const int2 qp_now = qp;
-            const float lse_now = lse;
+            const float lse_now = lse, far_now = far;
             if (it + 1 < i1) fetch(it + 1);
             // columns of dQ in turn between the two threads of a row
             bool fine = true;
@@ -694,7 +701,7 @@ __global__ void __launch_bounds__(2 * kRows, DP == 64 ? 2 : 1) k_attn_bwd_short(
                     __syncthreads();
                     const bool odd = row < rows && half_delta[row] + half_delta[kRows + row] != 0.0f && alive;
                     if (tid < kRows && query_again<T>(p, odd, k0, kvh, see, n, lse_now, delta))
-                        query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, delta, up, sd);
+                        query_row<T>(p, q0 + first + tid, head, k0, see, lse_now, far_now, delta, up, sd);
                 }
             }
             tc::fence_before();
@@ -840,6 +847,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
         const int tiles = (most + KT - 1) / KT;
         const int64_t token = t.begin + t.first + min(row, rows - 1);
         const float lse = live ? p.lse[static_cast<int64_t>(head) * p.tq + token] : INFINITY;
+        const float far = far_factor(p, static_cast<int64_t>(head) * p.tq + token, lse);
         const float delta = live ? p.delta[static_cast<int64_t>(head) * p.tq + token] : 0.0f;
         const int2 qp = entries > 0 ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0);
         auto fetch = [&](int kt) {
@@ -895,7 +903,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
             tc::fence_after();
             float s[N], dp[N];
             const bool whole = n == n16 && kt * KT + n <= least;
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - kt * KT, lse, mode, E, kp, qp);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - kt * KT, lse, far, mode, E, kp, qp);
             score_gradients(s, dp, delta, j0, whole, see - kt * KT);
             write_row<T>(sd, row, j0, dp, up);
             if (grad_bias) {
@@ -961,7 +969,7 @@ __global__ void __launch_bounds__(DqShape<DP>::kThreads, DP == 64 ? 2 : 1) k_att
                 stage16<T>(sq, row, o, c, alive ? p.scale / up : kNaN);
             }
             if (p.causal && query_again<T>(p, live && !fine && alive, t.obegin, kvh, see, most, lse, delta))
-                query_row<T>(p, token, head, t.obegin, see, lse, delta, up, sq);
+                query_row<T>(p, token, head, t.obegin, see, lse, far, delta, up, sq);
         }
         tc::fence_before();
         __syncthreads();
@@ -1038,13 +1046,14 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
         };
         // What a thread knows of its query of a tile; asked for a tile ahead.
         struct Row {
-            float lse, delta;
+            float lse, delta, far;
             int2 qp;
         };
         auto row_of = [&](int it) {
             const int head = kvh * group + it / qtiles, first = (it % qtiles) * kRows, rows = min(kRows, lq - first);
             const int64_t token = t.obegin + first + min(row, rows - 1), at = static_cast<int64_t>(head) * p.tq + token;
-            return Row{p.lse[at], p.delta[at], BIAS ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0)};
+            const float lse = p.lse[at];
+            return Row{lse, p.delta[at], far_factor(p, at, lse), BIAS ? bias_pos(p.bias.q_pos, p.bias.axes, token) : make_int2(0, 0)};
         };
         auto post_range = [&](const Row& r, int half) {
             const Range x = warp_range(r.qp);
@@ -1104,7 +1113,7 @@ __global__ void __launch_bounds__(DkvShape<DP>::kThreads, DP == 64 ? 2 : 1) k_at
             par_s ^= 1;
             tc::fence_after();
             float s[N], dp[N];
-            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, live ? now.lse : INFINITY, mode, E, kp, now.qp);
+            weights<KT, BIAS>(p, s, dp, ts, ts + KT, n16, j0, whole, see - t.first, live ? now.lse : INFINITY, now.far, mode, E, kp, now.qp);
             write_row<T>(sp, row, j0, s, 1.0f);
             score_gradients(s, dp, live ? now.delta : 0.0f, j0, whole, see - t.first);
             write_row<T>(sd, row, j0, dp, up);

@@ -249,8 +249,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_fwd(AttnParams p) {
 #pragma unroll
         for (int c = 0; c < CN; ++c)
             if (out_col<CN>(tx, c) < p.dim) out[out_col<CN>(tx, c)] = from_f<T>(o[i][c] * inv);
-        if (p.lse != nullptr && tx == 0)
-            p.lse[static_cast<int64_t>(head) * p.tq + token] = l[i] == 0.0f ? INFINITY : m[i] + log2f(l[i]);
+        if (p.lse != nullptr && tx == 0) store_lse(p, static_cast<int64_t>(head) * p.tq + token, m[i], l[i]);
     }
 }
 
@@ -293,8 +292,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_join(AttnParams p) {
         for (int c = 0; c < kMaxHeadDim / 32; ++c)
             if (lane + 32 * c < p.dim) lo[lane + 32 * c] = from_f<T>(lost_by<T>(o[c] * inv));
     }
-    if (p.lse != nullptr && lane == 0)
-        p.lse[(row % p.heads) * p.tq + row / p.heads] = l == 0.0f ? INFINITY : top + log2f(l);
+    if (p.lse != nullptr && lane == 0) store_lse(p, (row % p.heads) * p.tq + row / p.heads, top, l);
 }
 
 // Of 64 bits where it must be: such a division costs some ninety instructions more.
@@ -347,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_delta(AttnParams p) {
 template <int RM>
 __device__ __forceinline__ bool score_grads(const AttnParams& p, float (&s)[RM][4], float (&dp)[RM][4], int first, int rows,
                                             const AttnTile& w, bool by_query, int k0, int n, const float* lse,
-                                            const float* delta, const float* Es, int entries, const int2* qpos,
+                                            const float* delta, const float* far, const float* Es, int entries, const int2* qpos,
                                             const int2* kpos, int ty, int tx) {
     const int qlen = by_query ? w.len : w.olen, klen = by_query ? w.olen : w.len;
     const float c2 = p.scale * kLog2e;
@@ -362,7 +360,7 @@ __device__ __forceinline__ bool score_grads(const AttnParams& p, float (&s)[RM][
             if (j < n && k0 + j < see) {
                 float x = s[i][c] * c2;
                 if (entries > 0) x += Es[bias_index(p.bias, qpos[r], kpos[j])];
-                const float w2 = ex2(x - lse[r]);
+                const float w2 = ex2(x - lse[r]) * far[r];
                 s[i][c] = w2;
                 dp[i][c] = w2 * (dp[i][c] - delta[r]);
             } else {
@@ -391,6 +389,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p, int own_acc)
     float* Ds = sm.take(BM * LDP);
     float* lse = sm.take(BM);
     float* delta = sm.take(BM);
+    float* far = sm.take(BM);
     int2* qpos = reinterpret_cast<int2*>(sm.take(BM * 2));
     int2* kpos = reinterpret_cast<int2*>(sm.take(kKeys * 2));
     const int entries = bias_entries(p.bias);
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p, int own_acc)
         load_rows<T, DP, BM>(Gs, p.dout, p.do_st, p.do_sh, t.begin, head, 1, t.first, rows, p.dim);
         for (int r = tid; r < rows; r += kThreads) {
             const int64_t at = static_cast<int64_t>(head) * p.tq + t.begin + t.first + r;
-            lse[r] = p.lse[at];
+            lse[r] = p.lse[at], far[r] = far_factor(p, at, lse[r]);
             if (entries > 0) qpos[r] = bias_pos(p.bias.q_pos, p.bias.axes, t.begin + t.first + r);
         }
         __syncthreads();
@@ -463,7 +462,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dq(AttnParams p, int own_acc)
             float s[RM][4], dp[RM][4];
             dot_rows<DP, RM>(s, Qs, Ks, n, ty, tx);
             dot_rows<DP, RM>(dp, Gs, Vs, n, ty, tx);
-            const bool cut = score_grads<RM>(p, s, dp, t.first, rows, t, true, k0, n, lse, delta, Es, entries, qpos, kpos, ty, tx);
+            const bool cut = score_grads<RM>(p, s, dp, t.first, rows, t, true, k0, n, lse, delta, far, Es, entries, qpos, kpos, ty, tx);
 #pragma unroll
             for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -532,6 +531,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(AttnParams p) {
     float* Dt = sm.take(kKeys * LDP);
     float* lse = sm.take(BM);
     float* delta = sm.take(BM);
+    float* far = sm.take(BM);
     int2* qpos = reinterpret_cast<int2*>(sm.take(BM * 2));
     int2* kpos = reinterpret_cast<int2*>(sm.take(kKeys * 2));
     const int entries = bias_entries(p.bias);
@@ -561,14 +561,14 @@ __global__ void __launch_bounds__(kThreads) k_attn_dkv(AttnParams p) {
             load_rows<T, DP, BM>(Gs, p.dout, p.do_st, p.do_sh, t.obegin, head, 1, q0, rows, p.dim);
             for (int r = tid; r < rows; r += kThreads) {
                 const int64_t at = static_cast<int64_t>(head) * p.tq + t.obegin + q0 + r;
-                lse[r] = p.lse[at], delta[r] = p.delta[at];
+                lse[r] = p.lse[at], delta[r] = p.delta[at], far[r] = far_factor(p, at, lse[r]);
                 if (entries > 0) qpos[r] = bias_pos(p.bias.q_pos, p.bias.axes, t.obegin + q0 + r);
             }
             __syncthreads();
             float s[RM][4], dp[RM][4];
             dot_rows<DP, RM>(s, Qs, Ks, n, ty, tx);
             dot_rows<DP, RM>(dp, Gs, Vs, n, ty, tx);
-            const bool cut = score_grads<RM>(p, s, dp, q0, rows, t, false, t.first, n, lse, delta, Es, entries, qpos, kpos, ty, tx);
+            const bool cut = score_grads<RM>(p, s, dp, q0, rows, t, false, t.first, n, lse, delta, far, Es, entries, qpos, kpos, ty, tx);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // RM = 4: a row's four values together
                 *reinterpret_cast<float4*>(Pt + (tx + 16 * c) * LDP + ty * RM) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
@@ -692,7 +692,7 @@ template <typename T, int DP>
 cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s) {
     const int64_t entries = bias_entries(p.bias);
     const bool grad_bias = p.bias_part != nullptr;
-    int64_t dq_bytes = 4 * (4 * floats(64 * (DP + 4)) + floats(64 * 68) + 2 * 64 + 4 * 64 + floats(entries) * (grad_bias ? 3 : 1) +
+    int64_t dq_bytes = 4 * (4 * floats(64 * (DP + 4)) + floats(64 * 68) + 3 * 64 + 4 * 64 + floats(entries) * (grad_bias ? 3 : 1) +
                             (grad_bias ? 8 : 0));
     const int own_acc = grad_bias && dq_bytes + 4 * floats(2 * entries) <= kMaxSmem;
     if (own_acc) dq_bytes += 4 * floats(2 * entries);
@@ -706,7 +706,7 @@ cudaError_t bwd_dim(const AttnParams& p, cudaStream_t s) {
         k_attn_dq<T, DP, false><<<dim3(slots, p.heads), kThreads, dq_bytes, s>>>(p, 0);
     }
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    const int64_t kv_bytes = 4 * (4 * floats(64 * (DP + 4)) + 2 * floats(64 * 68) + 2 * 64 + 4 * 64 + floats(entries));
+    const int64_t kv_bytes = 4 * (4 * floats(64 * (DP + 4)) + 2 * floats(64 * 68) + 3 * 64 + 4 * 64 + floats(entries));
     if ((err = allow_smem(k_attn_dkv<T, DP>)) != cudaSuccess) return err;
     k_attn_dkv<T, DP><<<dim3(attn_slots(p.tk, p.windows, kKeys), p.kv_heads), kThreads, kv_bytes, s>>>(p);
     return cudaGetLastError();

@@ -345,9 +345,9 @@ __device__ __forceinline__ void tiny_forward(const AttnParams& p, int kvh, int g
                 if (r0 + g + 8 < r_end) store_row16<T, DB>(lo + to_step, p.dim, o, 1, 1.0f);
             }
             if (p.lse != nullptr && t == 0) {
-                float* lse = p.lse + static_cast<int64_t>(head) * p.tq + q0 + r0 + g;
-                if (r0 + g < r_end) lse[0] = sum.x == 0.0f ? INFINITY : top.x + log2f(sum.x);
-                if (r0 + g + 8 < r_end) lse[8] = sum.y == 0.0f ? INFINITY : top.y + log2f(sum.y);
+                const int64_t at = static_cast<int64_t>(head) * p.tq + q0 + r0 + g;
+                if (r0 + g < r_end) store_lse(p, at, top.x, sum.x);
+                if (r0 + g + 8 < r_end) store_lse(p, at + 8, top.y, sum.y);
             }
         }
     }
@@ -581,8 +581,21 @@ __device__ __forceinline__ void tiny_backward(const AttnParams& p, int kvh, int 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = BIAS ? fmaf(s[kb][i], c2, Eh[at[kb][i]]) - lse[i >> 1] : fmaf(s[kb][i], c2, -lse[i >> 1]);
+                    s[kb][i] = 8 * kb + (i & 1) < left ? ex2(x) : 0.0f;
+                }
+            if (__any_sync(0xffffffffu, is_far(lse[0]) || is_far(lse[1]))) {
+                const int64_t row = static_cast<int64_t>(head) * p.tq + q0 + r0 + g;
+                const float f[2] = {far_factor(p, row, lse[0]), far_factor(p, row + 8, lse[1])};
+#pragma unroll
+                for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[kb][i] *= f[i >> 1];
+            }
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
                     const bool on = 8 * kb + (i & 1) < left;
-                    s[kb][i] = on ? ex2(x) : 0.0f;
                     dp[kb][i] = on ? dp[kb][i] : 0.0f;
                     delta[i >> 1] = fmaf(s[kb][i], dp[kb][i], delta[i >> 1]);
                 }

@@ -1417,6 +1417,7 @@ extern "C" {
 
 int64_t oss_window_attention_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
                                            int64_t kv_heads, int64_t dim, int32_t causal, int64_t entries) {
+    dtype &= ~OSS_ATTENTION_LSE_PAIR;
     if (check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim) != OSS_OK || entries < 0 ||
         entries > oss::kMaxBiasEntries)
         return 0;
@@ -1432,6 +1433,8 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
                                  int32_t table_dtype, int64_t buckets, const int32_t* bucket_map, int64_t ry, int64_t rx,
                                  const int32_t* q_pos, const int32_t* k_pos, int32_t axes, void* out, float* lse,
                                  void* out_lo, void* scratch, int64_t scratch_bytes, void* stream) {
+    const bool lse_pair = (dtype & OSS_ATTENTION_LSE_PAIR) != 0;
+    dtype &= ~OSS_ATTENTION_LSE_PAIR;
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
     OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
@@ -1449,6 +1452,7 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
     p.q_off = q_offsets, p.k_off = k_offsets;
     p.scale = scale;
+    p.lse_rest = lse_pair && lse != nullptr ? lse + tq * heads : nullptr;
     p.out = out, p.lse = lse, p.out_lo = dtype == oss::kF32 ? nullptr : out_lo;
     attention_forward_plan(p, dtype, tq, tk, windows, heads, kv_heads, dim, causal != 0, entries);
     // without the backward's kernel for short windows, the warp-level kernels' would miss what it needs of them
@@ -1474,6 +1478,7 @@ int oss_window_attention_timeouts(uint32_t* count) {
 int64_t oss_window_attention_backward_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
                                                     int64_t kv_heads, int64_t dim, int32_t causal, int64_t entries,
                                                     int64_t buckets) {
+    dtype &= ~OSS_ATTENTION_LSE_PAIR;
     if (check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim) != OSS_OK || entries < 0 ||
         entries > oss::kMaxBiasEntries || buckets < 0 || buckets * heads > INT_MAX)
         return 0;
@@ -1492,6 +1497,8 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
                                   const int32_t* q_pos, const int32_t* k_pos, int32_t axes, const void* out,
                                   const float* lse, const void* out_lo, const void* d_out, int64_t do_st, int64_t do_sh, void* d_q, void* d_k,
                                   void* d_v, void* d_table, void* scratch, int64_t scratch_bytes, void* stream) {
+    const bool lse_pair = (dtype & OSS_ATTENTION_LSE_PAIR) != 0;
+    dtype &= ~OSS_ATTENTION_LSE_PAIR;
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
     OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
@@ -1519,6 +1526,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
     p.heads = static_cast<int>(heads), p.kv_heads = static_cast<int>(kv_heads), p.dim = static_cast<int>(dim);
     p.scale = scale, p.causal = causal != 0, p.pack = 1, p.splits = 1;
     p.out = const_cast<void*>(out), p.lse = const_cast<float*>(lse);
+    p.lse_rest = lse_pair && p.lse != nullptr ? p.lse + tq * heads : nullptr;
     p.out_lo = dtype == oss::kF32 ? nullptr : const_cast<void*>(out_lo);
     p.dout = d_out, p.do_st = do_st, p.do_sh = do_sh, p.dq = d_q, p.dk = d_k, p.dv = d_v;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

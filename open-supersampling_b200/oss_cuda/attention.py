@@ -20,6 +20,7 @@ from . import _lib
 from ._raster import check_int_cuda, check_no_tangent, on_device_of, stream_of
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LSE_PAIR = 16  # OSS_ATTENTION_LSE_PAIR
 MAX_HEAD_DIM = 128
 MAX_BIAS_ENTRIES = 4096
 MAX_TOKENS = 2**30
@@ -41,12 +42,12 @@ def _bias_args(table, buckets, q_pos, k_pos):
 _NO_BIAS = (None, 0, 0, None, 0, 0, None, None, 1)
 
 
-def _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos):
+def _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos, lse_pair=LSE_PAIR):
     """The arguments that the forward and the backward entry points begin with."""
     tq, h, d = q.shape
     tk, kv, _ = k.shape
     qs, ks, vs = q.stride(), k.stride(), v.stride()
-    return (DTYPES[q.dtype], tq, tk, q_offsets.size(0) - 1, h, kv, d, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+    return (DTYPES[q.dtype] | lse_pair, tq, tk, q_offsets.size(0) - 1, h, kv, d, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
             v.data_ptr(), vs[0], vs[1], q_offsets.data_ptr(), k_offsets.data_ptr(), scale, causal,
             *_bias_args(table, buckets, q_pos, k_pos))
 
@@ -59,7 +60,7 @@ def attention_forward(q, k, v, q_offsets, k_offsets, scale, causal, table, bucke
         args = _call_args(q, k, v, q_offsets, k_offsets, scale, causal, table, buckets, q_pos, k_pos)
         dev = q.device
         out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        lse = torch.empty((q.size(1), q.size(0)), device=dev, dtype=torch.float32) if want_lse else None
+        lse = torch.empty((2, q.size(1), q.size(0)), device=dev, dtype=torch.float32) if want_lse else None
         lo = torch.empty_like(out) if want_lse and q.dtype is not torch.float32 else None
         nbytes = lib.oss_window_attention_scratch_bytes(*args[:7], causal, 0 if table is None else buckets.numel())
         scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None

@@ -142,7 +142,7 @@ def test_host_threads_with_other_maps(cuda_device, dtype, keys):
         pos = [torch.randint(-20, 20, (t.shape[0], 2), generator=g).int().to(dev) for t in (q, k)]
         q, k, v, do = (t.to(dev) for t in (q, k, v, do))
         keep = (q, k, v, torch.tensor(qo, **i32), torch.tensor(ko, **i32), 0.2, 0, table, buckets, *pos)
-        args = attention._call_args(*keep)
+        args = attention._call_args(*keep, lse_pair=0)
         out, dq, dk, dv, dt = (torch.empty_like(t) for t in (q, q, k, v, table))
         lo, lse = torch.empty_like(q), torch.empty(1, q.shape[0], device=dev)
         sizes = (lib.oss_window_attention_scratch_bytes(*args[:7], 0, buckets.numel()),
@@ -309,5 +309,50 @@ def test_far_positions(cuda_device, dtype, keys, where, reach):
     ref = [x.clamp(-(2**29), 2**29) for x in at]
     want = window_attention(q, k, v, qo, ko, dout=do, table=table, buckets=buckets, q_pos=ref[0], k_pos=ref[1])
     got = run(cuda_device, q, k, v, qo, ko, do, table=table, buckets=buckets, q_pos=at[0], k_pos=at[1])
+    for n in want:
+        check(got[n], want[n], n)
+
+
+# value of the table, and its type where not fp32
+ALIKE = {"-1e9": (-1e9, None), "-3e7 of q's type": (-3e7, "same")}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", ALIKE)
+@pytest.mark.parametrize("keys", [13, 20, 50, 300])
+def test_rows_whose_keys_are_all_equally_far(cuda_device, dtype, bias, keys):
+    """A row all of whose keys stand at one very low (or high) finite bias weighs them as without it, and so do its gradients."""
+    t = TYPES[dtype]
+    value, table_type = ALIKE[bias]
+    tt = t if table_type == "same" else torch.float32
+    value = min(max(value, torch.finfo(tt).min), torch.finfo(tt).max)
+    (q, k, v, do), qo, ko, _ = inputs([40, 9], [keys, keys], 4, 2, 32, t, seed=keys)
+    q.zero_()  # equal scores: what rounding takes from a score of 0 beside the bias is nothing
+    table = torch.zeros(3, 4, dtype=tt)
+    kw = dict(buckets=torch.tensor([[0, 1, 2]], dtype=torch.int32), q_pos=torch.zeros(49, dtype=torch.int32),
+              k_pos=torch.full((2 * keys,), 5, dtype=torch.int32))
+    want = window_attention(q, k, v, qo, ko, dout=do, table=table, **kw)
+    table[2] = value
+    got = run(cuda_device, q, k, v, qo, ko, do, table=table, **kw)
+    for n in want:
+        check(got[n], want[n], n)
+    if value < 0:  # and beside one key that is not low, they count for nothing
+        kw["k_pos"][[3, keys + 3]] = 0
+        got = run(cuda_device, q, k, v, qo, ko, do, table=table, **kw)
+        # the weight of the one key is 1, dp less delta the difference of two fp32 sums of dim products
+        want = window_attention(q, k[[3, keys + 3]], v[[3, keys + 3]], qo, [0, 1, 2], dout=do, table=torch.zeros(3, 4, dtype=tt),
+                                **{**kw, "k_pos": kw["k_pos"][[3, keys + 3]]})
+        for n in ("out", "dq"):
+            check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_split_row_whose_keys_are_all_equally_far(cuda_device, dtype):
+    (q, k, v, do), qo, ko, _ = inputs([1, 1], [3000, 2100], 4, 2, 64, TYPES[dtype])
+    q.zero_()
+    kw = dict(buckets=torch.tensor([[0, 0, 0]], dtype=torch.int32), q_pos=torch.zeros(2, dtype=torch.int32),
+              k_pos=torch.zeros(5100, dtype=torch.int32))
+    want = window_attention(q, k, v, qo, ko, dout=do, causal=True, table=torch.zeros(1, 4), **kw)
+    got = run(cuda_device, q, k, v, qo, ko, do, causal=True, table=torch.full((1, 4), -1e9), **kw)
     for n in want:
         check(got[n], want[n], n)
