@@ -259,6 +259,7 @@ __device__ __forceinline__ void store_typed(void* p, int type, int64_t i, float 
         static_cast<__half*>(p)[i] = __float2half_rn(x);
 }
 
+__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -284,11 +285,14 @@ __device__ __forceinline__ float far_factor(const AttnParams& p, int64_t at, flo
 }
 
 // ---- bias ------------------------------------------------------------------
-// A head's expanded bias, times log2(e): entry (dy + ry) (2 rx + 1) + dx + rx.
+// A head's expanded bias, times log2(e): entry (dy + ry) (2 rx + 1) + dx + rx. A finite value stays finite: the
+// lowest value of fp32 or bf16 lowers its keys (all alike where a row has no others), only minus infinity hides them.
 __device__ __forceinline__ float bias_entry(const AttnBias& b, int heads, int head, int e) {
     const int bucket = __ldg(b.map + e);
     if (bucket < 0 || bucket >= b.buckets) return 0.0f;
-    return load_typed(b.table, b.table_type, static_cast<int64_t>(bucket) * heads + head) * kLog2e;
+    const float x = load_typed(b.table, b.table_type, static_cast<int64_t>(bucket) * heads + head);
+    constexpr float kMost = 3.4028234663852886e38f;
+    return is_finite(x) ? fminf(fmaxf(x * kLog2e, -kMost), kMost) : x;
 }
 __device__ __forceinline__ int2 bias_pos(const int32_t* pos, int axes, int64_t token) {
     int2 p = axes == 2 ? make_int2(__ldg(pos + token * 2), __ldg(pos + token * 2 + 1)) : make_int2(0, __ldg(pos + token));
@@ -323,7 +327,6 @@ __device__ __forceinline__ void bias_mark_bad(const AttnParams& p, int head, int
     if (bucket >= 0 && bucket < p.bias.buckets) p.bias_bad[static_cast<int64_t>(bucket) * p.heads + head] = 1u;
 }
 
-__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // The sum of finite |ds| of a warp's rows, negative where some is not finite.
 template <int N>
 __device__ __forceinline__ float warp_size(const float (&ds)[N]) {

@@ -160,7 +160,8 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
     scale        of the scores, positive; default D ** -0.5
     causal       query i of a window sees key j where j <= i + (keys - queries): the last query sees all
     bias_table   (num_buckets, H), fp32 or of q's type: bias_table[buckets[clamp(k_pos[j] - q_pos[i])], h] is
-                 added to the scaled score.  buckets is (2 ry + 1, 2 rx + 1) int32 of at most 4096 entries
+                 added to the scaled score (minus infinity hides the key, the lowest finite value only lowers it).
+                 buckets is (2 ry + 1, 2 rx + 1) int32 of at most 4096 entries
                  (window_position_buckets, log_position_buckets; an entry outside the table adds no bias),
                  q_pos (Tq, 2) and k_pos (Tk, 2) int32 (y, x), or (Tq,) and (Tk,) with a (1, 2 r + 1) map.
 

@@ -314,7 +314,8 @@ def test_far_positions(cuda_device, dtype, keys, where, reach):
 
 
 # value of the table, and its type where not fp32
-ALIKE = {"-1e9": (-1e9, None), "-3e7 of q's type": (-3e7, "same")}
+ALIKE = {"-1e9": (-1e9, None), "-3e7 of q's type": (-3e7, "same"), "lowest": (-math.inf, None), "lowest of q's type": (-math.inf, "same"),
+         "highest": (math.inf, None)}
 
 
 @pytest.mark.parametrize("dtype", TYPES)
