@@ -717,7 +717,7 @@ cudaError_t delta_lanes(const AttnParams& p, cudaStream_t s, int sms) {
     const int64_t blocks = (static_cast<int64_t>(p.tq) * p.heads * LANES + kThreads - 1) / kThreads;
     if (blocks == 0) return cudaSuccess;
     const unsigned grid = static_cast<unsigned>(blocks < 16 * sms ? blocks : 16 * sms);
-    const uintptr_t bytes = reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out);
+    const uintptr_t bytes = reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out_lo);
     const bool pairs = bytes % (2 * sizeof(T)) == 0 && ((p.do_st | p.do_sh | p.dim) & 1) == 0;
     if (pairs)
         k_attn_delta<T, LANES, true><<<grid, kThreads, 0, s>>>(p);

@@ -357,3 +357,29 @@ def test_split_row_whose_keys_are_all_equally_far(cuda_device, dtype):
     got = run(cuda_device, q, k, v, qo, ko, do, causal=True, table=torch.full((1, 4), -1e9), **kw)
     for n in want:
         check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("shift", [0, 1, 2, 4])
+def test_rounding_of_out_at_any_address(cuda_device, dtype, shift):
+    """The C entry points take what rounding took from out wherever its type may lie."""
+    from oss_cuda import _lib, attention
+
+    dev, lib, t = cuda_device, _lib.lib(), TYPES[dtype]
+    (q, k, v, do), qo, ko, _ = inputs([150, 20], [200, 90], 2, 2, 32, t)
+    want = window_attention(q, k, v, qo, ko, dout=do)
+    q, k, v, do = (x.to(dev) for x in (q, k, v, do))
+    off = [torch.tensor(o, dtype=torch.int32, device=dev) for o in (qo, ko)]
+    args = attention._call_args(q, k, v, *off, 32**-0.5, 0, None, None, None, None)
+    out, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+    lse = torch.empty(2, *q.shape[1::-1], device=dev)
+    lo = torch.empty(q.numel() + 8, dtype=t, device=dev)[shift:]
+    sizes = (lib.oss_window_attention_scratch_bytes(*args[:7], 0, 0), lib.oss_window_attention_backward_scratch_bytes(*args[:7], 0, 0, 0))
+    scratch = [torch.empty(n + 16, dtype=torch.uint8, device=dev) for n in sizes]
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    saved = (out.data_ptr(), lse.data_ptr(), lo.data_ptr())
+    _lib.check(lib.oss_window_attention_forward(*args, *saved, scratch[0].data_ptr(), sizes[0], stream), "forward")
+    _lib.check(lib.oss_window_attention_backward(*args, *saved, do.data_ptr(), do.stride(0), do.stride(1), dq.data_ptr(), dk.data_ptr(),
+                                                 dv.data_ptr(), None, scratch[1].data_ptr(), sizes[1], stream), "backward")
+    for n, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        check(got, want[n], n)
