@@ -663,7 +663,7 @@ OSS_API int oss_apply_prune_spawn(int64_t n, int64_t f, const int64_t* prune_idx
  *                      query's, clamped to +-ry and +-rx, to a row of the table; a value outside
  *                      [0, buckets) adds no bias.  At most 4096 entries.
  *   q_pos[tq][axes], k_pos[tk][axes]  int32 (y, x), or (x) with axes = 1; clamped to +-2^29
- * entries: (2 ry + 1)(2 rx + 1), 0 without a table.
+ * entries: (2 ry + 1)(2 rx + 1), 0 without a table.  scratch: 16-byte aligned.
  * ------------------------------------------------------------------------- */
 #define OSS_ATTENTION_LSE_PAIR 16
 OSS_API int64_t oss_window_attention_scratch_bytes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows,

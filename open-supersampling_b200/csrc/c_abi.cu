@@ -1461,6 +1461,7 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     const int64_t need = attention_forward_scratch(p, nullptr, 0);
     OSS_CHECK(need == 0 || (scratch != nullptr && scratch_bytes >= need), OSS_ERR_SCRATCH,
               "scratch smaller than oss_window_attention_scratch_bytes");
+    OSS_CHECK(need == 0 || aligned(scratch, 16), OSS_ERR_INVALID, "scratch must be 16-byte aligned");
     attention_forward_scratch(p, static_cast<char*>(scratch), scratch_bytes);
     OSS_CUDA_TRY(oss::launch_attn_forward(p, dtype, static_cast<cudaStream_t>(stream)));
     return OSS_OK;
@@ -1519,6 +1520,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
                   scratch_bytes >= oss_window_attention_backward_scratch_bytes(dtype, tq, tk, windows, heads, kv_heads, dim, causal,
                                                                                oss::bias_entries(p.bias), sums),
               OSS_ERR_SCRATCH, "scratch smaller than oss_window_attention_backward_scratch_bytes");
+    OSS_CHECK(aligned(scratch, 16), OSS_ERR_INVALID, "scratch must be 16-byte aligned");
     p.q = q, p.k = k, p.v = v;
     p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
     p.q_off = q_offsets, p.k_off = k_offsets;
