@@ -226,8 +226,14 @@ def log_position_buckets(num_buckets: int, max_distance: int, causal: bool = Fal
     near = side // 2
     if near < 1 or max_distance <= near or 2 * max_distance + 1 > MAX_BIAS_ENTRIES:
         raise ValueError("needs at least 2 buckets a side, max_distance above half of them and at most 2047")
+    wide = side - near
     r = torch.arange(max_distance + 1, dtype=torch.float64)
-    far = near + (r.clamp(min=1) / near).log() / math.log(max_distance / near) * (side - near)
-    b = torch.where(r < near, r, far.floor().clamp(max=side - 1)).to(torch.int32)
+    steps = (r.clamp(min=1) / near).log() / math.log(max_distance / near) * wide
+    # a distance beside a border is told by whole numbers: (max / near)^k <= (r / near)^wide
+    for i in ((steps - steps.round()).abs() < 1e-9).nonzero().flatten().tolist():
+        k = round(float(steps[i]))
+        if i > near:
+            steps[i] = k if max_distance**k * near ** (wide - k) <= i**wide else k - 1
+    b = torch.where(r < near, r, (near + steps.floor()).clamp(max=side - 1)).to(torch.int32)
     after = torch.zeros_like(b) if causal else b + side
     return torch.cat([b.flip(0), after[1:]]).view(1, -1).to(device)
