@@ -143,8 +143,10 @@ __device__ __forceinline__ float2 row_stats(const float (&u)[kElems], const Gate
     return make_float2(mean, rsqrtf(q[0] * p.inv_c + p.eps));
 }
 
-// The gate's values to their activations, and with SLOPE to its slopes as well.
-template <bool SLOPE>
+// The gate's values to their activations, and with SLOPE to its slopes as well. For 16-bit values __expf, off by 2^-21 and
+// more the farther from 0, and a quotient that is 0 beyond 2^126 are far below a rounding of theirs; fp32 values
+// get expf of a negative number, right to their last digits at either end.
+template <bool SLOPE, bool EXACT>
 __device__ __forceinline__ void activate(float (&g)[kElems], float (&slope)[kElems], int act) {
     if (act == 0) {
 #pragma unroll
@@ -153,7 +155,13 @@ __device__ __forceinline__ void activate(float (&g)[kElems], float (&slope)[kEle
     }
 #pragma unroll
     for (int i = 0; i < kElems; ++i) {
-        const float s = __fdividef(1.0f, 1.0f + __expf(-g[i]));
+        float s;
+        if (EXACT) {
+            const float t = expf(-fabsf(g[i]));
+            s = (g[i] < 0.0f ? t : 1.0f) / (1.0f + t);
+        } else {
+            s = __fdividef(1.0f, 1.0f + __expf(-g[i]));
+        }
         if (act == 1) {
             if (SLOPE) slope[i] = s * (1.0f - s);
             g[i] = s;
@@ -206,7 +214,7 @@ __global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup, TPR < 0 ? 1 : 3) k_ga
             for (int i = 0; i < kElems; ++i) g[i] = one;
         }
         fetch(row + step);
-        activate<false>(g, slope, p.act);
+        activate<false, sizeof(T) == 4>(g, slope, p.act);
         const float2 st1 = row_stats<TPR, V, FULL, LAYER>(h, p, lane, lanes, shared, turn);
 #pragma unroll
         for (int i = 0; i < kElems; ++i) x[i] = fmaf(g[i], LAYER ? fmaf((h[i] - st1.x) * st1.y, w[i], b[i]) : h[i] * st1.y * w[i], x[i]);
@@ -271,7 +279,7 @@ __global__ void __launch_bounds__(TPR < 0 ? 1024 : kGroup, TPR < 0 ? 1 : 2) k_ga
         float u[kElems];
         if (p.dz != nullptr) unpack_row<T, V, FULL>(u, rz, live, lane, lanes, p.c);
         fetch(row + step);
-        activate<true>(g, slope, p.act);
+        activate<true, sizeof(T) == 4>(g, slope, p.act);
         // y again, then its norm, from the forward's statistics
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
