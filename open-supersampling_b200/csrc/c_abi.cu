@@ -1368,9 +1368,10 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
         return static_cast<int>(tiles < per ? (tiles < 1 ? 1 : tiles) : per);
     };
     // The warp-level kernel: up to 32 columns and keys, where windows that short are likely, and the
-    // biases and sums of its warps leave room for two blocks on an SM.
+    // biases and sums of its warps leave room for two blocks on an SM. (Without a kernel for short windows, under
+    // large maps that take no gradient, the long ones' takes all: these were then found twice.)
     const int64_t side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
-    const bool tiny = !p.causal && p.dim <= 32 && p.tk <= 128 * windows &&
+    const bool tiny = p.short_max > 0 && !p.causal && p.dim <= 32 && p.tk <= 128 * windows &&
                       (entries * (4 * side + (sums ? 48 : 0)) + (sums ? 32 : 0)) * group <= 110 * 1024;
     p.tiny_max = tiny ? 32 : 0;
     p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;

@@ -383,3 +383,21 @@ def test_rounding_of_out_at_any_address(cuda_device, dtype, shift):
                                                  dv.data_ptr(), None, scratch[1].data_ptr(), sizes[1], stream), "backward")
     for n, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
         check(got, want[n], n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_large_map_without_its_gradient(cuda_device, dtype):
+    """Few keys a window under a map too large for the kernels of short windows, the table taking no gradient."""
+    from oss_cuda import fused_window_cross_attention
+
+    (q, k, v, do), qo, ko, g = inputs([70, 33, 20], [20, 50, 7], 4, 2, 32, TYPES[dtype])
+    kw = dict(table=torch.randn(4095, 4, generator=g), buckets=torch.arange(4095, dtype=torch.int32).view(63, 65),
+              q_pos=torch.randint(0, 32, (q.shape[0], 2), generator=g).int(), k_pos=torch.randint(0, 32, (k.shape[0], 2), generator=g).int())
+    want = window_attention(q, k, v, qo, ko, dout=do, **kw)
+    dev = cuda_device
+    leaves = [t.to(dev).requires_grad_(True) for t in (q, k, v)]
+    off = [torch.tensor(o, dtype=torch.int32, device=dev) for o in (qo, ko)]
+    kw = {n: t.to(dev) for n, t in kw.items()}
+    out = fused_window_cross_attention(*leaves, *off, bias_table=kw.pop("table"), **kw)
+    for n, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do.to(dev)))):
+        check(got, want[n], n)
