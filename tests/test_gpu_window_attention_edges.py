@@ -8,7 +8,7 @@ import threading
 import pytest
 import torch
 
-from attention_reference import check, window_attention
+from attention_reference import bias_of, check, window_attention
 from test_gpu_window_attention import TYPES, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -401,3 +401,33 @@ def test_large_map_without_its_gradient(cuda_device, dtype):
     out = fused_window_cross_attention(*leaves, *off, bias_table=kw.pop("table"), **kw)
     for n, got in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do.to(dev)))):
         check(got, want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv", [(128, 1, 1), (128, 4, 2), (32, 2, 2), (64, 2, 1)])
+@pytest.mark.parametrize("shape", [(63, 65), (1, 4095)])
+def test_largest_maps(cuda_device, dtype, dim, heads, kv, shape):
+    """As many entries as a map may have, under every kernel."""
+    (q, k, v, do), qo, ko, g = inputs([130, 60, 33], [200, 50, 20], heads, kv, dim, TYPES[dtype], seed=dim)
+    buckets = torch.arange(shape[0] * shape[1], dtype=torch.int32).view(shape)
+    table = torch.randn(buckets.numel(), heads, generator=g)
+    spread = [(n - 1) // 2 for n in shape]
+    pos = [torch.stack([torch.randint(-s // 2, s // 2 + 2, (x.shape[0],), generator=g) for s in spread], 1).int() for x in (q, k)]
+    kw = dict(table=table, buckets=buckets, q_pos=pos[0], k_pos=pos[1])
+    want = window_attention(q, k, v, qo, ko, dout=do, **kw)
+    # Most rows of the table have one pair, many of them with next to no gradient. A pair's term joins integers at
+    # 2^-30 of the sum of magnitudes of its tile (2^-60 in fp32), of which rounding takes half a step at most; a tile
+    # is no more than 128 queries by all keys of the window.
+    for a, b, c, e in zip(qo[:-1], qo[1:], ko[:-1], ko[1:]):
+        bias, row = bias_of(table, buckets, pos[0][a:b], pos[1][c:e])
+        qq, kk, vv, gg = (t.double() for t in (q[a:b], k[c:e].repeat_interleave(heads // kv, 1), v[c:e].repeat_interleave(heads // kv, 1), do[a:b]))
+        p = torch.softmax(torch.einsum("ihd,jhd->hij", qq, kk) / dim**0.5 + bias.permute(2, 0, 1), -1)
+        dp = torch.einsum("ihd,jhd->hij", gg, vv)
+        ds = (p * (dp - (p * dp).sum(-1, keepdim=True))).abs()
+        for i in range(0, b - a, 128):
+            step = ds[:, i:i + 128].sum((1, 2)) * 2.0 ** (-61 if dtype == "fp32" else -31)
+            rows = row[i:i + 128].reshape(-1)
+            want["dtable"][1].index_add_(0, rows, 1.05 * step.expand(rows.numel(), heads))
+    got = run(cuda_device, q, k, v, qo, ko, do, **kw)
+    for n in want:
+        check(got[n], want[n], n)
