@@ -1261,6 +1261,8 @@ namespace {
 
 constexpr int kSms = 148;  // sizes of scratch follow the B200's SM count on every host
 
+constexpr float kMaxScale = 1.7014118e38f;  // 2^127: times log2(e) it is finite still
+
 int check_attention_sizes(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads,
                           int64_t dim) {
     OSS_CHECK(dtype >= 0 && dtype <= 2, OSS_ERR_INVALID, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
@@ -1438,7 +1440,7 @@ int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, int64_t 
     dtype &= ~OSS_ATTENTION_LSE_PAIR;
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
-    OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
+    OSS_CHECK(scale > 0.0f && scale <= kMaxScale, OSS_ERR_INVALID, "scale must be positive, at most 2^127");
     oss::AttnParams p{};
     p.bias = {table, table_dtype, static_cast<int>(buckets), bucket_map, static_cast<int>(ry), static_cast<int>(rx),
               q_pos, k_pos, axes};
@@ -1503,7 +1505,7 @@ int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t
     dtype &= ~OSS_ATTENTION_LSE_PAIR;
     const int rc = check_attention_sizes(dtype, tq, tk, windows, heads, kv_heads, dim);
     if (rc != OSS_OK) return rc;
-    OSS_CHECK(scale > 0.0f && scale <= 3.0e38f, OSS_ERR_INVALID, "scale must be positive and finite");
+    OSS_CHECK(scale > 0.0f && scale <= kMaxScale, OSS_ERR_INVALID, "scale must be positive, at most 2^127");
     oss::AttnParams p{};
     p.bias = {table, table_dtype, static_cast<int>(buckets), bucket_map, static_cast<int>(ry), static_cast<int>(rx),
               q_pos, k_pos, axes};

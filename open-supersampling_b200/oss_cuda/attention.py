@@ -24,6 +24,7 @@ LSE_PAIR = 16  # OSS_ATTENTION_LSE_PAIR
 MAX_HEAD_DIM = 128
 MAX_BIAS_ENTRIES = 4096
 MAX_TOKENS = 2**30
+MAX_SCALE = 2.0**127
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -157,7 +158,7 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
                  [q_offsets[w], q_offsets[w + 1]) and keys [k_offsets[w], k_offsets[w + 1]).  They are not
                  read on the host, so nothing synchronises and the call can be captured in a CUDA graph
                  (values outside the tensors are clamped).  Windows may be empty on either side.
-    scale        of the scores, positive; default D ** -0.5
+    scale        of the scores, positive, at most 2**127; default D ** -0.5
     causal       query i of a window sees key j where j <= i + (keys - queries): the last query sees all
     bias_table   (num_buckets, H), fp32 or of q's type: bias_table[buckets[clamp(k_pos[j] - q_pos[i])], h] is
                  added to the scaled score (minus infinity hides the key, the lowest finite value only lowers it).
@@ -195,8 +196,8 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
     if bias_table is not None or buckets is not None or q_pos is not None or k_pos is not None:
         _check_bias(q, k, bias_table, buckets, q_pos, k_pos)
     scale = 1.0 / math.sqrt(qs[2]) if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError("scale must be positive and finite")
+    if not 0.0 < scale <= MAX_SCALE:
+        raise ValueError("scale must be positive, at most 2**127")
     check_no_tangent("fused_window_cross_attention", q, k, v, bias_table)
     if bias_table is not None:
         bias_table = bias_table.contiguous()
