@@ -1312,14 +1312,16 @@ int attention_splits(int64_t tq, int64_t tk, int64_t windows, int64_t heads, int
 
 // Keys of the windows that the forward's warp-level kernels take, 0: none. They are for windows of up
 // to 128 keys (32 with more than 32 columns: keys and values of more fill the registers) where the average
-// one has at most half of that; their blocks hold the biases of up to 4 key heads. 8160 windows of 256
-// under 24 keys: 430 us, 616 us by tcgen05 tiles of 64 keys, most of whose columns are empty then.
+// one has at most 64 (32); their blocks hold the biases of up to 4 key heads. In us, by them and by tcgen05 tiles
+// alone: 4000 windows of 256 under 40, 64, 100, 128 keys each, 4 heads of 32: 243 : 625, 249 : 584, 895 : 714,
+// 1024 : 675; 8160 under 24, 64, 90 on average, unevenly: 433 : 1217, 1065 : 1590, 1413 : 1810. Heads of 64, 4000
+// under 24, 32, 48 each: 280 : 677, 284 : 671, 682 : 676; 8160 under 16, 24, 40 unevenly: 888 : 1329, 1042 : 1346, 1263 : 1463.
 int attention_tiny(int32_t dtype, int64_t tk, int64_t windows, int64_t heads, int64_t kv_heads, int64_t dim, bool causal,
                    int64_t entries) {
-    const int64_t most = dim <= 32 ? 128 : 32, side = kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1;
-    return dtype != oss::kF32 && !causal && dim <= 64 && windows > 0 && 2 * tk <= most * windows &&
+    const int64_t side = kv_heads >= 4 ? 4 : kv_heads >= 2 ? 2 : 1;
+    return dtype != oss::kF32 && !causal && dim <= 64 && windows > 0 && tk <= (dim <= 32 ? 64 : 32) * windows &&
                    side * (heads / kv_heads) * entries <= 16384
-               ? static_cast<int>(most)
+               ? (dim <= 32 ? 128 : 32)
                : 0;
 }
 
@@ -1370,10 +1372,12 @@ void attention_backward_plan(oss::AttnParams& p, int64_t entries, bool sums) {
         return static_cast<int>(tiles < per ? (tiles < 1 ? 1 : tiles) : per);
     };
     // The warp-level kernel: up to 32 columns and keys, where windows that short are likely, and the
-    // biases and sums of its warps leave room for two blocks on an SM. (Without a kernel for short windows, under
+    // biases and sums of its warps leave room for two blocks on an SM. In us, forward and backward with it and without,
+    // 2040 windows of 256 queries, 4 heads of 32, uneven: with a bias gradient under 8, 24, 60, 120 keys 790 : 860,
+    // 1369 : 1307, 2280 : 2200, 3780 : 3620 (integer sums by shared atomics bound it); without, under 24 and 120, 851 : 929, 2355 : 2334. (Without a kernel for short windows, under
     // large maps that take no gradient, the long ones' takes all: these were then found twice.)
     const int64_t side = p.kv_heads >= 4 ? 4 : p.kv_heads >= 2 ? 2 : 1;
-    const bool tiny = p.short_max > 0 && !p.causal && p.dim <= 32 && p.tk <= 128 * windows &&
+    const bool tiny = p.short_max > 0 && !p.causal && p.dim <= 32 && p.tk <= (sums ? 16 : 128) * windows &&
                       (entries * (4 * side + (sums ? 48 : 0)) + (sums ? 32 : 0)) * group <= 110 * 1024;
     p.tiny_max = tiny ? 32 : 0;
     p.tiny_blocks = tiny ? oss::attn_tiny_backward_blocks(p) : 0;

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from attention_reference import bias_of, check, window_attention
-from test_gpu_window_attention import TYPES, inputs, run
+from test_gpu_window_attention import TYPES, both, inputs, run
 
 pytestmark = pytest.mark.gpu
 
@@ -431,3 +431,18 @@ def test_largest_maps(cuda_device, dtype, dim, heads, kv, shape):
     got = run(cuda_device, q, k, v, qo, ko, do, **kw)
     for n in want:
         check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,kv", [(7, 4, 2), (30, 3, 3), (32, 8, 2)])
+@pytest.mark.parametrize("reach", [2, 6])
+def test_few_keys_on_average_with_a_bias_gradient(cuda_device, dtype, dim, heads, kv, reach):
+    """Windows of either class of the few-keys backward, and some of more keys, where the average has few."""
+    from oss_cuda import window_position_buckets
+
+    kl = [32, 17, 0, 31, 20, 16, 9, 60, 8, 1, 70] + [2] * 25
+    ql = [64, 130, 5, 33, 16, 70, 3, 40, 90, 1, 20] + [7, 0, 40, 1, 18] * 5
+    (q, k, v, do), qo, ko, g = inputs(ql, kl, heads, kv, dim, TYPES[dtype], seed=dim, qfirst=2, ktail=3)
+    buckets = window_position_buckets(reach, reach)
+    both(cuda_device, q, k, v, qo, ko, do, table=torch.randn(buckets.numel(), heads, generator=g).to(TYPES[dtype]), buckets=buckets,
+         q_pos=torch.randint(0, 5, (q.shape[0], 2), generator=g).int(), k_pos=torch.randint(0, 5, (k.shape[0], 2), generator=g).int())
