@@ -677,8 +677,8 @@ OSS_API int oss_window_attention_forward(int32_t dtype, int64_t tq, int64_t tk, 
                                          const int32_t* bucket_map, int64_t ry, int64_t rx, const int32_t* q_pos,
                                          const int32_t* k_pos, int32_t axes, void* out, float* lse, void* out_lo,
                                          void* scratch, int64_t scratch_bytes, void* stream);
-/* Waits inside the tensor-core kernels are bounded; one that runs out (which would be a fault of the
- * library) leaves NaN in its rows and is counted.  count: blocks that this happened to on the current
+/* Waits inside the tensor-core kernels are bounded, at about ten seconds; one that runs out (which would be a fault
+ * of the library) ends what relies on it, leaves NaN in its block's rows and is counted.  count: blocks that this happened to on the current
  * device since the library was loaded.  Synchronises. */
 OSS_API int oss_window_attention_timeouts(uint32_t* count);
 /* buckets: rows of the table whose gradient is wanted, else 0; 0 bytes where an argument is out of range. */
@@ -686,7 +686,9 @@ OSS_API int64_t oss_window_attention_backward_scratch_bytes(int32_t dtype, int64
                                                             int64_t heads, int64_t kv_heads, int64_t dim,
                                                             int32_t causal, int64_t entries, int64_t buckets);
 /* d_table[buckets][heads] in the table's dtype, null: not wanted.  Every gradient is the same
- * on every run: sums have a fixed order, those of d_table are 64-bit integers. */
+ * on every run: sums have a fixed order, or join integers at a power of two that follows from their tile (for d_table
+ * 2^-30 of the tile's sum of magnitudes in 32 bits, 2^-60 in 64 for fp32, at least 2^-20 of 16 rows' where windows have
+ * up to 32 keys), which join fp64 sums in a fixed order. */
 OSS_API int oss_window_attention_backward(int32_t dtype, int64_t tq, int64_t tk, int64_t windows, int64_t heads,
                                           int64_t kv_heads, int64_t dim, const void* q, int64_t q_st, int64_t q_sh,
                                           const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,

@@ -15,8 +15,8 @@
 namespace oss {
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Entries of the expanded position bias, (2 ry + 1) (2 rx + 1): a head's bias and its 64-bit
-// gradient sums stay in shared memory beside the tiles (16 + 32 KB).
+// Entries of the expanded position bias, (2 ry + 1) (2 rx + 1): a head's bias, its integer gradient sums and
+// (in fp32 only where they fit) their fp64 sums stay in shared memory beside the tiles (16 + 16 + 32 KB; fp32 16 + 32 + 32).
 constexpr int kMaxBiasEntries = 4096;
 constexpr int kMaxHeadDim = 128;
 // Positions are clamped to this magnitude on load, so that their differences stay within int32. Linear

@@ -9,9 +9,10 @@
 // S of the next tile is computed into a second buffer while the softmax runs, and two blocks share an
 // SM, so that the exponentials (16 a clock and SM) hardly pause. Keys and values arrive by tensor
 // copies, two tiles ahead; 16- or 4-byte copies or plain loads where strides or alignment allow none.
-// One causal window of 16320, 8 heads over 2 of 128: 705 us, 775 TFLOP/s of the formula's products; the
-// exponentials and the reads of S from tensor memory bound it (a single buffer of S and keys loaded by
-// the softmax warps took 975 us). 68 single tokens over 8160 keys, split: 95 us, 3.4 TB/s of keys and values.
+// One causal window of 16320, 8 heads over 2 of 128: 686 us, 796 TFLOP/s of the formula's products (a single buffer
+// of S and keys loaded by the softmax warps took 975 us). Products and softmax wait for one another: S of a tile for
+// P V of two tiles before, the softmax for O of the one before; the tensor pipe, the exponentials and the issue
+// slots are each less than half taken. 68 single tokens over 8160 keys, split: 94 us, 3.4 TB/s of keys and values.
 // Tiles end at the window's last key rounded up to 16: N of S and K of P V are set by it.
 // The running maximum that the weights are taken against moves only when a row exceeds it by
 // 2^8: O has to be scaled in tensor memory then, which after the first tiles hardly happens.

@@ -745,7 +745,8 @@ __device__ __forceinline__ bool walk_range(AttnWalk<ROWS>& walk, int slots, cons
 // ---- long windows: dq ------------------------------------------------------------------------
 // dq: with up to 64 columns 64 keys a tile and two blocks on an SM, which fill each other's waits;
 // with more, tensor memory holds one block, of 512 threads. 135 windows of 256 under 576, 6 heads of 30, with
-// the bias gradient: 395 us, half of the issue slots taken, by the softmax's arithmetic and the bias's sums.
+// the bias gradient: 384 us; latency at 24% of an SM's warps, with half of the issue slots and of shared memory's pipe
+// taken by the softmax's arithmetic and the bias's sums, and 3% of the tensor pipe.
 template <int DP>
 struct DqShape {
     static constexpr int KT = DP == 64 ? 64 : 128, kThreads = 4 * KT, N = 32;
@@ -756,7 +757,7 @@ struct DqShape {
     static constexpr int kCols = DP == 64 ? 256 : 512;  // S, dP, dQ
 };
 // dk, dv: the same. Products of 64 keys leave half of their 128 rows unused, but two blocks fill each other's
-// waits: 420 us for those windows, against 596 us with 128 keys and one block of 512 threads, and 486 us when
+// waits: 413 us for those windows, against 596 us with 128 keys and one block of 512 threads, and 486 us when
 // that had three buffers of queries and one barrier a step.
 template <int DP>
 struct DkvShape {

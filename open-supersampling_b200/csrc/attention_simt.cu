@@ -3,9 +3,10 @@
 // Tiles of BM queries x 64 keys. 256 threads as 16 x 16: thread (ty, tx) holds rows ty RM + i and
 // keys tx + 16 c of a tile of scores, and rows ty RM + i, columns tx CN + c of an output tile.
 // Every product runs on the FP32 pipe from shared memory, 16 RM FMAs for RM + 4 16-byte loads, two
-// FMAs an instruction, so that the pipe (128 lanes a clock and SM) bounds it and not shared memory.
-// 510 windows of 64 queries under 144 keys, 4 heads of 32, forward and backward: 684 us (785 us with one
-// FMA an instruction and whole tiles at the windows' ends), 12.4 TFLOP/s of 14 dim flops a pair and head.
+// FMAs an instruction. 510 windows of 64 queries under 144 keys, 4 heads of 32, forward and backward: 693 us (785 us
+// with one FMA an instruction and whole tiles at the windows' ends), 12.2 TFLOP/s of 14 dim flops a pair and head where
+// the pipe has 74: S and dP are found in both backward kernels, and at 24% of an SM's warps (128 registers) latency
+// bounds all three, with half of shared memory's pipe, 45% of the issue slots and 19% of the FP32 pipe taken.
 #include "attention.cuh"
 #include "internal.h"
 

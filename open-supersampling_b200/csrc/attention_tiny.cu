@@ -16,8 +16,11 @@
 // P and dS go from accumulators to operands without leaving the lane, transposed in registers
 // for P^T and dS^T.
 //
-// 8160 windows of 256 under 24 keys on average, 4 heads over 2 of 32: 430 us (616 us by tcgen05 tiles alone), of
-// which 223 us for up to 32 keys, 101 us for 33 to 64, 66 us for 65 to 128. Issue of instructions bounds it.
+// 8160 windows of 256 under 24 keys on average, 4 heads over 2 of 32: 424 us (1217 us by the tcgen05 kernel), of
+// which 218 us for up to 32 keys, 102 us for 33 to 64, 67 us for 65 to 128. Latency bounds it: their registers leave
+// 11 to 25% of an SM's warps, which wait for loads and for one instruction after the other; half of the issue
+// slots (a quarter with 65 keys and more) and 43% of DRAM at most are taken. The backward, 2040 windows under 8 keys
+// with a bias gradient: 278 us for up to 16 keys, 78 us for 17 to 32, at 12% of the warps and 28% of the issue slots.
 #include "attention_mma.cuh"
 #include "internal.h"
 

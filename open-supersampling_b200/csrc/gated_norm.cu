@@ -5,14 +5,15 @@
 // Each row belongs to a group of lanes (8, 16 or 32 of a warp, or a whole block for rows of
 // more than 256 channels, of up to 256 threads or 1024); a lane keeps its 8 columns of the row and
 // of the parameters in registers, so that a call reads every activation once and writes every
-// result once: HBM bounds it. Blocks stay and walk rows; the next row's values are on their way
+// result once. Blocks stay and walk rows; the next row's values are on their way
 // while one is worked on. The backward takes x, h and the gate again and recomputes n and y in
 // fp32 (y as written would carry its rounding into every gradient), with the means and deviations
 // of the forward. Sums over rows go lane by lane in fp32 (one lane adds at most rows / groups terms),
 // over the groups of a block in order, then over the blocks in double, always in the same order.
-// 522240 rows of 128 in bf16 with a full gate, forward: 148 us, 4.5 TB/s (271 us without the next row's
-// values on their way). 32640 rows of 1024 in bf16, silu gate, forward and backward: 353 us, 1.9 TB/s; the
-// backward's registers bound it.
+// 522240 rows of 128 in bf16 with a full gate, forward: 148 us, 4.5 TB/s, 69% of a copy's (271 us without the next
+// row's values on their way); the latency of its loads bounds it, at 37% of an SM's warps. 32640 rows of 1024 in bf16,
+// silu gate, forward and backward: 353 us, 1.9 TB/s; the backward's 128 registers leave 24% of the warps, too few for
+// its loads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -168,8 +168,9 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
 
     A query that sees no key, or lies outside every window, gives zeros.  Differentiable once, in q, k, v and
     bias_table, in reverse mode, with the same bits on every run.  Scores, softmax and sums are held in fp32; with 16-bit
-    inputs the weights are rounded to their type before they meet v.  A value that is not finite reaches only
-    the rows whose window and mask show it.  To capture a backward into a graph, drop earlier eager graphs of
+    inputs the weights are rounded to their type before they meet v.  Where a gradient is wanted, long windows of
+    those types also multiply what that rounding took, so that out's last bit may differ from a call without.
+    A value that is not finite reaches only the rows whose window and mask show it.  To capture a backward into a graph, drop earlier eager graphs of
     the same leaves first."""
     dtype, dev, qs, ks = q.dtype, q.device, q.shape, k.shape
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
