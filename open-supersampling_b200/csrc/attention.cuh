@@ -286,7 +286,7 @@ __device__ __forceinline__ float far_factor(const AttnParams& p, int64_t at, flo
 
 // ---- bias ------------------------------------------------------------------
 // A head's expanded bias, times log2(e): entry (dy + ry) (2 rx + 1) + dx + rx. A finite value stays finite: the
-// lowest value of fp32 or bf16 lowers its keys (all alike where a row has no others), only minus infinity hides them.
+// lowest value of fp32 or bf16 lowers its keys (all alike where a row has no others), only minus infinity leaves them no weight.
 __device__ __forceinline__ float bias_entry(const AttnBias& b, int heads, int head, int e) {
     const int bucket = __ldg(b.map + e);
     if (bucket < 0 || bucket >= b.buckets) return 0.0f;

@@ -161,17 +161,18 @@ def fused_window_cross_attention(q, k, v, q_offsets, k_offsets, *, scale=None, c
     scale        of the scores, positive, at most 2**127; default D ** -0.5
     causal       query i of a window sees key j where j <= i + (keys - queries): the last query sees all
     bias_table   (num_buckets, H), fp32 or of q's type: bias_table[buckets[clamp(k_pos[j] - q_pos[i])], h] is
-                 added to the scaled score (minus infinity hides the key, the lowest finite value only lowers it).
-                 buckets is (2 ry + 1, 2 rx + 1) int32 of at most 4096 entries
+                 added to the scaled score (minus infinity leaves a key no weight, the lowest finite value only
+                 lowers it).  buckets is (2 ry + 1, 2 rx + 1) int32 of at most 4096 entries
                  (window_position_buckets, log_position_buckets; an entry outside the table adds no bias),
                  q_pos (Tq, 2) and k_pos (Tk, 2) int32 (y, x), or (Tq,) and (Tk,) with a (1, 2 r + 1) map.
 
-    A query that sees no key, or lies outside every window, gives zeros.  Differentiable once, in q, k, v and
-    bias_table, in reverse mode, with the same bits on every run.  Scores, softmax and sums are held in fp32; with 16-bit
-    inputs the weights are rounded to their type before they meet v.  Where a gradient is wanted, long windows of
-    those types also multiply what that rounding took, so that out's last bit may differ from a call without.
-    A value that is not finite reaches only the rows whose window and mask show it.  To capture a backward into a graph, drop earlier eager graphs of
-    the same leaves first."""
+    A query that sees no key (or only keys whose score is minus infinity), or lies outside every window, gives
+    zeros.  Differentiable once, in q, k, v and bias_table, in reverse mode, with the same bits on every run.
+    Scores, softmax and sums are held in fp32; with 16-bit inputs the weights are rounded to their type before
+    they meet v.  Where a gradient is wanted, long windows of those types also multiply what that rounding took,
+    so that out's last bit may differ from a call without.  A value that is not finite reaches only the rows
+    whose window and causal mask show it.  To capture a backward into a graph, drop earlier eager graphs of the
+    same leaves first."""
     dtype, dev, qs, ks = q.dtype, q.device, q.shape, k.shape
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if not t.is_cuda:
